@@ -246,6 +246,45 @@ int o1d_colsum(const void *x, float *out, void *workspace, size_t workspace_byte
 int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y,
                      int N, int Cin, long long HW, int Cout, int dtype, void *stream);
 
+/* Activation checkpoints in 8 bits: what a training step keeps of a tensor between its forward and its
+ * backward pass (the reference keeps every activation whole, through autograd; models/convnext.py:304-318).
+ * x is [rows, C], fp32 or bf16.  Each row is cut into groups of 128 columns (the last may be shorter).  With lo, hi
+ * the least and greatest value of a group, s = (hi - lo) * (1/255) and q = round_to_even((v - lo) * (1/s)), every
+ * operation in fp32 and rounded on its own; the code q stands for lo + q * s.  A group of equal values (or whose s is
+ * below the normal numbers) has s = 0 and stands for lo; a group that holds a NaN or an infinity, or whose range
+ * overflows, has s = NaN and stands for NaN.  codes: [rows, C] bytes; ranges: [rows, ceil(C / 128), 2] floats,
+ * 8-byte aligned: lo, s. */
+int o1d_keep8(const void *x, uint8_t *codes, float *ranges, long long rows, int C, int dtype, void *stream);
+int o1d_restore8(const uint8_t *codes, const float *ranges, void *y, long long rows, int C, int dtype, void *stream);
+
+/* y = GELU(x + bias) (exact, erf; bias [C] or NULL), and the checkpoint of x + bias in the same pass (codes NULL:
+ * none).  The pass between the two Linear layers of a block (models/convnext.py:311).  bias is fp32, or bf16 with
+ * dtype | O1D_FLAG_PARAMS_BF16. */
+int o1d_gelu_keep8(const void *x, const float *bias, void *y, uint8_t *codes, float *ranges, long long rows, int C,
+                   int dtype, void *stream);
+/* Its backward pass from the checkpoint h' of x + bias: dx = dy * GELU'(h'); dbias = the column sums of dx before
+ * they are rounded (NULL: not wanted; summed in a fixed order; fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16);
+ * y = GELU(h') once more (NULL: not wanted), which a weight gradient of the layer behind reads.
+ * workspace: o1d_gelu_keep8_bwd_workspace_bytes(rows, C) bytes, uninitialised; read only when dbias is given. */
+size_t o1d_gelu_keep8_bwd_workspace_bytes(long long rows, int C);
+int o1d_gelu_keep8_bwd(const uint8_t *codes, const float *ranges, const void *dy, void *dx, void *y, float *dbias,
+                       void *workspace, size_t workspace_bytes, long long rows, int C, int dtype, void *stream);
+
+/* LayerNorm over rows of any length up to 8192, y = (x - mean) * rstd * gamma + beta, and the checkpoint of x in the
+ * same pass; stats: [rows, 2] floats (mean, rstd), 8-byte aligned.  gamma, beta [C] fp32, or bf16 with
+ * dtype | O1D_FLAG_PARAMS_BF16.  (models/convnext.py:28-56; o1d_layernorm_cl keeps x whole and takes rows of whole
+ * vectors only.) */
+int o1d_layernorm_keep8(const void *x, const float *gamma, const float *beta, void *y, uint8_t *codes, float *ranges,
+                        float *stats, long long rows, int C, float eps, int dtype, void *stream);
+/* Its backward pass from the checkpoint of x and the statistics of the true x: dx in the element type, dgamma and
+ * dbeta in the parameters' type, summed in a fixed order.  y: NULL, or the forward pass's output once more, from the
+ * checkpoint (beta is read only then).  workspace: o1d_layernorm_keep8_bwd_workspace_bytes(rows, C) bytes,
+ * uninitialised. */
+size_t o1d_layernorm_keep8_bwd_workspace_bytes(long long rows, int C);
+int o1d_layernorm_keep8_bwd(const uint8_t *codes, const float *ranges, const float *stats, const void *dy,
+                            const float *gamma, const float *beta, void *dx, void *y, float *dgamma, float *dbeta,
+                            void *workspace, size_t workspace_bytes, long long rows, int C, int dtype, void *stream);
+
 /* Batched 2-D transpose [n, a, b] -> [n, b, a].  Replaces nhwc_to_nchw / nchw_to_nhwc
  * (kernels.cu:56-68, nhwc_utils.h:46-110): NHWC->NCHW is (n=N, a=H*W, b=C),
  * NCHW->NHWC is (n=N, a=C, b=H*W). */

@@ -47,6 +47,14 @@ SIGNATURES = {
     "o1d_colsum_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int, _c_int]),
     "o1d_colsum": (_c_int, [_c_void_p] * 3 + [_c_size_t, ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
     "o1d_pointwise_in": (_c_int, [_c_void_p] * 4 + [_c_int, _c_int, ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
+    "o1d_keep8": (_c_int, [_c_void_p] * 3 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
+    "o1d_restore8": (_c_int, [_c_void_p] * 3 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
+    "o1d_gelu_keep8": (_c_int, [_c_void_p] * 5 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
+    "o1d_gelu_keep8_bwd_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int]),
+    "o1d_gelu_keep8_bwd": (_c_int, [_c_void_p] * 7 + [_c_size_t, ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
+    "o1d_layernorm_keep8": (_c_int, [_c_void_p] * 7 + [ctypes.c_longlong, _c_int, ctypes.c_float, _c_int, _c_void_p]),
+    "o1d_layernorm_keep8_bwd_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int]),
+    "o1d_layernorm_keep8_bwd": (_c_int, [_c_void_p] * 11 + [_c_size_t, ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
     "o1d_transpose": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p]),
 }
 

@@ -19,6 +19,7 @@
 #include "o1d_seg.h"
 #include "o1d_wline.h"
 #include "o1d_walk.h"
+#include "o1d_keep8.h"
 
 using namespace o1d;
 
@@ -1281,6 +1282,110 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y, 
 #undef O1D_PW
     O1D_CUDA(cudaGetLastError());
     return O1D_OK;
+}
+
+extern "C++" {
+namespace {
+bool bad_rows(long long rows, int C, int dtype) { return rows <= 0 || C <= 0 || (dtype != O1D_F32 && dtype != O1D_BF16); }
+// Ranges and statistics are read and written as pairs of floats.
+bool misaligned8(const void *p) { return ((uintptr_t)p & 7) != 0; }
+int keep_call(int kind, const KeepArgs &a, int dtype, void *stream, const char *what) {
+    if (misaligned8(a.ranges)) return O1D_ERR_UNSUPPORTED;
+    DeviceInfo d;
+    int rc = device_info(&d);
+    if (rc) return rc;
+    const cudaError_t e = keep_launch(kind, dtype == O1D_BF16, a, d.sms, (cudaStream_t)stream);
+    return e == cudaSuccess ? O1D_OK : cuda_fail(e, what);
+}
+}  // namespace
+}  // extern "C++"
+
+int o1d_keep8(const void *x, uint8_t *codes, float *ranges, long long rows, int C, int dtype, void *stream) {
+    if (!x || !codes || !ranges || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
+    KeepArgs a{};
+    a.x = x; a.codes = codes; a.ranges = ranges; a.rows = rows; a.C = C;
+    return keep_call(KEEP_FWD, a, dtype, stream, "keep8 launch");
+}
+
+int o1d_restore8(const uint8_t *codes, const float *ranges, void *y, long long rows, int C, int dtype, void *stream) {
+    if (!codes || !ranges || !y || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
+    KeepArgs a{};
+    a.codes = const_cast<uint8_t *>(codes); a.ranges = const_cast<float *>(ranges); a.y = y; a.rows = rows; a.C = C;
+    return keep_call(KEEP_RESTORE, a, dtype, stream, "restore8 launch");
+}
+
+int o1d_gelu_keep8(const void *x, const float *bias, void *y, uint8_t *codes, float *ranges, long long rows, int C, int dtype,
+                   void *stream) {
+    const int pbf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
+    dtype &= ~O1D_FLAG_PARAMS_BF16;
+    if (!x || !y || !codes != !ranges || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
+    KeepArgs a{};
+    a.x = x; a.bias = bias; a.y = y; a.codes = codes; a.ranges = ranges; a.rows = rows; a.C = C; a.pbf16 = pbf16;
+    return keep_call(KEEP_GELU_FWD, a, dtype, stream, "GELU checkpoint launch");
+}
+
+size_t o1d_gelu_keep8_bwd_workspace_bytes(long long rows, int C) {
+    DeviceInfo d;
+    if (rows <= 0 || C <= 0 || device_info(&d)) return 0;
+    return (size_t)keep_slices(rows, C, d.sms) * (size_t)C * sizeof(float);
+}
+
+int o1d_gelu_keep8_bwd(const uint8_t *codes, const float *ranges, const void *dy, void *dx, void *y, float *dbias, void *workspace,
+                       size_t workspace_bytes, long long rows, int C, int dtype, void *stream) {
+    const int pbf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
+    dtype &= ~O1D_FLAG_PARAMS_BF16;
+    if (!codes || !ranges || !dy || !dx || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
+    if (dbias && (!workspace || workspace_bytes < o1d_gelu_keep8_bwd_workspace_bytes(rows, C))) return O1D_ERR_WORKSPACE;
+    KeepArgs a{};
+    a.x = dy; a.codes = const_cast<uint8_t *>(codes); a.ranges = const_cast<float *>(ranges); a.y = y; a.dx = dx; a.dbias = dbias;
+    a.partial = (float *)workspace; a.rows = rows; a.C = C; a.pbf16 = pbf16;
+    return keep_call(KEEP_GELU_BWD, a, dtype, stream, "GELU checkpoint backward launch");
+}
+
+extern "C++" {
+namespace {
+int ln_keep_call(bool backward, const LnKeepArgs &a, int dtype, void *stream, const char *what) {
+    if (a.C > kKeepMaxRow || misaligned8(a.ranges) || misaligned8(a.stats)) return O1D_ERR_UNSUPPORTED;
+    DeviceInfo d;
+    int rc = device_info(&d);
+    if (rc) return rc;
+    const cudaError_t e = ln_keep_launch(backward, dtype == O1D_BF16, a, d.sms, (cudaStream_t)stream);
+    return e == cudaSuccess ? O1D_OK : cuda_fail(e, what);
+}
+}  // namespace
+}  // extern "C++"
+
+int o1d_layernorm_keep8(const void *x, const float *gamma, const float *beta, void *y, uint8_t *codes, float *ranges, float *stats,
+                        long long rows, int C, float eps, int dtype, void *stream) {
+    const int pbf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
+    dtype &= ~O1D_FLAG_PARAMS_BF16;
+    if (!x || !gamma || !beta || !y || !codes || !ranges || !stats || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
+    LnKeepArgs a{};
+    a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.codes = codes; a.ranges = ranges; a.stats = stats; a.rows = rows; a.C = C;
+    a.eps = eps; a.pbf16 = pbf16;
+    return ln_keep_call(false, a, dtype, stream, "LayerNorm checkpoint launch");
+}
+
+size_t o1d_layernorm_keep8_bwd_workspace_bytes(long long rows, int C) {
+    DeviceInfo d;
+    if (rows <= 0 || C <= 0 || C > kKeepMaxRow || device_info(&d)) return 0;
+    return (size_t)ln_keep_ctas(rows, C, d.sms) * 2 * (size_t)C * sizeof(float);
+}
+
+int o1d_layernorm_keep8_bwd(const uint8_t *codes, const float *ranges, const float *stats, const void *dy, const float *gamma,
+                            const float *beta, void *dx, void *y, float *dgamma, float *dbeta, void *workspace,
+                            size_t workspace_bytes, long long rows, int C, int dtype, void *stream) {
+    const int pbf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
+    dtype &= ~O1D_FLAG_PARAMS_BF16;
+    if (!codes || !ranges || !stats || !dy || !gamma || (y && !beta) || !dx || !dgamma || !dbeta || bad_rows(rows, C, dtype))
+        return O1D_ERR_INVALID;
+    if (C > kKeepMaxRow) return O1D_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < o1d_layernorm_keep8_bwd_workspace_bytes(rows, C)) return O1D_ERR_WORKSPACE;
+    LnKeepArgs a{};
+    a.x = dy; a.gamma = gamma; a.beta = beta; a.y = y; a.codes = const_cast<uint8_t *>(codes);
+    a.ranges = const_cast<float *>(ranges); a.stats = const_cast<float *>(stats); a.dx = dx; a.dgamma = dgamma; a.dbeta = dbeta;
+    a.partial = (float *)workspace; a.rows = rows; a.C = C; a.pbf16 = pbf16;
+    return ln_keep_call(true, a, dtype, stream, "LayerNorm checkpoint backward launch");
 }
 
 int o1d_transpose(const void *in, void *out, int n, int a, int b, int dtype, void *stream) {

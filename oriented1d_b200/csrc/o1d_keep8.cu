@@ -1,0 +1,110 @@
+// Launches of the 8-bit checkpoint kernels.
+#include "o1d_keep8.cuh"
+#include "o1d_slices.cuh"
+
+namespace o1d {
+
+namespace {
+
+inline int groups_of(int C) { return (C + kKeepGroup - 1) / kKeepGroup; }
+inline bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+// Lanes that hold a row of at most 128 columns, four values each.
+inline int lanes_of(int C) { return C <= 32 ? 8 : C <= 64 ? 16 : 32; }
+
+template <int KIND, typename T, bool VEC, int L>
+cudaError_t keep_go(const KeepArgs &a, int sms, cudaStream_t st) {
+    constexpr int UN = 4;
+    const dim3 grid(groups_of(a.C), keep_slices(a.rows, a.C, sms));
+    keep_kernel<KIND, T, VEC, L, UN><<<grid, kKeepThreads, 0, st>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess && KIND == KEEP_GELU_BWD && a.dbias ? sum_slices(a.partial, a.dbias, a.C, nullptr, 0, a.pbf16, (int)grid.y, st) : e;
+}
+template <int KIND, typename T, bool VEC>
+cudaError_t keep_lanes(const KeepArgs &a, int sms, cudaStream_t st) {
+    switch (lanes_of(a.C)) {
+        case 8: return keep_go<KIND, T, VEC, 8>(a, sms, st);
+        case 16: return keep_go<KIND, T, VEC, 16>(a, sms, st);
+        default: return keep_go<KIND, T, VEC, 32>(a, sms, st);
+    }
+}
+template <int KIND, typename T>
+cudaError_t keep_vec(const KeepArgs &a, int sms, cudaStream_t st) {
+    const int vb = 4 * (int)sizeof(T);
+    const bool vec = a.C % 4 == 0 && aligned(a.x, vb) && aligned(a.y, vb) && aligned(a.dx, vb) && aligned(a.codes, 4);
+    return vec ? keep_lanes<KIND, T, true>(a, sms, st) : keep_lanes<KIND, T, false>(a, sms, st);
+}
+template <typename T>
+cudaError_t keep_kind(int kind, const KeepArgs &a, int sms, cudaStream_t st) {
+    switch (kind) {
+        case KEEP_FWD: return keep_vec<KEEP_FWD, T>(a, sms, st);
+        case KEEP_RESTORE: return keep_vec<KEEP_RESTORE, T>(a, sms, st);
+        case KEEP_GELU_FWD: return keep_vec<KEEP_GELU_FWD, T>(a, sms, st);
+        default: return keep_vec<KEEP_GELU_BWD, T>(a, sms, st);
+    }
+}
+
+// Rows a CTA of the LayerNorm kernels holds at once, and warps that share one.
+inline int ln_team(int C) { return C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : 8; }
+inline int ln_cta_rows(int C) { return C <= 128 ? kKeepWarps * (32 / lanes_of(C)) : kKeepWarps / ln_team(C); }
+
+template <bool BWD, typename T, bool VEC, int L, int TEAM, int NG>
+cudaError_t ln_go(const LnKeepArgs &a, int sms, cudaStream_t st) {
+    const int grid = ln_keep_ctas(a.rows, a.C, sms);
+    if constexpr (BWD) {
+        constexpr int TEAMS = kKeepWarps / TEAM;
+        const int smem = TEAMS > 1 ? TEAMS * 2 * a.C * (int)sizeof(float) : 0;        // at most 32 KB
+        ln_keep_bwd_kernel<T, VEC, L, TEAM, NG><<<grid, kKeepThreads, smem, st>>>(a);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        return sum_slices(a.partial, a.dgamma, a.C, a.dbeta, a.C, a.pbf16, grid, st);
+    } else {
+        ln_keep_kernel<T, VEC, L, TEAM, NG><<<grid, kKeepThreads, 0, st>>>(a);
+        return cudaGetLastError();
+    }
+}
+template <bool BWD, typename T, bool VEC>
+cudaError_t ln_width(const LnKeepArgs &a, int sms, cudaStream_t st) {
+    const int C = a.C;
+    if (C <= 32) return ln_go<BWD, T, VEC, 8, 1, 1>(a, sms, st);
+    if (C <= 64) return ln_go<BWD, T, VEC, 16, 1, 1>(a, sms, st);
+    if (C <= 128) return ln_go<BWD, T, VEC, 32, 1, 1>(a, sms, st);
+    if (C <= 256) return ln_go<BWD, T, VEC, 32, 1, 2>(a, sms, st);
+    if (C <= 512) return ln_go<BWD, T, VEC, 32, 1, 4>(a, sms, st);
+    if (C <= 1024) return ln_go<BWD, T, VEC, 32, 2, 4>(a, sms, st);
+    if (C <= 2048) return ln_go<BWD, T, VEC, 32, 4, 4>(a, sms, st);
+    if (C <= 4096) return ln_go<BWD, T, VEC, 32, 8, 4>(a, sms, st);
+    return ln_go<BWD, T, VEC, 32, 8, 8>(a, sms, st);
+}
+template <bool BWD, typename T>
+cudaError_t ln_vec(const LnKeepArgs &a, int sms, cudaStream_t st) {
+    const int vb = 4 * (int)sizeof(T);
+    const bool vec = a.C % 4 == 0 && aligned(a.x, vb) && aligned(a.y, vb) && aligned(a.dx, vb) && aligned(a.codes, 4);
+    return vec ? ln_width<BWD, T, true>(a, sms, st) : ln_width<BWD, T, false>(a, sms, st);
+}
+
+}  // namespace
+
+int keep_slices(long long rows, int C, int sms) {
+    const int per = kKeepWarps * (C <= 128 ? 32 / lanes_of(C) : 1), G = groups_of(C);
+    const long long most = (rows + per - 1) / per;                       // a row for every warp
+    long long s = ((long long)sms * 16 + G - 1) / G;
+    s = s < most ? s : most;
+    return (int)(s < 1 ? 1 : s > 65535 ? 65535 : s);
+}
+
+cudaError_t keep_launch(int kind, bool bf16, const KeepArgs &a, int sms, cudaStream_t st) {
+    return bf16 ? keep_kind<__nv_bfloat16>(kind, a, sms, st) : keep_kind<float>(kind, a, sms, st);
+}
+
+int ln_keep_ctas(long long rows, int C, int sms) {
+    const int per = ln_cta_rows(C);
+    const long long need = (rows + per - 1) / per, cap = (long long)sms * 4;
+    return (int)(need < cap ? need : cap);
+}
+
+cudaError_t ln_keep_launch(bool backward, bool bf16, const LnKeepArgs &a, int sms, cudaStream_t st) {
+    if (backward) return bf16 ? ln_vec<true, __nv_bfloat16>(a, sms, st) : ln_vec<true, float>(a, sms, st);
+    return bf16 ? ln_vec<false, __nv_bfloat16>(a, sms, st) : ln_vec<false, float>(a, sms, st);
+}
+
+}  // namespace o1d

@@ -370,6 +370,219 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 };
 Tensor linear_train(const Tensor &x, const Tensor &w, const Tensor &b) { return LinearFn::apply(x, w, b); }
 
+// ---- 8-bit activation checkpoints --------------------------------------------------------------------
+// All tensors of a call live on one device: the library launches there, on that device's current stream.
+void need_device(const Tensor &t, const Tensor &like, const char *what) {
+    need_cuda(t);
+    if (t.device() != like.device())
+        throw py::value_error(std::string(what) + " is on " + t.device().str() + ", the first tensor on " + like.device().str());
+}
+// The nodes below differentiate once; a graph of their backward pass would silently leave them out.
+void need_first_order(const char *what) {
+    if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + " has no second derivative (create_graph=True)");
+}
+// [rows, C] of a tensor whose last axis is a row; no rows is a valid tensor, no columns is not.
+struct Rows {
+    int64_t rows, C;
+    explicit Rows(const Tensor &x) {
+        if (x.dim() == 0 || x.size(-1) == 0) throw py::value_error("expected a tensor with at least one column");
+        C = x.size(-1);
+        rows = x.numel() / C;
+        if (C > INT32_MAX) throw py::value_error("rows of more than 2^31 - 1 elements are not supported");
+    }
+};
+struct Kept { Tensor codes, ranges; };
+Kept empty_kept(const Tensor &x) {
+    auto shape = x.sizes().vec();
+    shape.back() = (shape.back() + 127) / 128;
+    shape.push_back(2);
+    return {at::empty(x.sizes(), x.options().dtype(at::kByte)), at::empty(shape, x.options().dtype(at::kFloat))};
+}
+void need_kept(const Tensor &codes, const Tensor &ranges) {
+    if (codes.scalar_type() != at::kByte || ranges.scalar_type() != at::kFloat)
+        throw py::type_error("a checkpoint is uint8 codes and float32 ranges");
+    const Rows r(codes);
+    auto want = codes.sizes().vec();
+    want.back() = (want.back() + 127) / 128;
+    want.push_back(2);
+    if (ranges.sizes() != at::IntArrayRef(want)) {
+        std::ostringstream s;
+        s << "ranges have shape " << ranges.sizes() << ", codes of shape " << codes.sizes() << " need " << at::IntArrayRef(want);
+        throw py::value_error(s.str());
+    }
+}
+
+std::tuple<Tensor, Tensor> keep8(const Tensor &x_) {
+    const Rows r(x_);
+    const int code = dtype_code(x_);
+    need_cuda(x_);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = x_.contiguous();
+    Kept k = empty_kept(x);
+    if (r.rows)
+        check(o1d_keep8(ptr(x), (uint8_t *)k.codes.data_ptr(), (float *)k.ranges.data_ptr(), r.rows, (int)r.C, code, stream()), "o1d_keep8");
+    return {k.codes, k.ranges};
+}
+
+Tensor restore8(const Tensor &codes_, const Tensor &ranges_, bool bf16) {
+    need_kept(codes_, ranges_);
+    const Rows r(codes_);
+    need_cuda(codes_); need_device(ranges_, codes_, "ranges");
+    const c10::cuda::CUDAGuard guard(codes_.device());
+    const Tensor codes = codes_.contiguous(), ranges = ranges_.contiguous();
+    Tensor y = at::empty(codes.sizes(), codes.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+    if (r.rows)
+        check(o1d_restore8((const uint8_t *)ptr(codes), (const float *)ptr(ranges), y.data_ptr(), r.rows, (int)r.C, bf16 ? O1D_BF16 : O1D_F32, stream()),
+              "o1d_restore8");
+    return y;
+}
+
+// GELU(x + bias), and the checkpoint of x + bias when `keep` is set.
+std::tuple<Tensor, Kept> gelu_forward(const Tensor &x_, const OptTensor &bias, bool keep) {
+    const Rows r(x_);
+    const int code = dtype_code(x_);
+    if (bias) need_numel(*bias, r.C, "bias");
+    need_cuda(x_);
+    if (bias) need_device(*bias, x_, "bias");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = x_.contiguous();
+    Tensor b;
+    if (bias) b = is_bf16(*bias) ? bias->contiguous() : as_f32(*bias);
+    Tensor y = at::empty(x.sizes(), x.options());
+    Kept k;
+    if (keep) k = empty_kept(x);
+    if (r.rows)
+        check(o1d_gelu_keep8(ptr(x), (const float *)ptr(b), y.data_ptr(), keep ? (uint8_t *)k.codes.data_ptr() : nullptr,
+                             keep ? (float *)k.ranges.data_ptr() : nullptr, r.rows, (int)r.C,
+                             code | (bias && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+              "o1d_gelu_keep8");
+    return {y, k};
+}
+
+struct GeluGrads { Tensor dx, db, y; };
+// dx; the bias gradient in `db_type` when `with_db` is set; the activation once more when `with_y` is.
+GeluGrads gelu_backward(const Kept &k, const Tensor &dy_, bool with_db, at::ScalarType db_type, bool with_y) {
+    const Rows r(k.codes);
+    const c10::cuda::CUDAGuard guard(dy_.device());
+    const Tensor dy = dy_.contiguous();
+    const int code = dtype_code(dy);
+    GeluGrads g{at::empty(dy.sizes(), dy.options()), {}, {}};
+    if (with_y) g.y = at::empty(dy.sizes(), dy.options());
+    const bool db16 = db_type == at::kBFloat16;
+    Tensor ws;
+    size_t bytes = 0;
+    if (with_db) {
+        auto opts = dy.options().dtype(db16 ? at::kBFloat16 : at::kFloat);
+        g.db = r.rows ? at::empty({r.C}, opts) : at::zeros({r.C}, opts);
+        bytes = o1d_gelu_keep8_bwd_workspace_bytes(r.rows, (int)r.C);
+        ws = at::empty({(int64_t)std::max<size_t>(bytes, 4)}, dy.options().dtype(at::kByte));
+    }
+    if (r.rows)
+        check(o1d_gelu_keep8_bwd((const uint8_t *)ptr(k.codes), (const float *)ptr(k.ranges), ptr(dy), g.dx.data_ptr(),
+                                 with_y ? g.y.data_ptr() : nullptr, with_db ? (float *)g.db.data_ptr() : nullptr,
+                                 with_db ? ws.data_ptr() : nullptr, bytes, r.rows, (int)r.C, code | (db16 ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+              "o1d_gelu_keep8_bwd");
+    if (with_db && g.db.scalar_type() != db_type) g.db = g.db.to(db_type);
+    return g;
+}
+
+struct GeluKeep8Fn : torch::autograd::Function<GeluKeep8Fn> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const OptTensor &bias) {
+        auto [y, k] = gelu_forward(x, bias, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({k.codes, k.ranges});
+        ctx->saved_data["p"] = std::vector<int64_t>{(int64_t)x.scalar_type(), bias ? (int64_t)bias->scalar_type() : (int64_t)at::kFloat, bias.has_value()};
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(2);
+        if (!grads[0].defined()) return out;
+        need_first_order("gelu_keep8");
+        const auto saved = ctx->get_saved_variables();
+        const auto p = ctx->saved_data["p"].toIntVector();
+        const bool need_db = p[2] && ctx->needs_input_grad(1);
+        GeluGrads g = gelu_backward({saved[0], saved[1]}, grads[0].to((at::ScalarType)p[0]), need_db, (at::ScalarType)p[1], false);
+        if (ctx->needs_input_grad(0)) out[0] = g.dx;
+        if (need_db) out[1] = g.db;
+        return out;
+    }
+};
+bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
+bool wants_grad(const OptTensor &t) { return t && t->requires_grad(); }
+Tensor gelu_keep8(const Tensor &x, const OptTensor &bias) {
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(bias))) return GeluKeep8Fn::apply(x, bias);
+    return std::get<0>(gelu_forward(x, bias, false));
+}
+
+struct LnKept { Kept x; Tensor stats; };
+std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, const Tensor &b, double eps) {
+    const Rows r(x_);
+    const int code = dtype_code(x_);
+    need_numel(g, r.C, "weight");
+    need_numel(b, r.C, "bias");
+    need_cuda(x_); need_device(g, x_, "weight"); need_device(b, x_, "bias");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = x_.contiguous();
+    Params p(g, b);
+    Tensor y = at::empty(x.sizes(), x.options());
+    LnKept k{empty_kept(x), at::empty({r.rows, 2}, x.options().dtype(at::kFloat))};
+    if (r.rows)
+        check(o1d_layernorm_keep8(ptr(x), (const float *)ptr(p.w), (const float *)ptr(p.b), y.data_ptr(), (uint8_t *)k.x.codes.data_ptr(),
+                                  (float *)k.x.ranges.data_ptr(), (float *)k.stats.data_ptr(), r.rows, (int)r.C, (float)eps, code | p.flag(), stream()),
+              "o1d_layernorm_keep8");
+    return {y, k};
+}
+
+struct LnGrads { Tensor dx, dg, db, y; };
+LnGrads ln_keep_backward(const LnKept &k, const Tensor &dy_, const Tensor &g, const Tensor &b, bool with_y) {
+    const Rows r(k.x.codes);
+    const c10::cuda::CUDAGuard guard(dy_.device());
+    const Tensor dy = dy_.contiguous();
+    const int code = dtype_code(dy);
+    Params p(g, b);
+    LnGrads out{at::empty(dy.sizes(), dy.options()), {}, {}, {}};
+    auto opts = dy.options().dtype(p.bf16 ? at::kBFloat16 : at::kFloat);
+    out.dg = r.rows ? at::empty({r.C}, opts) : at::zeros({r.C}, opts);
+    out.db = r.rows ? at::empty({r.C}, opts) : at::zeros({r.C}, opts);
+    if (with_y) out.y = at::empty(dy.sizes(), dy.options());
+    const size_t bytes = o1d_layernorm_keep8_bwd_workspace_bytes(r.rows, (int)r.C);
+    Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 4)}, dy.options().dtype(at::kByte));
+    if (r.rows)
+        check(o1d_layernorm_keep8_bwd((const uint8_t *)ptr(k.x.codes), (const float *)ptr(k.x.ranges), (const float *)ptr(k.stats), ptr(dy),
+                                      (const float *)ptr(p.w), (const float *)ptr(p.b), out.dx.data_ptr(), with_y ? out.y.data_ptr() : nullptr,
+                                      (float *)out.dg.data_ptr(), (float *)out.db.data_ptr(), ws.data_ptr(), bytes, r.rows, (int)r.C,
+                                      code | p.flag(), stream()),
+              "o1d_layernorm_keep8_bwd");
+    if (out.dg.scalar_type() != g.scalar_type()) out.dg = out.dg.to(g.scalar_type());
+    if (out.db.scalar_type() != b.scalar_type()) out.db = out.db.to(b.scalar_type());
+    return out;
+}
+
+struct LayerNormKeep8Fn : torch::autograd::Function<LayerNormKeep8Fn> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
+        auto [y, k] = ln_keep_forward(x, g, b, eps);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({k.x.codes, k.x.ranges, k.stats, g, b});
+        ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(4);
+        if (!grads[0].defined()) return out;
+        need_first_order("layer_norm_keep8");
+        const auto s = ctx->get_saved_variables();
+        LnGrads g = ln_keep_backward({{s[0], s[1]}, s[2]}, grads[0].to((at::ScalarType)ctx->saved_data["dtype"].toInt()), s[3], s[4], false);
+        if (ctx->needs_input_grad(0)) out[0] = g.dx;
+        if (ctx->needs_input_grad(1)) out[1] = g.dg.reshape(s[3].sizes());
+        if (ctx->needs_input_grad(2)) out[2] = g.db.reshape(s[4].sizes());
+        return out;
+    }
+};
+Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(g) || wants_grad(b))) return LayerNormKeep8Fn::apply(x, g, b, eps);
+    return std::get<0>(ln_keep_forward(x, g, b, eps));
+}
+
 Tensor conv(const Tensor &x, const Tensor &w, const Tensor &theta, const OptTensor &bias, const Tensor &host, const Tensor &dev,
             int64_t plan_c, int64_t K, int64_t stride, bool nhwc, bool via, bool identity, bool gelu) {
     return ConvFn::apply(x, w, theta, bias, host, dev, plan_c, K, stride, nhwc, via, identity, gelu);
@@ -390,4 +603,8 @@ PYBIND11_MODULE(_o1d_torch, m) {
     m.def("layer_norm_cl_bwd", &layer_norm_cl_bwd, py::call_guard<py::gil_scoped_release>());
     m.def("colsum", &colsum, py::call_guard<py::gil_scoped_release>());
     m.def("pointwise_in", &pointwise_in, py::call_guard<py::gil_scoped_release>());
+    m.def("keep8", &keep8, py::call_guard<py::gil_scoped_release>());
+    m.def("restore8", &restore8, py::call_guard<py::gil_scoped_release>());
+    m.def("gelu_keep8", &gelu_keep8, py::call_guard<py::gil_scoped_release>());
+    m.def("layer_norm_keep8", &layer_norm_keep8, py::call_guard<py::gil_scoped_release>());
 }

@@ -160,6 +160,34 @@ def pointwise_in(x, weight, bias):
     return ext.pointwise_in(x, weight, bias)
 
 
+def keep8(x):
+    """An 8-bit checkpoint of x [..., C]: (codes uint8 [..., C], ranges fp32 [..., ceil(C/128), 2]).  Each group of 128
+    columns of a row has its least value `lo` and a step `s` (a 255th of its range); code q stands for lo + q*s, at most
+    half a step from the value.  A group with a NaN or an infinity in it is NaN when it is read back.  No autograd."""
+    return ext.keep8(x.detach())
+
+
+def restore8(codes, ranges, dtype: torch.dtype = torch.float32):
+    """The values that a checkpoint made by keep8() stands for, in fp32 or bf16."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"oriented1d_b200 supports float32 and bfloat16 tensors, got {dtype}")
+    return ext.restore8(codes, ranges, dtype == torch.bfloat16)
+
+
+def gelu_keep8(x, bias=None):
+    """Exact GELU of x + bias (bias [C], broadcast over the rows; or None), keeping for the backward pass 1.06 bytes an
+    element in place of the tensor: the checkpoint keep8() makes of x + bias.  The output is that of F.gelu; dx and the
+    bias gradient are taken at the values the checkpoint stands for.  Without gradients nothing is kept."""
+    return ext.gelu_keep8(x, bias)
+
+
+def layer_norm_keep8(x, weight, bias, eps: float = 1e-6):
+    """LayerNorm over the last axis (1 to 8192 columns, any alignment), keeping for the backward pass the checkpoint
+    keep8() makes of x and two floats a row in place of x.  The output and the row statistics are those of x itself; dx
+    and the weight gradient read the checkpoint."""
+    return ext.layer_norm_keep8(x, weight, bias, float(eps))
+
+
 def uses_tiled(plan: Plan, N: int, H: int, W: int, stride: int, nhwc: bool, dtype: torch.dtype) -> bool:
     """Would this request run on one of the TMA-staged families (tiled, direct, segments; True) or on the
     general kernels (False)?"""

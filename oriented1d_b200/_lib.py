@@ -47,6 +47,11 @@ SIGNATURES = {
     "o1d_colsum_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int, _c_int]),
     "o1d_colsum": (_c_int, [_c_void_p] * 3 + [_c_size_t, ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
     "o1d_pointwise_in": (_c_int, [_c_void_p] * 4 + [_c_int, _c_int, ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
+    "o1d_linear_xent_workspace_bytes": (_c_size_t, [ctypes.c_longlong] + [_c_int] * 4),
+    "o1d_linear_xent": (_c_int, [_c_void_p] * 8 + [_c_size_t, ctypes.c_longlong, _c_int, _c_int, ctypes.c_longlong, ctypes.c_float, _c_int,
+                                                 _c_int, _c_void_p]),
+    "o1d_linear_xent_bwd": (_c_int, [_c_void_p] * 11 + [_c_size_t, ctypes.c_longlong, _c_int, _c_int, ctypes.c_longlong, ctypes.c_float,
+                                                      _c_int, _c_int, _c_void_p]),
     "o1d_keep8": (_c_int, [_c_void_p] * 3 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
     "o1d_restore8": (_c_int, [_c_void_p] * 3 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
     "o1d_gelu_keep8": (_c_int, [_c_void_p] * 5 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p]),
@@ -62,6 +67,7 @@ ABI_VERSION = 2
 NCHW, NHWC = 0, 1
 F32, BF16 = 0, 1
 FLAG_IDENTITY, FLAG_GELU_INPUT = 1, 2
+XENT_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 class O1dError(RuntimeError):

@@ -20,6 +20,7 @@
 #include "o1d_wline.h"
 #include "o1d_walk.h"
 #include "o1d_keep8.h"
+#include "o1d_xent.h"
 
 using namespace o1d;
 
@@ -1282,6 +1283,63 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y, 
 #undef O1D_PW
     O1D_CUDA(cudaGetLastError());
     return O1D_OK;
+}
+
+extern "C++" {
+namespace {
+bool bad_xent(const XentArgs &a, int dtype) {
+    return !a.x || !a.w || !a.target || !a.lse || a.N <= 0 || a.D <= 0 || a.V <= 0 || (dtype != O1D_F32 && dtype != O1D_BF16) ||
+           !(a.smoothing >= 0.f && a.smoothing <= 1.f) || a.reduction < O1D_XENT_NONE || a.reduction > O1D_XENT_MEAN;
+}
+int xent_call(const XentArgs &a, bool backward, void *stream) {
+    if (a.N > 0x7fffff00LL || a.V > 0x7fffff00) return O1D_ERR_UNSUPPORTED;
+    DeviceInfo d;
+    int rc = device_info(&d), *flag = nullptr;
+    if (!rc) rc = device_flag_ptr(&flag);
+    if (rc) return rc;
+    if (!a.workspace || ((uintptr_t)a.workspace & 255) || a.workspace_bytes < xent_workspace(a, backward, d.sms)) return O1D_ERR_WORKSPACE;
+    cudaError_t e = cudaSuccess;
+    int encode = 0;
+    rc = backward ? xent_backward(a, d.sms, flag, (cudaStream_t)stream, &e, &encode) : xent_forward(a, d.sms, flag, (cudaStream_t)stream, &e, &encode);
+    if (e != cudaSuccess) return cuda_fail(e, "linear cross entropy launch");
+    if (encode) { last_encode_result() = encode; return map_fail("linear cross entropy"); }
+    return rc;
+}
+}  // namespace
+}  // extern "C++"
+
+size_t o1d_linear_xent_workspace_bytes(long long N, int D, int V, int dtype, int backward) {
+    XentArgs a{};
+    a.N = N; a.D = D; a.V = V; a.bf16 = dtype == O1D_BF16;
+    DeviceInfo d;
+    if (N <= 0 || D <= 0 || V <= 0 || N > 0x7fffff00LL || V > 0x7fffff00 || (dtype != O1D_F32 && dtype != O1D_BF16) || device_info(&d)) return 0;
+    return xent_workspace(a, backward != 0, d.sms);
+}
+
+int o1d_linear_xent(const void *x, const void *w, const void *bias, const long long *target, float *loss, float *lse, float *count,
+                    void *workspace, size_t workspace_bytes, long long N, int D, int V, long long ignore_index, float label_smoothing,
+                    int reduction, int dtype, void *stream) {
+    XentArgs a{};
+    a.bias_bf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
+    dtype &= ~O1D_FLAG_PARAMS_BF16;
+    a.x = x; a.w = w; a.bias = bias; a.target = target; a.N = N; a.D = D; a.V = V; a.bf16 = dtype == O1D_BF16; a.ignore = ignore_index;
+    a.smoothing = label_smoothing; a.reduction = reduction; a.loss = loss; a.lse = lse; a.count = count; a.workspace = workspace;
+    a.workspace_bytes = workspace_bytes;
+    if (bad_xent(a, dtype) || !loss || (!count && reduction != O1D_XENT_NONE)) return O1D_ERR_INVALID;
+    return xent_call(a, false, stream);
+}
+
+int o1d_linear_xent_bwd(const void *x, const void *w, const void *bias, const long long *target, const float *lse, const float *count,
+                        const float *dloss, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes, long long N, int D,
+                        int V, long long ignore_index, float label_smoothing, int reduction, int dtype, void *stream) {
+    XentArgs a{};
+    a.bias_bf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
+    dtype &= ~O1D_FLAG_PARAMS_BF16;
+    a.x = x; a.w = w; a.bias = bias; a.target = target; a.N = N; a.D = D; a.V = V; a.bf16 = dtype == O1D_BF16; a.ignore = ignore_index;
+    a.smoothing = label_smoothing; a.reduction = reduction; a.lse = const_cast<float *>(lse); a.count = const_cast<float *>(count);
+    a.dloss = dloss; a.dx = dx; a.dw = dw; a.db = db; a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+    if (bad_xent(a, dtype) || !dloss || (!count && reduction == O1D_XENT_MEAN)) return O1D_ERR_INVALID;
+    return xent_call(a, true, stream);
 }
 
 extern "C++" {

@@ -583,6 +583,105 @@ Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, doubl
     return std::get<0>(ln_keep_forward(x, g, b, eps));
 }
 
+// ---- softmax cross entropy of a linear classifier ----------------------------------------------------
+struct XentShape {
+    int64_t N, D, V;
+    XentShape(const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target, double smoothing) {
+        if (x.dim() == 0 || x.size(-1) == 0) throw py::value_error("x must have at least one feature");
+        D = x.size(-1);
+        N = x.numel() / D;
+        if (w.dim() != 2 || w.size(1) != D || w.size(0) == 0)
+            throw py::value_error("weight must be [classes, " + std::to_string(D) + "]");
+        V = w.size(0);
+        if (w.scalar_type() != x.scalar_type()) throw py::type_error("x and weight must have the same dtype");
+        if (bias) need_numel(*bias, V, "bias");
+        if (target.scalar_type() != at::kLong) throw py::type_error("target must be int64 class indices");
+        if (target.sizes() != x.sizes().slice(0, x.dim() - 1)) {
+            std::ostringstream s;
+            s << "target has shape " << target.sizes() << ", x of shape " << x.sizes() << " needs " << x.sizes().slice(0, x.dim() - 1);
+            throw py::value_error(s.str());
+        }
+        if (!(smoothing >= 0. && smoothing <= 1.)) throw py::value_error("label_smoothing must be between 0 and 1");
+        if (D > INT32_MAX || V > 0x7fffff00 || N > 0x7fffff00) throw py::value_error("more than 2^31 rows, classes or features are not supported");
+        need_cuda(x); need_device(w, x, "weight"); need_device(target, x, "target");
+        if (bias) need_device(*bias, x, "bias");
+    }
+};
+Tensor xent_bias(const OptTensor &b) { return !b ? Tensor() : is_bf16(*b) ? b->contiguous() : as_f32(*b); }
+Tensor xent_workspace(const XentShape &s, const Tensor &like, int code, bool backward, size_t *bytes) {
+    *bytes = o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, backward);
+    return at::empty({(int64_t)std::max<size_t>(*bytes, 256)}, like.options().dtype(at::kByte));
+}
+struct XentOut { Tensor loss, lse, count; };
+XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, const Tensor &target_, int64_t ignore, double smoothing,
+                     int64_t reduction) {
+    const int code = dtype_code(x_);
+    const XentShape s(x_, w_, bias, target_, smoothing);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = x_.contiguous(), w = w_.contiguous(), target = target_.contiguous(), b = xent_bias(bias);
+    const auto f32 = x.options().dtype(at::kFloat);
+    const bool each = reduction == O1D_XENT_NONE;
+    XentOut o{each ? at::empty(target.sizes(), f32) : at::empty({}, f32), at::empty({s.N}, f32), each ? Tensor() : at::empty({}, f32)};
+    if (s.N == 0) {                                       // the sum of nothing, the mean of nothing
+        if (!each) { o.loss.fill_(reduction == O1D_XENT_SUM ? 0. : NAN); o.count.zero_(); }
+        return o;
+    }
+    size_t bytes;
+    Tensor ws = xent_workspace(s, x, code, false, &bytes);
+    check(o1d_linear_xent(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (float *)o.loss.data_ptr(), (float *)o.lse.data_ptr(),
+                          each ? nullptr : (float *)o.count.data_ptr(), ws.data_ptr(), bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing,
+                          (int)reduction, code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+          "o1d_linear_xent");
+    return o;
+}
+
+struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target,
+                          int64_t ignore, double smoothing, int64_t reduction) {
+        XentOut o = xent_forward(x, w, bias, target, ignore, smoothing, reduction);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, w, bias ? *bias : Tensor(), target, o.lse, o.count});
+        ctx->saved_data["p"] = std::vector<int64_t>{ignore, reduction};
+        ctx->saved_data["smoothing"] = smoothing;
+        return o.loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(7);
+        if (!grads[0].defined()) return out;
+        need_first_order("linear_cross_entropy");
+        const auto saved = ctx->get_saved_variables();
+        const OptTensor bias = saved[2].defined() ? OptTensor(saved[2]) : std::nullopt;
+        const auto p = ctx->saved_data["p"].toIntVector();
+        const double smoothing = ctx->saved_data["smoothing"].toDouble();
+        const XentShape s(saved[0], saved[1], bias, saved[3], smoothing);
+        const c10::cuda::CUDAGuard guard(saved[0].device());
+        const Tensor x = saved[0].contiguous(), w = saved[1].contiguous(), target = saved[3].contiguous(), b = xent_bias(bias), lse = saved[4], count = saved[5];
+        const Tensor dloss = as_f32(grads[0]);
+        const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), b.defined() && ctx->needs_input_grad(2)};
+        const bool none = s.N == 0;
+        if (need[0]) out[0] = at::empty(x.sizes(), x.options());
+        if (need[1]) out[1] = none ? at::zeros(w.sizes(), w.options()) : at::empty(w.sizes(), w.options());
+        if (need[2]) out[2] = none ? at::zeros(b.sizes(), b.options()) : at::empty(b.sizes(), b.options());
+        if (!none) {
+            const int code = dtype_code(x);
+            size_t bytes;
+            Tensor ws = xent_workspace(s, x, code, true, &bytes);
+            check(o1d_linear_xent_bwd(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (const float *)ptr(lse), (const float *)ptr(count),
+                                      (const float *)ptr(dloss), need[0] ? out[0].data_ptr() : nullptr, need[1] ? out[1].data_ptr() : nullptr,
+                                      need[2] ? out[2].data_ptr() : nullptr, ws.data_ptr(), bytes, s.N, (int)s.D, (int)s.V, p[0], (float)smoothing,
+                                      (int)p[1], code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+                  "o1d_linear_xent_bwd");
+        }
+        if (need[2]) out[2] = out[2].to(bias->scalar_type()).reshape(bias->sizes());
+        return out;
+    }
+};
+Tensor linear_xent(const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target, int64_t ignore, double smoothing, int64_t reduction) {
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(bias)))
+        return LinearXentFn::apply(x, w, bias, target, ignore, smoothing, reduction);
+    return xent_forward(x, w, bias, target, ignore, smoothing, reduction).loss;
+}
+
 Tensor conv(const Tensor &x, const Tensor &w, const Tensor &theta, const OptTensor &bias, const Tensor &host, const Tensor &dev,
             int64_t plan_c, int64_t K, int64_t stride, bool nhwc, bool via, bool identity, bool gelu) {
     return ConvFn::apply(x, w, theta, bias, host, dev, plan_c, K, stride, nhwc, via, identity, gelu);
@@ -606,5 +705,6 @@ PYBIND11_MODULE(_o1d_torch, m) {
     m.def("keep8", &keep8, py::call_guard<py::gil_scoped_release>());
     m.def("restore8", &restore8, py::call_guard<py::gil_scoped_release>());
     m.def("gelu_keep8", &gelu_keep8, py::call_guard<py::gil_scoped_release>());
+    m.def("linear_xent", &linear_xent, py::call_guard<py::gil_scoped_release>());
     m.def("layer_norm_keep8", &layer_norm_keep8, py::call_guard<py::gil_scoped_release>());
 }

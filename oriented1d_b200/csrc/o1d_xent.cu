@@ -1,0 +1,309 @@
+// Linear cross entropy: cutting the work into pieces, tensor maps, launches.
+#include "o1d_xent.cuh"
+#include "o1d_tma_host.cuh"
+#include "o1d_xent.h"
+
+namespace o1d {
+
+namespace {
+
+// Bytes of G that are held at once: about half the L2 cache, so that the two products that read a piece find it there.
+constexpr long long kPieceBytes = 64ll << 20;
+constexpr int kMinSplitSteps = 8;                // K steps that a part of a split axis has at least
+
+inline long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
+inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// A bf16 matrix as the tensor copies see it.
+struct Mat {
+    const __nv_bfloat16 *p;
+    long long rows;
+    int cols;                // that exist
+    long long ld, plane;     // elements between rows / planes
+    int planes;
+};
+Mat sub_rows(const Mat &m, long long row0, long long rows) {
+    Mat r = m;
+    r.p += row0 * m.ld;
+    r.rows = rows;
+    return r;
+}
+
+int encode(CUtensorMap *map, const Mat &m, int box_rows) {
+    thread_local bool bound = false;
+    if (!bound) { bind_primary_context(); bound = true; }
+    PFN_encodeTiled enc = encode_tiled_fn();
+    if (!enc) return -1;
+    const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)m.ld * 2, (cuuint64_t)m.plane * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)kXK, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
+    CUresult r = CUDA_SUCCESS;
+    for (int attempt = 0; attempt < 2; attempt++) {
+        r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16 *>(m.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r == CUDA_SUCCESS) return 0;
+        bind_primary_context();
+    }
+    return (int)r;
+}
+
+struct Run {                 // of one call
+    const XentArgs &a;
+    int sms, *err_flag;
+    cudaStream_t st;
+    cudaError_t *cuda;
+    int *enc;
+    int fail(cudaError_t e) { *cuda = e; return O1D_ERR_CUDA; }
+
+    template <int KIND, bool SPLIT>
+    int product(const Mat &ma, const Mat &mb, XentParams p) {
+        using S = XentShape<SPLIT>;
+        constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
+        CUtensorMap a_map, b_map;
+        if ((*enc = encode(&a_map, ma, A_MN ? kXK : kXM)) || (*enc = encode(&b_map, mb, B_MN ? kXK : S::BN))) return O1D_ERR_CUDA;
+        p.M = (int)(A_MN ? ma.cols : ma.rows);
+        p.N = (int)(B_MN ? mb.cols : mb.rows);
+        const long long m_tiles = cdiv(p.M, kXM), n_tiles = cdiv(p.N, S::BN);
+        p.k_steps = cdiv(A_MN ? ma.rows : ma.cols, kXK);
+        if (p.splits < 1) p.splits = 1;
+        if (m_tiles * n_tiles * p.splits > 0x7fffffff) return O1D_ERR_UNSUPPORTED;
+        p.m_tiles = (int)m_tiles;
+        p.n_tiles = (int)n_tiles;
+        p.tiles = p.m_tiles * p.n_tiles * p.splits;
+        p.err_flag = err_flag;
+        auto kern = xent_kernel<KIND, SPLIT>;
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e != cudaSuccess) return fail(e);
+        kern<<<p.tiles < sms ? p.tiles : sms, kXThreads, S::SMEM, st>>>(a_map, b_map, p);
+        e = cudaGetLastError();
+        return e == cudaSuccess ? O1D_OK : fail(e);
+    }
+};
+
+// x or w as planes: in place where it can be, else in the workspace.
+struct Operand { bool copy; long long rows; int D, ld, planes; size_t bytes; };
+Operand operand_of(const void *p, long long rows, int D, bool bf16) {
+    Operand o;
+    o.copy = !bf16 || D % 8 != 0 || ((uintptr_t)p & 15);
+    o.rows = rows; o.D = D;
+    o.planes = bf16 ? 1 : 3;
+    o.ld = o.copy ? (int)up_to(D, 8) : D;
+    o.bytes = o.copy ? (size_t)up_to((long long)o.planes * rows * o.ld * 2, 256) : 0;
+    return o;
+}
+// Workspaces are sized for operands that need the copy: an address is not part of the request.
+size_t operand_bytes(long long rows, int D, bool bf16) { return operand_of((const void *)1, rows, D, bf16).bytes; }
+
+int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, Mat *m) {
+    m->rows = o.rows; m->cols = o.D; m->ld = o.ld; m->plane = o.rows * o.ld; m->planes = o.planes;
+    if (!o.copy) { m->p = (const __nv_bfloat16 *)src; return O1D_OK; }
+    __nv_bfloat16 *to = (__nv_bfloat16 *)*ws;
+    *ws += o.bytes;
+    m->p = to;
+    const long long n = o.rows * o.D, blocks = (n + 255) / 256;
+    const int grid = (int)(blocks < (long long)r.sms * 32 ? blocks : (long long)r.sms * 32);
+    if (o.planes == 3) xent_planes_kernel<float><<<grid, 256, 0, r.st>>>((const float *)src, to, o.rows, o.D, o.ld);
+    else xent_planes_kernel<__nv_bfloat16><<<grid, 256, 0, r.st>>>((const __nv_bfloat16 *)src, to, o.rows, o.D, o.ld);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? O1D_OK : r.fail(e);
+}
+
+// Forward: CTAs that a row tile's vocabulary is spread over, at most.
+int forward_slots(long long N, int V, bool bf16, int sms) {
+    const long long n_tiles = cdiv(V, bf16 ? 256 : 128), tiles = cdiv(N, kXM) * n_tiles;
+    const long long ctas = tiles < sms ? tiles : sms, least = tiles / ctas;
+    return 2 * (int)(cdiv(n_tiles, least) + 1);
+}
+
+// Backward: how G is cut, and into how many parts the K axes of the two products are.
+struct Cut {
+    bool by_rows;
+    long long piece;         // rows, or columns of the vocabulary
+    int pieces, ld;          // ld: columns of G in memory
+    long long rows;          // rows of a piece
+    int dx_parts, dw_parts;  // fp32 sums; 0: the product writes its result
+    int col_slices;
+};
+int parts_of(long long m, long long n, long long k, int bn, int sms, bool adds) {
+    const long long tiles = (long long)cdiv(m, kXM) * cdiv(n, bn), steps = cdiv(k, kXK);
+    long long s = sms / tiles;
+    if (s > steps / kMinSplitSteps) s = steps / kMinSplitSteps;
+    if (s < 1) s = 1;
+    return s == 1 && !adds ? 0 : (int)s;
+}
+Cut cut_of(const XentArgs &a, int sms) {
+    const int bn = a.bf16 ? 256 : 128, planes = a.bf16 ? 1 : 3;
+    Cut c;
+    c.by_rows = a.N > a.V;
+    const long long all_ld = up_to(a.V, 64), axis = c.by_rows ? a.N : a.V;
+    long long most = c.by_rows ? kPieceBytes / (2 * planes * all_ld) / kXM * kXM : kPieceBytes / (2 * planes * a.N) / 256 * 256;
+    if (most < 256) most = 256;
+    c.pieces = cdiv(axis, most);
+    c.piece = c.pieces == 1 ? axis : up_to(cdiv(axis, c.pieces), 256);
+    c.pieces = cdiv(axis, c.piece);
+    c.ld = (int)(c.by_rows ? all_ld : up_to(c.piece, 64));
+    c.rows = c.by_rows ? c.piece : a.N;
+    c.dx_parts = parts_of(c.rows, a.D, c.by_rows ? a.V : c.piece, bn, sms, !c.by_rows && c.pieces > 1);
+    c.dw_parts = parts_of(c.by_rows ? a.V : c.piece, a.D, c.rows, bn, sms, c.by_rows && c.pieces > 1);
+    const int col_blocks = cdiv(c.ld, 256);
+    long long s = cdiv(4ll * sms, col_blocks);
+    if (s > cdiv(c.rows, 32)) s = cdiv(c.rows, 32);
+    c.col_slices = (int)s;
+    return c;
+}
+struct BackwardBytes { size_t x, w, g, dx, dw, col; };
+BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
+    const int planes = a.bf16 ? 1 : 3;
+    BackwardBytes b;
+    b.x = operand_bytes(a.N, a.D, a.bf16);
+    b.w = operand_bytes(a.V, a.D, a.bf16);
+    b.g = (size_t)up_to(2ll * planes * c.rows * c.ld, 256);
+    // by rows, dx is complete with its piece; by vocabulary, dw is
+    b.dx = (size_t)up_to(4ll * c.dx_parts * c.rows * a.D, 256);
+    b.dw = (size_t)up_to(4ll * c.dw_parts * (c.by_rows ? a.V : c.piece) * a.D, 256);
+    b.col = (size_t)up_to(4ll * (c.by_rows ? c.pieces : 1) * c.col_slices * up_to(a.V, 64), 256);
+    return b;
+}
+
+template <bool SPLIT>
+int forward(Run &r) {
+    const XentArgs &a = r.a;
+    unsigned char *ws = (unsigned char *)a.workspace;
+    Mat x, w;
+    int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
+    if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
+    if (rc) return rc;
+    const int slots = forward_slots(a.N, a.V, a.bf16, r.sms);
+    XentParams p{};
+    p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
+    p.part = (float2 *)ws; ws += up_to(8ll * slots * a.N, 256);
+    p.target_logit = (float *)ws; ws += up_to(4 * a.N, 256);
+    p.smooth = a.smoothing > 0.f;
+    p.part_sum = (float *)ws; ws += up_to(4ll * slots * a.N, 256);
+    double2 *sums = (double2 *)ws;
+    p.part_rows = a.N;
+    rc = r.product<XENT_LOGITS, SPLIT>(x, w, p);
+    if (rc) return rc;
+    const int n_tiles = cdiv(a.V, XentShape<SPLIT>::BN), tiles = cdiv(a.N, kXM) * n_tiles, blocks = cdiv(a.N, 256);
+    const bool each = a.reduction == O1D_XENT_NONE;
+    xent_rows_kernel<<<blocks, 256, 0, r.st>>>(p.part, p.part_sum, p.target_logit, a.target, a.ignore, a.smoothing, a.V, a.N, a.N, n_tiles, tiles,
+                                               tiles < r.sms ? tiles : r.sms, a.lse, each ? a.loss : nullptr, each ? nullptr : sums);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && !each) {
+        xent_total_kernel<<<1, 256, 0, r.st>>>(sums, blocks, a.reduction == O1D_XENT_MEAN, a.loss, a.count);
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? O1D_OK : r.fail(e);
+}
+
+template <typename T>
+cudaError_t finish(const float *sums, void *out, long long n, int slots, const float *up, const float *count, float f, int sms, cudaStream_t st) {
+    const long long blocks = (n + 255) / 256;
+    xent_finish_kernel<T><<<(int)(blocks < sms * 16ll ? blocks : sms * 16ll), 256, 0, st>>>(sums, (T *)out, n, slots, up, count, f);
+    return cudaGetLastError();
+}
+
+template <bool SPLIT>
+int backward(Run &r) {
+    const XentArgs &a = r.a;
+    const Cut c = cut_of(a, r.sms);
+    const BackwardBytes b = backward_bytes(a, c);
+    unsigned char *ws = (unsigned char *)a.workspace;
+    const int es = a.bf16 ? 2 : 4;
+    __nv_bfloat16 *g = (__nv_bfloat16 *)ws; ws += b.g;
+    float *dxs = (float *)ws; ws += b.dx;
+    float *dws = (float *)ws; ws += b.dw;
+    float *cols = (float *)ws; ws += b.col;
+    Mat x, w;
+    int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
+    if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
+    if (rc) return rc;
+
+    const bool each = a.reduction == O1D_XENT_NONE;
+    const float f = a.smoothing < 1.f ? 1.f - a.smoothing : 1.f;
+    const float *up = each ? nullptr : a.dloss, *count = a.reduction == O1D_XENT_MEAN ? a.count : nullptr;
+    const long long part_ld = up_to(a.V, 64);
+    // One product's way out: its result at once, or sums that `finish` turns into it.
+    auto out_of = [&](XentParams &p, int parts, bool first, void *result, float *sums, long long elems, long long k) {
+        p.splits = parts < 1 ? 1 : parts;
+        const long long steps = cdiv(k, kXK);
+        if (p.splits > steps) p.splits = (int)steps;                  // a short last piece
+        p.out = parts ? (void *)sums : result;
+        p.split_elems = elems;
+        p.out_kind = parts ? (first ? 2 : 3) : a.bf16 ? 0 : 1;
+        p.vec = ((uintptr_t)p.out & 15) == 0 && (long long)a.D * (p.out_kind == 0 ? 2 : 4) % 16 == 0;
+        p.alpha_up = up; p.alpha_count = count; p.alpha = f;
+    };
+    auto end = [&](int parts, float *sums, void *result, long long elems) {
+        if (!parts) return cudaSuccess;
+        return a.bf16 ? finish<__nv_bfloat16>(sums, result, elems, parts, up, count, f, r.sms, r.st)
+                      : finish<float>(sums, result, elems, parts, up, count, f, r.sms, r.st);
+    };
+    for (int i = 0; i < c.pieces; i++) {
+        const long long at = i * c.piece, axis = c.by_rows ? a.N : a.V, n = axis - at < c.piece ? axis - at : c.piece;
+        const long long row0 = c.by_rows ? at : 0, rows = c.by_rows ? n : a.N;
+        const int col0 = c.by_rows ? 0 : (int)at, colsn = c.by_rows ? a.V : (int)n, ld = (int)up_to(colsn, 64);
+        const Mat xs = sub_rows(x, row0, rows), wp = sub_rows(w, col0, colsn);
+        const Mat gm{g, rows, ld, ld, rows * ld, SPLIT ? 3 : 1};
+        XentParams p{};
+        p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.col0 = col0; p.V = a.V; p.target = a.target + row0; p.ignore = a.ignore;
+        p.smooth = a.smoothing > 0.f;
+        p.lse = a.lse + row0; p.up = each ? a.dloss + row0 : nullptr;
+        p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
+        p.g = g; p.g_plane = gm.plane; p.g_ld = ld;
+        // exp(l - lse) / f = exp2(l2 - (lse2 + log2 f))
+        if ((rc = r.product<XENT_GRAD, SPLIT>(xs, wp, p))) return rc;
+        cudaError_t e = cudaSuccess;
+        if (a.dx) {
+            XentParams q{};
+            void *to = (char *)a.dx + row0 * a.D * es;
+            out_of(q, c.dx_parts, c.by_rows || i == 0, to, dxs, rows * a.D, ld);
+            if ((rc = r.product<XENT_DX, SPLIT>(gm, wp, q))) return rc;
+            if (c.by_rows || i == c.pieces - 1) e = end(c.dx_parts, dxs, to, rows * a.D);
+        }
+        if (e == cudaSuccess && a.dw) {
+            XentParams q{};
+            void *to = (char *)a.dw + (long long)col0 * a.D * es;
+            Mat gv = gm;
+            gv.cols = colsn;                                          // rows of dw that exist
+            out_of(q, c.dw_parts, !c.by_rows || i == 0, to, dws, (long long)colsn * a.D, rows);
+            if ((rc = r.product<XENT_DW, SPLIT>(gv, xs, q))) return rc;
+            if (!c.by_rows || i == c.pieces - 1) e = end(c.dw_parts, dws, to, (long long)colsn * a.D);
+        }
+        if (e == cudaSuccess && a.db) {
+            xent_colsum_kernel<<<dim3(cdiv(ld, 256), c.col_slices), 256, 0, r.st>>>(g, gm.plane, gm.planes, (int)rows, ld,
+                                                                                    cols + (long long)(c.by_rows ? i : 0) * c.col_slices * part_ld + col0, (int)part_ld);
+            e = cudaGetLastError();
+        }
+        if (e != cudaSuccess) return r.fail(e);
+    }
+    if (a.db) {
+        xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(cols, (int)part_ld, (c.by_rows ? c.pieces : 1) * c.col_slices, a.db, a.bias_bf16, a.V,
+                                                                   up, count, f);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return r.fail(e);
+    }
+    return O1D_OK;
+}
+
+}  // namespace
+
+size_t xent_workspace(const XentArgs &a, bool back, int sms) {
+    if (back) {
+        const BackwardBytes b = backward_bytes(a, cut_of(a, sms));
+        return b.x + b.w + b.g + b.dx + b.dw + b.col;
+    }
+    const int slots = forward_slots(a.N, a.V, a.bf16, sms);
+    return operand_bytes(a.N, a.D, a.bf16) + operand_bytes(a.V, a.D, a.bf16) + (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) +
+           up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 256), 256));
+}
+int xent_forward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {
+    Run r{a, sms, err_flag, st, cuda, enc};
+    return a.bf16 ? forward<false>(r) : forward<true>(r);
+}
+int xent_backward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {
+    Run r{a, sms, err_flag, st, cuda, enc};
+    return a.bf16 ? backward<false>(r) : backward<true>(r);
+}
+
+}  // namespace o1d

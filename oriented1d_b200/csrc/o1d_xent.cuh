@@ -1,0 +1,622 @@
+// Softmax cross entropy of a linear classifier, without the logits.
+//   l[n, v] = sum_d x[n, d] w[v, d] + b[v],  lse[n] = log sum_v exp l[n, v],  e = label smoothing,
+//   loss[n] = lse[n] - (1-e) l[n, t_n] - (e/V) sum_v l[n, v],
+//   G[n, v] = u_n (exp(l[n, v] - lse[n]) - (1-e) [v = t_n] - e/V),   dx = G w,  dw = G^T x,  db = G^T 1.
+// Three matrix products on the tensor cores with one kernel body (xent_kernel):
+//   LOGITS   tiles of x w^T stay in tensor memory; the epilogue keeps a running maximum and sum a row and writes two
+//            floats a row and CTA run: the logits exist nowhere else.
+//   GRAD     the same tiles once more; the epilogue turns a piece of them into G (bf16) in the workspace.
+//   OUT      G w and G^T x over that piece, to the output or to fp32 sums that later pieces (and the other parts of a
+//            split K axis) add to in a fixed order.
+// Logits are formed twice (8NDV operations where 6NDV would do) because to keep them in fp32 costs more in traffic than
+// the product does, and to keep them in bf16 costs the softmax its accuracy.
+//
+// fp32 inputs are cut into three bf16 planes each (x = x0 + x1 + x2 exactly, 8 bits a plane); of the nine products of
+// planes the six above 2^-24 are taken.  x0 w0 has an accumulator of its own, the five small ones share another, and
+// both are added to fp32 registers every 256 of K: a tensor core adds with truncation, which over thousands of steps
+// would show.
+//
+// Rounding: G is rounded to bf16 for bf16 inputs (half a unit of 2^-8, random from element to element; dx and dw are
+// rounded so themselves).  So that the rounding of the coefficient 1-e, which every row shares, cannot add up, G is kept divided
+// by 1-e and the factor applied to the fp32 sums.  All sums, statistics and the loss are fp32 or wider.
+#pragma once
+
+#include "o1d_common.cuh"
+#include "o1d_tc.cuh"
+
+namespace o1d {
+
+enum : int { XENT_LOGITS = 0, XENT_GRAD, XENT_DX, XENT_DW };
+
+constexpr int kXM = 128, kXK = 64;               // tile rows; K elements of a stage (one 128-byte swizzled row)
+constexpr int kXThreads = 384;                   // warp 0 loads, 1 multiplies, 2 owns tensor memory, 4-11 finish tiles
+constexpr int kXStaging = 2048;                  // bytes of a warp's store buffer: 32 rows of 64 bytes
+constexpr int kXChunk = 4;                       // fp32: stages of one accumulation
+template <bool SPLIT> struct XentShape {
+    static constexpr int BN = SPLIT ? 128 : 256, PL = SPLIT ? 3 : 1, STAGES = SPLIT ? 2 : 4;
+    static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = BN * kXK * 2, STAGE = PL * (A_BYTES + B_BYTES);
+    static constexpr int SMEM = STAGES * STAGE + 8 * kXStaging + 8 * (BN / 2) * (int)sizeof(float) + 256 + 1024;
+};
+
+struct XentParams {
+    int M, N;                    // extents of the product
+    int m_tiles, n_tiles, k_steps;
+    int splits;                  // OUT: parts of the K axis
+    int tiles;                   // m_tiles * n_tiles * splits
+    // LOGITS, GRAD
+    const void *bias;
+    int bias_bf16;
+    int col0, V;                 // vocabulary index of the product's first column; size of the vocabulary
+    const long long *target;     // of the product's first row
+    long long ignore;
+    // LOGITS: [slots][rows] of (maximum, sum) and, when smoothing, of the sum of logits; the target's logit a row
+    float2 *part;
+    float *part_sum, *target_logit;
+    long long part_rows;
+    int smooth;
+    // GRAD
+    const float *lse, *up;       // up: per-row gradient of the loss, or null
+    float factor_log2, one, eps_v;   // log2(1-e), coefficient of the target, e/V; both divided by 1-e
+    __nv_bfloat16 *g;
+    long long g_plane;           // elements of a plane of G
+    int g_ld;
+    // OUT
+    void *out;                   // dx or dw (rows of N elements), or the fp32 sums of split 0
+    long long split_elems;       // elements of one split's sums
+    int out_kind;                // 0: bf16 result, 1: fp32 result, 2: fp32 sums, written, 3: fp32 sums, added to
+    int vec;                     // rows of the output start on 16 bytes
+    const float *alpha_up, *alpha_count;
+    float alpha;
+    int *err_flag;
+};
+
+// Gradient of the loss with respect to a row's loss where all rows share it, times the factor kept out of G.
+__device__ __forceinline__ float xent_alpha(const float *up, const float *count, float f) {
+    if (up) f *= __ldg(up);
+    if (count) { const float c = __ldg(count); f = c > 0.f ? f / c : 0.f; }      // no row counts: nothing has a gradient
+    return f;
+}
+
+__device__ __forceinline__ float exp2_fast(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+
+// Tile t of a CTA's work.
+struct XentTile { int m, n, k0, k1, split; };
+template <int KIND>
+__device__ __forceinline__ XentTile xent_tile(const XentParams &p, int t) {
+    XentTile r;
+    if (KIND == XENT_LOGITS) {                       // along the vocabulary: a CTA keeps its rows' statistics in registers
+        r.m = t / p.n_tiles; r.n = t - r.m * p.n_tiles; r.k0 = 0; r.k1 = p.k_steps; r.split = 0;
+    } else {
+        const int mn = p.m_tiles * p.n_tiles;
+        r.split = t / mn; t -= r.split * mn;
+        r.n = t / p.m_tiles; r.m = t - r.n * p.m_tiles;
+        r.k0 = (int)((long long)p.k_steps * r.split / p.splits); r.k1 = (int)((long long)p.k_steps * (r.split + 1) / p.splits);
+    }
+    return r;
+}
+// First tile of CTA i: LOGITS gives each a contiguous run, so that the runs differ by one tile at most.
+__host__ __device__ inline int xent_run(int i, int tiles, int ctas) { return (int)((long long)i * tiles / ctas); }
+// CTA whose run holds tile t.
+__host__ __device__ inline int xent_owner(int t, int tiles, int ctas) { return (int)((((long long)t + 1) * ctas - 1) / tiles); }
+
+// Moves 32 rows x 64 bytes from the lanes that own the rows to memory: `vals` are the lane's four 16-byte pieces.
+// Rows go out as whole 64-byte segments.  F(row, piece, value) stores one piece.
+template <typename F>
+__device__ __forceinline__ void xent_transpose(char *stage, int lane, const uint4 (&vals)[4], F &&store) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) *reinterpret_cast<uint4 *>(stage + lane * 64 + ((j ^ (lane >> 1)) & 3) * 16) = vals[j];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int row = i * 8 + (lane >> 2), piece = lane & 3;
+        store(row, piece, *reinterpret_cast<const uint4 *>(stage + row * 64 + ((piece ^ (row >> 1)) & 3) * 16));
+    }
+    __syncwarp();
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// The next 8 bits of v, and what is left of it.  Zero is left of what is not finite.
+__device__ __forceinline__ float take_bf16(float &v) {
+    const float top = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    if (fabsf(v) <= 3.402823466e38f) { v -= top; return top; }
+    const float r = isnan(v) ? __uint_as_float(0x7fc00000u) : top;
+    v = 0.f;
+    return r;
+}
+
+template <int KIND, bool SPLIT>
+__global__ void __launch_bounds__(kXThreads, 1)
+xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XentParams p) {
+    using S = XentShape<SPLIT>;
+    constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
+    constexpr int BN = S::BN, HALF = BN / 2, PIECES = HALF / 32;
+    constexpr uint32_t INSTR = tc::instruction<BN, A_MN, B_MN>();
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char *smem = raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u);
+    char *staging = reinterpret_cast<char *>(smem + S::STAGES * S::STAGE);
+    float *bias_s = reinterpret_cast<float *>(staging + 8 * kXStaging);                 // [epilogue warp][HALF]
+    uint64_t *full = reinterpret_cast<uint64_t *>(bias_s + 8 * HALF), *empty = full + S::STAGES;
+    uint64_t *done = empty + S::STAGES, *taken = done + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(taken + 2);
+    volatile int *dead = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; i++) { tc::bar_init(full + i, 1); tc::bar_init(empty + i, 1); }
+        for (int i = 0; i < 2; i++) { tc::bar_init(done + i, 1); tc::bar_init(taken + i, 8); }
+        *dead = 0;
+        tc::bar_init_fence();
+        tc::tma_prefetch(&map_a);
+        tc::tma_prefetch(&map_b);
+    }
+    if (warp == 2) tc::tmem_alloc(tmem_slot, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int t_begin = KIND == XENT_LOGITS ? xent_run(blockIdx.x, p.tiles, gridDim.x) : blockIdx.x;
+    const int t_end = KIND == XENT_LOGITS ? xent_run(blockIdx.x + 1, p.tiles, gridDim.x) : p.tiles;
+    const int t_step = KIND == XENT_LOGITS ? 1 : gridDim.x;
+
+    if (warp == 0 && lane == 0) {                                   // ---- loads
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = t_begin; ok && t < t_end; t += t_step) {
+            const XentTile w = xent_tile<KIND>(p, t);
+            for (int k = w.k0; k < w.k1; k++) {
+                if (!(ok = tc::bar_wait(empty + stage, phase ^ 1, dead, p.err_flag))) break;
+                tc::bar_expect(full + stage, S::STAGE);
+                unsigned char *a = smem + stage * S::STAGE, *b = a + S::PL * S::A_BYTES;
+#pragma unroll
+                for (int pl = 0; pl < S::PL; pl++) {
+                    if (A_MN) {
+#pragma unroll
+                        for (int j = 0; j < kXM / 64; j++)
+                            tc::tma_load3(a + pl * S::A_BYTES + j * 8192, &map_a, full + stage, w.m * kXM + j * 64, k * kXK, pl);
+                    } else {
+                        tc::tma_load3(a + pl * S::A_BYTES, &map_a, full + stage, k * kXK, w.m * kXM, pl);
+                    }
+                    if (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < BN / 64; j++)
+                            tc::tma_load3(b + pl * S::B_BYTES + j * 8192, &map_b, full + stage, w.n * BN + j * 64, k * kXK, pl);
+                    } else {
+                        tc::tma_load3(b + pl * S::B_BYTES, &map_b, full + stage, k * kXK, w.n * BN, pl);
+                    }
+                }
+                issued++;
+                if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
+            }
+        }
+        if (!ok) {                                                  // copies in flight end before the CTA does
+            for (int i = 0; i < S::STAGES && i < issued; i++) {
+                stage = stage == 0 ? S::STAGES - 1 : stage - 1;
+                if (stage == S::STAGES - 1) phase ^= 1;
+                tc::bar_drain(full + stage, phase);
+            }
+        }
+    } else if (warp == 1 && lane == 0) {                            // ---- products
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int t = t_begin; ok && t < t_end; t += t_step) {
+            const XentTile w = xent_tile<KIND>(p, t);
+            for (int c = w.k0; ok && c < w.k1; c += SPLIT ? kXChunk : w.k1 - w.k0) {
+                const int c_end = SPLIT ? min(c + kXChunk, w.k1) : w.k1;
+                if (!(ok = tc::bar_wait(taken + acc, acc_phase ^ 1, dead, p.err_flag))) break;
+                tc::fence_after();
+                const uint32_t d = tmem + acc * 256;
+                for (int k = c; k < c_end; k++) {
+                    if (!(ok = tc::bar_wait(full + stage, phase, dead, p.err_flag))) break;
+                    tc::fence_after();
+                    unsigned char *a = smem + stage * S::STAGE, *b = a + S::PL * S::A_BYTES;
+                    uint64_t da[S::PL], db[S::PL];
+#pragma unroll
+                    for (int pl = 0; pl < S::PL; pl++) {
+                        da[pl] = tc::operand(a + pl * S::A_BYTES, A_MN ? 8192 : 16, 1024);
+                        db[pl] = tc::operand(b + pl * S::B_BYTES, B_MN ? 8192 : 16, 1024);
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < kXK / 16; kk++) {         // 16 of K: 32 bytes of a K-major row, or 16 rows
+                        const uint64_t oa = kk * (A_MN ? 128 : 2), ob = kk * (B_MN ? 128 : 2);
+                        const bool add = k > c || kk > 0;
+                        tc::mma(d, da[0] + oa, db[0] + ob, INSTR, add);
+                        if constexpr (SPLIT) {
+                            tc::mma(d + 128, da[0] + oa, db[2] + ob, INSTR, add);
+                            tc::mma(d + 128, da[1] + oa, db[1] + ob, INSTR, true);
+                            tc::mma(d + 128, da[2] + oa, db[0] + ob, INSTR, true);
+                            tc::mma(d + 128, da[0] + oa, db[1] + ob, INSTR, true);
+                            tc::mma(d + 128, da[1] + oa, db[0] + ob, INSTR, true);
+                        }
+                    }
+                    tc::commit(empty + stage);
+                    if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                tc::commit(done + acc);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
+            }
+        }
+        if (!ok) {                                                  // products in flight read shared memory: wait for them
+            tc::commit(done + acc);
+            tc::bar_drain(done + acc, acc_phase);
+        }
+    } else if (warp >= 4) {                                         // ---- epilogue: a thread owns a row's half
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        float *bs = bias_s + (warp - 4) * HALF;
+        char *stage = staging + (warp - 4) * kXStaging;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * HALF;
+        int acc = 0, m_now = -1;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        // LOGITS: running maximum and sum of the row's half, in units of log2
+        float mx = 0.f, sum = 0.f, total = 0.f;
+        long long tgt = -1;
+        float lse = 0.f, scale = 0.f;
+        bool ignored = false;
+        float alpha = 1.f;
+        if (KIND >= XENT_DX && p.out_kind < 2) alpha = xent_alpha(p.alpha_up, p.alpha_count, p.alpha);
+
+        auto flush = [&]() {
+            const long long row = (long long)m_now * kXM + quarter * 32 + lane;
+            if (row >= p.M) return;
+            const int slot = ((int)blockIdx.x - xent_owner(m_now * p.n_tiles, p.tiles, gridDim.x)) * 2 + half;
+            p.part[(long long)slot * p.part_rows + row] = make_float2(mx, sum);
+            if (p.smooth) p.part_sum[(long long)slot * p.part_rows + row] = total;
+        };
+
+        for (int t = t_begin; ok && t < t_end; t += t_step) {
+            const XentTile w = xent_tile<KIND>(p, t);
+            const int row = w.m * kXM + quarter * 32 + lane, n0 = w.n * BN;
+            if constexpr (KIND <= XENT_GRAD) {
+                if (w.m != m_now) {
+                    if (KIND == XENT_LOGITS && m_now >= 0) flush();
+                    m_now = w.m;
+                    mx = __int_as_float(0xff800000); sum = 0.f; total = 0.f;
+                    tgt = row < p.M ? __ldg(p.target + row) : p.ignore;
+                    ignored = tgt == p.ignore;
+                    if (KIND == XENT_GRAD && row < p.M) {
+                        lse = __ldg(p.lse + row) + p.factor_log2;
+                        if (tgt < 0 || tgt >= p.V) lse = __int_as_float(0x7fffffff);      // no such class: NaN, not silence
+                        scale = p.up ? __ldg(p.up + row) : 1.f;
+                    }
+                }
+                // the tile's bias in units of log2; -inf where the vocabulary ends, so that those columns weigh nothing
+                // (every warp keeps its own: no warp ever waits for another without a limit)
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < HALF / 32; i++) {
+                    const int c = n0 + half * HALF + i * 32 + lane;
+                    bs[i * 32 + lane] = c >= p.N ? __int_as_float(0xff800000) : p.bias ? 1.4426950408889634f * ld_param(p.bias, p.col0 + c, p.bias_bf16) : 0.f;
+                }
+                __syncwarp();
+            }
+            float v[SPLIT ? PIECES : 1][32];
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int pc = 0; pc < PIECES; pc++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[pc][i] = 0.f;
+                for (int c = w.k0; c < w.k1; c += kXChunk) {
+                    ok = __all_sync(0xffffffffu, tc::bar_wait(done + acc, acc_phase, dead, p.err_flag));
+                    if (!ok) break;
+                    tc::fence_after();
+#pragma unroll
+                    for (int pc = 0; pc < PIECES; pc++) {
+                        uint32_t r[32], s[32];
+                        tc::tmem_load32(lane_base + acc * 256 + pc * 32, r);
+                        tc::tmem_load32(lane_base + acc * 256 + 128 + pc * 32, s);
+                        tc::tmem_wait32(r);
+                        tc::tmem_wait32(s);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[pc][i] += __uint_as_float(r[i]) + __uint_as_float(s[i]);
+                    }
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::bar_arrive(taken + acc);
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
+                }
+            } else {
+                ok = __all_sync(0xffffffffu, tc::bar_wait(done + acc, acc_phase, dead, p.err_flag));
+                if (ok) tc::fence_after();
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int pc = 0; pc < PIECES; pc++) {
+                float (&a)[32] = v[SPLIT ? pc : 0];
+                const int c0 = n0 + half * HALF + pc * 32;          // first column of the piece
+                if constexpr (!SPLIT) {
+                    uint32_t r[32];
+                    tc::tmem_load32(lane_base + acc * 256 + pc * 32, r);
+                    tc::tmem_wait32(r);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) a[i] = __uint_as_float(r[i]);
+                    if (pc == PIECES - 1) {
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::bar_arrive(taken + acc);
+                        acc ^= 1;
+                        if (acc == 0) acc_phase ^= 1;
+                    }
+                }
+                if constexpr (KIND <= XENT_GRAD) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 b = *reinterpret_cast<const float4 *>(bs + pc * 32 + i);
+                        a[i] = fmaf(a[i], 1.4426950408889634f, b.x);
+                        a[i + 1] = fmaf(a[i + 1], 1.4426950408889634f, b.y);
+                        a[i + 2] = fmaf(a[i + 2], 1.4426950408889634f, b.z);
+                        a[i + 3] = fmaf(a[i + 3], 1.4426950408889634f, b.w);
+                    }
+                    const long long off = tgt - p.col0 - c0;         // where the target lies in this piece
+                    const bool hit = off >= 0 && off < 32;
+                    const int at = (int)off;
+                    if constexpr (KIND == XENT_LOGITS) {
+                        if (hit) {
+                            float l = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 32; i++) l = at == i ? a[i] : l;
+                            if (row < p.M) p.target_logit[row] = l;
+                        }
+                        if (p.smooth) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) total += c0 + i < p.N ? a[i] : 0.f;
+                        }
+                        float top = a[0];
+#pragma unroll
+                        for (int i = 1; i < 32; i++) top = fmaxf(top, a[i]);
+                        top = fmaxf(top, mx);
+                        const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
+                        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) { s0 += exp2_fast(a[i] - ref); s1 += exp2_fast(a[i + 1] - ref); }
+                        sum = sum * exp2_fast(mx - ref) + (s0 + s1);
+                        mx = top;
+                    } else {
+                        if (c0 < p.g_ld) {                           // the same for the whole warp
+#pragma unroll
+                            for (int i = 0; i < 32; i++) {
+                                float g = exp2_fast(a[i] - lse);
+                                if (p.smooth) g -= c0 + i < p.N ? p.eps_v : 0.f;
+                                a[i] = g;
+                            }
+                            if (hit) {
+#pragma unroll
+                                for (int i = 0; i < 32; i++) a[i] -= at == i ? p.one : 0.f;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i] * scale;
+#pragma unroll
+                            for (int pl = 0; pl < S::PL; pl++) {
+                                uint4 out[4];
+                                uint32_t *o = reinterpret_cast<uint32_t *>(out);
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    if constexpr (SPLIT) {
+                                        const float lo = take_bf16(a[2 * i]), hi = take_bf16(a[2 * i + 1]);
+                                        o[i] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
+                                    } else {
+                                        o[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
+                                    }
+                                }
+                                __nv_bfloat16 *to = p.g + pl * p.g_plane + c0;
+                                const int r0 = w.m * kXM + quarter * 32;
+                                xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
+                                    if (r0 + r < p.M) *reinterpret_cast<uint4 *>(to + (long long)(r0 + r) * p.g_ld + piece * 8) = val;
+                                });
+                            }
+                        }
+                    }
+                } else {
+                    const int r0 = w.m * kXM + quarter * 32;
+                    if (p.out_kind == 0) {
+                        uint4 out[4];
+                        uint32_t *o = reinterpret_cast<uint32_t *>(out);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[i] = pack_bf16(alpha * a[2 * i], alpha * a[2 * i + 1]);
+                        __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(p.out);
+                        xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
+                            const int c = c0 + piece * 8;
+                            if (r0 + r >= p.M || c >= p.N) return;
+                            __nv_bfloat16 *q = to + (long long)(r0 + r) * p.N + c;
+                            if (p.vec && c + 8 <= p.N) { *reinterpret_cast<uint4 *>(q) = val; return; }
+                            const uint32_t x[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                if (c + i < p.N) q[i] = __ushort_as_bfloat16((unsigned short)(x[i >> 1] >> (16 * (i & 1))));
+                        });
+                    } else {
+                        float *to = static_cast<float *>(p.out) + (p.out_kind >= 2 ? w.split * p.split_elems : 0);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            uint4 out[4];
+                            float *o = reinterpret_cast<float *>(out);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] = alpha * a[h * 16 + i];
+                            xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
+                                const int c = c0 + h * 16 + piece * 4;
+                                if (r0 + r >= p.M || c >= p.N) return;
+                                float *q = to + (long long)(r0 + r) * p.N + c;
+                                const float x[4] = {__uint_as_float(val.x), __uint_as_float(val.y), __uint_as_float(val.z), __uint_as_float(val.w)};
+                                if (p.vec && c + 4 <= p.N) {
+                                    float4 s = make_float4(x[0], x[1], x[2], x[3]);
+                                    if (p.out_kind == 3) {
+                                        const float4 old = *reinterpret_cast<const float4 *>(q);
+                                        s.x += old.x; s.y += old.y; s.z += old.z; s.w += old.w;
+                                    }
+                                    *reinterpret_cast<float4 *>(q) = s;
+                                    return;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    if (c + i < p.N) q[i] = p.out_kind == 3 ? q[i] + x[i] : x[i];
+                            });
+                        }
+                    }
+                }
+            }
+        }
+        if (KIND == XENT_LOGITS && ok && m_now >= 0) flush();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 2) tc::tmem_free(tmem, 512);
+}
+
+// One matrix as the bf16 planes that tensor copies read: fp32 cut into three, bf16 whose rows do not start on 16 bytes
+// copied.  planes: [3 or 1][rows][ld], ld a multiple of 8 (what lies past D is never read).
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_planes_kernel(const T *__restrict__ x, __nv_bfloat16 *__restrict__ planes, long long rows, int D, int ld) {
+    const long long n = rows * D, plane = rows * ld, step = (long long)gridDim.x * blockDim.x;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
+        const long long r = i / D;
+        __nv_bfloat16 *to = planes + r * ld + (i - r * D);
+        if constexpr (sizeof(T) == 2) {
+            *to = x[i];
+        } else {
+            float v = x[i];
+#pragma unroll
+            for (int pl = 0; pl < 3; pl++) to[pl * plane] = __float2bfloat16_rn(take_bf16(v));      // exact: eight bits each
+        }
+    }
+}
+
+// Loss of every row from the CTAs' statistics, and lse (in units of log2) for the backward pass.  Each block also sums its
+// rows' losses and counts the rows that have one.
+__global__ void __launch_bounds__(256)
+xent_rows_kernel(const float2 *__restrict__ part, const float *__restrict__ part_sum, const float *__restrict__ target_logit,
+                 const long long *__restrict__ target, long long ignore, float smoothing, int V, long long rows, long long part_rows, int n_tiles,
+                 int tiles, int ctas, float *__restrict__ lse, float *__restrict__ loss_rows, double2 *__restrict__ sums) {
+    const long long row = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    double loss = 0., counted = 0.;
+    if (row < rows) {
+        const int m = (int)(row / kXM);
+        const int slots = 2 * (xent_owner((m + 1) * n_tiles - 1, tiles, ctas) - xent_owner(m * n_tiles, tiles, ctas) + 1);
+        float top = __int_as_float(0xff800000), total = 0.f;
+        for (int s = 0; s < slots; s++) top = fmaxf(top, part[s * part_rows + row].x);
+        const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
+        float sum = 0.f;
+        for (int s = 0; s < slots; s++) {
+            const float2 v = part[s * part_rows + row];
+            sum += v.y * exp2f(v.x - ref);
+            if (smoothing > 0.f) total += part_sum[s * part_rows + row];
+        }
+        const float l2 = ref + log2f(sum);
+        lse[row] = l2;
+        const long long t = target[row];
+        float out = 0.f;
+        if (t != ignore) {
+            if (t < 0 || t >= V) out = __int_as_float(0x7fffffff);
+            else {
+                out = smoothing < 1.f ? l2 - (1.f - smoothing) * target_logit[row] : l2;
+                if (smoothing > 0.f) out -= smoothing / (float)V * total;
+                out *= 0.6931471805599453f;
+            }
+            loss = out;
+            counted = 1.;
+        }
+        if (loss_rows) loss_rows[row] = out;
+    }
+    if (!sums) return;
+    __shared__ double red[2][8];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        counted += __shfl_xor_sync(0xffffffffu, counted, o);
+    }
+    if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = loss; red[1][threadIdx.x >> 5] = counted; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double a = 0., b = 0.;
+        for (int w = 0; w < 8; w++) { a += red[0][w]; b += red[1][w]; }
+        sums[blockIdx.x] = make_double2(a, b);
+    }
+}
+__global__ void __launch_bounds__(256)
+xent_total_kernel(const double2 *__restrict__ sums, int blocks, int mean, float *__restrict__ loss, float *__restrict__ count) {
+    __shared__ double red[2][256];
+    double a = 0., b = 0.;
+    for (int i = threadIdx.x; i < blocks; i += 256) { a += sums[i].x; b += sums[i].y; }
+    red[0][threadIdx.x] = a; red[1][threadIdx.x] = b;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if (threadIdx.x < o) { red[0][threadIdx.x] += red[0][threadIdx.x + o]; red[1][threadIdx.x] += red[1][threadIdx.x + o]; }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        *count = (float)red[1][0];
+        *loss = (float)(mean ? red[0][0] / red[1][0] : red[0][0]);        // no row counts: 0 / 0, as the mean of nothing
+    }
+}
+
+// out = alpha * sum over slots of sums[slot], in order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_finish_kernel(const float *__restrict__ sums, T *__restrict__ out, long long n, int slots, const float *up, const float *count, float f) {
+    const float alpha = xent_alpha(up, count, f);
+    const long long step = (long long)gridDim.x * blockDim.x;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
+        float s = sums[i];
+        for (int k = 1; k < slots; k++) s += sums[k * n + i];
+        st(out + i, alpha * s);
+    }
+}
+
+// Column sums of a piece of G: CTA (bx, by) adds rows by*8+warp, ... of 256 columns; partial [slice][part_ld].
+__global__ void __launch_bounds__(256)
+xent_colsum_kernel(const __nv_bfloat16 *__restrict__ g, long long plane, int planes, int rows, int ld, float *__restrict__ partial, int part_ld) {
+    __shared__ float red[8][256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 256 + lane * 8;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < ld)
+        for (int pl = planes - 1; pl >= 0; pl--)                     // small planes first
+#pragma unroll 4
+            for (int r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(g + pl * plane + (long long)r * ld + c));
+                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    s[2 * i] += __uint_as_float(x[i] << 16);
+                    s[2 * i + 1] += __uint_as_float(x[i] & 0xffff0000u);
+                }
+            }
+#pragma unroll
+    for (int i = 0; i < 8; i++) red[warp][lane * 8 + i] = s[i];
+    __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col < ld) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; w++) t += red[w][threadIdx.x];
+        partial[(long long)blockIdx.y * part_ld + col] = t;
+    }
+}
+// db = alpha * sum over slices of partial, in a fixed order.  Block (32, 32).
+__global__ void __launch_bounds__(1024)
+xent_bias_kernel(const float *__restrict__ partial, int part_ld, int slices, void *__restrict__ db, int bf16, int V, const float *up,
+                 const float *count, float f) {
+    __shared__ float part[32][33];
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    float s = 0.f;
+    if (c < V)
+        for (int k = threadIdx.y; k < slices; k += 32) s += partial[(long long)k * part_ld + c];
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < V) {
+        float t = 0.f;
+#pragma unroll
+        for (int y = 0; y < 32; y++) t += part[y][threadIdx.x];
+        st_param(db, c, bf16, xent_alpha(up, count, f) * t);
+    }
+}
+
+}  // namespace o1d

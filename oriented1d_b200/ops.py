@@ -160,6 +160,21 @@ def pointwise_in(x, weight, bias):
     return ext.pointwise_in(x, weight, bias)
 
 
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean"):
+    """F.cross_entropy(F.linear(x, weight, bias), target, ...) without the logits: features x [..., D], weight [V, D],
+    bias [V] or None, int64 class indices target [...]; the loss is fp32, a scalar or (reduction="none") of target's
+    shape.  Differentiable in x, weight and bias.  The logits exist a tile at a time on the chip, and their gradient a piece
+    of the classes at a time; what is kept between the passes is one float a row.
+
+    A row with target == ignore_index has no loss and no gradient; a target that is no class makes the row's loss (and the
+    gradients) NaN, where torch stops the process.  weight is brought to x's dtype where it differs."""
+    if reduction not in _lib.XENT_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {', '.join(_lib.XENT_REDUCTIONS)}, got {reduction!r}")
+    if weight.dtype != x.dtype:
+        weight = weight.to(x.dtype)
+    return ext.linear_xent(x, weight, bias, target, int(ignore_index), float(label_smoothing), _lib.XENT_REDUCTIONS[reduction])
+
+
 def keep8(x):
     """An 8-bit checkpoint of x [..., C]: (codes uint8 [..., C], ranges fp32 [..., ceil(C/128), 2]).  Each group of 128
     columns of a row has its least value `lo` and a step `s` (a 255th of its range); code q stands for lo + q*s, at most

@@ -8,12 +8,16 @@ namespace {
 
 inline int groups_of(int C) { return (C + kKeepGroup - 1) / kKeepGroup; }
 inline bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
-// Lanes that hold a row of at most 128 columns, four values each.
-inline int lanes_of(int C) { return C <= 32 ? 8 : C <= 64 ? 16 : 32; }
+// Lanes that hold a group's part of a row, eight values each.
+inline int lanes_of(int C) { return C <= 32 ? 4 : C <= 64 ? 8 : 16; }
+// Whole vectors: rows of eight values, 16 bytes of the elements, 8 of the codes.
+inline bool vectors(int C, const void *x, const void *y, const void *dx, const void *codes) {
+    return C % 8 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(dx, 16) && aligned(codes, 8);
+}
 
 template <int KIND, typename T, bool VEC, int L>
 cudaError_t keep_go(const KeepArgs &a, int sms, cudaStream_t st) {
-    constexpr int UN = 4;
+    constexpr int UN = sizeof(T) == 2 ? 4 : 2;
     const dim3 grid(groups_of(a.C), keep_slices(a.rows, a.C, sms));
     keep_kernel<KIND, T, VEC, L, UN><<<grid, kKeepThreads, 0, st>>>(a);
     const cudaError_t e = cudaGetLastError();
@@ -22,16 +26,14 @@ cudaError_t keep_go(const KeepArgs &a, int sms, cudaStream_t st) {
 template <int KIND, typename T, bool VEC>
 cudaError_t keep_lanes(const KeepArgs &a, int sms, cudaStream_t st) {
     switch (lanes_of(a.C)) {
+        case 4: return keep_go<KIND, T, VEC, 4>(a, sms, st);
         case 8: return keep_go<KIND, T, VEC, 8>(a, sms, st);
-        case 16: return keep_go<KIND, T, VEC, 16>(a, sms, st);
-        default: return keep_go<KIND, T, VEC, 32>(a, sms, st);
+        default: return keep_go<KIND, T, VEC, 16>(a, sms, st);
     }
 }
 template <int KIND, typename T>
 cudaError_t keep_vec(const KeepArgs &a, int sms, cudaStream_t st) {
-    const int vb = 4 * (int)sizeof(T);
-    const bool vec = a.C % 4 == 0 && aligned(a.x, vb) && aligned(a.y, vb) && aligned(a.dx, vb) && aligned(a.codes, 4);
-    return vec ? keep_lanes<KIND, T, true>(a, sms, st) : keep_lanes<KIND, T, false>(a, sms, st);
+    return vectors(a.C, a.x, a.y, a.dx, a.codes) ? keep_lanes<KIND, T, true>(a, sms, st) : keep_lanes<KIND, T, false>(a, sms, st);
 }
 template <typename T>
 cudaError_t keep_kind(int kind, const KeepArgs &a, int sms, cudaStream_t st) {
@@ -43,49 +45,48 @@ cudaError_t keep_kind(int kind, const KeepArgs &a, int sms, cudaStream_t st) {
     }
 }
 
-// Rows a CTA of the LayerNorm kernels holds at once, and warps that share one.
+// Warps that share a row of the LayerNorm kernels, and rows that a CTA holds at once: two groups a warp up to 256
+// columns, four beyond, eight for the longest rows.
 inline int ln_team(int C) { return C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : 8; }
 inline int ln_cta_rows(int C) { return C <= 128 ? kKeepWarps * (32 / lanes_of(C)) : kKeepWarps / ln_team(C); }
 
-template <bool BWD, typename T, bool VEC, int L, int TEAM, int NG>
+template <bool BWD, typename T, bool VEC, int LR, int TEAM, int NG, int UN>
 cudaError_t ln_go(const LnKeepArgs &a, int sms, cudaStream_t st) {
     const int grid = ln_keep_ctas(a.rows, a.C, sms);
     if constexpr (BWD) {
         constexpr int TEAMS = kKeepWarps / TEAM;
         const int smem = TEAMS > 1 ? TEAMS * 2 * a.C * (int)sizeof(float) : 0;        // at most 32 KB
-        ln_keep_bwd_kernel<T, VEC, L, TEAM, NG><<<grid, kKeepThreads, smem, st>>>(a);
+        ln_keep_bwd_kernel<T, VEC, LR, TEAM, NG, UN><<<grid, kKeepThreads, smem, st>>>(a);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         return sum_slices(a.partial, a.dgamma, a.C, a.dbeta, a.C, a.pbf16, grid, st);
     } else {
-        ln_keep_kernel<T, VEC, L, TEAM, NG><<<grid, kKeepThreads, 0, st>>>(a);
+        ln_keep_kernel<T, VEC, LR, TEAM, NG, UN><<<grid, kKeepThreads, 0, st>>>(a);
         return cudaGetLastError();
     }
 }
 template <bool BWD, typename T, bool VEC>
 cudaError_t ln_width(const LnKeepArgs &a, int sms, cudaStream_t st) {
     const int C = a.C;
-    if (C <= 32) return ln_go<BWD, T, VEC, 8, 1, 1>(a, sms, st);
-    if (C <= 64) return ln_go<BWD, T, VEC, 16, 1, 1>(a, sms, st);
-    if (C <= 128) return ln_go<BWD, T, VEC, 32, 1, 1>(a, sms, st);
-    if (C <= 256) return ln_go<BWD, T, VEC, 32, 1, 2>(a, sms, st);
-    if (C <= 512) return ln_go<BWD, T, VEC, 32, 1, 4>(a, sms, st);
-    if (C <= 1024) return ln_go<BWD, T, VEC, 32, 2, 4>(a, sms, st);
-    if (C <= 2048) return ln_go<BWD, T, VEC, 32, 4, 4>(a, sms, st);
-    if (C <= 4096) return ln_go<BWD, T, VEC, 32, 8, 4>(a, sms, st);
-    return ln_go<BWD, T, VEC, 32, 8, 8>(a, sms, st);
+    if (C <= 32) return ln_go<BWD, T, VEC, 4, 1, 1, 2>(a, sms, st);
+    if (C <= 64) return ln_go<BWD, T, VEC, 8, 1, 1, 2>(a, sms, st);
+    if (C <= 128) return ln_go<BWD, T, VEC, 16, 1, 1, 2>(a, sms, st);
+    if (C <= 256) return ln_go<BWD, T, VEC, 32, 1, 1, 2>(a, sms, st);
+    if (C <= 512) return ln_go<BWD, T, VEC, 32, 1, 2, 1>(a, sms, st);
+    if (C <= 1024) return ln_go<BWD, T, VEC, 32, 2, 2, 1>(a, sms, st);
+    if (C <= 2048) return ln_go<BWD, T, VEC, 32, 4, 2, 1>(a, sms, st);
+    if (C <= 4096) return ln_go<BWD, T, VEC, 32, 8, 2, 1>(a, sms, st);
+    return ln_go<BWD, T, VEC, 32, 8, 4, 1>(a, sms, st);
 }
 template <bool BWD, typename T>
 cudaError_t ln_vec(const LnKeepArgs &a, int sms, cudaStream_t st) {
-    const int vb = 4 * (int)sizeof(T);
-    const bool vec = a.C % 4 == 0 && aligned(a.x, vb) && aligned(a.y, vb) && aligned(a.dx, vb) && aligned(a.codes, 4);
-    return vec ? ln_width<BWD, T, true>(a, sms, st) : ln_width<BWD, T, false>(a, sms, st);
+    return vectors(a.C, a.x, a.y, a.dx, a.codes) ? ln_width<BWD, T, true>(a, sms, st) : ln_width<BWD, T, false>(a, sms, st);
 }
 
 }  // namespace
 
 int keep_slices(long long rows, int C, int sms) {
-    const int per = kKeepWarps * (C <= 128 ? 32 / lanes_of(C) : 1), G = groups_of(C);
+    const int per = kKeepWarps * (32 / lanes_of(C)), G = groups_of(C);
     const long long most = (rows + per - 1) / per;                       // a row for every warp
     long long s = ((long long)sms * 16 + G - 1) / G;
     s = s < most ? s : most;

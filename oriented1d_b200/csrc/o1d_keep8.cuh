@@ -18,24 +18,12 @@ namespace o1d {
 
 constexpr int kKeepThreads = 256;
 constexpr int kKeepWarps = kKeepThreads / 32;
+constexpr int kKeepLane = 8;             // values of a lane: 16 lanes hold a group, 16 bytes of bf16 each
 
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// Least and greatest value over the L lanes that share a group; a NaN anywhere gives NaN.
-template <int L>
-__device__ __forceinline__ void group_range(float &lo, float &hi) {
-    if constexpr (L == 32) {
-        asm volatile("redux.sync.min.NaN.f32 %0, %0, 0xffffffff;" : "+f"(lo));
-        asm volatile("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(hi));
-    } else {
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) {
-            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-    }
-}
+// Sum over the L lanes that share something.
 template <int L>
 __device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
@@ -43,126 +31,178 @@ __device__ __forceinline__ float lane_sum(float v) {
     return v;
 }
 
-// Four values of a lane.  VEC: columns c .. c+3, one vector access (C % 4 == 0 and aligned, so all four exist or none);
-// otherwise columns c, c+L, c+2L, c+3L, one element each.
+// Exact GELU and its slope without erff, of which the passes below would be nothing else (20 instructions a value each).
+//   P(-|h|) = erfc(z)/2,  z = |h|/sqrt 2,  erfc(z) = t q(t) exp(-z^2),  t = 1/(1 + 0.33 z)
+// the form of Abramowitz and Stegun 7.1.26, with a polynomial q of degree 7 fitted to exp(z^2) erfc(z) on 0 <= z <= 10 by
+// iterated weighted least squares: relative error 1e-7 in both tails.  One reciprocal and one exponential, which the slope
+// GELU'(h) = P(h) + h exp(-h^2/2) / sqrt(2 pi) needs anyway.
+struct Normal { float cdf, bell; };                 // P(h), exp(-h^2/2)
+__device__ __forceinline__ Normal normal_of(float h) {
+    float t, e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(fabsf(h), 0.33f * 0.70710678f, 1.f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-0.72134752f * h * h));
+    float q = fmaf(t, -0.1353452503681183f, 0.4602353572845459f);
+    q = fmaf(t, q, -0.35114675760269165f);
+    q = fmaf(t, q, 0.40849733352661133f);
+    q = fmaf(t, q, 0.04722202196717262f);
+    q = fmaf(t, q, 0.2012234777212143f);
+    q = fmaf(t, q, 0.1829560101032257f);
+    q = fmaf(t, q, 0.1863577961921692f);
+    q *= 0.5f * t * e;
+    return {h < 0.f ? q : 1.f - q, e};
+}
+
+// A lane's eight values of a group of L lanes.  VEC: columns c .. c+7 (C % 8 == 0 and all aligned, so that all exist or
+// none); otherwise columns c, c+L, ..., c+7L, one element each.  `end`: the columns of the row, or of its part, that exist.
 template <bool VEC, int L> __device__ __forceinline__ int col_of(int c, int i) { return VEC ? c + i : c + i * L; }
+template <bool VEC> __device__ __forceinline__ int first_col(int lane) { return VEC ? lane * kKeepLane : lane; }
 
+__device__ __forceinline__ float from_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float from_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// A lane's eight values as they come from memory (bf16 vectors stay packed until they are used: half the registers in flight).
+template <typename T, bool VEC> struct Raw8 { float f[8]; };
+template <> struct Raw8<__nv_bfloat16, true> { uint4 v; };
 template <bool VEC, int L, typename T>
-__device__ __forceinline__ void load4(const T *row, int c, int C, float fill, float (&f)[4]) {
-    if constexpr (VEC) {
-        if (c < C) {
-            if constexpr (sizeof(T) == 4) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(row + c));
-                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-            } else {
-                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(row + c));
-                f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
-                f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = fill;
+__device__ __forceinline__ void load8(const T *row, int c, int end, Raw8<T, VEC> &r) {
+    if constexpr (VEC && sizeof(T) == 2) {
+        r.v = c < end ? __ldg(reinterpret_cast<const uint4 *>(row + c)) : make_uint4(0u, 0u, 0u, 0u);
+    } else if constexpr (VEC) {
+        const bool on = c < end;
+        const float4 a = on ? __ldg(reinterpret_cast<const float4 *>(row + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 b = on ? __ldg(reinterpret_cast<const float4 *>(row + c) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        r.f[0] = a.x; r.f[1] = a.y; r.f[2] = a.z; r.f[3] = a.w; r.f[4] = b.x; r.f[5] = b.y; r.f[6] = b.z; r.f[7] = b.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = c + i * L < C ? ld(row + c + i * L) : fill;
+        for (int i = 0; i < 8; i++) r.f[i] = c + i * L < end ? ld(row + c + i * L) : 0.f;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void unpack8(const Raw8<T, VEC> &r, float (&f)[8]) {
+    if constexpr (VEC && sizeof(T) == 2) {
+        f[0] = from_lo(r.v.x); f[1] = from_hi(r.v.x); f[2] = from_lo(r.v.y); f[3] = from_hi(r.v.y);
+        f[4] = from_lo(r.v.z); f[5] = from_hi(r.v.z); f[6] = from_lo(r.v.w); f[7] = from_hi(r.v.w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = r.f[i];
     }
 }
 template <bool VEC, int L, typename T>
-__device__ __forceinline__ void store4(T *row, int c, int C, const float (&f)[4]) {
+__device__ __forceinline__ void store8(T *row, int c, int end, const float (&f)[8]) {
     if constexpr (VEC) {
-        if (c >= C) return;
+        if (c >= end) return;
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(row + c) = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4 *>(row + c)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4 *>(row + c)[1] = make_float4(f[4], f[5], f[6], f[7]);
         } else {
-            __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
-            *reinterpret_cast<uint2 *>(row + c) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                u[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+            *reinterpret_cast<uint4 *>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (c + i * L < C) st(row + c + i * L, f[i]);
+        for (int i = 0; i < 8; i++)
+            if (c + i * L < end) st(row + c + i * L, f[i]);
     }
 }
+// Parameters of the lane's columns (0 where there is none).
 template <bool VEC, int L>
-__device__ __forceinline__ void load_codes(const uint8_t *row, int c, int C, uint32_t (&q)[4]) {
-    if constexpr (VEC) {
-        const uint32_t v = c < C ? __ldg(reinterpret_cast<const uint32_t *>(row + c)) : 0u;
+__device__ __forceinline__ void load_params(const void *p, int bf16, int c, int end, float (&f)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) q[i] = (v >> (8 * i)) & 0xffu;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) q[i] = c + i * L < C ? __ldg(row + c + i * L) : 0u;
-    }
+    for (int i = 0; i < 8; i++) f[i] = p && col_of<VEC, L>(c, i) < end ? ld_param(p, col_of<VEC, L>(c, i), bf16) : 0.f;
 }
+// Codes travel as bytes and become numbers in the mantissa of 2^23 + q: integer conversions run at an eighth of the rate.
 template <bool VEC, int L>
-__device__ __forceinline__ void store_codes(uint8_t *row, int c, int C, const uint32_t (&q)[4]) {
-    if constexpr (VEC) {
-        if (c < C) *reinterpret_cast<uint32_t *>(row + c) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
-    } else {
+__device__ __forceinline__ uint2 load_codes(const uint8_t *row, int c, int end) {
+    if constexpr (VEC) return c < end ? __ldg(reinterpret_cast<const uint2 *>(row + c)) : make_uint2(0u, 0u);
+    uint32_t w[2] = {0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (c + i * L < C) row[c + i * L] = (uint8_t)q[i];
+    for (int i = 0; i < 8; i++)
+        if (c + i * L < end) w[i >> 2] |= (uint32_t)__ldg(row + c + i * L) << (8 * (i & 3));
+    return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void restore_codes(uint2 q, float2 range, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float v = __uint_as_float(__byte_perm(i < 4 ? q.x : q.y, 0x4b000000u, 0x7650 | (i & 3))) - 8388608.f;
+        f[i] = fmaf(v, range.y, range.x);
     }
 }
 
-// Codes of the lane's four values, and the group's range (written by the group's first lane).
+// Codes of the lane's eight values, and their group's range (stored by the group's first lane, when `store` is set).
 template <bool VEC, int L>
-__device__ __forceinline__ void keep_group(const float (&f)[4], int c, int C, int lane, uint8_t *codes, float *range) {
+__device__ __forceinline__ void keep_group(const float (&f)[8], int c, int end, bool store, uint8_t *codes, float *range) {
     float lo = __int_as_float(0x7f800000), hi = -lo;
+    if (VEC) {
+        if (c < end) {
+            lo = min_nan(min_nan(min_nan(f[0], f[1]), min_nan(f[2], f[3])), min_nan(min_nan(f[4], f[5]), min_nan(f[6], f[7])));
+            hi = max_nan(max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3])), max_nan(max_nan(f[4], f[5]), max_nan(f[6], f[7])));
+        }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (col_of<VEC, L>(c, i) >= C) continue;
-        lo = min_nan(lo, f[i]);
-        hi = max_nan(hi, f[i]);
+        for (int i = 0; i < 8; i++)
+            if (c + i * L < end) { lo = min_nan(lo, f[i]); hi = max_nan(hi, f[i]); }
     }
-    group_range<L>(lo, hi);
-    float step = __fmul_rn(__fsub_rn(hi, lo), 1.f / 255.f);
-    if (!(step <= 3.402823466e38f)) step = __int_as_float(0x7fffffff);        // NaN or infinite: the group is lost
-    float inv = 0.f;
-    if (step < 1.175494351e-38f) step = 0.f; else inv = __frcp_rn(step);
-    uint32_t q[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) q[i] = min(__float2uint_rn(__fmul_rn(__fsub_rn(f[i], lo), inv)), 255u);
-    store_codes<VEC, L>(codes, c, C, q);
-    if (lane == 0) *reinterpret_cast<float2 *>(range) = make_float2(lo, step);
+    for (int o = L / 2; o > 0; o >>= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    float step = __fmul_rn(__fsub_rn(hi, lo), 1.f / 255.f), inv = 0.f;
+    if (!(step <= 3.402823466e38f)) step = __int_as_float(0x7fffffff);        // NaN or infinite: the group is lost
+    else if (step < 1.175494351e-38f) step = 0.f;
+    else inv = __frcp_rn(step);
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)                       // 2^23 + t has round(t) in its lowest bits; fmaxf: 0 for NaN
+        q[i] = __float_as_uint(__fadd_rn(fmaxf(__fmul_rn(__fsub_rn(f[i], lo), inv), 0.f), 8388608.f));
+    if constexpr (VEC) {
+        if (c < end)
+            *reinterpret_cast<uint2 *>(codes + c) = make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                                                               __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (c + i * L < end) codes[c + i * L] = (uint8_t)q[i];
+    }
+    if (store) *reinterpret_cast<float2 *>(range) = make_float2(lo, step);
 }
-__device__ __forceinline__ float restored(uint32_t q, float2 range) { return fmaf((float)q, range.y, range.x); }
 
-// The elementwise kinds.  CTA (bx, by): the columns of group bx, rows by*8+warp, ... in steps of gridDim.y*8 (a warp
-// holds 32/L rows at once where rows are short).  Column sums of the GELU backward (its bias gradient) stay in
-// registers over all rows of a thread and leave as one partial per (by, column), added in a fixed order by
-// sum_slices_kernel.  UN rows of a warp are in flight at once: the kernels are bound by memory, and a lane's piece of
-// a row is only 8 or 16 bytes.
+// The elementwise kinds.  CTA (bx, by): the columns of group bx, rows in steps of all the grid's; L lanes hold a row's part of
+// the group, 32/L rows a warp.  Column sums of the GELU backward (its bias gradient) stay in registers over all rows
+// of a thread and leave as one partial per (by, column), added in a fixed order by sum_slices_kernel.  UN rows of a lane are in
+// flight at once.
 template <int KIND, typename T, bool VEC, int L, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 keep_kernel(const KeepArgs a) {
     constexpr int RW = 32 / L;                                   // rows of a warp
     const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, warp = threadIdx.x >> 5;
     const int g = blockIdx.x, G = gridDim.x, C = a.C;
-    const int c = g * kKeepGroup + (VEC ? lane * 4 : lane);
+    const int c = g * kKeepGroup + first_col<VEC>(lane);
     const int lim = min(C, (g + 1) * kKeepGroup);                // end of the group
     const long long stride = (long long)gridDim.y * kKeepWarps * RW;
     const T *x = static_cast<const T *>(a.x);
     T *y = static_cast<T *>(a.y), *dx = static_cast<T *>(a.dx);
-    float b[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (KIND == KEEP_GELU_FWD && a.bias) {
+    float b[8], sum[8];
+    if (KIND == KEEP_GELU_FWD) load_params<VEC, L>(a.bias, a.pbf16, c, lim, b);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (col_of<VEC, L>(c, i) < lim) b[i] = ld_param(a.bias, col_of<VEC, L>(c, i), a.pbf16);
-    }
+    for (int i = 0; i < 8; i++) sum[i] = 0.f;
     // whole warps leave the loop together (the groups' ranges are found with warp-wide instructions)
     for (long long r0 = ((long long)blockIdx.y * kKeepWarps + warp) * RW; r0 < a.rows; r0 += stride * UN) {
-        float f[UN][4];
-        uint32_t q[UN][4];
+        Raw8<T, VEC> raw[UN];
+        uint2 q[UN];
         float2 range[UN];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             const long long r = r0 + sub + u * stride;
             const bool act = r < a.rows;
-            if (KIND != KEEP_RESTORE) load4<VEC, L>(x + (act ? r : 0) * C, c, act ? lim : 0, 0.f, f[u]);
+            if (KIND != KEEP_RESTORE) load8<VEC, L>(x + (act ? r : 0) * C, c, act ? lim : 0, raw[u]);
             if (KIND == KEEP_RESTORE || KIND == KEEP_GELU_BWD) {
-                load_codes<VEC, L>(a.codes + (act ? r : 0) * C, c, act ? lim : 0, q[u]);
+                q[u] = load_codes<VEC, L>(a.codes + (act ? r : 0) * C, c, act ? lim : 0);
                 range[u] = __ldg(reinterpret_cast<const float2 *>(a.ranges) + (act ? r : 0) * G + g);
             }
         }
@@ -172,32 +212,38 @@ keep_kernel(const KeepArgs a) {
             const bool act = r < a.rows;
             const int end = act ? lim : 0;                       // a row past the last one has no columns
             const long long ro = (act ? r : 0) * C;
+            float f[8];
+            if constexpr (KIND != KEEP_RESTORE) unpack8<T, VEC>(raw[u], f);
             if constexpr (KIND == KEEP_FWD || KIND == KEEP_GELU_FWD) {
                 if constexpr (KIND == KEEP_GELU_FWD) {
-                    float v[4];
+                    float v[8];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        f[u][i] = __fadd_rn(f[u][i], b[i]);
-                        v[i] = gelu_exact(f[u][i]);
+                    for (int i = 0; i < 8; i++) {
+                        f[i] = __fadd_rn(f[i], b[i]);
+                        v[i] = f[i] * normal_of(f[i]).cdf;
                     }
-                    store4<VEC, L>(y + ro, c, end, v);
+                    store8<VEC, L>(y + ro, c, end, v);
                 }
                 if (KIND == KEEP_FWD || a.codes)
-                    keep_group<VEC, L>(f[u], c, end, act ? lane : 1, a.codes + ro, a.ranges + ((act ? r : 0) * G + g) * 2);
+                    keep_group<VEC, L>(f, c, end, act && lane == 0, a.codes + ro, a.ranges + ((act ? r : 0) * G + g) * 2);
             } else {
-                float v[4], d[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = restored(q[u][i], range[u]);
+                float v[8];
+                restore_codes(q[u], range[u], v);
                 if constexpr (KIND == KEEP_GELU_BWD) {
+                    float d[8];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        d[i] = f[u][i] * gelu_exact_grad(v[i]);
-                        if (col_of<VEC, L>(c, i) < end) sum[i] += d[i];
-                        v[i] = gelu_exact(v[i]);
+                    for (int i = 0; i < 8; i++) {
+                        const Normal n = normal_of(v[i]);
+                        d[i] = f[i] * fmaf(v[i] * 0.3989422804014327f, n.bell, n.cdf);
+                        v[i] *= n.cdf;
                     }
-                    store4<VEC, L>(dx + ro, c, end, d);
+                    if (a.dbias) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) sum[i] += col_of<VEC, L>(c, i) < end ? d[i] : 0.f;
+                    }
+                    store8<VEC, L>(dx + ro, c, end, d);
                 }
-                if (KIND == KEEP_RESTORE || y) store4<VEC, L>(y + ro, c, end, v);
+                if (KIND == KEEP_RESTORE || y) store8<VEC, L>(y + ro, c, end, v);
             }
         }
     }
@@ -205,10 +251,10 @@ keep_kernel(const KeepArgs a) {
         if (!a.dbias) return;
         __shared__ float red[kKeepWarps][kKeepGroup];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 8; i++) {
 #pragma unroll
             for (int o = L; o < 32; o <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-            if (sub == 0) red[warp][col_of<VEC, L>(VEC ? lane * 4 : lane, i)] = sum[i];
+            if (sub == 0) red[warp][col_of<VEC, L>(first_col<VEC>(lane), i)] = sum[i];
         }
         __syncthreads();
         if (threadIdx.x < lim - g * kKeepGroup) {
@@ -239,61 +285,103 @@ __device__ __forceinline__ void team_sum(float (&v)[NV], float (*slot)[NV], int 
     }
 }
 
-// LayerNorm over rows of up to 8192 columns, y = (x - mean) * rstd * gamma + beta.  A row is held in registers by L lanes
-// (short rows: 32/L rows a warp), by a warp (up to 512 columns) or by a team of TEAM warps, NG groups of 128 columns a
-// warp.  Statistics are two-pass, fp32.  Kept for the backward pass: the codes of x, mean and rstd.
-template <typename T, bool VEC, int L, int TEAM, int NG>
+// How a row is held: LR lanes (4 to 16 for one group, 32/LR rows a warp; 32 for two groups side by side), a team of TEAM
+// warps, NG passes of a warp's lanes along the row.  L: lanes of a group.
+template <int LR, int TEAM, int NG> struct LnRow {
+    static constexpr int L = LR < 16 ? LR : 16, PER_PASS = LR == 32 ? 2 : 1, RW = 32 / LR, TEAMS = kKeepWarps / TEAM;
+    int lane, sub, team, wt, half;                   // lane within its group; row of the warp; group of the pass
+    __device__ __forceinline__ LnRow() {
+        const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+        lane = l % L; sub = l / LR; half = LR == 32 ? l / 16 : 0; team = warp / TEAM; wt = warp % TEAM;
+    }
+    __device__ __forceinline__ int group(int j) const { return (wt * NG + j) * PER_PASS + half; }
+};
+
+// LayerNorm over rows of up to 8192 columns, y = (x - mean) * rstd * gamma + beta, the row held in registers.  Statistics are
+// two-pass, fp32.  Kept for the backward pass: the codes of x, mean and rstd.  UN rows of a lane are in flight at once
+// (short rows: what bounds the kernel is memory, and a lane's piece of a row is 16 bytes).
+template <typename T, bool VEC, int LR, int TEAM, int NG, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 ln_keep_kernel(const LnKeepArgs a) {
-    constexpr int RW = 32 / L, TEAMS = kKeepWarps / TEAM;
-    __shared__ float s1[kKeepWarps][1], s2[kKeepWarps][1];
-    const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, warp = threadIdx.x >> 5;
-    const int team = warp / TEAM, wt = warp % TEAM, C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
+    using R = LnRow<LR, TEAM, NG>;
+    constexpr int L = R::L;
+    __shared__ float s1[kKeepWarps][UN], s2[kKeepWarps][UN];
+    const R w;
+    const int C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
     const T *x = static_cast<const T *>(a.x);
     T *y = static_cast<T *>(a.y);
     const float inv_c = 1.f / (float)C;
-    for (long long r0 = ((long long)blockIdx.x * TEAMS + team) * RW; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS * RW) {
-        const long long r = r0 + sub;
-        const bool act = r < a.rows;
-        const long long ro = (act ? r : 0) * C;
-        float f[NG][4], s[1] = {0.f};
+    const long long stride = (long long)gridDim.x * R::TEAMS * R::RW;
+    float gm[NG][8], bt[NG][8];
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const int c = (wt * NG + j) * kKeepGroup + (VEC ? lane * 4 : lane);
-            load4<VEC, L>(x + ro, c, act ? min(C, (wt * NG + j + 1) * kKeepGroup) : 0, 0.f, f[j]);
-        }
+    for (int j = 0; j < NG; j++) {
+        const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), lim = min(C, (g + 1) * kKeepGroup);
+        load_params<VEC, L>(a.gamma, a.pbf16, c, lim, gm[j]);
+        load_params<VEC, L>(a.beta, a.pbf16, c, lim, bt[j]);
+    }
+    for (long long r0 = ((long long)blockIdx.x * R::TEAMS + w.team) * R::RW; r0 < a.rows; r0 += stride * UN) {
+        Raw8<T, VEC> raw[UN][NG];
+        float s[UN], mean[UN];
 #pragma unroll
-        for (int j = 0; j < NG; j++) s[0] += (f[j][0] + f[j][1]) + (f[j][2] + f[j][3]);
-        s[0] = lane_sum<L>(s[0]);
-        team_sum<TEAM, 1>(s, s1, team, wt);
-        const float mean = s[0] * inv_c;
-        s[0] = 0.f;
+        for (int u = 0; u < UN; u++) {
+            const long long r = r0 + w.sub + u * stride;
+            const bool act = r < a.rows;
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const int c = (wt * NG + j) * kKeepGroup + (VEC ? lane * 4 : lane);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float d = f[j][i] - mean;
-                if (col_of<VEC, L>(c, i) < C) s[0] += d * d;
+            for (int j = 0; j < NG; j++) {
+                const int g = w.group(j);
+                load8<VEC, L>(x + (act ? r : 0) * C, g * kKeepGroup + first_col<VEC>(w.lane), act ? min(C, (g + 1) * kKeepGroup) : 0, raw[u][j]);
             }
         }
-        s[0] = lane_sum<L>(s[0]);
-        team_sum<TEAM, 1>(s, s2, team, wt);
-        const float rstd = rsqrtf(s[0] * inv_c + a.eps);
-        if (act && lane == 0 && wt == 0) *reinterpret_cast<float2 *>(a.stats + r * 2) = make_float2(mean, rstd);
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const int g = wt * NG + j, c = g * kKeepGroup + (VEC ? lane * 4 : lane);
-            if (g >= G) break;
-            const int end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-            float o[4];
+        for (int u = 0; u < UN; u++) {
+            s[u] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int k = col_of<VEC, L>(c, i);
-                o[i] = k < end ? (f[j][i] - mean) * rstd * ld_param(a.gamma, k, a.pbf16) + ld_param(a.beta, k, a.pbf16) : 0.f;
+            for (int j = 0; j < NG; j++) {
+                float f[8];
+                unpack8<T, VEC>(raw[u][j], f);
+                s[u] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
             }
-            store4<VEC, L>(y + ro, c, end, o);
-            keep_group<VEC, L>(f[j], c, end, act ? lane : 1, a.codes + ro, a.ranges + ((act ? r : 0) * G + g) * 2);
+            s[u] = lane_sum<LR>(s[u]);
+        }
+        team_sum<TEAM, UN>(s, s1, w.team, w.wt);
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            mean[u] = s[u] * inv_c;
+            s[u] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
+                float t = 0.f, f[8];
+                unpack8<T, VEC>(raw[u][j], f);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float d = f[i] - mean[u];
+                    if (VEC || c + i * L < min(C, (g + 1) * kKeepGroup)) t = fmaf(d, d, t);
+                }
+                if (!VEC || c < C) s[u] += t;
+            }
+            s[u] = lane_sum<LR>(s[u]);
+        }
+        team_sum<TEAM, UN>(s, s2, w.team, w.wt);
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            const long long r = r0 + w.sub + u * stride;
+            const bool act = r < a.rows;
+            const long long ro = (act ? r : 0) * C;
+            const float rstd = rsqrtf(s[u] * inv_c + a.eps);
+            if (act && w.lane == 0 && w.half == 0 && w.wt == 0) *reinterpret_cast<float2 *>(a.stats + r * 2) = make_float2(mean[u], rstd);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
+                if ((w.wt * NG + j) * R::PER_PASS >= G) break;                  // the same for the whole warp
+                const int end = act ? min(C, (g + 1) * kKeepGroup) : 0;
+                float f[8], o[8];
+                unpack8<T, VEC>(raw[u][j], f);
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = fmaf((f[i] - mean[u]) * rstd, gm[j][i], bt[j][i]);
+                store8<VEC, L>(y + ro, c, end, o);
+                keep_group<VEC, L>(f, c, end, act && w.lane == 0 && g < G, a.codes + ro, a.ranges + ((act ? r : 0) * G + (g < G ? g : 0)) * 2);
+            }
         }
     }
 }
@@ -302,105 +390,128 @@ ln_keep_kernel(const LnKeepArgs a) {
 //   dx = rstd * (g - mean_C(g) - xhat * mean_C(g * xhat)),  dgamma = sum_rows dy * xhat,  dbeta = sum_rows dy.
 // Column sums as in layernorm_cl_bwd_kernel: registers, then the CTA's teams in order, then the CTAs in order
 // (sum_slices_kernel).  Dynamic shared memory: teams x 2 x C floats where a CTA has more than one team.
-template <typename T, bool VEC, int L, int TEAM, int NG>
+template <typename T, bool VEC, int LR, int TEAM, int NG, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 ln_keep_bwd_kernel(const LnKeepArgs a) {
-    constexpr int RW = 32 / L, TEAMS = kKeepWarps / TEAM;
+    using R = LnRow<LR, TEAM, NG>;
+    constexpr int L = R::L;
     extern __shared__ float ln_cols[];
-    __shared__ float s1[2][kKeepWarps][2];
-    const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, warp = threadIdx.x >> 5;
-    const int team = warp / TEAM, wt = warp % TEAM, C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
+    __shared__ float s1[2][kKeepWarps][2 * UN];
+    const R w;
+    const int C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
     const T *dy = static_cast<const T *>(a.x);
     T *dx = static_cast<T *>(a.dx), *y = static_cast<T *>(a.y);
     const float inv_c = 1.f / (float)C;
-    float gm[NG][4], sg[NG][4], sb[NG][4];
+    const long long stride = (long long)gridDim.x * R::TEAMS * R::RW;
+    float gm[NG][8], sg[NG][8], sb[NG][8];
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        const int c = (wt * NG + j) * kKeepGroup + (VEC ? lane * 4 : lane);
+        const int g = w.group(j);
+        load_params<VEC, L>(a.gamma, a.pbf16, g * kKeepGroup + first_col<VEC>(w.lane), min(C, (g + 1) * kKeepGroup), gm[j]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = col_of<VEC, L>(c, i);
-            gm[j][i] = k < min(C, (wt * NG + j + 1) * kKeepGroup) ? ld_param(a.gamma, k, a.pbf16) : 0.f;
-            sg[j][i] = sb[j][i] = 0.f;
-        }
+        for (int i = 0; i < 8; i++) sg[j][i] = sb[j][i] = 0.f;
     }
+    // xhat of the lane's values.  Of a group that is NaN, single columns may still not exist.
+    auto normalised = [&](uint2 q, float2 range, float2 st, int g, float (&h)[8]) {
+        restore_codes(q, range, h);
+        const int c = g * kKeepGroup + first_col<VEC>(w.lane), lim = min(C, (g + 1) * kKeepGroup);
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = VEC || c + i * L < lim ? (h[i] - st.x) * st.y : 0.f;
+    };
     int turn = 0;
-    for (long long r0 = ((long long)blockIdx.x * TEAMS + team) * RW; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS * RW) {
-        const long long r = r0 + sub;
-        const bool act = r < a.rows;
-        const long long ro = (act ? r : 0) * C;
-        const float2 st = __ldg(reinterpret_cast<const float2 *>(a.stats) + (act ? r : 0));
-        float d[NG][4], h[NG][4], s[2] = {0.f, 0.f};
+    for (long long r0 = ((long long)blockIdx.x * R::TEAMS + w.team) * R::RW; r0 < a.rows; r0 += stride * UN) {
+        Raw8<T, VEC> raw[UN][NG];
+        float s[2 * UN];
+        float2 st[UN], range[UN][NG];
+        uint2 q[UN][NG];
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const int g = wt * NG + j, c = g * kKeepGroup + (VEC ? lane * 4 : lane);
-            const int end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-            uint32_t q[4];
-            load4<VEC, L>(dy + ro, c, end, 0.f, d[j]);
-            load_codes<VEC, L>(a.codes + ro, c, end, q);
-            const float2 range = g < G ? __ldg(reinterpret_cast<const float2 *>(a.ranges) + (act ? r : 0) * G + g) : make_float2(0.f, 0.f);
+        for (int u = 0; u < UN; u++) {
+            const long long r = r0 + w.sub + u * stride;
+            const bool act = r < a.rows;
+            const long long ro = (act ? r : 0) * C;
+            st[u] = __ldg(reinterpret_cast<const float2 *>(a.stats) + (act ? r : 0));
 #pragma unroll
-            for (int i = 0; i < 4; i++) h[j][i] = col_of<VEC, L>(c, i) < end ? (restored(q[i], range) - st.x) * st.y : 0.f;
+            for (int j = 0; j < NG; j++) {
+                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), end = act ? min(C, (g + 1) * kKeepGroup) : 0;
+                load8<VEC, L>(dy + ro, c, end, raw[u][j]);
+                q[u][j] = load_codes<VEC, L>(a.codes + ro, c, end);
+                // (columns that do not exist: dy, gamma and this are zero, whatever their group holds)
+                range[u][j] = c < end ? __ldg(reinterpret_cast<const float2 *>(a.ranges) + r * G + g) : make_float2(0.f, 0.f);
+            }
+            if (!act) st[u] = make_float2(0.f, 0.f);
         }
 #pragma unroll
-        for (int j = 0; j < NG; j++)
+        for (int u = 0; u < UN; u++) {
+            s[2 * u] = s[2 * u + 1] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float gg = d[j][i] * gm[j][i];
-                s[0] += gg;
-                s[1] += gg * h[j][i];
-                sg[j][i] += d[j][i] * h[j][i];
-                sb[j][i] += d[j][i];
-            }
-        s[0] = lane_sum<L>(s[0]);
-        s[1] = lane_sum<L>(s[1]);
-        team_sum<TEAM, 2>(s, s1[turn], team, wt);
-        turn ^= 1;
-        const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
+            for (int j = 0; j < NG; j++) {
+                float d[8], h[8];
+                normalised(q[u][j], range[u][j], st[u], w.group(j), h);
+                unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const int g = wt * NG + j, c = g * kKeepGroup + (VEC ? lane * 4 : lane);
-            if (g >= G) break;
-            const int end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-            float o[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = st.y * (d[j][i] * gm[j][i] - c1 - h[j][i] * c2);
-            store4<VEC, L>(dx + ro, c, end, o);
-            if (y) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int k = col_of<VEC, L>(c, i);
-                    o[i] = k < end ? h[j][i] * gm[j][i] + ld_param(a.beta, k, a.pbf16) : 0.f;
+                for (int i = 0; i < 8; i++) {
+                    const float gg = d[i] * gm[j][i];
+                    s[2 * u] += gg;
+                    s[2 * u + 1] = fmaf(gg, h[i], s[2 * u + 1]);
+                    sg[j][i] = fmaf(d[i], h[i], sg[j][i]);
+                    sb[j][i] += d[i];
                 }
-                store4<VEC, L>(y + ro, c, end, o);
+            }
+            s[2 * u] = lane_sum<LR>(s[2 * u]);
+            s[2 * u + 1] = lane_sum<LR>(s[2 * u + 1]);
+        }
+        team_sum<TEAM, 2 * UN>(s, s1[turn], w.team, w.wt);
+        turn ^= 1;
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            const long long r = r0 + w.sub + u * stride;
+            const bool act = r < a.rows;
+            const long long ro = (act ? r : 0) * C;
+            const float c1 = s[2 * u] * inv_c, c2 = s[2 * u + 1] * inv_c;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), end = act ? min(C, (g + 1) * kKeepGroup) : 0;
+                float d[8], h[8], o[8];
+                normalised(q[u][j], range[u][j], st[u], g, h);
+                unpack8<T, VEC>(raw[u][j], d);
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = st[u].y * (d[i] * gm[j][i] - c1 - h[i] * c2);
+                store8<VEC, L>(dx + ro, c, end, o);
+                if (y) {
+                    float bt[8];
+                    load_params<VEC, L>(a.beta, a.pbf16, c, end, bt);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[i] = fmaf(h[i], gm[j][i], bt[i]);
+                    store8<VEC, L>(y + ro, c, end, o);
+                }
             }
         }
     }
     float *out = a.partial + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        const int c = (wt * NG + j) * kKeepGroup + (VEC ? lane * 4 : lane);
+        const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 8; i++) {
             const int k = col_of<VEC, L>(c, i);
 #pragma unroll
-            for (int o = L; o < 32; o <<= 1) {
+            for (int o = LR; o < 32; o <<= 1) {
                 sg[j][i] += __shfl_xor_sync(0xffffffffu, sg[j][i], o);
                 sb[j][i] += __shfl_xor_sync(0xffffffffu, sb[j][i], o);
             }
-            if (sub == 0 && k < min(C, (wt * NG + j + 1) * kKeepGroup)) {
-                float *to = TEAMS > 1 ? ln_cols + (size_t)team * 2 * C : out;
+            if (w.sub == 0 && k < min(C, (g + 1) * kKeepGroup)) {
+                float *to = R::TEAMS > 1 ? ln_cols + (size_t)w.team * 2 * C : out;
                 to[k] = sg[j][i];
                 to[C + k] = sb[j][i];
             }
         }
     }
-    if constexpr (TEAMS > 1) {
+    if constexpr (R::TEAMS > 1) {
         __syncthreads();
         for (int e = threadIdx.x; e < 2 * C; e += kKeepThreads) {
             float t = 0.f;
 #pragma unroll
-            for (int w = 0; w < TEAMS; w++) t += ln_cols[(size_t)w * 2 * C + e];
+            for (int k = 0; k < R::TEAMS; k++) t += ln_cols[(size_t)k * 2 * C + e];
             out[e] = t;
         }
     }

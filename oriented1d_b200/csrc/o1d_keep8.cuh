@@ -20,8 +20,20 @@ constexpr int kKeepThreads = 256;
 constexpr int kKeepWarps = kKeepThreads / 32;
 constexpr int kKeepLane = 8;             // values of a lane: 16 lanes hold a group, 16 bytes of bf16 each
 
+// Two fp32 numbers that one instruction works on (fma.rn.f32x2 and the like): the passes below are bound by instruction
+// issue, and a packed instruction takes one slot for two values.  Each half is rounded as the scalar instruction rounds.
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 two(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ F2 both(float a) { return two(a, a); }
+__device__ __forceinline__ float2 apart(F2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v)); return r; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float min_nan(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
 // Sum over the L lanes that share something.
 template <int L>
@@ -35,21 +47,37 @@ __device__ __forceinline__ float lane_sum(float v) {
 //   P(-|h|) = erfc(z)/2,  z = |h|/sqrt 2,  erfc(z) = t q(t) exp(-z^2),  t = 1/(1 + 0.33 z)
 // the form of Abramowitz and Stegun 7.1.26, with a polynomial q of degree 7 fitted to exp(z^2) erfc(z) on 0 <= z <= 10 by
 // iterated weighted least squares: relative error 1e-7 in both tails.  One reciprocal and one exponential, which the slope
-// GELU'(h) = P(h) + h exp(-h^2/2) / sqrt(2 pi) needs anyway.
-struct Normal { float cdf, bell; };                 // P(h), exp(-h^2/2)
-__device__ __forceinline__ Normal normal_of(float h) {
-    float t, e;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(fabsf(h), 0.33f * 0.70710678f, 1.f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-0.72134752f * h * h));
-    float q = fmaf(t, -0.1353452503681183f, 0.4602353572845459f);
-    q = fmaf(t, q, -0.35114675760269165f);
-    q = fmaf(t, q, 0.40849733352661133f);
-    q = fmaf(t, q, 0.04722202196717262f);
-    q = fmaf(t, q, 0.2012234777212143f);
-    q = fmaf(t, q, 0.1829560101032257f);
-    q = fmaf(t, q, 0.1863577961921692f);
-    q *= 0.5f * t * e;
-    return {h < 0.f ? q : 1.f - q, e};
+// needs anyway.
+// For a pair of values: m = |h| (at most 64), q = -P(-|h|), bell = exp(-h^2/2).  Then GELU(h) = max(h, 0) + m q and
+// GELU'(h) = 1/2 + sign(h) (1/2 + q + m bell / sqrt(2 pi)).
+struct Normal { F2 m, q, bell; };
+__device__ __forceinline__ Normal normal_of(F2 h) {
+    const float2 a = apart(h);
+    const F2 m = two(fminf(fabsf(a.x), 64.f), fminf(fabsf(a.y), 64.f));      // (q is 0 there: an infinity times it would be NaN)
+    const float2 d = apart(fma2(m, both(0.33f * 0.70710678f), both(1.f))), z = apart(mul2(mul2(h, h), both(-0.72134752f)));
+    float2 r, e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(z.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(z.y));
+    const F2 t = two(r.x, r.y), bell = two(e.x, e.y);
+    F2 q = fma2(t, both(0.5f * 0.1353452503681183f), both(-0.5f * 0.4602353572845459f));
+    q = fma2(t, q, both(0.5f * 0.35114675760269165f));
+    q = fma2(t, q, both(-0.5f * 0.40849733352661133f));
+    q = fma2(t, q, both(-0.5f * 0.04722202196717262f));
+    q = fma2(t, q, both(-0.5f * 0.2012234777212143f));
+    q = fma2(t, q, both(-0.5f * 0.1829560101032257f));
+    q = fma2(t, q, both(-0.5f * 0.1863577961921692f));
+    return {m, mul2(q, mul2(t, bell)), bell};
+}
+__device__ __forceinline__ F2 gelu_of(F2 h, const Normal &n) {
+    const float2 a = apart(h);
+    return fma2(n.m, n.q, two(fmaxf(a.x, 0.f), fmaxf(a.y, 0.f)));            // (NaN comes back through q)
+}
+__device__ __forceinline__ F2 gelu_slope(F2 h, const Normal &n) {
+    const float2 a = apart(h), w = apart(add2(fma2(mul2(n.m, both(0.3989422804014327f)), n.bell, n.q), both(0.5f)));
+    return add2(two(__uint_as_float(__float_as_uint(w.x) ^ (__float_as_uint(a.x) & 0x80000000u)),
+                    __uint_as_float(__float_as_uint(w.y) ^ (__float_as_uint(a.y) & 0x80000000u))), both(0.5f));
 }
 
 // A lane's eight values of a group of L lanes.  VEC: columns c .. c+7 (C % 8 == 0 and all aligned, so that all exist or
@@ -78,32 +106,29 @@ __device__ __forceinline__ void load8(const T *row, int c, int end, Raw8<T, VEC>
     }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void unpack8(const Raw8<T, VEC> &r, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const Raw8<T, VEC> &r, F2 (&f)[4]) {
     if constexpr (VEC && sizeof(T) == 2) {
-        f[0] = from_lo(r.v.x); f[1] = from_hi(r.v.x); f[2] = from_lo(r.v.y); f[3] = from_hi(r.v.y);
-        f[4] = from_lo(r.v.z); f[5] = from_hi(r.v.z); f[6] = from_lo(r.v.w); f[7] = from_hi(r.v.w);
+        f[0] = two(from_lo(r.v.x), from_hi(r.v.x)); f[1] = two(from_lo(r.v.y), from_hi(r.v.y));
+        f[2] = two(from_lo(r.v.z), from_hi(r.v.z)); f[3] = two(from_lo(r.v.w), from_hi(r.v.w));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = r.f[i];
+        for (int i = 0; i < 4; i++) f[i] = two(r.f[2 * i], r.f[2 * i + 1]);
     }
 }
 template <bool VEC, int L, typename T>
-__device__ __forceinline__ void store8(T *row, int c, int end, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T *row, int c, int end, const F2 (&v)[4]) {
+    const float2 a = apart(v[0]), b = apart(v[1]), d = apart(v[2]), e = apart(v[3]);
     if constexpr (VEC) {
         if (c >= end) return;
         if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4 *>(row + c)[0] = make_float4(f[0], f[1], f[2], f[3]);
-            reinterpret_cast<float4 *>(row + c)[1] = make_float4(f[4], f[5], f[6], f[7]);
+            reinterpret_cast<float4 *>(row + c)[0] = make_float4(a.x, a.y, b.x, b.y);
+            reinterpret_cast<float4 *>(row + c)[1] = make_float4(d.x, d.y, e.x, e.y);
         } else {
-            uint32_t u[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-                u[i] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-            *reinterpret_cast<uint4 *>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
+            const __nv_bfloat162 h[4] = {__float22bfloat162_rn(a), __float22bfloat162_rn(b), __float22bfloat162_rn(d), __float22bfloat162_rn(e)};
+            *reinterpret_cast<uint4 *>(row + c) = *reinterpret_cast<const uint4 *>(h);
         }
     } else {
+        const float f[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (c + i * L < end) st(row + c + i * L, f[i]);
@@ -111,9 +136,12 @@ __device__ __forceinline__ void store8(T *row, int c, int end, const float (&f)[
 }
 // Parameters of the lane's columns (0 where there is none).
 template <bool VEC, int L>
-__device__ __forceinline__ void load_params(const void *p, int bf16, int c, int end, float (&f)[8]) {
+__device__ __forceinline__ void load_params(const void *p, int bf16, int c, int end, F2 (&v)[4]) {
+    float f[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = p && col_of<VEC, L>(c, i) < end ? ld_param(p, col_of<VEC, L>(c, i), bf16) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = two(f[2 * i], f[2 * i + 1]);
 }
 // Codes travel as bytes and become numbers in the mantissa of 2^23 + q: integer conversions run at an eighth of the rate.
 template <bool VEC, int L>
@@ -125,49 +153,66 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t *row, int c, int end) 
         if (c + i * L < end) w[i >> 2] |= (uint32_t)__ldg(row + c + i * L) << (8 * (i & 3));
     return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void restore_codes(uint2 q, float2 range, float (&f)[8]) {
+__device__ __forceinline__ void restore_codes(uint2 q, float2 range, F2 (&f)[4]) {
+    const F2 step = both(range.y), lo = both(range.x);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float v = __uint_as_float(__byte_perm(i < 4 ? q.x : q.y, 0x4b000000u, 0x7650 | (i & 3))) - 8388608.f;
-        f[i] = fmaf(v, range.y, range.x);
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = i < 2 ? q.x : q.y;
+        const F2 v = two(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 | (2 * i & 3))), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 | ((2 * i + 1) & 3))));
+        f[i] = fma2(add2(v, both(-8388608.f)), step, lo);
     }
 }
 
 // Codes of the lane's eight values, and their group's range (stored by the group's first lane, when `store` is set).
 template <bool VEC, int L>
-__device__ __forceinline__ void keep_group(const float (&f)[8], int c, int end, bool store, uint8_t *codes, float *range) {
-    float lo = __int_as_float(0x7f800000), hi = -lo;
+__device__ __forceinline__ void keep_group(const F2 (&f)[4], int c, int end, bool store, uint8_t *codes, float *range) {
+    const float none = __int_as_float(0x7f800000);
+    const float2 a = apart(f[0]), b = apart(f[1]), d = apart(f[2]), e = apart(f[3]);
+    float lo, hi;
     if (VEC) {
-        if (c < end) {
-            lo = min_nan(min_nan(min_nan(f[0], f[1]), min_nan(f[2], f[3])), min_nan(min_nan(f[4], f[5]), min_nan(f[6], f[7])));
-            hi = max_nan(max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3])), max_nan(max_nan(f[4], f[5]), max_nan(f[6], f[7])));
-        }
+        lo = min_nan(min_nan(a.x, a.y, b.x), min_nan(b.y, d.x, d.y), min_nan(e.x, e.y));
+        hi = max_nan(max_nan(a.x, a.y, b.x), max_nan(b.y, d.x, d.y), max_nan(e.x, e.y));
+        if (c >= end) { lo = none; hi = -none; }
     } else {
+        const float v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
+        lo = none; hi = -none;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (c + i * L < end) { lo = min_nan(lo, f[i]); hi = max_nan(hi, f[i]); }
+            if (c + i * L < end) { lo = min_nan(lo, v[i]); hi = max_nan(hi, v[i]); }
     }
+    // One butterfly finds both: the lanes of the upper half take over the (negated) greatest values, those of the lower
+    // half the least ones, and the last exchange hands each the other's result.
+    const bool upper = threadIdx.x & (L / 2);
+    float m = upper ? -hi : lo;
+    m = min_nan(m, __shfl_xor_sync(0xffffffffu, upper ? lo : -hi, L / 2));
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
+    for (int o = L / 4; o > 0; o >>= 1) m = min_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float other = __shfl_xor_sync(0xffffffffu, m, L / 2);
+    lo = upper ? other : m;
+    hi = -(upper ? m : other);
     float step = __fmul_rn(__fsub_rn(hi, lo), 1.f / 255.f), inv = 0.f;
-    if (!(step <= 3.402823466e38f)) step = __int_as_float(0x7fffffff);        // NaN or infinite: the group is lost
+    uint32_t mask = 0xffffffffu;
+    if (!(step <= 3.402823466e38f)) { step = __int_as_float(0x7fffffff); mask = 0u; }        // NaN or infinite: the group is lost
     else if (step < 1.175494351e-38f) step = 0.f;
     else inv = __frcp_rn(step);
     uint32_t q[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++)                       // 2^23 + t has round(t) in its lowest bits; fmaxf: 0 for NaN
-        q[i] = __float_as_uint(__fadd_rn(fmaxf(__fmul_rn(__fsub_rn(f[i], lo), inv), 0.f), 8388608.f));
+    for (int i = 0; i < 4; i++) {
+        // 2^23 + t has round(t) in its lowest bits.  (Not a packed sum: the assembler makes one operation of a packed product
+        // and the packed sum behind it, with one rounding, which on ties is another code.)
+        const float2 t = apart(mul2(add2(f[i], both(-lo)), both(inv)));
+        q[2 * i] = __float_as_uint(__fadd_rn(t.x, 8388608.f));
+        q[2 * i + 1] = __float_as_uint(__fadd_rn(t.y, 8388608.f));
+    }
     if constexpr (VEC) {
         if (c < end)
-            *reinterpret_cast<uint2 *>(codes + c) = make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
-                                                               __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+            *reinterpret_cast<uint2 *>(codes + c) =
+                make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410) & mask,
+                           __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410) & mask);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (c + i * L < end) codes[c + i * L] = (uint8_t)q[i];
+            if (c + i * L < end) codes[c + i * L] = (uint8_t)(q[i] & mask);
     }
     if (store) *reinterpret_cast<float2 *>(range) = make_float2(lo, step);
 }
@@ -187,10 +232,10 @@ keep_kernel(const KeepArgs a) {
     const long long stride = (long long)gridDim.y * kKeepWarps * RW;
     const T *x = static_cast<const T *>(a.x);
     T *y = static_cast<T *>(a.y), *dx = static_cast<T *>(a.dx);
-    float b[8], sum[8];
+    F2 b[4], sum[4];
     if (KIND == KEEP_GELU_FWD) load_params<VEC, L>(a.bias, a.pbf16, c, lim, b);
 #pragma unroll
-    for (int i = 0; i < 8; i++) sum[i] = 0.f;
+    for (int i = 0; i < 4; i++) sum[i] = both(0.f);
     // whole warps leave the loop together (the groups' ranges are found with warp-wide instructions)
     for (long long r0 = ((long long)blockIdx.y * kKeepWarps + warp) * RW; r0 < a.rows; r0 += stride * UN) {
         Raw8<T, VEC> raw[UN];
@@ -212,35 +257,34 @@ keep_kernel(const KeepArgs a) {
             const bool act = r < a.rows;
             const int end = act ? lim : 0;                       // a row past the last one has no columns
             const long long ro = (act ? r : 0) * C;
-            float f[8];
+            F2 f[4];
             if constexpr (KIND != KEEP_RESTORE) unpack8<T, VEC>(raw[u], f);
             if constexpr (KIND == KEEP_FWD || KIND == KEEP_GELU_FWD) {
                 if constexpr (KIND == KEEP_GELU_FWD) {
-                    float v[8];
+                    F2 v[4];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        f[i] = __fadd_rn(f[i], b[i]);
-                        v[i] = f[i] * normal_of(f[i]).cdf;
+                    for (int i = 0; i < 4; i++) {
+                        f[i] = add2(f[i], b[i]);
+                        v[i] = gelu_of(f[i], normal_of(f[i]));
                     }
                     store8<VEC, L>(y + ro, c, end, v);
                 }
                 if (KIND == KEEP_FWD || a.codes)
                     keep_group<VEC, L>(f, c, end, act && lane == 0, a.codes + ro, a.ranges + ((act ? r : 0) * G + g) * 2);
             } else {
-                float v[8];
+                F2 v[4];
                 restore_codes(q[u], range[u], v);
                 if constexpr (KIND == KEEP_GELU_BWD) {
-                    float d[8];
+                    F2 d[4];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 4; i++) {
                         const Normal n = normal_of(v[i]);
-                        d[i] = f[i] * fmaf(v[i] * 0.3989422804014327f, n.bell, n.cdf);
-                        v[i] *= n.cdf;
+                        d[i] = mul2(f[i], gelu_slope(v[i], n));
+                        if (y) v[i] = gelu_of(v[i], n);
                     }
-                    if (a.dbias) {
+                    // columns that do not exist add dy = 0, unless their group is NaN; their sums are never read
 #pragma unroll
-                        for (int i = 0; i < 8; i++) sum[i] += col_of<VEC, L>(c, i) < end ? d[i] : 0.f;
-                    }
+                    for (int i = 0; i < 4; i++) sum[i] = add2(sum[i], act ? d[i] : both(0.f));
                     store8<VEC, L>(dx + ro, c, end, d);
                 }
                 if (KIND == KEEP_RESTORE || y) store8<VEC, L>(y + ro, c, end, v);
@@ -252,9 +296,10 @@ keep_kernel(const KeepArgs a) {
         __shared__ float red[kKeepWarps][kKeepGroup];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
+            float t = i & 1 ? apart(sum[i >> 1]).y : apart(sum[i >> 1]).x;
 #pragma unroll
-            for (int o = L; o < 32; o <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-            if (sub == 0) red[warp][col_of<VEC, L>(first_col<VEC>(lane), i)] = sum[i];
+            for (int o = L; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (sub == 0) red[warp][col_of<VEC, L>(first_col<VEC>(lane), i)] = t;
         }
         __syncthreads();
         if (threadIdx.x < lim - g * kKeepGroup) {
@@ -312,7 +357,7 @@ ln_keep_kernel(const LnKeepArgs a) {
     T *y = static_cast<T *>(a.y);
     const float inv_c = 1.f / (float)C;
     const long long stride = (long long)gridDim.x * R::TEAMS * R::RW;
-    float gm[NG][8], bt[NG][8];
+    F2 gm[NG][4], bt[NG][4];
 #pragma unroll
     for (int j = 0; j < NG; j++) {
         const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), lim = min(C, (g + 1) * kKeepGroup);
@@ -337,9 +382,10 @@ ln_keep_kernel(const LnKeepArgs a) {
             s[u] = 0.f;
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                float f[8];
+                F2 f[4];
                 unpack8<T, VEC>(raw[u][j], f);
-                s[u] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+                const float2 t = apart(add2(add2(f[0], f[1]), add2(f[2], f[3])));
+                s[u] += t.x + t.y;
             }
             s[u] = lane_sum<LR>(s[u]);
         }
@@ -351,14 +397,20 @@ ln_keep_kernel(const LnKeepArgs a) {
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
-                float t = 0.f, f[8];
+                F2 f[4], sq = both(0.f);
                 unpack8<T, VEC>(raw[u][j], f);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float d = f[i] - mean[u];
-                    if (VEC || c + i * L < min(C, (g + 1) * kKeepGroup)) t = fmaf(d, d, t);
+                for (int i = 0; i < 4; i++) {
+                    F2 d = add2(f[i], both(-mean[u]));
+                    if (!VEC) {
+                        const int lim = min(C, (g + 1) * kKeepGroup);
+                        const float2 v = apart(d);
+                        d = two(c + 2 * i * L < lim ? v.x : 0.f, c + (2 * i + 1) * L < lim ? v.y : 0.f);
+                    }
+                    sq = fma2(d, d, sq);
                 }
-                if (!VEC || c < C) s[u] += t;
+                const float2 t = apart(sq);
+                if (!VEC || c < C) s[u] += t.x + t.y;
             }
             s[u] = lane_sum<LR>(s[u]);
         }
@@ -375,10 +427,10 @@ ln_keep_kernel(const LnKeepArgs a) {
                 const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
                 if ((w.wt * NG + j) * R::PER_PASS >= G) break;                  // the same for the whole warp
                 const int end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-                float f[8], o[8];
+                F2 f[4], o[4];
                 unpack8<T, VEC>(raw[u][j], f);
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[i] = fmaf((f[i] - mean[u]) * rstd, gm[j][i], bt[j][i]);
+                for (int i = 0; i < 4; i++) o[i] = fma2(mul2(add2(f[i], both(-mean[u])), both(rstd)), gm[j][i], bt[j][i]);
                 store8<VEC, L>(y + ro, c, end, o);
                 keep_group<VEC, L>(f, c, end, act && w.lane == 0 && g < G, a.codes + ro, a.ranges + ((act ? r : 0) * G + (g < G ? g : 0)) * 2);
             }
@@ -403,20 +455,26 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
     T *dx = static_cast<T *>(a.dx), *y = static_cast<T *>(a.y);
     const float inv_c = 1.f / (float)C;
     const long long stride = (long long)gridDim.x * R::TEAMS * R::RW;
-    float gm[NG][8], sg[NG][8], sb[NG][8];
+    F2 gm[NG][4], sg[NG][4], sb[NG][4];
 #pragma unroll
     for (int j = 0; j < NG; j++) {
         const int g = w.group(j);
         load_params<VEC, L>(a.gamma, a.pbf16, g * kKeepGroup + first_col<VEC>(w.lane), min(C, (g + 1) * kKeepGroup), gm[j]);
 #pragma unroll
-        for (int i = 0; i < 8; i++) sg[j][i] = sb[j][i] = 0.f;
+        for (int i = 0; i < 4; i++) sg[j][i] = sb[j][i] = both(0.f);
     }
     // xhat of the lane's values.  Of a group that is NaN, single columns may still not exist.
-    auto normalised = [&](uint2 q, float2 range, float2 st, int g, float (&h)[8]) {
+    auto normalised = [&](uint2 q, float2 range, float2 st, int g, F2 (&h)[4]) {
         restore_codes(q, range, h);
         const int c = g * kKeepGroup + first_col<VEC>(w.lane), lim = min(C, (g + 1) * kKeepGroup);
 #pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = VEC || c + i * L < lim ? (h[i] - st.x) * st.y : 0.f;
+        for (int i = 0; i < 4; i++) {
+            h[i] = mul2(add2(h[i], both(-st.x)), both(st.y));
+            if (!VEC) {
+                const float2 v = apart(h[i]);
+                h[i] = two(c + 2 * i * L < lim ? v.x : 0.f, c + (2 * i + 1) * L < lim ? v.y : 0.f);
+            }
+        }
     };
     int turn = 0;
     for (long long r0 = ((long long)blockIdx.x * R::TEAMS + w.team) * R::RW; r0 < a.rows; r0 += stride * UN) {
@@ -442,21 +500,23 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            s[2 * u] = s[2 * u + 1] = 0.f;
+            F2 t1 = both(0.f), t2 = both(0.f);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                float d[8], h[8];
+                F2 d[4], h[4];
                 normalised(q[u][j], range[u][j], st[u], w.group(j), h);
                 unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float gg = d[i] * gm[j][i];
-                    s[2 * u] += gg;
-                    s[2 * u + 1] = fmaf(gg, h[i], s[2 * u + 1]);
-                    sg[j][i] = fmaf(d[i], h[i], sg[j][i]);
-                    sb[j][i] += d[i];
+                for (int i = 0; i < 4; i++) {
+                    const F2 gg = mul2(d[i], gm[j][i]);
+                    t1 = add2(t1, gg);
+                    t2 = fma2(gg, h[i], t2);
+                    sg[j][i] = fma2(d[i], h[i], sg[j][i]);
+                    sb[j][i] = add2(sb[j][i], d[i]);
                 }
             }
+            s[2 * u] = apart(t1).x + apart(t1).y;
+            s[2 * u + 1] = apart(t2).x + apart(t2).y;
             s[2 * u] = lane_sum<LR>(s[2 * u]);
             s[2 * u + 1] = lane_sum<LR>(s[2 * u + 1]);
         }
@@ -471,17 +531,18 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-                float d[8], h[8], o[8];
+                F2 d[4], h[4], o[4];
                 normalised(q[u][j], range[u][j], st[u], g, h);
                 unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[i] = st[u].y * (d[i] * gm[j][i] - c1 - h[i] * c2);
+                for (int i = 0; i < 4; i++)
+                    o[i] = mul2(fma2(h[i], both(-c2), fma2(d[i], gm[j][i], both(-c1))), both(st[u].y));
                 store8<VEC, L>(dx + ro, c, end, o);
                 if (y) {
-                    float bt[8];
+                    F2 bt[4];
                     load_params<VEC, L>(a.beta, a.pbf16, c, end, bt);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[i] = fmaf(h[i], gm[j][i], bt[i]);
+                    for (int i = 0; i < 4; i++) o[i] = fma2(h[i], gm[j][i], bt[i]);
                     store8<VEC, L>(y + ro, c, end, o);
                 }
             }
@@ -494,15 +555,16 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int k = col_of<VEC, L>(c, i);
+            float tg = i & 1 ? apart(sg[j][i >> 1]).y : apart(sg[j][i >> 1]).x, tb = i & 1 ? apart(sb[j][i >> 1]).y : apart(sb[j][i >> 1]).x;
 #pragma unroll
             for (int o = LR; o < 32; o <<= 1) {
-                sg[j][i] += __shfl_xor_sync(0xffffffffu, sg[j][i], o);
-                sb[j][i] += __shfl_xor_sync(0xffffffffu, sb[j][i], o);
+                tg += __shfl_xor_sync(0xffffffffu, tg, o);
+                tb += __shfl_xor_sync(0xffffffffu, tb, o);
             }
             if (w.sub == 0 && k < min(C, (g + 1) * kKeepGroup)) {
                 float *to = R::TEAMS > 1 ? ln_cols + (size_t)w.team * 2 * C : out;
-                to[k] = sg[j][i];
-                to[C + k] = sb[j][i];
+                to[k] = tg;
+                to[C + k] = tb;
             }
         }
     }

@@ -271,7 +271,7 @@ int o1d_linear_xent_bwd(const void *x, const void *w, const void *bias, const lo
 
 /* Activation checkpoints in 8 bits: what a training step keeps of a tensor between its forward and its
  * backward pass (the reference keeps every activation whole, through autograd; models/convnext.py:304-318).
- * x is [rows, C], fp32 or bf16.  Each row is cut into groups of 128 columns (the last may be shorter).  With lo, hi
+ * x is [rows, C], fp32 or bf16, C at most 2^24.  Each row is cut into groups of 128 columns (the last may be shorter).  With lo, hi
  * the least and greatest value of a group, s = (hi - lo) * (1/255) and q = round_to_even((v - lo) * (1/s)), every
  * operation in fp32 and rounded on its own; the code q stands for lo + q * s.  A group of equal values (or whose s is
  * below the normal numbers) has s = 0 and stands for lo; a group that holds a NaN or an infinity, or whose range

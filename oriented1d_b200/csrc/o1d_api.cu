@@ -1348,7 +1348,7 @@ bool bad_rows(long long rows, int C, int dtype) { return rows <= 0 || C <= 0 || 
 // Ranges and statistics are read and written as pairs of floats.
 bool misaligned8(const void *p) { return ((uintptr_t)p & 7) != 0; }
 int keep_call(int kind, const KeepArgs &a, int dtype, void *stream, const char *what) {
-    if (misaligned8(a.ranges)) return O1D_ERR_UNSUPPORTED;
+    if (misaligned8(a.ranges) || a.C > kKeepMaxColumns) return O1D_ERR_UNSUPPORTED;
     DeviceInfo d;
     int rc = device_info(&d);
     if (rc) return rc;

@@ -15,11 +15,16 @@ inline bool vectors(int C, const void *x, const void *y, const void *dx, const v
     return C % 8 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(dx, 16) && aligned(codes, 8);
 }
 
+// Rows of a lane in flight: two where there are rows enough for four CTAs on every SM, else one, so that short tensors
+// reach all SMs.
+constexpr int kKeepFlight = 2;
+inline bool keep_many(long long rows, int C, int sms) { return rows * groups_of(C) >= (long long)kKeepWarps * (32 / lanes_of(C)) * kKeepFlight * sms * 4; }
+
 template <int KIND, typename T, bool VEC, int L>
 cudaError_t keep_go(const KeepArgs &a, int sms, cudaStream_t st) {
-    constexpr int UN = sizeof(T) == 2 ? 4 : 2;
     const dim3 grid(groups_of(a.C), keep_slices(a.rows, a.C, sms));
-    keep_kernel<KIND, T, VEC, L, UN><<<grid, kKeepThreads, 0, st>>>(a);
+    if (keep_many(a.rows, a.C, sms)) keep_kernel<KIND, T, VEC, L, kKeepFlight><<<grid, kKeepThreads, 0, st>>>(a);
+    else keep_kernel<KIND, T, VEC, L, 1><<<grid, kKeepThreads, 0, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess && KIND == KEEP_GELU_BWD && a.dbias ? sum_slices(a.partial, a.dbias, a.C, nullptr, 0, a.pbf16, (int)grid.y, st) : e;
 }
@@ -50,6 +55,9 @@ cudaError_t keep_kind(int kind, const KeepArgs &a, int sms, cudaStream_t st) {
 inline int ln_team(int C) { return C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : 8; }
 inline int ln_cta_rows(int C) { return C <= 128 ? kKeepWarps * (32 / lanes_of(C)) : kKeepWarps / ln_team(C); }
 
+// Short rows: two of a lane in flight where there are rows enough for four CTAs on every SM.
+inline int ln_flight(long long rows, int C, int sms) { return C <= 256 && rows >= 2ll * ln_cta_rows(C) * sms * 4 ? 2 : 1; }
+
 template <bool BWD, typename T, bool VEC, int LR, int TEAM, int NG, int UN>
 cudaError_t ln_go(const LnKeepArgs &a, int sms, cudaStream_t st) {
     const int grid = ln_keep_ctas(a.rows, a.C, sms);
@@ -65,13 +73,17 @@ cudaError_t ln_go(const LnKeepArgs &a, int sms, cudaStream_t st) {
         return cudaGetLastError();
     }
 }
+template <bool BWD, typename T, bool VEC, int LR>
+cudaError_t ln_short(const LnKeepArgs &a, int sms, cudaStream_t st) {
+    return ln_flight(a.rows, a.C, sms) == 2 ? ln_go<BWD, T, VEC, LR, 1, 1, 2>(a, sms, st) : ln_go<BWD, T, VEC, LR, 1, 1, 1>(a, sms, st);
+}
 template <bool BWD, typename T, bool VEC>
 cudaError_t ln_width(const LnKeepArgs &a, int sms, cudaStream_t st) {
     const int C = a.C;
-    if (C <= 32) return ln_go<BWD, T, VEC, 4, 1, 1, 2>(a, sms, st);
-    if (C <= 64) return ln_go<BWD, T, VEC, 8, 1, 1, 2>(a, sms, st);
-    if (C <= 128) return ln_go<BWD, T, VEC, 16, 1, 1, 2>(a, sms, st);
-    if (C <= 256) return ln_go<BWD, T, VEC, 32, 1, 1, 2>(a, sms, st);
+    if (C <= 32) return ln_short<BWD, T, VEC, 4>(a, sms, st);
+    if (C <= 64) return ln_short<BWD, T, VEC, 8>(a, sms, st);
+    if (C <= 128) return ln_short<BWD, T, VEC, 16>(a, sms, st);
+    if (C <= 256) return ln_short<BWD, T, VEC, 32>(a, sms, st);
     if (C <= 512) return ln_go<BWD, T, VEC, 32, 1, 2, 1>(a, sms, st);
     if (C <= 1024) return ln_go<BWD, T, VEC, 32, 2, 2, 1>(a, sms, st);
     if (C <= 2048) return ln_go<BWD, T, VEC, 32, 4, 2, 1>(a, sms, st);
@@ -86,8 +98,8 @@ cudaError_t ln_vec(const LnKeepArgs &a, int sms, cudaStream_t st) {
 }  // namespace
 
 int keep_slices(long long rows, int C, int sms) {
-    const int per = kKeepWarps * (32 / lanes_of(C)), G = groups_of(C);
-    const long long most = (rows + per - 1) / per;                       // a row for every warp
+    const int per = kKeepWarps * (32 / lanes_of(C)) * (keep_many(rows, C, sms) ? kKeepFlight : 1), G = groups_of(C);
+    const long long most = (rows + per - 1) / per;                       // rows of one round of a CTA
     long long s = ((long long)sms * 16 + G - 1) / G;
     s = s < most ? s : most;
     return (int)(s < 1 ? 1 : s > 65535 ? 65535 : s);
@@ -98,7 +110,7 @@ cudaError_t keep_launch(int kind, bool bf16, const KeepArgs &a, int sms, cudaStr
 }
 
 int ln_keep_ctas(long long rows, int C, int sms) {
-    const int per = ln_cta_rows(C);
+    const int per = ln_cta_rows(C) * ln_flight(rows, C, sms);
     const long long need = (rows + per - 1) / per, cap = (long long)sms * 4;
     return (int)(need < cap ? need : cap);
 }

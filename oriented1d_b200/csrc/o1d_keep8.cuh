@@ -35,12 +35,13 @@ __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.N
 __device__ __forceinline__ float min_nan(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
-// Sum over the L lanes that share something.
-template <int L>
-__device__ __forceinline__ float lane_sum(float v) {
+// Sums over the L lanes that share something, for U of them at once.
+template <int L, int U>
+__device__ __forceinline__ void lane_sums(float (&v)[U]) {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
 }
 
 // Exact GELU and its slope without erff, of which the passes below would be nothing else (20 instructions a value each).
@@ -81,7 +82,8 @@ __device__ __forceinline__ F2 gelu_slope(F2 h, const Normal &n) {
 }
 
 // A lane's eight values of a group of L lanes.  VEC: columns c .. c+7 (C % 8 == 0 and all aligned, so that all exist or
-// none); otherwise columns c, c+L, ..., c+7L, one element each.  `end`: the columns of the row, or of its part, that exist.
+// none); otherwise columns c, c+L, ..., c+7L, one element each.  `at`: the address of column c; `end`: the columns of the row, or
+// of its part, that exist.
 template <bool VEC, int L> __device__ __forceinline__ int col_of(int c, int i) { return VEC ? c + i : c + i * L; }
 template <bool VEC> __device__ __forceinline__ int first_col(int lane) { return VEC ? lane * kKeepLane : lane; }
 
@@ -92,17 +94,17 @@ __device__ __forceinline__ float from_hi(uint32_t v) { return __uint_as_float(v 
 template <typename T, bool VEC> struct Raw8 { float f[8]; };
 template <> struct Raw8<__nv_bfloat16, true> { uint4 v; };
 template <bool VEC, int L, typename T>
-__device__ __forceinline__ void load8(const T *row, int c, int end, Raw8<T, VEC> &r) {
+__device__ __forceinline__ void load8(const T *at, int c, int end, Raw8<T, VEC> &r) {
     if constexpr (VEC && sizeof(T) == 2) {
-        r.v = c < end ? __ldg(reinterpret_cast<const uint4 *>(row + c)) : make_uint4(0u, 0u, 0u, 0u);
+        r.v = c < end ? __ldg(reinterpret_cast<const uint4 *>(at)) : make_uint4(0u, 0u, 0u, 0u);
     } else if constexpr (VEC) {
         const bool on = c < end;
-        const float4 a = on ? __ldg(reinterpret_cast<const float4 *>(row + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 b = on ? __ldg(reinterpret_cast<const float4 *>(row + c) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 a = on ? __ldg(reinterpret_cast<const float4 *>(at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 b = on ? __ldg(reinterpret_cast<const float4 *>(at) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
         r.f[0] = a.x; r.f[1] = a.y; r.f[2] = a.z; r.f[3] = a.w; r.f[4] = b.x; r.f[5] = b.y; r.f[6] = b.z; r.f[7] = b.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) r.f[i] = c + i * L < end ? ld(row + c + i * L) : 0.f;
+        for (int i = 0; i < 8; i++) r.f[i] = c + i * L < end ? ld(at + i * L) : 0.f;
     }
 }
 template <typename T, bool VEC>
@@ -116,22 +118,22 @@ __device__ __forceinline__ void unpack8(const Raw8<T, VEC> &r, F2 (&f)[4]) {
     }
 }
 template <bool VEC, int L, typename T>
-__device__ __forceinline__ void store8(T *row, int c, int end, const F2 (&v)[4]) {
+__device__ __forceinline__ void store8(T *at, int c, int end, const F2 (&v)[4]) {
     const float2 a = apart(v[0]), b = apart(v[1]), d = apart(v[2]), e = apart(v[3]);
     if constexpr (VEC) {
         if (c >= end) return;
         if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4 *>(row + c)[0] = make_float4(a.x, a.y, b.x, b.y);
-            reinterpret_cast<float4 *>(row + c)[1] = make_float4(d.x, d.y, e.x, e.y);
+            reinterpret_cast<float4 *>(at)[0] = make_float4(a.x, a.y, b.x, b.y);
+            reinterpret_cast<float4 *>(at)[1] = make_float4(d.x, d.y, e.x, e.y);
         } else {
             const __nv_bfloat162 h[4] = {__float22bfloat162_rn(a), __float22bfloat162_rn(b), __float22bfloat162_rn(d), __float22bfloat162_rn(e)};
-            *reinterpret_cast<uint4 *>(row + c) = *reinterpret_cast<const uint4 *>(h);
+            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(h);
         }
     } else {
         const float f[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (c + i * L < end) st(row + c + i * L, f[i]);
+            if (c + i * L < end) st(at + i * L, f[i]);
     }
 }
 // Parameters of the lane's columns (0 where there is none).
@@ -145,12 +147,12 @@ __device__ __forceinline__ void load_params(const void *p, int bf16, int c, int 
 }
 // Codes travel as bytes and become numbers in the mantissa of 2^23 + q: integer conversions run at an eighth of the rate.
 template <bool VEC, int L>
-__device__ __forceinline__ uint2 load_codes(const uint8_t *row, int c, int end) {
-    if constexpr (VEC) return c < end ? __ldg(reinterpret_cast<const uint2 *>(row + c)) : make_uint2(0u, 0u);
+__device__ __forceinline__ uint2 load_codes(const uint8_t *at, int c, int end) {
+    if constexpr (VEC) return c < end ? __ldg(reinterpret_cast<const uint2 *>(at)) : make_uint2(0u, 0u);
     uint32_t w[2] = {0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        if (c + i * L < end) w[i >> 2] |= (uint32_t)__ldg(row + c + i * L) << (8 * (i & 3));
+        if (c + i * L < end) w[i >> 2] |= (uint32_t)__ldg(at + i * L) << (8 * (i & 3));
     return make_uint2(w[0], w[1]);
 }
 __device__ __forceinline__ void restore_codes(uint2 q, float2 range, F2 (&f)[4]) {
@@ -163,131 +165,162 @@ __device__ __forceinline__ void restore_codes(uint2 q, float2 range, F2 (&f)[4])
     }
 }
 
-// Codes of the lane's eight values, and their group's range (stored by the group's first lane, when `store` is set).
-template <bool VEC, int L>
-__device__ __forceinline__ void keep_group(const F2 (&f)[4], int c, int end, bool store, uint8_t *codes, float *range) {
+// Codes of the lane's eight values and their group's range, for U groups at once (each step of the butterflies waits for the
+// one before it, and shuffles stay in the order they are written in: one group after the other, those waits were what the
+// kernels did).  end: 0 for a row that does not exist.
+template <bool VEC, int L, int U>
+__device__ __forceinline__ void keep_groups(const F2 (&f)[U][4], int c, const int (&end)[U], uint2 (&codes)[U], float2 (&range)[U]) {
     const float none = __int_as_float(0x7f800000);
-    const float2 a = apart(f[0]), b = apart(f[1]), d = apart(f[2]), e = apart(f[3]);
-    float lo, hi;
-    if (VEC) {
-        lo = min_nan(min_nan(a.x, a.y, b.x), min_nan(b.y, d.x, d.y), min_nan(e.x, e.y));
-        hi = max_nan(max_nan(a.x, a.y, b.x), max_nan(b.y, d.x, d.y), max_nan(e.x, e.y));
-        if (c >= end) { lo = none; hi = -none; }
-    } else {
-        const float v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
-        lo = none; hi = -none;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (c + i * L < end) { lo = min_nan(lo, v[i]); hi = max_nan(hi, v[i]); }
-    }
-    // One butterfly finds both: the lanes of the upper half take over the (negated) greatest values, those of the lower
-    // half the least ones, and the last exchange hands each the other's result.
     const bool upper = threadIdx.x & (L / 2);
-    float m = upper ? -hi : lo;
-    m = min_nan(m, __shfl_xor_sync(0xffffffffu, upper ? lo : -hi, L / 2));
+    float m[U], send[U], lo[U], inv[U], step[U];
+    uint32_t mask[U];
 #pragma unroll
-    for (int o = L / 4; o > 0; o >>= 1) m = min_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float other = __shfl_xor_sync(0xffffffffu, m, L / 2);
-    lo = upper ? other : m;
-    hi = -(upper ? m : other);
-    float step = __fmul_rn(__fsub_rn(hi, lo), 1.f / 255.f), inv = 0.f;
-    uint32_t mask = 0xffffffffu;
-    if (!(step <= 3.402823466e38f)) { step = __int_as_float(0x7fffffff); mask = 0u; }        // NaN or infinite: the group is lost
-    else if (step < 1.175494351e-38f) step = 0.f;
-    else inv = __frcp_rn(step);
-    uint32_t q[8];
+    for (int u = 0; u < U; u++) {
+        const float2 a = apart(f[u][0]), b = apart(f[u][1]), d = apart(f[u][2]), e = apart(f[u][3]);
+        float least, most;
+        if (VEC) {
+            least = min_nan(min_nan(a.x, a.y, b.x), min_nan(b.y, d.x, d.y), min_nan(e.x, e.y));
+            most = max_nan(max_nan(a.x, a.y, b.x), max_nan(b.y, d.x, d.y), max_nan(e.x, e.y));
+            if (c >= end[u]) { least = none; most = -none; }
+        } else {
+            const float v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
+            least = none; most = -none;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        // 2^23 + t has round(t) in its lowest bits.  (Not a packed sum: the assembler makes one operation of a packed product
-        // and the packed sum behind it, with one rounding, which on ties is another code.)
-        const float2 t = apart(mul2(add2(f[i], both(-lo)), both(inv)));
-        q[2 * i] = __float_as_uint(__fadd_rn(t.x, 8388608.f));
-        q[2 * i + 1] = __float_as_uint(__fadd_rn(t.y, 8388608.f));
+            for (int i = 0; i < 8; i++)
+                if (c + i * L < end[u]) { least = min_nan(least, v[i]); most = max_nan(most, v[i]); }
+        }
+        // One butterfly finds both ends: the lanes of the upper half take over the (negated) greatest values, those of the
+        // lower half the least ones, and the last exchange hands each the other's result.
+        m[u] = upper ? -most : least;
+        send[u] = upper ? least : -most;
     }
+#pragma unroll
+    for (int u = 0; u < U; u++) m[u] = min_nan(m[u], __shfl_xor_sync(0xffffffffu, send[u], L / 2));
+#pragma unroll
+    for (int o = L / 4; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; u++) m[u] = min_nan(m[u], __shfl_xor_sync(0xffffffffu, m[u], o));
+#pragma unroll
+    for (int u = 0; u < U; u++) send[u] = __shfl_xor_sync(0xffffffffu, m[u], L / 2);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        lo[u] = upper ? send[u] : m[u];
+        const float hi = -(upper ? m[u] : send[u]);
+        step[u] = __fmul_rn(__fsub_rn(hi, lo[u]), 1.f / 255.f);
+        inv[u] = 0.f;
+        mask[u] = 0xffffffffu;
+        if (!(step[u] <= 3.402823466e38f)) { step[u] = __int_as_float(0x7fffffff); mask[u] = 0u; }        // NaN or infinite: the group is lost
+        else if (step[u] < 1.175494351e-38f) step[u] = 0.f;
+        else inv[u] = __frcp_rn(step[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        uint32_t q[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // 2^23 + t has round(t) in its lowest bits.  (Not a packed sum: the assembler makes one operation of a packed
+            // product and the packed sum behind it, with one rounding, which on ties is another code.)
+            const float2 t = apart(mul2(add2(f[u][i], both(-lo[u])), both(inv[u])));
+            q[2 * i] = __float_as_uint(__fadd_rn(t.x, 8388608.f));
+            q[2 * i + 1] = __float_as_uint(__fadd_rn(t.y, 8388608.f));
+        }
+        codes[u] = make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410) & mask[u],
+                              __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410) & mask[u]);
+        range[u] = make_float2(lo[u], step[u]);
+    }
+}
+template <bool VEC, int L>
+__device__ __forceinline__ void store_codes(uint8_t *row, int c, int end, uint2 q) {
     if constexpr (VEC) {
-        if (c < end)
-            *reinterpret_cast<uint2 *>(codes + c) =
-                make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410) & mask,
-                           __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410) & mask);
+        if (c < end) *reinterpret_cast<uint2 *>(row) = q;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (c + i * L < end) codes[c + i * L] = (uint8_t)(q[i] & mask);
+            if (c + i * L < end) row[i * L] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
     }
-    if (store) *reinterpret_cast<float2 *>(range) = make_float2(lo, step);
 }
 
-// The elementwise kinds.  CTA (bx, by): the columns of group bx, rows in steps of all the grid's; L lanes hold a row's part of
-// the group, 32/L rows a warp.  Column sums of the GELU backward (its bias gradient) stay in registers over all rows
-// of a thread and leave as one partial per (by, column), added in a fixed order by sum_slices_kernel.  UN rows of a lane are in
-// flight at once.
+// The elementwise kinds.  CTA (bx, by): the columns of group bx, blocks of UN * ROWS rows in steps of all the grid's; L lanes
+// hold a row's part of the group, 32/L rows a warp, UN rows of a lane are in flight at once.  Column sums of the GELU
+// backward (its bias gradient) stay in registers over all rows of a thread and leave as one partial per (by, column),
+// added in a fixed order by sum_slices_kernel.  Addresses are a base that the whole CTA shares plus an offset that never
+// changes: as 64-bit products of row and column for every access they were half of all instructions.
 template <int KIND, typename T, bool VEC, int L, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 keep_kernel(const KeepArgs a) {
-    constexpr int RW = 32 / L;                                   // rows of a warp
+    constexpr int RW = 32 / L, ROWS = kKeepWarps * RW;           // rows of a warp, of the CTA
     const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, warp = threadIdx.x >> 5;
     const int g = blockIdx.x, G = gridDim.x, C = a.C;
     const int c = g * kKeepGroup + first_col<VEC>(lane);
     const int lim = min(C, (g + 1) * kKeepGroup);                // end of the group
-    const long long stride = (long long)gridDim.y * kKeepWarps * RW;
-    const T *x = static_cast<const T *>(a.x);
-    T *y = static_cast<T *>(a.y), *dx = static_cast<T *>(a.dx);
+    const int my_row = warp * RW + sub;
+    const unsigned off = (unsigned)my_row * (unsigned)C + (unsigned)c, range_off = (unsigned)my_row * (unsigned)G + (unsigned)g;
     F2 b[4], sum[4];
     if (KIND == KEEP_GELU_FWD) load_params<VEC, L>(a.bias, a.pbf16, c, lim, b);
 #pragma unroll
     for (int i = 0; i < 4; i++) sum[i] = both(0.f);
-    // whole warps leave the loop together (the groups' ranges are found with warp-wide instructions)
-    for (long long r0 = ((long long)blockIdx.y * kKeepWarps + warp) * RW; r0 < a.rows; r0 += stride * UN) {
+    // whole CTAs go round together (the groups' ranges are found with warp-wide instructions)
+    for (long long r0 = (long long)blockIdx.y * (UN * ROWS); r0 < a.rows; r0 += (long long)gridDim.y * (UN * ROWS)) {
+        const T *x = static_cast<const T *>(a.x) + r0 * C;
+        T *y = static_cast<T *>(a.y) + r0 * C, *dx = static_cast<T *>(a.dx) + r0 * C;
+        uint8_t *codes = a.codes + r0 * C;
+        float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G;
+        const int left = (int)min(a.rows - r0, (long long)(UN * ROWS));
         Raw8<T, VEC> raw[UN];
         uint2 q[UN];
         float2 range[UN];
+        int end[UN];                                             // a row past the last one has no columns
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const long long r = r0 + sub + u * stride;
-            const bool act = r < a.rows;
-            if (KIND != KEEP_RESTORE) load8<VEC, L>(x + (act ? r : 0) * C, c, act ? lim : 0, raw[u]);
+            const long long ub = (long long)(u * ROWS) * C;
+            end[u] = u * ROWS + my_row < left ? lim : 0;
+            if (KIND != KEEP_RESTORE) load8<VEC, L>(x + ub + off, c, end[u], raw[u]);
             if (KIND == KEEP_RESTORE || KIND == KEEP_GELU_BWD) {
-                q[u] = load_codes<VEC, L>(a.codes + (act ? r : 0) * C, c, act ? lim : 0);
-                range[u] = __ldg(reinterpret_cast<const float2 *>(a.ranges) + (act ? r : 0) * G + g);
+                q[u] = load_codes<VEC, L>(codes + ub + off, c, end[u]);
+                range[u] = end[u] ? __ldg(ranges + (long long)(u * ROWS) * G + range_off) : make_float2(0.f, 0.f);
             }
         }
+        if constexpr (KIND == KEEP_FWD || KIND == KEEP_GELU_FWD) {
+            F2 f[UN][4];
 #pragma unroll
-        for (int u = 0; u < UN; u++) {
-            const long long r = r0 + sub + u * stride;
-            const bool act = r < a.rows;
-            const int end = act ? lim : 0;                       // a row past the last one has no columns
-            const long long ro = (act ? r : 0) * C;
-            F2 f[4];
-            if constexpr (KIND != KEEP_RESTORE) unpack8<T, VEC>(raw[u], f);
-            if constexpr (KIND == KEEP_FWD || KIND == KEEP_GELU_FWD) {
+            for (int u = 0; u < UN; u++) {
+                unpack8<T, VEC>(raw[u], f[u]);
                 if constexpr (KIND == KEEP_GELU_FWD) {
                     F2 v[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        f[i] = add2(f[i], b[i]);
-                        v[i] = gelu_of(f[i], normal_of(f[i]));
+                        f[u][i] = add2(f[u][i], b[i]);
+                        v[i] = gelu_of(f[u][i], normal_of(f[u][i]));
                     }
-                    store8<VEC, L>(y + ro, c, end, v);
+                    store8<VEC, L>(y + (long long)(u * ROWS) * C + off, c, end[u], v);
                 }
-                if (KIND == KEEP_FWD || a.codes)
-                    keep_group<VEC, L>(f, c, end, act && lane == 0, a.codes + ro, a.ranges + ((act ? r : 0) * G + g) * 2);
-            } else {
+            }
+            if (KIND == KEEP_FWD || a.codes) {
+                keep_groups<VEC, L, UN>(f, c, end, q, range);
+#pragma unroll
+                for (int u = 0; u < UN; u++) {
+                    store_codes<VEC, L>(codes + (long long)(u * ROWS) * C + off, c, end[u], q[u]);
+                    if (end[u] && lane == 0) ranges[(long long)(u * ROWS) * G + range_off] = range[u];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
                 F2 v[4];
                 restore_codes(q[u], range[u], v);
                 if constexpr (KIND == KEEP_GELU_BWD) {
-                    F2 d[4];
+                    F2 d[4], f[4];
+                    unpack8<T, VEC>(raw[u], f);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const Normal n = normal_of(v[i]);
                         d[i] = mul2(f[i], gelu_slope(v[i], n));
-                        if (y) v[i] = gelu_of(v[i], n);
+                        sum[i] = add2(sum[i], d[i]);             // rows that do not exist add zeros; columns are never read
+                        if (a.y) v[i] = gelu_of(v[i], n);
                     }
-                    // columns that do not exist add dy = 0, unless their group is NaN; their sums are never read
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[i] = add2(sum[i], act ? d[i] : both(0.f));
-                    store8<VEC, L>(dx + ro, c, end, d);
+                    store8<VEC, L>(dx + (long long)(u * ROWS) * C + off, c, end[u], d);
                 }
-                if (KIND == KEEP_RESTORE || y) store8<VEC, L>(y + ro, c, end, v);
+                if (KIND == KEEP_RESTORE || a.y) store8<VEC, L>(y + (long long)(u * ROWS) * C + off, c, end[u], v);
             }
         }
     }
@@ -334,10 +367,11 @@ __device__ __forceinline__ void team_sum(float (&v)[NV], float (*slot)[NV], int 
 // warps, NG passes of a warp's lanes along the row.  L: lanes of a group.
 template <int LR, int TEAM, int NG> struct LnRow {
     static constexpr int L = LR < 16 ? LR : 16, PER_PASS = LR == 32 ? 2 : 1, RW = 32 / LR, TEAMS = kKeepWarps / TEAM;
-    int lane, sub, team, wt, half;                   // lane within its group; row of the warp; group of the pass
+    static constexpr int ROWS = TEAMS * RW;          // rows of a CTA
+    int lane, team, wt, half, row;                   // lane within its group; group of the pass; row of the CTA
     __device__ __forceinline__ LnRow() {
         const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
-        lane = l % L; sub = l / LR; half = LR == 32 ? l / 16 : 0; team = warp / TEAM; wt = warp % TEAM;
+        lane = l % L; half = LR == 32 ? l / 16 : 0; team = warp / TEAM; wt = warp % TEAM; row = team * RW + l / LR;
     }
     __device__ __forceinline__ int group(int j) const { return (wt * NG + j) * PER_PASS + half; }
 };
@@ -353,29 +387,32 @@ ln_keep_kernel(const LnKeepArgs a) {
     __shared__ float s1[kKeepWarps][UN], s2[kKeepWarps][UN];
     const R w;
     const int C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
-    const T *x = static_cast<const T *>(a.x);
-    T *y = static_cast<T *>(a.y);
     const float inv_c = 1.f / (float)C;
-    const long long stride = (long long)gridDim.x * R::TEAMS * R::RW;
+    const unsigned off = (unsigned)(w.row * C), range_off = (unsigned)(w.row * G);
     F2 gm[NG][4], bt[NG][4];
+    int c[NG], lim[NG];
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), lim = min(C, (g + 1) * kKeepGroup);
-        load_params<VEC, L>(a.gamma, a.pbf16, c, lim, gm[j]);
-        load_params<VEC, L>(a.beta, a.pbf16, c, lim, bt[j]);
+        const int g = w.group(j);
+        c[j] = g * kKeepGroup + first_col<VEC>(w.lane);
+        lim[j] = min(C, (g + 1) * kKeepGroup);
+        load_params<VEC, L>(a.gamma, a.pbf16, c[j], lim[j], gm[j]);
+        load_params<VEC, L>(a.beta, a.pbf16, c[j], lim[j], bt[j]);
     }
-    for (long long r0 = ((long long)blockIdx.x * R::TEAMS + w.team) * R::RW; r0 < a.rows; r0 += stride * UN) {
+    for (long long r0 = (long long)blockIdx.x * (UN * R::ROWS); r0 < a.rows; r0 += (long long)gridDim.x * (UN * R::ROWS)) {
+        const T *x = static_cast<const T *>(a.x) + r0 * C;
+        T *y = static_cast<T *>(a.y) + r0 * C;
+        uint8_t *codes = a.codes + r0 * C;
+        float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G, *stats = reinterpret_cast<float2 *>(a.stats) + r0;
+        const int left = (int)min(a.rows - r0, (long long)(UN * R::ROWS));
         Raw8<T, VEC> raw[UN][NG];
         float s[UN], mean[UN];
+        bool act[UN];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const long long r = r0 + w.sub + u * stride;
-            const bool act = r < a.rows;
+            act[u] = u * R::ROWS + w.row < left;
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const int g = w.group(j);
-                load8<VEC, L>(x + (act ? r : 0) * C, g * kKeepGroup + first_col<VEC>(w.lane), act ? min(C, (g + 1) * kKeepGroup) : 0, raw[u][j]);
-            }
+            for (int j = 0; j < NG; j++) load8<VEC, L>(x + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], act[u] ? lim[j] : 0, raw[u][j]);
         }
 #pragma unroll
         for (int u = 0; u < UN; u++) {
@@ -387,8 +424,8 @@ ln_keep_kernel(const LnKeepArgs a) {
                 const float2 t = apart(add2(add2(f[0], f[1]), add2(f[2], f[3])));
                 s[u] += t.x + t.y;
             }
-            s[u] = lane_sum<LR>(s[u]);
         }
+        lane_sums<LR, UN>(s);
         team_sum<TEAM, UN>(s, s1, w.team, w.wt);
 #pragma unroll
         for (int u = 0; u < UN; u++) {
@@ -396,43 +433,49 @@ ln_keep_kernel(const LnKeepArgs a) {
             s[u] = 0.f;
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
                 F2 f[4], sq = both(0.f);
                 unpack8<T, VEC>(raw[u][j], f);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     F2 d = add2(f[i], both(-mean[u]));
                     if (!VEC) {
-                        const int lim = min(C, (g + 1) * kKeepGroup);
                         const float2 v = apart(d);
-                        d = two(c + 2 * i * L < lim ? v.x : 0.f, c + (2 * i + 1) * L < lim ? v.y : 0.f);
+                        d = two(c[j] + 2 * i * L < lim[j] ? v.x : 0.f, c[j] + (2 * i + 1) * L < lim[j] ? v.y : 0.f);
                     }
                     sq = fma2(d, d, sq);
                 }
                 const float2 t = apart(sq);
-                if (!VEC || c < C) s[u] += t.x + t.y;
+                if (!VEC || c[j] < C) s[u] += t.x + t.y;
             }
-            s[u] = lane_sum<LR>(s[u]);
         }
+        lane_sums<LR, UN>(s);
         team_sum<TEAM, UN>(s, s2, w.team, w.wt);
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const long long r = r0 + w.sub + u * stride;
-            const bool act = r < a.rows;
-            const long long ro = (act ? r : 0) * C;
-            const float rstd = rsqrtf(s[u] * inv_c + a.eps);
-            if (act && w.lane == 0 && w.half == 0 && w.wt == 0) *reinterpret_cast<float2 *>(a.stats + r * 2) = make_float2(mean[u], rstd);
+            s[u] = rsqrtf(s[u] * inv_c + a.eps);
+            if (act[u] && w.lane == 0 && w.half == 0 && w.wt == 0) stats[u * R::ROWS + w.row] = make_float2(mean[u], s[u]);
+        }
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
-                if ((w.wt * NG + j) * R::PER_PASS >= G) break;                  // the same for the whole warp
-                const int end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-                F2 f[4], o[4];
-                unpack8<T, VEC>(raw[u][j], f);
+        for (int j = 0; j < NG; j++) {
+            if ((w.wt * NG + j) * R::PER_PASS >= G) break;                      // the same for the whole warp
+            F2 f[UN][4];
+            int end[UN];
+            uint2 q[UN];
+            float2 range[UN];
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = fma2(mul2(add2(f[i], both(-mean[u])), both(rstd)), gm[j][i], bt[j][i]);
-                store8<VEC, L>(y + ro, c, end, o);
-                keep_group<VEC, L>(f, c, end, act && w.lane == 0 && g < G, a.codes + ro, a.ranges + ((act ? r : 0) * G + (g < G ? g : 0)) * 2);
+            for (int u = 0; u < UN; u++) {
+                end[u] = act[u] ? lim[j] : 0;
+                F2 o[4];
+                unpack8<T, VEC>(raw[u][j], f[u]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = fma2(mul2(add2(f[u][i], both(-mean[u])), both(s[u])), gm[j][i], bt[j][i]);
+                store8<VEC, L>(y + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end[u], o);
+            }
+            keep_groups<VEC, L, UN>(f, c[j], end, q, range);
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
+                store_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end[u], q[u]);
+                if (act[u] && w.lane == 0 && w.group(j) < G) ranges[(long long)(u * R::ROWS) * G + (range_off + w.group(j))] = range[u];
             }
         }
     }
@@ -451,52 +494,55 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
     __shared__ float s1[2][kKeepWarps][2 * UN];
     const R w;
     const int C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
-    const T *dy = static_cast<const T *>(a.x);
-    T *dx = static_cast<T *>(a.dx), *y = static_cast<T *>(a.y);
     const float inv_c = 1.f / (float)C;
-    const long long stride = (long long)gridDim.x * R::TEAMS * R::RW;
+    const unsigned off = (unsigned)(w.row * C), range_off = (unsigned)(w.row * G);
     F2 gm[NG][4], sg[NG][4], sb[NG][4];
+    int c[NG], lim[NG];
 #pragma unroll
     for (int j = 0; j < NG; j++) {
         const int g = w.group(j);
-        load_params<VEC, L>(a.gamma, a.pbf16, g * kKeepGroup + first_col<VEC>(w.lane), min(C, (g + 1) * kKeepGroup), gm[j]);
+        c[j] = g * kKeepGroup + first_col<VEC>(w.lane);
+        lim[j] = min(C, (g + 1) * kKeepGroup);
+        load_params<VEC, L>(a.gamma, a.pbf16, c[j], lim[j], gm[j]);
 #pragma unroll
         for (int i = 0; i < 4; i++) sg[j][i] = sb[j][i] = both(0.f);
     }
     // xhat of the lane's values.  Of a group that is NaN, single columns may still not exist.
-    auto normalised = [&](uint2 q, float2 range, float2 st, int g, F2 (&h)[4]) {
+    auto normalised = [&](uint2 q, float2 range, float2 st, int j, F2 (&h)[4]) {
         restore_codes(q, range, h);
-        const int c = g * kKeepGroup + first_col<VEC>(w.lane), lim = min(C, (g + 1) * kKeepGroup);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             h[i] = mul2(add2(h[i], both(-st.x)), both(st.y));
             if (!VEC) {
                 const float2 v = apart(h[i]);
-                h[i] = two(c + 2 * i * L < lim ? v.x : 0.f, c + (2 * i + 1) * L < lim ? v.y : 0.f);
+                h[i] = two(c[j] + 2 * i * L < lim[j] ? v.x : 0.f, c[j] + (2 * i + 1) * L < lim[j] ? v.y : 0.f);
             }
         }
     };
     int turn = 0;
-    for (long long r0 = ((long long)blockIdx.x * R::TEAMS + w.team) * R::RW; r0 < a.rows; r0 += stride * UN) {
+    for (long long r0 = (long long)blockIdx.x * (UN * R::ROWS); r0 < a.rows; r0 += (long long)gridDim.x * (UN * R::ROWS)) {
+        const T *dy = static_cast<const T *>(a.x) + r0 * C;
+        T *dx = static_cast<T *>(a.dx) + r0 * C, *y = static_cast<T *>(a.y) + r0 * C;
+        const uint8_t *codes = a.codes + r0 * C;
+        const float2 *ranges = reinterpret_cast<const float2 *>(a.ranges) + r0 * G, *stats = reinterpret_cast<const float2 *>(a.stats) + r0;
+        const int left = (int)min(a.rows - r0, (long long)(UN * R::ROWS));
         Raw8<T, VEC> raw[UN][NG];
         float s[2 * UN];
         float2 st[UN], range[UN][NG];
         uint2 q[UN][NG];
+        bool act[UN];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const long long r = r0 + w.sub + u * stride;
-            const bool act = r < a.rows;
-            const long long ro = (act ? r : 0) * C;
-            st[u] = __ldg(reinterpret_cast<const float2 *>(a.stats) + (act ? r : 0));
+            act[u] = u * R::ROWS + w.row < left;
+            st[u] = act[u] ? __ldg(stats + u * R::ROWS + w.row) : make_float2(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), end = act ? min(C, (g + 1) * kKeepGroup) : 0;
-                load8<VEC, L>(dy + ro, c, end, raw[u][j]);
-                q[u][j] = load_codes<VEC, L>(a.codes + ro, c, end);
+                const int end = act[u] ? lim[j] : 0;
+                load8<VEC, L>(dy + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end, raw[u][j]);
+                q[u][j] = load_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end);
                 // (columns that do not exist: dy, gamma and this are zero, whatever their group holds)
-                range[u][j] = c < end ? __ldg(reinterpret_cast<const float2 *>(a.ranges) + r * G + g) : make_float2(0.f, 0.f);
+                range[u][j] = c[j] < end ? __ldg(ranges + (long long)(u * R::ROWS) * G + (range_off + w.group(j))) : make_float2(0.f, 0.f);
             }
-            if (!act) st[u] = make_float2(0.f, 0.f);
         }
 #pragma unroll
         for (int u = 0; u < UN; u++) {
@@ -504,7 +550,7 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 F2 d[4], h[4];
-                normalised(q[u][j], range[u][j], st[u], w.group(j), h);
+                normalised(q[u][j], range[u][j], st[u], j, h);
                 unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -517,33 +563,29 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
             }
             s[2 * u] = apart(t1).x + apart(t1).y;
             s[2 * u + 1] = apart(t2).x + apart(t2).y;
-            s[2 * u] = lane_sum<LR>(s[2 * u]);
-            s[2 * u + 1] = lane_sum<LR>(s[2 * u + 1]);
         }
+        lane_sums<LR, 2 * UN>(s);
         team_sum<TEAM, 2 * UN>(s, s1[turn], w.team, w.wt);
         turn ^= 1;
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const long long r = r0 + w.sub + u * stride;
-            const bool act = r < a.rows;
-            const long long ro = (act ? r : 0) * C;
             const float c1 = s[2 * u] * inv_c, c2 = s[2 * u + 1] * inv_c;
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane), end = act ? min(C, (g + 1) * kKeepGroup) : 0;
+                const int end = act[u] ? lim[j] : 0;
                 F2 d[4], h[4], o[4];
-                normalised(q[u][j], range[u][j], st[u], g, h);
+                normalised(q[u][j], range[u][j], st[u], j, h);
                 unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     o[i] = mul2(fma2(h[i], both(-c2), fma2(d[i], gm[j][i], both(-c1))), both(st[u].y));
-                store8<VEC, L>(dx + ro, c, end, o);
-                if (y) {
+                store8<VEC, L>(dx + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end, o);
+                if (a.y) {
                     F2 bt[4];
-                    load_params<VEC, L>(a.beta, a.pbf16, c, end, bt);
+                    load_params<VEC, L>(a.beta, a.pbf16, c[j], end, bt);
 #pragma unroll
                     for (int i = 0; i < 4; i++) o[i] = fma2(h[i], gm[j][i], bt[i]);
-                    store8<VEC, L>(y + ro, c, end, o);
+                    store8<VEC, L>(y + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end, o);
                 }
             }
         }
@@ -551,17 +593,16 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
     float *out = a.partial + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        const int g = w.group(j), c = g * kKeepGroup + first_col<VEC>(w.lane);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int k = col_of<VEC, L>(c, i);
+            const int k = col_of<VEC, L>(c[j], i);
             float tg = i & 1 ? apart(sg[j][i >> 1]).y : apart(sg[j][i >> 1]).x, tb = i & 1 ? apart(sb[j][i >> 1]).y : apart(sb[j][i >> 1]).x;
 #pragma unroll
             for (int o = LR; o < 32; o <<= 1) {
                 tg += __shfl_xor_sync(0xffffffffu, tg, o);
                 tb += __shfl_xor_sync(0xffffffffu, tb, o);
             }
-            if (w.sub == 0 && k < min(C, (g + 1) * kKeepGroup)) {
+            if (w.row % R::RW == 0 && k < lim[j]) {
                 float *to = R::TEAMS > 1 ? ln_cols + (size_t)w.team * 2 * C : out;
                 to[k] = tg;
                 to[C + k] = tb;

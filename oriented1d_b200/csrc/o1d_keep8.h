@@ -8,6 +8,7 @@ namespace o1d {
 
 constexpr int kKeepGroup = 128;          // columns that share a range
 constexpr int kKeepMaxRow = 8192;        // longest row of the LayerNorm kernels
+constexpr int kKeepMaxColumns = 1 << 24; // and of the elementwise ones (32-bit offsets within a block of rows)
 
 enum : int { KEEP_FWD = 0, KEEP_RESTORE, KEEP_GELU_FWD, KEEP_GELU_BWD };
 

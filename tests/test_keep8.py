@@ -315,6 +315,7 @@ def test_entry_points_reject_bad_arguments():
     assert lib.o1d_keep8(p, p, p, 0, 8, 0, None) == 1
     assert lib.o1d_keep8(p, p, p, 1, 8, 2, None) == 1
     assert lib.o1d_keep8(p, p, p + 4, 1, 8, 0, None) == 2
+    assert lib.o1d_keep8(p, p, p, 1, 2 ** 24 + 1, 0, None) == 2
     assert lib.o1d_restore8(p, None, p, 1, 8, 0, None) == 1
     assert lib.o1d_gelu_keep8(p, None, p, p, None, 1, 8, 0, None) == 1          # codes without ranges
     assert lib.o1d_gelu_keep8_bwd(p, p, p, None, None, None, None, 0, 1, 8, 0, None) == 1

@@ -207,11 +207,11 @@ __device__ __forceinline__ void keep_groups(const F2 (&f)[U][4], int c, const in
         lo[u] = upper ? send[u] : m[u];
         const float hi = -(upper ? m[u] : send[u]);
         step[u] = __fmul_rn(__fsub_rn(hi, lo[u]), 1.f / 255.f);
-        inv[u] = 0.f;
-        mask[u] = 0xffffffffu;
-        if (!(step[u] <= 3.402823466e38f)) { step[u] = __int_as_float(0x7fffffff); mask[u] = 0u; }        // NaN or infinite: the group is lost
-        else if (step[u] < 1.175494351e-38f) step[u] = 0.f;
-        else inv[u] = __frcp_rn(step[u]);
+        const bool lost = !(step[u] <= 3.402823466e38f), some = step[u] >= 1.175494351e-38f;        // (neither, either, not both)
+        inv[u] = __frcp_rn(fmaxf(step[u], 1.175494351e-38f));
+        inv[u] = some && !lost ? inv[u] : 0.f;
+        step[u] = lost ? __int_as_float(0x7fffffff) : some ? step[u] : 0.f;
+        mask[u] = lost ? 0u : 0xffffffffu;                            // a NaN or an infinity: the group is lost
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -259,27 +259,42 @@ keep_kernel(const KeepArgs a) {
     if (KIND == KEEP_GELU_FWD) load_params<VEC, L>(a.bias, a.pbf16, c, lim, b);
 #pragma unroll
     for (int i = 0; i < 4; i++) sum[i] = both(0.f);
-    // whole CTAs go round together (the groups' ranges are found with warp-wide instructions)
-    for (long long r0 = (long long)blockIdx.y * (UN * ROWS); r0 < a.rows; r0 += (long long)gridDim.y * (UN * ROWS)) {
-        const T *x = static_cast<const T *>(a.x) + r0 * C;
-        T *y = static_cast<T *>(a.y) + r0 * C, *dx = static_cast<T *>(a.dx) + r0 * C;
-        uint8_t *codes = a.codes + r0 * C;
-        float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G;
-        const int left = (int)min(a.rows - r0, (long long)(UN * ROWS));
+    struct Rows {
         Raw8<T, VEC> raw[UN];
         uint2 q[UN];
         float2 range[UN];
-        int end[UN];                                             // a row past the last one has no columns
+    };
+    // end of the row part of round r0, row u: a row past the last one has no columns
+    auto row_end = [&](long long r0, int u) { return my_row < a.rows - r0 - u * ROWS ? lim : 0; };
+    auto load = [&](long long r0, Rows &w) {
+        const T *x = static_cast<const T *>(a.x) + r0 * C;
+        const uint8_t *codes = a.codes + r0 * C;
+        const float2 *ranges = reinterpret_cast<const float2 *>(a.ranges) + r0 * G;
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const long long ub = (long long)(u * ROWS) * C;
-            end[u] = u * ROWS + my_row < left ? lim : 0;
-            if (KIND != KEEP_RESTORE) load8<VEC, L>(x + ub + off, c, end[u], raw[u]);
+            const int end = row_end(r0, u);
+            if (KIND != KEEP_RESTORE) load8<VEC, L>(x + (long long)(u * ROWS) * C + off, c, end, w.raw[u]);
             if (KIND == KEEP_RESTORE || KIND == KEEP_GELU_BWD) {
-                q[u] = load_codes<VEC, L>(codes + ub + off, c, end[u]);
-                range[u] = end[u] ? __ldg(ranges + (long long)(u * ROWS) * G + range_off) : make_float2(0.f, 0.f);
+                w.q[u] = load_codes<VEC, L>(codes + (long long)(u * ROWS) * C + off, c, end);
+                w.range[u] = end ? __ldg(ranges + (long long)(u * ROWS) * G + range_off) : make_float2(0.f, 0.f);
             }
         }
+    };
+    // Whole CTAs go round together (the groups' ranges are found with warp-wide instructions).  The next round's values are
+    // on their way while this one's are worked on.
+    Rows next;
+    const long long round = (long long)gridDim.y * (UN * ROWS);
+    load((long long)blockIdx.y * (UN * ROWS), next);
+    for (long long r0 = (long long)blockIdx.y * (UN * ROWS); r0 < a.rows; r0 += round) {
+        T *y = static_cast<T *>(a.y) + r0 * C, *dx = static_cast<T *>(a.dx) + r0 * C;
+        uint8_t *codes = a.codes + r0 * C;
+        float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G;
+        const Rows now = next;
+        load(r0 + round, next);
+        const Raw8<T, VEC> (&raw)[UN] = now.raw;
+        int end[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++) end[u] = row_end(r0, u);
         if constexpr (KIND == KEEP_FWD || KIND == KEEP_GELU_FWD) {
             F2 f[UN][4];
 #pragma unroll
@@ -296,6 +311,8 @@ keep_kernel(const KeepArgs a) {
                 }
             }
             if (KIND == KEEP_FWD || a.codes) {
+                uint2 q[UN];
+                float2 range[UN];
                 keep_groups<VEC, L, UN>(f, c, end, q, range);
 #pragma unroll
                 for (int u = 0; u < UN; u++) {
@@ -307,7 +324,7 @@ keep_kernel(const KeepArgs a) {
 #pragma unroll
             for (int u = 0; u < UN; u++) {
                 F2 v[4];
-                restore_codes(q[u], range[u], v);
+                restore_codes(now.q[u], now.range[u], v);
                 if constexpr (KIND == KEEP_GELU_BWD) {
                     F2 d[4], f[4];
                     unpack8<T, VEC>(raw[u], f);

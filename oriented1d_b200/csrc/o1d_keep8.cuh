@@ -416,21 +416,31 @@ ln_keep_kernel(const LnKeepArgs a) {
         load_params<VEC, L>(a.gamma, a.pbf16, c[j], lim[j], gm[j]);
         load_params<VEC, L>(a.beta, a.pbf16, c[j], lim[j], bt[j]);
     }
-    for (long long r0 = (long long)blockIdx.x * (UN * R::ROWS); r0 < a.rows; r0 += (long long)gridDim.x * (UN * R::ROWS)) {
+    struct Rows { Raw8<T, VEC> raw[UN][NG]; };
+    auto exists = [&](long long r0, int u) { return w.row < a.rows - r0 - u * R::ROWS; };
+    auto load = [&](long long r0, Rows &to) {
         const T *x = static_cast<const T *>(a.x) + r0 * C;
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+#pragma unroll
+            for (int j = 0; j < NG; j++)
+                load8<VEC, L>(x + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], exists(r0, u) ? lim[j] : 0, to.raw[u][j]);
+    };
+    // the next round's rows are on their way while this one's are worked on
+    Rows next;
+    const long long round = (long long)gridDim.x * (UN * R::ROWS);
+    load((long long)blockIdx.x * (UN * R::ROWS), next);
+    for (long long r0 = (long long)blockIdx.x * (UN * R::ROWS); r0 < a.rows; r0 += round) {
         T *y = static_cast<T *>(a.y) + r0 * C;
         uint8_t *codes = a.codes + r0 * C;
         float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G, *stats = reinterpret_cast<float2 *>(a.stats) + r0;
-        const int left = (int)min(a.rows - r0, (long long)(UN * R::ROWS));
-        Raw8<T, VEC> raw[UN][NG];
+        const Rows now = next;
+        load(r0 + round, next);
+        const Raw8<T, VEC> (&raw)[UN][NG] = now.raw;
         float s[UN], mean[UN];
         bool act[UN];
 #pragma unroll
-        for (int u = 0; u < UN; u++) {
-            act[u] = u * R::ROWS + w.row < left;
-#pragma unroll
-            for (int j = 0; j < NG; j++) load8<VEC, L>(x + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], act[u] ? lim[j] : 0, raw[u][j]);
-        }
+        for (int u = 0; u < UN; u++) act[u] = exists(r0, u);
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             s[u] = 0.f;
@@ -536,31 +546,48 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
             }
         }
     };
-    int turn = 0;
-    for (long long r0 = (long long)blockIdx.x * (UN * R::ROWS); r0 < a.rows; r0 += (long long)gridDim.x * (UN * R::ROWS)) {
-        const T *dy = static_cast<const T *>(a.x) + r0 * C;
-        T *dx = static_cast<T *>(a.dx) + r0 * C, *y = static_cast<T *>(a.y) + r0 * C;
-        const uint8_t *codes = a.codes + r0 * C;
-        const float2 *ranges = reinterpret_cast<const float2 *>(a.ranges) + r0 * G, *stats = reinterpret_cast<const float2 *>(a.stats) + r0;
-        const int left = (int)min(a.rows - r0, (long long)(UN * R::ROWS));
+    struct Rows {
         Raw8<T, VEC> raw[UN][NG];
-        float s[2 * UN];
         float2 st[UN], range[UN][NG];
         uint2 q[UN][NG];
-        bool act[UN];
+    };
+    auto exists = [&](long long r0, int u) { return w.row < a.rows - r0 - u * R::ROWS; };
+    auto load = [&](long long r0, Rows &to) {
+        const T *dy = static_cast<const T *>(a.x) + r0 * C;
+        const uint8_t *codes = a.codes + r0 * C;
+        const float2 *ranges = reinterpret_cast<const float2 *>(a.ranges) + r0 * G, *stats = reinterpret_cast<const float2 *>(a.stats) + r0;
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            act[u] = u * R::ROWS + w.row < left;
-            st[u] = act[u] ? __ldg(stats + u * R::ROWS + w.row) : make_float2(0.f, 0.f);
+            const bool on = exists(r0, u);
+            to.st[u] = on ? __ldg(stats + u * R::ROWS + w.row) : make_float2(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const int end = act[u] ? lim[j] : 0;
-                load8<VEC, L>(dy + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end, raw[u][j]);
-                q[u][j] = load_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end);
+                const int end = on ? lim[j] : 0;
+                load8<VEC, L>(dy + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end, to.raw[u][j]);
+                to.q[u][j] = load_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end);
                 // (columns that do not exist: dy, gamma and this are zero, whatever their group holds)
-                range[u][j] = c[j] < end ? __ldg(ranges + (long long)(u * R::ROWS) * G + (range_off + w.group(j))) : make_float2(0.f, 0.f);
+                to.range[u][j] = c[j] < end ? __ldg(ranges + (long long)(u * R::ROWS) * G + (range_off + w.group(j))) : make_float2(0.f, 0.f);
             }
         }
+    };
+    // the next round's rows are on their way while this one's are worked on, where there are registers for both
+    constexpr bool AHEAD = NG * UN <= 2;
+    Rows next;
+    const long long round = (long long)gridDim.x * (UN * R::ROWS);
+    if (AHEAD) load((long long)blockIdx.x * (UN * R::ROWS), next);
+    int turn = 0;
+    for (long long r0 = (long long)blockIdx.x * (UN * R::ROWS); r0 < a.rows; r0 += round) {
+        T *dx = static_cast<T *>(a.dx) + r0 * C, *y = static_cast<T *>(a.y) + r0 * C;
+        if (!AHEAD) load(r0, next);
+        const Rows now = next;
+        if (AHEAD) load(r0 + round, next);
+        const Raw8<T, VEC> (&raw)[UN][NG] = now.raw;
+        const float2 (&st)[UN] = now.st, (&range)[UN][NG] = now.range;
+        const uint2 (&q)[UN][NG] = now.q;
+        float s[2 * UN];
+        bool act[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++) act[u] = exists(r0, u);
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             F2 t1 = both(0.f), t2 = both(0.f);

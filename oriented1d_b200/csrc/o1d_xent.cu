@@ -7,9 +7,12 @@ namespace o1d {
 
 namespace {
 
-// Bytes of G that are held at once: about half the L2 cache, so that the two products that read a piece find it there.
-constexpr long long kPieceBytes = 64ll << 20;
+// Bytes of G that are held at once.  Larger pieces have fewer waves that end half empty and fewer rounds of adding to fp32
+// sums, which is worth more than finding a piece in the L2 cache; 4096 x 1024 x 21841 bf16, gradient alone: 40 MB 557 us,
+// 80 MB 512, 128 MB 489, all 179 MB in one piece 452.
+constexpr long long kPieceBytes = 128ll << 20;
 constexpr int kMinSplitSteps = 8;                // K steps that a part of a split axis has at least
+constexpr int kSlicesAtOnce = 512;               // column sums of more slices are added in two steps
 
 inline long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -47,6 +50,15 @@ int encode(CUtensorMap *map, const Mat &m, int box_rows) {
     return (int)r;
 }
 
+// Columns of a tile: 256 reads a third less for each product, 128 wastes less of a narrow matrix and gives twice the tiles.  Waves of
+// tiles times their steps, a step of 128 columns being 0.6 of one of 256 (measured: 0.25 and 0.42 us).
+int width_of(long long m, long long n, long long k, bool split, int sms) {
+    if (split) return 128;
+    const long long steps = cdiv(k, kXK) + 6, wide = cdiv((long long)cdiv(m, kXM) * cdiv(n, 256), sms) * steps * 5,
+                    narrow = cdiv((long long)cdiv(m, kXM) * cdiv(n, 128), sms) * steps * 3;
+    return narrow < wide ? 128 : 256;
+}
+
 struct Run {                 // of one call
     const XentArgs &a;
     int sms, *err_flag;
@@ -56,14 +68,21 @@ struct Run {                 // of one call
     int fail(cudaError_t e) { *cuda = e; return O1D_ERR_CUDA; }
 
     template <int KIND, bool SPLIT>
-    int product(const Mat &ma, const Mat &mb, XentParams p) {
-        using S = XentShape<SPLIT>;
+    int product(const Mat &ma, const Mat &mb, const XentParams &p) {
+        constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
+        if constexpr (!SPLIT)
+            if (width_of(A_MN ? ma.cols : ma.rows, B_MN ? mb.cols : mb.rows, A_MN ? ma.rows : ma.cols, false, sms) == 256) return run<KIND, false, 256>(ma, mb, p);
+        return run<KIND, SPLIT, 128>(ma, mb, p);
+    }
+    template <int KIND, bool SPLIT, int BN>
+    int run(const Mat &ma, const Mat &mb, XentParams p) {
+        using S = XentShape<SPLIT, BN>;
         constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
         CUtensorMap a_map, b_map;
-        if ((*enc = encode(&a_map, ma, A_MN ? kXK : kXM)) || (*enc = encode(&b_map, mb, B_MN ? kXK : S::BN))) return O1D_ERR_CUDA;
+        if ((*enc = encode(&a_map, ma, A_MN ? kXK : kXM)) || (*enc = encode(&b_map, mb, B_MN ? kXK : BN))) return O1D_ERR_CUDA;
         p.M = (int)(A_MN ? ma.cols : ma.rows);
         p.N = (int)(B_MN ? mb.cols : mb.rows);
-        const long long m_tiles = cdiv(p.M, kXM), n_tiles = cdiv(p.N, S::BN);
+        const long long m_tiles = cdiv(p.M, kXM), n_tiles = cdiv(p.N, BN);
         p.k_steps = cdiv(A_MN ? ma.rows : ma.cols, kXK);
         if (p.splits < 1) p.splits = 1;
         if (m_tiles * n_tiles * p.splits > 0x7fffffff) return O1D_ERR_UNSUPPORTED;
@@ -71,7 +90,7 @@ struct Run {                 // of one call
         p.n_tiles = (int)n_tiles;
         p.tiles = p.m_tiles * p.n_tiles * p.splits;
         p.err_flag = err_flag;
-        auto kern = xent_kernel<KIND, SPLIT>;
+        auto kern = xent_kernel<KIND, SPLIT, BN>;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
         if (e != cudaSuccess) return fail(e);
         kern<<<p.tiles < sms ? p.tiles : sms, kXThreads, S::SMEM, st>>>(a_map, b_map, p);
@@ -109,8 +128,8 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
 }
 
 // Forward: CTAs that a row tile's vocabulary is spread over, at most.
-int forward_slots(long long N, int V, bool bf16, int sms) {
-    const long long n_tiles = cdiv(V, bf16 ? 256 : 128), tiles = cdiv(N, kXM) * n_tiles;
+int forward_slots(long long N, int D, int V, bool bf16, int sms) {
+    const long long n_tiles = cdiv(V, width_of(N, V, D, !bf16, sms)), tiles = cdiv(N, kXM) * n_tiles;
     const long long ctas = tiles < sms ? tiles : sms, least = tiles / ctas;
     return 2 * (int)(cdiv(n_tiles, least) + 1);
 }
@@ -122,36 +141,64 @@ struct Cut {
     int pieces, ld;          // ld: columns of G in memory
     long long rows;          // rows of a piece
     int dx_parts, dw_parts;  // fp32 sums; 0: the product writes its result
-    int col_slices;
+    int col_blocks() const { return cdiv(cdiv(rows, 32), kSlicesAtOnce); }
+    bool col_once() const { return pieces == 1 && col_blocks() == 1; }
 };
-int parts_of(long long m, long long n, long long k, int bn, int sms, bool adds) {
+int parts_of(long long m, long long n, long long k, bool split, int sms, bool adds) {
+    const int bn = width_of(m, n, k, split, sms);
     const long long tiles = (long long)cdiv(m, kXM) * cdiv(n, bn), steps = cdiv(k, kXK);
     long long s = sms / tiles;
     if (s > steps / kMinSplitSteps) s = steps / kMinSplitSteps;
     if (s < 1) s = 1;
     return s == 1 && !adds ? 0 : (int)s;
 }
+// Time of a cut in units of one K step of one tile (0.4 us): waves of tiles times their steps, which an epilogue of
+// about six steps bounds from below, and six steps for each launch to begin and end.
+long long cost_of(const XentArgs &a, bool by_rows, long long piece, int sms, int bn) {
+    const long long axis = by_rows ? a.N : a.V;
+    long long total = 0;
+    auto waves = [&](long long tiles, long long steps) { return (tiles + sms - 1) / sms * (steps < 6 ? 6 : steps) + 6; };
+    auto one = [&](long long n) {
+        const long long rows = by_rows ? n : a.N, cols = by_rows ? a.V : n, m = cdiv(rows, kXM), d = cdiv(a.D, bn);
+        return waves(m * cdiv(cols, bn), cdiv(a.D, kXK)) + waves(m * d, cdiv(cols, kXK)) + waves(cdiv(cols, kXM) * d, cdiv(rows, kXK));
+    };
+    total = axis / piece * one(piece);
+    if (axis % piece) total += one(axis % piece);
+    return total;
+}
 Cut cut_of(const XentArgs &a, int sms) {
     const int bn = a.bf16 ? 256 : 128, planes = a.bf16 ? 1 : 3;
     Cut c;
     c.by_rows = a.N > a.V;
     const long long all_ld = up_to(a.V, 64), axis = c.by_rows ? a.N : a.V;
-    long long most = c.by_rows ? kPieceBytes / (2 * planes * all_ld) / kXM * kXM : kPieceBytes / (2 * planes * a.N) / 256 * 256;
+    long long most = kPieceBytes / (2 * planes * (c.by_rows ? all_ld : a.N)) / 256 * 256;
     if (most < 256) most = 256;
-    c.pieces = cdiv(axis, most);
-    c.piece = c.pieces == 1 ? axis : up_to(cdiv(axis, c.pieces), 256);
+    c.piece = axis;
+    if (axis > most) {
+        // equal pieces, or such as make whole waves of the tiles along the cut axis: whichever costs least
+        long long best = 0;
+        auto consider = [&](long long p) {
+            if (p < 256 || p > most) return;
+            const long long t = cost_of(a, c.by_rows, p, sms, bn);
+            if (!best || t < best) { best = t; c.piece = p; }
+        };
+        const long long least = (axis + most - 1) / most;
+        for (long long k = least; k < least + 3; k++) consider(up_to((axis + k - 1) / k, 256));
+        const long long d = cdiv(a.D, bn);
+        for (int w = 1; w <= 4; w++) {
+            consider(w * sms / d * kXM / 256 * 256);
+            if (!c.by_rows) consider(w * sms / cdiv(a.N, kXM) * bn / 256 * 256);
+        }
+        if (!best) c.piece = most;
+    }
     c.pieces = cdiv(axis, c.piece);
     c.ld = (int)(c.by_rows ? all_ld : up_to(c.piece, 64));
     c.rows = c.by_rows ? c.piece : a.N;
-    c.dx_parts = parts_of(c.rows, a.D, c.by_rows ? a.V : c.piece, bn, sms, !c.by_rows && c.pieces > 1);
-    c.dw_parts = parts_of(c.by_rows ? a.V : c.piece, a.D, c.rows, bn, sms, c.by_rows && c.pieces > 1);
-    const int col_blocks = cdiv(c.ld, 256);
-    long long s = cdiv(4ll * sms, col_blocks);
-    if (s > cdiv(c.rows, 32)) s = cdiv(c.rows, 32);
-    c.col_slices = (int)s;
+    c.dx_parts = parts_of(c.rows, a.D, c.by_rows ? a.V : c.piece, !a.bf16, sms, !c.by_rows && c.pieces > 1);
+    c.dw_parts = parts_of(c.by_rows ? a.V : c.piece, a.D, c.rows, !a.bf16, sms, c.by_rows && c.pieces > 1);
     return c;
 }
-struct BackwardBytes { size_t x, w, g, dx, dw, col; };
+struct BackwardBytes { size_t x, w, g, dx, dw, col, more; };
 BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
     const int planes = a.bf16 ? 1 : 3;
     BackwardBytes b;
@@ -161,7 +208,9 @@ BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
     // by rows, dx is complete with its piece; by vocabulary, dw is
     b.dx = (size_t)up_to(4ll * c.dx_parts * c.rows * a.D, 256);
     b.dw = (size_t)up_to(4ll * c.dw_parts * (c.by_rows ? a.V : c.piece) * a.D, 256);
-    b.col = (size_t)up_to(4ll * (c.by_rows ? c.pieces : 1) * c.col_slices * up_to(a.V, 64), 256);
+    // column sums of a piece, in slices of 32 rows; and of all pieces, in slices of kSlicesAtOnce of those
+    b.col = (size_t)up_to(4ll * cdiv(c.rows, 32) * c.ld, 256);
+    b.more = (size_t)up_to(4ll * c.col_blocks() * (c.by_rows ? c.pieces : 1) * up_to(a.V, 64), 256);
     return b;
 }
 
@@ -173,7 +222,7 @@ int forward(Run &r) {
     int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
     if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
     if (rc) return rc;
-    const int slots = forward_slots(a.N, a.V, a.bf16, r.sms);
+    const int slots = forward_slots(a.N, a.D, a.V, a.bf16, r.sms);
     XentParams p{};
     p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
     p.part = (float2 *)ws; ws += up_to(8ll * slots * a.N, 256);
@@ -184,7 +233,7 @@ int forward(Run &r) {
     p.part_rows = a.N;
     rc = r.product<XENT_LOGITS, SPLIT>(x, w, p);
     if (rc) return rc;
-    const int n_tiles = cdiv(a.V, XentShape<SPLIT>::BN), tiles = cdiv(a.N, kXM) * n_tiles, blocks = cdiv(a.N, 256);
+    const int n_tiles = cdiv(a.V, width_of(a.N, a.V, a.D, SPLIT, r.sms)), tiles = cdiv(a.N, kXM) * n_tiles, blocks = cdiv(a.N, 256);
     const bool each = a.reduction == O1D_XENT_NONE;
     xent_rows_kernel<<<blocks, 256, 0, r.st>>>(p.part, p.part_sum, p.target_logit, a.target, a.ignore, a.smoothing, a.V, a.N, a.N, n_tiles, tiles,
                                                tiles < r.sms ? tiles : r.sms, a.lse, each ? a.loss : nullptr, each ? nullptr : sums);
@@ -197,12 +246,11 @@ int forward(Run &r) {
 }
 
 template <typename T>
-cudaError_t finish(const float *sums, void *out, long long n, int slots, const float *up, const float *count, float f, int sms, cudaStream_t st) {
-    const long long blocks = (n + 255) / 256;
-    xent_finish_kernel<T><<<(int)(blocks < sms * 16ll ? blocks : sms * 16ll), 256, 0, st>>>(sums, (T *)out, n, slots, up, count, f);
+cudaError_t finish(const float *sums, void *out, long long n, int slots, const float *up, const float *count, float f, cudaStream_t st) {
+    if (slots > 4) xent_finish_kernel<T><<<cdiv(n, 32), dim3(32, 8), 0, st>>>(sums, (T *)out, n, slots, up, count, f);
+    else xent_finish_few_kernel<T><<<cdiv(n, 1024), 256, 0, st>>>(sums, (T *)out, n, slots, up, count, f);
     return cudaGetLastError();
 }
-
 template <bool SPLIT>
 int backward(Run &r) {
     const XentArgs &a = r.a;
@@ -214,6 +262,7 @@ int backward(Run &r) {
     float *dxs = (float *)ws; ws += b.dx;
     float *dws = (float *)ws; ws += b.dw;
     float *cols = (float *)ws; ws += b.col;
+    float *more = (float *)ws; ws += b.more;
     Mat x, w;
     int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
     if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
@@ -236,9 +285,10 @@ int backward(Run &r) {
     };
     auto end = [&](int parts, float *sums, void *result, long long elems) {
         if (!parts) return cudaSuccess;
-        return a.bf16 ? finish<__nv_bfloat16>(sums, result, elems, parts, up, count, f, r.sms, r.st)
-                      : finish<float>(sums, result, elems, parts, up, count, f, r.sms, r.st);
+        return a.bf16 ? finish<__nv_bfloat16>(sums, result, elems, parts, up, count, f, r.st)
+                      : finish<float>(sums, result, elems, parts, up, count, f, r.st);
     };
+    int more_slices = 0;
     for (int i = 0; i < c.pieces; i++) {
         const long long at = i * c.piece, axis = c.by_rows ? a.N : a.V, n = axis - at < c.piece ? axis - at : c.piece;
         const long long row0 = c.by_rows ? at : 0, rows = c.by_rows ? n : a.N;
@@ -251,6 +301,7 @@ int backward(Run &r) {
         p.lse = a.lse + row0; p.up = each ? a.dloss + row0 : nullptr;
         p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
         p.g = g; p.g_plane = gm.plane; p.g_ld = ld;
+        p.cols = a.db ? cols : nullptr; p.cols_ld = ld;
         // exp(l - lse) / f = exp2(l2 - (lse2 + log2 f))
         if ((rc = r.product<XENT_GRAD, SPLIT>(xs, wp, p))) return rc;
         cudaError_t e = cudaSuccess;
@@ -271,15 +322,20 @@ int backward(Run &r) {
             if (!c.by_rows || i == c.pieces - 1) e = end(c.dw_parts, dws, to, (long long)colsn * a.D);
         }
         if (e == cudaSuccess && a.db) {
-            xent_colsum_kernel<<<dim3(cdiv(ld, 256), c.col_slices), 256, 0, r.st>>>(g, gm.plane, gm.planes, (int)rows, ld,
-                                                                                    cols + (long long)(c.by_rows ? i : 0) * c.col_slices * part_ld + col0, (int)part_ld);
+            const int slices = cdiv(rows, 32);
+            if (c.col_once())
+                xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(cols, ld, slices, slices, a.db, a.bias_bf16, nullptr, 0, a.V, up, count, f);
+            else
+                xent_bias_kernel<<<dim3(cdiv(colsn, 32), cdiv(slices, kSlicesAtOnce)), dim3(32, 32), 0, r.st>>>(
+                    cols, ld, slices, kSlicesAtOnce, nullptr, 0, more + (long long)(c.by_rows ? i : 0) * c.col_blocks() * part_ld + col0, part_ld, colsn, nullptr,
+                    nullptr, 1.f);
+            more_slices = c.by_rows ? i * c.col_blocks() + cdiv(slices, kSlicesAtOnce) : c.col_blocks();
             e = cudaGetLastError();
         }
         if (e != cudaSuccess) return r.fail(e);
     }
-    if (a.db) {
-        xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(cols, (int)part_ld, (c.by_rows ? c.pieces : 1) * c.col_slices, a.db, a.bias_bf16, a.V,
-                                                                   up, count, f);
+    if (a.db && !c.col_once()) {
+        xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(more, part_ld, more_slices, more_slices, a.db, a.bias_bf16, nullptr, 0, a.V, up, count, f);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return r.fail(e);
     }
@@ -291,9 +347,9 @@ int backward(Run &r) {
 size_t xent_workspace(const XentArgs &a, bool back, int sms) {
     if (back) {
         const BackwardBytes b = backward_bytes(a, cut_of(a, sms));
-        return b.x + b.w + b.g + b.dx + b.dw + b.col;
+        return b.x + b.w + b.g + b.dx + b.dw + b.col + b.more;
     }
-    const int slots = forward_slots(a.N, a.V, a.bf16, sms);
+    const int slots = forward_slots(a.N, a.D, a.V, a.bf16, sms);
     return operand_bytes(a.N, a.D, a.bf16) + operand_bytes(a.V, a.D, a.bf16) + (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) +
            up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 256), 256));
 }

@@ -32,8 +32,10 @@ constexpr int kXM = 128, kXK = 64;               // tile rows; K elements of a s
 constexpr int kXThreads = 384;                   // warp 0 loads, 1 multiplies, 2 owns tensor memory, 4-11 finish tiles
 constexpr int kXStaging = 2048;                  // bytes of a warp's store buffer: 32 rows of 64 bytes
 constexpr int kXChunk = 4;                       // fp32: stages of one accumulation
-template <bool SPLIT> struct XentShape {
-    static constexpr int BN = SPLIT ? 128 : 256, PL = SPLIT ? 3 : 1, STAGES = SPLIT ? 2 : 4;
+// Tiles of 256 columns, or of 128: fp32 (its two accumulators would not fit twice), and bf16 products of few columns or too
+// few tiles to go round (see width_of in o1d_xent.cu).
+template <bool SPLIT, int BN_> struct XentShape {
+    static constexpr int BN = BN_, PL = SPLIT ? 3 : 1, STAGES = SPLIT ? 2 : BN == 256 ? 4 : 6;
     static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = BN * kXK * 2, STAGE = PL * (A_BYTES + B_BYTES);
     static constexpr int SMEM = STAGES * STAGE + 8 * kXStaging + 8 * (BN / 2) * (int)sizeof(float) + 256 + 1024;
 };
@@ -60,6 +62,8 @@ struct XentParams {
     __nv_bfloat16 *g;
     long long g_plane;           // elements of a plane of G
     int g_ld;
+    float *cols;                 // [rows / 32][cols_ld] column sums of G, or null
+    long long cols_ld;
     // OUT
     void *out;                   // dx or dw (rows of N elements), or the fp32 sums of split 0
     long long split_elems;       // elements of one split's sums
@@ -127,12 +131,28 @@ __device__ __forceinline__ float take_bf16(float &v) {
     return r;
 }
 
-template <int KIND, bool SPLIT>
+// Sums over the warp's lanes of 32 values each: lane i gets the sum of value i.  Each step exchanges half of what is left
+// (31 shuffles; 32 sums one after the other would be 160).  All lanes add in the same fixed order.
+__device__ __forceinline__ float column_sums(const float (&a)[32], int lane) {
+    float t[16];
+    const bool u = lane & 16;
+#pragma unroll
+    for (int i = 0; i < 16; i++) t[i] = (u ? a[i + 16] : a[i]) + __shfl_xor_sync(0xffffffffu, u ? a[i] : a[i + 16], 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        const bool v = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; i++) t[i] = (v ? t[i + o] : t[i]) + __shfl_xor_sync(0xffffffffu, v ? t[i] : t[i + o], o);
+    }
+    return t[0];
+}
+
+template <int KIND, bool SPLIT, int BN>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XentParams p) {
-    using S = XentShape<SPLIT>;
+    using S = XentShape<SPLIT, BN>;
     constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
-    constexpr int BN = S::BN, HALF = BN / 2, PIECES = HALF / 32;
+    constexpr int HALF = BN / 2, PIECES = HALF / 32;
     constexpr uint32_t INSTR = tc::instruction<BN, A_MN, B_MN>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *smem = raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u);
@@ -251,7 +271,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         float *bs = bias_s + (warp - 4) * HALF;
         char *stage = staging + (warp - 4) * kXStaging;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * HALF;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * 32;      // every second piece of 32 columns
         int acc = 0, m_now = -1;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -271,6 +291,29 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             if (p.smooth) p.part_sum[(long long)slot * p.part_rows + row] = total;
         };
 
+        // What a tile needs from memory, fetched while the one before it is worked on.  Bias in units of log2; -inf where the
+        // vocabulary ends, so that those columns weigh nothing.
+        struct Ahead { long long tgt; float lse, scale, bias[HALF / 32]; };
+        auto fetch = [&](int t) {
+            Ahead f{p.ignore, 0.f, 1.f, {}};
+            if (KIND > XENT_GRAD || t >= t_end) return f;
+            const XentTile w = xent_tile<KIND>(p, t);
+            const int row = w.m * kXM + quarter * 32 + lane;
+            if (row < p.M) {
+                f.tgt = __ldg(p.target + row);
+                if (KIND == XENT_GRAD) {
+                    f.lse = __ldg(p.lse + row) + p.factor_log2;
+                    if (p.up) f.scale = __ldg(p.up + row);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < HALF / 32; i++) {
+                const int c = w.n * BN + (2 * i + half) * 32 + lane;
+                f.bias[i] = c >= p.N ? __int_as_float(0xff800000) : p.bias ? 1.4426950408889634f * ld_param(p.bias, p.col0 + c, p.bias_bf16) : 0.f;
+            }
+            return f;
+        };
+        Ahead next = fetch(t_begin);
         for (int t = t_begin; ok && t < t_end; t += t_step) {
             const XentTile w = xent_tile<KIND>(p, t);
             const int row = w.m * kXM + quarter * 32 + lane, n0 = w.n * BN;
@@ -279,23 +322,17 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (KIND == XENT_LOGITS && m_now >= 0) flush();
                     m_now = w.m;
                     mx = __int_as_float(0xff800000); sum = 0.f; total = 0.f;
-                    tgt = row < p.M ? __ldg(p.target + row) : p.ignore;
-                    ignored = tgt == p.ignore;
-                    if (KIND == XENT_GRAD && row < p.M) {
-                        lse = __ldg(p.lse + row) + p.factor_log2;
-                        if (tgt < 0 || tgt >= p.V) lse = __int_as_float(0x7fffffff);      // no such class: NaN, not silence
-                        scale = p.up ? __ldg(p.up + row) : 1.f;
-                    }
                 }
-                // the tile's bias in units of log2; -inf where the vocabulary ends, so that those columns weigh nothing
-                // (every warp keeps its own: no warp ever waits for another without a limit)
+                tgt = next.tgt;
+                ignored = tgt == p.ignore;
+                lse = !ignored && (tgt < 0 || tgt >= p.V) ? __int_as_float(0x7fffffff) : next.lse;      // no such class: NaN, not silence
+                scale = next.scale;
+                // (every warp keeps its own copy of the bias: no warp ever waits for another without a limit)
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < HALF / 32; i++) {
-                    const int c = n0 + half * HALF + i * 32 + lane;
-                    bs[i * 32 + lane] = c >= p.N ? __int_as_float(0xff800000) : p.bias ? 1.4426950408889634f * ld_param(p.bias, p.col0 + c, p.bias_bf16) : 0.f;
-                }
+                for (int i = 0; i < HALF / 32; i++) bs[i * 32 + lane] = next.bias[i];
                 __syncwarp();
+                next = fetch(t + t_step);
             }
             float v[SPLIT ? PIECES : 1][32];
             if constexpr (SPLIT) {
@@ -310,8 +347,8 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                     for (int pc = 0; pc < PIECES; pc++) {
                         uint32_t r[32], s[32];
-                        tc::tmem_load32(lane_base + acc * 256 + pc * 32, r);
-                        tc::tmem_load32(lane_base + acc * 256 + 128 + pc * 32, s);
+                        tc::tmem_load32(lane_base + acc * 256 + pc * 64, r);
+                        tc::tmem_load32(lane_base + acc * 256 + 128 + pc * 64, s);
                         tc::tmem_wait32(r);
                         tc::tmem_wait32(s);
 #pragma unroll
@@ -331,13 +368,16 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
             for (int pc = 0; pc < PIECES; pc++) {
                 float (&a)[32] = v[SPLIT ? pc : 0];
-                const int c0 = n0 + half * HALF + pc * 32;          // first column of the piece
+                const int c0 = n0 + (2 * pc + half) * 32;           // first column of the piece
+                const bool some = c0 < (KIND == XENT_GRAD ? p.g_ld : p.N);      // the same for the whole warp
                 if constexpr (!SPLIT) {
-                    uint32_t r[32];
-                    tc::tmem_load32(lane_base + acc * 256 + pc * 32, r);
-                    tc::tmem_wait32(r);
+                    if (some) {
+                        uint32_t r[32];
+                        tc::tmem_load32(lane_base + acc * 256 + pc * 64, r);
+                        tc::tmem_wait32(r);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) a[i] = __uint_as_float(r[i]);
+                        for (int i = 0; i < 32; i++) a[i] = __uint_as_float(r[i]);
+                    }
                     if (pc == PIECES - 1) {
                         tc::fence_before();
                         __syncwarp();
@@ -346,6 +386,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         if (acc == 0) acc_phase ^= 1;
                     }
                 }
+                if (!some) continue;
                 if constexpr (KIND <= XENT_GRAD) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
@@ -380,38 +421,37 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         sum = sum * exp2_fast(mx - ref) + (s0 + s1);
                         mx = top;
                     } else {
-                        if (c0 < p.g_ld) {                           // the same for the whole warp
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                float g = exp2_fast(a[i] - lse);
-                                if (p.smooth) g -= c0 + i < p.N ? p.eps_v : 0.f;
-                                a[i] = g;
-                            }
-                            if (hit) {
+                        for (int i = 0; i < 32; i++) {
+                            float g = exp2_fast(a[i] - lse);
+                            if (p.smooth) g -= c0 + i < p.N ? p.eps_v : 0.f;
+                            a[i] = g;
+                        }
+                        if (hit) {
 #pragma unroll
-                                for (int i = 0; i < 32; i++) a[i] -= at == i ? p.one : 0.f;
-                            }
+                            for (int i = 0; i < 32; i++) a[i] -= at == i ? p.one : 0.f;
+                        }
 #pragma unroll
-                            for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i] * scale;
+                        for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i] * scale;
+                        const int r0 = w.m * kXM + quarter * 32;
+                        if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + lane] = column_sums(a, lane);
 #pragma unroll
-                            for (int pl = 0; pl < S::PL; pl++) {
-                                uint4 out[4];
-                                uint32_t *o = reinterpret_cast<uint32_t *>(out);
+                        for (int pl = 0; pl < S::PL; pl++) {
+                            uint4 out[4];
+                            uint32_t *o = reinterpret_cast<uint32_t *>(out);
 #pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    if constexpr (SPLIT) {
-                                        const float lo = take_bf16(a[2 * i]), hi = take_bf16(a[2 * i + 1]);
-                                        o[i] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
-                                    } else {
-                                        o[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
-                                    }
+                            for (int i = 0; i < 16; i++) {
+                                if constexpr (SPLIT) {
+                                    const float lo = take_bf16(a[2 * i]), hi = take_bf16(a[2 * i + 1]);
+                                    o[i] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
+                                } else {
+                                    o[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
                                 }
-                                __nv_bfloat16 *to = p.g + pl * p.g_plane + c0;
-                                const int r0 = w.m * kXM + quarter * 32;
-                                xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
-                                    if (r0 + r < p.M) *reinterpret_cast<uint4 *>(to + (long long)(r0 + r) * p.g_ld + piece * 8) = val;
-                                });
                             }
+                            __nv_bfloat16 *to = p.g + pl * p.g_plane + c0;
+                            xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
+                                if (r0 + r < p.M) *reinterpret_cast<uint4 *>(to + (long long)(r0 + r) * p.g_ld + piece * 8) = val;
+                            });
                         }
                     }
                 } else {
@@ -558,64 +598,66 @@ xent_total_kernel(const double2 *__restrict__ sums, int blocks, int mean, float 
     }
 }
 
-// out = alpha * sum over slots of sums[slot], in order.
+// out = alpha * sum over slots of sums[slot], in a fixed order.  Block (32, 8): 32 elements, the slots congruent to y modulo 8.
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_finish_kernel(const float *__restrict__ sums, T *__restrict__ out, long long n, int slots, const float *up, const float *count, float f) {
-    const float alpha = xent_alpha(up, count, f);
-    const long long step = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        float s = sums[i];
-        for (int k = 1; k < slots; k++) s += sums[k * n + i];
-        st(out + i, alpha * s);
-    }
-}
-
-// Column sums of a piece of G: CTA (bx, by) adds rows by*8+warp, ... of 256 columns; partial [slice][part_ld].
-__global__ void __launch_bounds__(256)
-xent_colsum_kernel(const __nv_bfloat16 *__restrict__ g, long long plane, int planes, int rows, int ld, float *__restrict__ partial, int part_ld) {
-    __shared__ float red[8][256];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 256 + lane * 8;
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < ld)
-        for (int pl = planes - 1; pl >= 0; pl--)                     // small planes first
+    __shared__ float part[8][33];
+    const long long i = (long long)blockIdx.x * 32 + threadIdx.x;
+    float s = 0.f;
+    if (i < n)
 #pragma unroll 4
-            for (int r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(g + pl * plane + (long long)r * ld + c));
-                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    s[2 * i] += __uint_as_float(x[i] << 16);
-                    s[2 * i + 1] += __uint_as_float(x[i] & 0xffff0000u);
-                }
-            }
-#pragma unroll
-    for (int i = 0; i < 8; i++) red[warp][lane * 8 + i] = s[i];
+        for (int k = threadIdx.y; k < slots; k += 8) s += sums[k * n + i];
+    part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    const int col = blockIdx.x * 256 + threadIdx.x;
-    if (col < ld) {
+    if (threadIdx.y == 0 && i < n) {
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; w++) t += red[w][threadIdx.x];
-        partial[(long long)blockIdx.y * part_ld + col] = t;
+        for (int y = 0; y < 8; y++) t += part[y][threadIdx.x];
+        st(out + i, xent_alpha(up, count, f) * t);
     }
 }
-// db = alpha * sum over slices of partial, in a fixed order.  Block (32, 32).
+// The same where there are few slots and many elements: four elements a thread.
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_finish_few_kernel(const float *__restrict__ sums, T *__restrict__ out, long long n, int slots, const float *up, const float *count, float f) {
+    const float alpha = xent_alpha(up, count, f);
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool whole = n % 4 == 0;                       // every slot then starts on a vector
+    for (int k = 0; k < slots; k++) {
+        if (whole) {
+            const float4 v = *reinterpret_cast<const float4 *>(sums + k * n + i);
+            s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+        } else {
+            for (int j = 0; j < 4; j++)
+                if (i + j < n) s[j] += sums[k * n + i + j];
+        }
+    }
+    for (int j = 0; j < 4; j++)
+        if (i + j < n) st(out + i + j, alpha * s[j]);
+}
+
+// Column sums over slices of 32 rows, in a fixed order.  Block (32, 32); CTA (bx, by): columns 32 bx .., slices by * per ..
+// With one CTA along y the result is db (times alpha), else partial sums again.
 __global__ void __launch_bounds__(1024)
-xent_bias_kernel(const float *__restrict__ partial, int part_ld, int slices, void *__restrict__ db, int bf16, int V, const float *up,
-                 const float *count, float f) {
+xent_bias_kernel(const float *__restrict__ partial, long long part_ld, int slices, int per, void *__restrict__ db, int bf16, float *__restrict__ more,
+                 long long more_ld, int V, const float *up, const float *count, float f) {
     __shared__ float part[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
+    const int c = blockIdx.x * 32 + threadIdx.x, end = min(slices, (int)(blockIdx.y + 1) * per);
     float s = 0.f;
     if (c < V)
-        for (int k = threadIdx.y; k < slices; k += 32) s += partial[(long long)k * part_ld + c];
+#pragma unroll 4
+        for (int k = blockIdx.y * per + threadIdx.y; k < end; k += 32) s += partial[k * part_ld + c];
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < V) {
         float t = 0.f;
 #pragma unroll
         for (int y = 0; y < 32; y++) t += part[y][threadIdx.x];
-        st_param(db, c, bf16, xent_alpha(up, count, f) * t);
+        if (more) more[blockIdx.y * more_ld + c] = t;
+        else st_param(db, c, bf16, xent_alpha(up, count, f) * t);
     }
 }
 

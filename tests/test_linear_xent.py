@@ -124,10 +124,10 @@ def test_options(smoothing, bias, reduction, dtype):
 
 @gpu
 @pytest.mark.parametrize("N,D,V,dtype,reduction", [
-    (2100, 64, 20001, "bf16", "mean"),        # pieces of the classes
-    (1500, 72, 9001, "fp32", "none"),
-    (40001, 32, 1000, "bf16", "none"),        # pieces of the rows
-    (20003, 24, 700, "fp32", "mean"),
+    (2100, 64, 40001, "bf16", "mean"),        # pieces of the classes
+    (1500, 72, 20001, "fp32", "none"),
+    (80001, 32, 1000, "bf16", "none"),        # pieces of the rows
+    (40003, 24, 700, "fp32", "mean"),
     (30000, 64, 10, "bf16", "mean"),          # the gradient of the weight has one tile and a long K axis: parts
     (9000, 100, 3, "fp32", "sum"),
     (5, 64, 30011, "bf16", "sum"),            # dx has one tile and a long K axis
@@ -284,8 +284,8 @@ def test_repeats_bit_for_bit_streams_and_graphs():
 
 @gpu
 def test_the_logits_are_not_kept():
-    """1000 classes more cost the weight's rows and no logits: 16384 x 9000 bf16 logits alone would be 295 MB."""
-    x, w, b, t = make(16384, 64, 9000, "bf16")
+    """16384 x 30000 bf16 logits alone would be 983 MB."""
+    x, w, b, t = make(16384, 64, 30000, "bf16")
     leaves = [v.requires_grad_(True) for v in (x, w, b)]
     torch.cuda.synchronize()
     base = torch.cuda.memory_allocated()
@@ -294,7 +294,7 @@ def test_the_logits_are_not_kept():
     assert torch.cuda.memory_allocated() - base <= 16384 * 4 + 8192       # one float a row
     torch.autograd.grad(loss, leaves)
     torch.cuda.synchronize()
-    assert torch.cuda.max_memory_allocated() - base <= 120 << 20
+    assert torch.cuda.max_memory_allocated() - base <= 256 << 20
 
 
 def test_refusals():

@@ -119,10 +119,10 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
     __nv_bfloat16 *to = (__nv_bfloat16 *)*ws;
     *ws += o.bytes;
     m->p = to;
-    const long long n = o.rows * o.D, blocks = (n + 255) / 256;
-    const int grid = (int)(blocks < (long long)r.sms * 32 ? blocks : (long long)r.sms * 32);
-    if (o.planes == 3) xent_planes_kernel<float><<<grid, 256, 0, r.st>>>((const float *)src, to, o.rows, o.D, o.ld);
-    else xent_planes_kernel<__nv_bfloat16><<<grid, 256, 0, r.st>>>((const __nv_bfloat16 *)src, to, o.rows, o.D, o.ld);
+    const long long blocks = (o.rows + 7) / 8;
+    const int grid = (int)(blocks < (long long)r.sms * 16 ? blocks : (long long)r.sms * 16), vec = o.D % 4 == 0 && ((uintptr_t)src & 15) == 0;
+    if (o.planes == 3) xent_planes_kernel<float><<<grid, 256, 0, r.st>>>((const float *)src, to, o.rows, o.D, o.ld, vec);
+    else xent_planes_kernel<__nv_bfloat16><<<grid, 256, 0, r.st>>>((const __nv_bfloat16 *)src, to, o.rows, o.D, o.ld, vec);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? O1D_OK : r.fail(e);
 }
@@ -131,7 +131,7 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
 int forward_slots(long long N, int D, int V, bool bf16, int sms) {
     const long long n_tiles = cdiv(V, width_of(N, V, D, !bf16, sms)), tiles = cdiv(N, kXM) * n_tiles;
     const long long ctas = tiles < sms ? tiles : sms, least = tiles / ctas;
-    return 2 * (int)(cdiv(n_tiles, least) + 1);
+    return 4 * (int)(cdiv(n_tiles, least) + 1);
 }
 
 // Backward: how G is cut, and into how many parts the K axes of the two products are.

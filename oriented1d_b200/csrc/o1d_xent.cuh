@@ -22,6 +22,7 @@
 #pragma once
 
 #include "o1d_common.cuh"
+#include "o1d_pair.cuh"
 #include "o1d_tc.cuh"
 
 namespace o1d {
@@ -29,7 +30,9 @@ namespace o1d {
 enum : int { XENT_LOGITS = 0, XENT_GRAD, XENT_DX, XENT_DW };
 
 constexpr int kXM = 128, kXK = 64;               // tile rows; K elements of a stage (one 128-byte swizzled row)
-constexpr int kXThreads = 384;                   // warp 0 loads, 1 multiplies, 2 owns tensor memory, 4-11 finish tiles
+constexpr int kXFinish = 16;                     // warps that finish tiles: four a scheduler (with two, half the issue slots stayed
+                                                 // empty behind the chain load, exponential, pack, store of a piece)
+constexpr int kXThreads = 128 + 32 * kXFinish;   // warp 0 loads, 1 multiplies, 2 owns tensor memory, 4-19 finish tiles
 constexpr int kXStaging = 2048;                  // bytes of a warp's store buffer: 32 rows of 64 bytes
 constexpr int kXChunk = 4;                       // fp32: stages of one accumulation
 // Tiles of 256 columns, or of 128: fp32 (its two accumulators would not fit twice), and bf16 products of few columns or too
@@ -37,7 +40,7 @@ constexpr int kXChunk = 4;                       // fp32: stages of one accumula
 template <bool SPLIT, int BN_> struct XentShape {
     static constexpr int BN = BN_, PL = SPLIT ? 3 : 1, STAGES = SPLIT ? 2 : BN == 256 ? 4 : 6;
     static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = BN * kXK * 2, STAGE = PL * (A_BYTES + B_BYTES);
-    static constexpr int SMEM = STAGES * STAGE + 8 * kXStaging + 8 * (BN / 2) * (int)sizeof(float) + 256 + 1024;
+    static constexpr int SMEM = STAGES * STAGE + kXFinish * kXStaging + 256 + 1024;
 };
 
 struct XentParams {
@@ -152,13 +155,12 @@ __global__ void __launch_bounds__(kXThreads, 1)
 xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XentParams p) {
     using S = XentShape<SPLIT, BN>;
     constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
-    constexpr int HALF = BN / 2, PIECES = HALF / 32;
+    constexpr int PIECES = BN / 128;                 // of 32 columns, for each of the four warps that share 32 rows
     constexpr uint32_t INSTR = tc::instruction<BN, A_MN, B_MN>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *smem = raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u);
     char *staging = reinterpret_cast<char *>(smem + S::STAGES * S::STAGE);
-    float *bias_s = reinterpret_cast<float *>(staging + 8 * kXStaging);                 // [epilogue warp][HALF]
-    uint64_t *full = reinterpret_cast<uint64_t *>(bias_s + 8 * HALF), *empty = full + S::STAGES;
+    uint64_t *full = reinterpret_cast<uint64_t *>(staging + kXFinish * kXStaging), *empty = full + S::STAGES;
     uint64_t *done = empty + S::STAGES, *taken = done + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(taken + 2);
     volatile int *dead = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -166,7 +168,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; i++) { tc::bar_init(full + i, 1); tc::bar_init(empty + i, 1); }
-        for (int i = 0; i < 2; i++) { tc::bar_init(done + i, 1); tc::bar_init(taken + i, 8); }
+        for (int i = 0; i < 2; i++) { tc::bar_init(done + i, 1); tc::bar_init(taken + i, kXFinish); }
         *dead = 0;
         tc::bar_init_fence();
         tc::tma_prefetch(&map_a);
@@ -267,15 +269,14 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             tc::commit(done + acc);
             tc::bar_drain(done + acc, acc_phase);
         }
-    } else if (warp >= 4) {                                         // ---- epilogue: a thread owns a row's half
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        float *bs = bias_s + (warp - 4) * HALF;
+    } else if (warp >= 4) {                                         // ---- epilogue: a thread owns a quarter of a row
+        const int quarter = warp & 3, part = (warp - 4) >> 2;
         char *stage = staging + (warp - 4) * kXStaging;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + half * 32;      // every second piece of 32 columns
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + part * 32;      // every fourth piece of 32 columns
         int acc = 0, m_now = -1;
         uint32_t acc_phase = 0;
         bool ok = true;
-        // LOGITS: running maximum and sum of the row's half, in units of log2
+        // LOGITS: running maximum and sum of the row's columns that this warp sees, in units of log2
         float mx = 0.f, sum = 0.f, total = 0.f;
         long long tgt = -1;
         float lse = 0.f, scale = 0.f;
@@ -286,14 +287,14 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         auto flush = [&]() {
             const long long row = (long long)m_now * kXM + quarter * 32 + lane;
             if (row >= p.M) return;
-            const int slot = ((int)blockIdx.x - xent_owner(m_now * p.n_tiles, p.tiles, gridDim.x)) * 2 + half;
+            const int slot = ((int)blockIdx.x - xent_owner(m_now * p.n_tiles, p.tiles, gridDim.x)) * 4 + part;
             p.part[(long long)slot * p.part_rows + row] = make_float2(mx, sum);
             if (p.smooth) p.part_sum[(long long)slot * p.part_rows + row] = total;
         };
 
         // What a tile needs from memory, fetched while the one before it is worked on.  Bias in units of log2; -inf where the
         // vocabulary ends, so that those columns weigh nothing.
-        struct Ahead { long long tgt; float lse, scale, bias[HALF / 32]; };
+        struct Ahead { long long tgt; float lse, scale, bias[PIECES]; };
         auto fetch = [&](int t) {
             Ahead f{p.ignore, 0.f, 1.f, {}};
             if (KIND > XENT_GRAD || t >= t_end) return f;
@@ -307,8 +308,8 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 }
             }
 #pragma unroll
-            for (int i = 0; i < HALF / 32; i++) {
-                const int c = w.n * BN + (2 * i + half) * 32 + lane;
+            for (int i = 0; i < PIECES; i++) {
+                const int c = w.n * BN + (4 * i + part) * 32 + lane;
                 f.bias[i] = c >= p.N ? __int_as_float(0xff800000) : p.bias ? 1.4426950408889634f * ld_param(p.bias, p.col0 + c, p.bias_bf16) : 0.f;
             }
             return f;
@@ -317,6 +318,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         for (int t = t_begin; ok && t < t_end; t += t_step) {
             const XentTile w = xent_tile<KIND>(p, t);
             const int row = w.m * kXM + quarter * 32 + lane, n0 = w.n * BN;
+            float bias[PIECES];
             if constexpr (KIND <= XENT_GRAD) {
                 if (w.m != m_now) {
                     if (KIND == XENT_LOGITS && m_now >= 0) flush();
@@ -327,11 +329,8 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 ignored = tgt == p.ignore;
                 lse = !ignored && (tgt < 0 || tgt >= p.V) ? __int_as_float(0x7fffffff) : next.lse;      // no such class: NaN, not silence
                 scale = next.scale;
-                // (every warp keeps its own copy of the bias: no warp ever waits for another without a limit)
-                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < HALF / 32; i++) bs[i * 32 + lane] = next.bias[i];
-                __syncwarp();
+                for (int i = 0; i < PIECES; i++) bias[i] = next.bias[i];
                 next = fetch(t + t_step);
             }
             float v[SPLIT ? PIECES : 1][32];
@@ -345,15 +344,15 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (!ok) break;
                     tc::fence_after();
 #pragma unroll
-                    for (int pc = 0; pc < PIECES; pc++) {
-                        uint32_t r[32], s[32];
-                        tc::tmem_load32(lane_base + acc * 256 + pc * 64, r);
-                        tc::tmem_load32(lane_base + acc * 256 + 128 + pc * 64, s);
-                        tc::tmem_wait32(r);
-                        tc::tmem_wait32(s);
+                    for (int pc = 0; pc < PIECES; pc++)
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[pc][i] += __uint_as_float(r[i]) + __uint_as_float(s[i]);
-                    }
+                        for (int part_sum = 1; part_sum >= 0; part_sum--) {          // the five small products, then x0 w0
+                            uint32_t r[32];
+                            tc::tmem_load32(lane_base + acc * 256 + part_sum * 128 + pc * 128, r);
+                            tc::tmem_wait32(r);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) v[pc][i] += __uint_as_float(r[i]);
+                        }
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) tc::bar_arrive(taken + acc);
@@ -368,12 +367,12 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
             for (int pc = 0; pc < PIECES; pc++) {
                 float (&a)[32] = v[SPLIT ? pc : 0];
-                const int c0 = n0 + (2 * pc + half) * 32;           // first column of the piece
+                const int c0 = n0 + (4 * pc + part) * 32;           // first column of the piece
                 const bool some = c0 < (KIND == XENT_GRAD ? p.g_ld : p.N);      // the same for the whole warp
                 if constexpr (!SPLIT) {
                     if (some) {
                         uint32_t r[32];
-                        tc::tmem_load32(lane_base + acc * 256 + pc * 64, r);
+                        tc::tmem_load32(lane_base + acc * 256 + pc * 128, r);
                         tc::tmem_wait32(r);
 #pragma unroll
                         for (int i = 0; i < 32; i++) a[i] = __uint_as_float(r[i]);
@@ -388,51 +387,70 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 }
                 if (!some) continue;
                 if constexpr (KIND <= XENT_GRAD) {
+                    // logits in units of log2; the piece's bias through the store buffer, from lane i to every lane's value i
+                    const F2 log2e = both(1.4426950408889634f);
+                    float *bs = reinterpret_cast<float *>(stage);
+                    bs[lane] = bias[pc];
+                    __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        const float4 b = *reinterpret_cast<const float4 *>(bs + pc * 32 + i);
-                        a[i] = fmaf(a[i], 1.4426950408889634f, b.x);
-                        a[i + 1] = fmaf(a[i + 1], 1.4426950408889634f, b.y);
-                        a[i + 2] = fmaf(a[i + 2], 1.4426950408889634f, b.z);
-                        a[i + 3] = fmaf(a[i + 3], 1.4426950408889634f, b.w);
+                        const float4 b = *reinterpret_cast<const float4 *>(bs + i);
+                        const float2 u = apart(fma2(two(a[i], a[i + 1]), log2e, two(b.x, b.y))), v = apart(fma2(two(a[i + 2], a[i + 3]), log2e, two(b.z, b.w)));
+                        a[i] = u.x; a[i + 1] = u.y; a[i + 2] = v.x; a[i + 3] = v.y;
                     }
+                    __syncwarp();
                     const long long off = tgt - p.col0 - c0;         // where the target lies in this piece
-                    const bool hit = off >= 0 && off < 32;
-                    const int at = (int)off;
+                    const int at = off >= 0 && off < 32 ? (int)off : -1;
+                    const bool hit = __any_sync(0xffffffffu, at >= 0);
                     if constexpr (KIND == XENT_LOGITS) {
                         if (hit) {
                             float l = 0.f;
 #pragma unroll
                             for (int i = 0; i < 32; i++) l = at == i ? a[i] : l;
-                            if (row < p.M) p.target_logit[row] = l;
+                            if (at >= 0 && row < p.M) p.target_logit[row] = l;
                         }
                         if (p.smooth) {
 #pragma unroll
                             for (int i = 0; i < 32; i++) total += c0 + i < p.N ? a[i] : 0.f;
                         }
-                        float top = a[0];
+                        float top = mx;
 #pragma unroll
-                        for (int i = 1; i < 32; i++) top = fmaxf(top, a[i]);
-                        top = fmaxf(top, mx);
+                        for (int i = 0; i < 32; i++) top = fmaxf(top, a[i]);
                         const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
-                        float s0 = 0.f, s1 = 0.f;
+                        F2 s0 = both(0.f), s1 = both(0.f);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) { s0 += exp2_fast(a[i] - ref); s1 += exp2_fast(a[i + 1] - ref); }
-                        sum = sum * exp2_fast(mx - ref) + (s0 + s1);
+                        for (int i = 0; i < 32; i += 4) {
+                            const float2 u = apart(add2(two(a[i], a[i + 1]), both(-ref))), v = apart(add2(two(a[i + 2], a[i + 3]), both(-ref)));
+                            s0 = add2(s0, two(exp2_fast(u.x), exp2_fast(u.y)));
+                            s1 = add2(s1, two(exp2_fast(v.x), exp2_fast(v.y)));
+                        }
+                        const float2 s2 = apart(add2(s0, s1));
+                        sum = sum * exp2_fast(mx - ref) + (s2.x + s2.y);
                         mx = top;
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            float g = exp2_fast(a[i] - lse);
-                            if (p.smooth) g -= c0 + i < p.N ? p.eps_v : 0.f;
-                            a[i] = g;
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 u = apart(add2(two(a[i], a[i + 1]), both(-lse)));
+                            a[i] = exp2_fast(u.x);
+                            a[i + 1] = exp2_fast(u.y);
+                        }
+                        if (p.smooth) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) a[i] -= c0 + i < p.N ? p.eps_v : 0.f;
                         }
                         if (hit) {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) a[i] -= at == i ? p.one : 0.f;
+                            for (int i = 0; i < 32; i++)
+                                if (at == i) a[i] -= p.one;
                         }
+                        if (p.up) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i] * scale;
+                            for (int i = 0; i < 32; i++) a[i] *= scale;
+                        }
+                        if (__any_sync(0xffffffffu, ignored)) {      // (whatever the row held: nothing comes of it)
+#pragma unroll
+                            for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i];
+                        }
                         const int r0 = w.m * kXM + quarter * 32;
                         if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + lane] = column_sums(a, lane);
 #pragma unroll
@@ -512,20 +530,41 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // One matrix as the bf16 planes that tensor copies read: fp32 cut into three, bf16 whose rows do not start on 16 bytes
-// copied.  planes: [3 or 1][rows][ld], ld a multiple of 8 (what lies past D is never read).
+// copied.  planes: [3 or 1][rows][ld], ld a multiple of 8 (what lies past D is never read).  A warp a row; `vec`: four
+// values a lane, where the rows of x start on a vector.
 template <typename T>
 __global__ void __launch_bounds__(256)
-xent_planes_kernel(const T *__restrict__ x, __nv_bfloat16 *__restrict__ planes, long long rows, int D, int ld) {
-    const long long n = rows * D, plane = rows * ld, step = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const long long r = i / D;
-        __nv_bfloat16 *to = planes + r * ld + (i - r * D);
-        if constexpr (sizeof(T) == 2) {
-            *to = x[i];
-        } else {
-            float v = x[i];
+xent_planes_kernel(const T *__restrict__ x, __nv_bfloat16 *__restrict__ planes, long long rows, int D, int ld, int vec) {
+    const long long plane = rows * ld;
+    const int lane = threadIdx.x & 31;
+    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
+        const T *from = x + r * D;
+        __nv_bfloat16 *to = planes + r * ld;
+        if constexpr (sizeof(T) == 4) {
+            if (vec) {
+#pragma unroll 2
+                for (int c = lane * 4; c < D; c += 128) {
+                    const float4 q = __ldg(reinterpret_cast<const float4 *>(from + c));
+                    float v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int pl = 0; pl < 3; pl++) to[pl * plane] = __float2bfloat16_rn(take_bf16(v));      // exact: eight bits each
+                    for (int pl = 0; pl < 3; pl++) {
+                        uint32_t b[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) b[i] = __float_as_uint(take_bf16(v[i]));              // exact: eight bits each
+                        *reinterpret_cast<uint2 *>(to + pl * plane + c) = make_uint2(b[0] >> 16 | (b[1] & 0xffff0000u), b[2] >> 16 | (b[3] & 0xffff0000u));
+                    }
+                }
+                continue;
+            }
+        }
+        for (int c = lane; c < D; c += 32) {
+            if constexpr (sizeof(T) == 2) {
+                to[c] = from[c];
+            } else {
+                float v = from[c];
+#pragma unroll
+                for (int pl = 0; pl < 3; pl++) to[pl * plane + c] = __float2bfloat16_rn(take_bf16(v));
+            }
         }
     }
 }
@@ -540,7 +579,7 @@ xent_rows_kernel(const float2 *__restrict__ part, const float *__restrict__ part
     double loss = 0., counted = 0.;
     if (row < rows) {
         const int m = (int)(row / kXM);
-        const int slots = 2 * (xent_owner((m + 1) * n_tiles - 1, tiles, ctas) - xent_owner(m * n_tiles, tiles, ctas) + 1);
+        const int slots = 4 * (xent_owner((m + 1) * n_tiles - 1, tiles, ctas) - xent_owner(m * n_tiles, tiles, ctas) + 1);
         float top = __int_as_float(0xff800000), total = 0.f;
         for (int s = 0; s < slots; s++) top = fmaxf(top, part[s * part_rows + row].x);
         const float ref = top == __int_as_float(0xff800000) ? 0.f : top;

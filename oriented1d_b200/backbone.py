@@ -62,11 +62,11 @@ class ConvNeXt1DBackbone(ConvNeXt1D):
     -> tuple of normalised stage maps [N,C_i,ceil(H/4/2^i),ceil(W/4/2^i)] for i in out_indices."""
 
     def __init__(self, in_chans=3, depths=(3, 3, 9, 3), dims=(96, 192, 384, 768), drop_path_rate=0.0,
-                 layer_scale_init_value=1e-6, out_indices=(0, 1, 2, 3), variant="1d", N=8, stem_dim1=64):
+                 layer_scale_init_value=1e-6, out_indices=(0, 1, 2, 3), variant="1d", N=8, stem_dim1=64, keep8=False):
         super().__init__(in_chans=in_chans, num_classes=1, depths=depths, dims=dims, drop_path_rate=drop_path_rate,
                          layer_scale_init_value=layer_scale_init_value, variant=variant, N=N, stem_dim1=stem_dim1,
                          arbitrary_size=True, block_kernels=BACKBONE_BLOCK_KERNELS[variant],
-                         stem_kernel=BACKBONE_STEM_KERNEL[variant])
+                         stem_kernel=BACKBONE_STEM_KERNEL[variant], keep8=keep8)
         del self.norm, self.head
         _wrap_convs(self)
         self.out_indices = tuple(out_indices)

@@ -123,13 +123,20 @@ class Block1D(nn.Module):
         self.dwconv = get_convolution_1d(dim, kernel_size=kernel_sizes[0], padding=kernel_sizes[0] // 2, nhwc=True,
                                          N=N, layer_offset=layer_offset, arbitrary_size=arbitrary_size)
 
+    keep8 = False        # keep 8-bit checkpoints of the MLP's tensors for the backward pass (set by ConvNeXt1D)
+
     def _mlp_in(self, x, gelu=True):
         h = ops.linear_cl(self.pwconv1, self.norm(x))
         return F.gelu(h) if gelu else h
 
+    def _mlp(self, x):
+        if self.keep8 and x.is_cuda and torch.is_grad_enabled():
+            return ops.mlp_keep8(x, self.norm.weight, self.norm.bias, self.pwconv1.weight, self.pwconv1.bias, self.pwconv2.weight,
+                                 self.pwconv2.bias, self.norm.eps)
+        return ops.linear_cl(self.pwconv2, self._mlp_in(x))
+
     def forward(self, x):
-        y = ops.linear_cl(self.pwconv2, self._mlp_in(self.dwconv(x)))
-        return self._residual(x, y)
+        return self._residual(x, self._mlp(self.dwconv(x)))
 
     def _residual(self, x, y):
         """x + drop_path(gamma * y) (convnext.py:314-318); one fused pass when nothing is dropped."""
@@ -176,8 +183,7 @@ class Block2D(Block1D):
         return conv(x.permute(0, 3, 1, 2)).permute(0, 2, 3, 1)
 
     def forward(self, x):
-        y = ops.linear_cl(self.pwconv2, self._mlp_in(self._dw2d(self.dwconv, x)))
-        return self._residual(x, y)
+        return self._residual(x, self._mlp(self._dw2d(self.dwconv, x)))
 
 
 class Block2DPP(Block2D):
@@ -242,9 +248,11 @@ class ConvNeXt1D(nn.Module):
 
     def __init__(self, in_chans=3, num_classes=1000, depths=(3, 3, 9, 3), dims=(96, 192, 384, 768),
                  drop_path_rate=0.0, layer_scale_init_value=1e-6, head_init_scale=1.0, variant="1d", N=8,
-                 stem_dim1=64, arbitrary_size=False, block_kernels=None, stem_kernel=None, fuse_gelu=False):
+                 stem_dim1=64, arbitrary_size=False, block_kernels=None, stem_kernel=None, fuse_gelu=False, keep8=False):
         super().__init__()
         assert variant in BLOCKS
+        if keep8 and variant not in ("1d", "2d"):
+            raise ValueError("keep8 needs blocks whose hidden tensor goes from GELU straight to the second Linear: variants 1d and 2d")
         Block = BLOCKS[variant]
         block_kernels = BLOCK_KERNELS[variant] if block_kernels is None else block_kernels
         stem_kernel = STEM_KERNEL[variant] if stem_kernel is None else stem_kernel
@@ -269,6 +277,9 @@ class ConvNeXt1D(nn.Module):
                 # only the operator module itself knows the flag (a wrapper for arbitrary sizes keeps the separate pass)
                 if isinstance(m, (Block1DPP, Block2DPP)) and hasattr(m.dwconv2, "_apply_op"):
                     m.dwconv2.gelu_input = fuse_gelu
+        for stage in self.stages:
+            for block in stage:
+                block.keep8 = bool(keep8)
         self.norm = nn.LayerNorm(dims[-1], eps=1e-6)
         self.head = nn.Linear(dims[-1], num_classes)
         self.apply(self._init_weights)
@@ -295,6 +306,12 @@ class ConvNeXt1D(nn.Module):
     def forward(self, x):
         x = self.forward_features(x)
         return self.head(self.norm(x.mean([-2, -1])))
+
+    def loss(self, x, target, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
+        """F.cross_entropy(self(x).float(), target, ...) without the logits (ops.linear_cross_entropy); fp32."""
+        x = self.norm(self.forward_features(x).mean([-2, -1]))
+        return ops.linear_cross_entropy(x, self.head.weight, target, self.head.bias, ignore_index=ignore_index,
+                                        label_smoothing=label_smoothing, reduction=reduction)
 
 
 def convnext_tiny(variant="1d", drop_path_rate=0.1, **kw):

@@ -583,6 +583,68 @@ Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, doubl
     return std::get<0>(ln_keep_forward(x, g, b, eps));
 }
 
+// ---- a block's LayerNorm -> Linear -> GELU -> Linear with 8-bit checkpoints -------------------------------
+// Kept between the passes: the codes of x (from which LayerNorm's output, the first Linear's input, is formed again) and
+// of the first Linear's output (from which the activation is); the four matrix products stay with the GEMM library.
+Tensor sum_rows(const Tensor &dy, at::ScalarType dt) {
+    const int64_t ve = dy.scalar_type() == at::kFloat ? 4 : 8;
+    Tensor s = dy.numel() && dy.size(-1) % ve == 0 ? colsum(dy, dt == at::kBFloat16) : dy.sum(0, false, at::kFloat);
+    return s.scalar_type() == dt ? s : s.to(dt);
+}
+struct MlpKeep8Fn : torch::autograd::Function<MlpKeep8Fn> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &g, const Tensor &b, const Tensor &w1, const Tensor &b1,
+                          const Tensor &w2, const Tensor &b2, double eps) {
+        auto [y, kx] = ln_keep_forward(x, g, b, eps);
+        auto [a, kh] = gelu_forward(at::linear(y, w1), b1, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({kx.x.codes, kx.x.ranges, kx.stats, g, b, kh.codes, kh.ranges, w1, w2});
+        ctx->saved_data["p"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)b1.scalar_type(), (int64_t)b2.scalar_type()};
+        return at::linear(a, w2, b2);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(8);
+        if (!grads[0].defined()) return out;
+        need_first_order("mlp_keep8");
+        const auto s = ctx->get_saved_variables();
+        const auto p = ctx->saved_data["p"].toIntVector();
+        const Tensor &w1 = s[7], &w2 = s[8], dz = grads[0].to((at::ScalarType)p[0]);
+        const Tensor dz2 = dz.reshape({-1, dz.size(-1)});
+        const c10::cuda::CUDAGuard guard(dz.device());
+        auto need = [&](int i) { return ctx->needs_input_grad(i); };
+        if (need(6)) out[6] = sum_rows(dz2, (at::ScalarType)p[2]);
+        GeluGrads h = gelu_backward({s[5], s[6]}, dz.matmul(w2), need(4), (at::ScalarType)p[1], need(5));
+        if (need(4)) out[4] = h.db;
+        if (need(5)) out[5] = dz2.t().matmul(h.y.reshape({-1, h.y.size(-1)}));
+        h.y = Tensor();
+        if (!(need(0) || need(1) || need(2) || need(3))) return out;
+        LnGrads n = ln_keep_backward({{s[0], s[1]}, s[2]}, h.dx.matmul(w1), s[3], s[4], need(3));
+        if (need(0)) out[0] = n.dx;
+        if (need(1)) out[1] = n.dg.reshape(s[3].sizes());
+        if (need(2)) out[2] = n.db.reshape(s[4].sizes());
+        if (need(3)) out[3] = h.dx.reshape({-1, h.dx.size(-1)}).t().matmul(n.y.reshape({-1, n.y.size(-1)}));
+        return out;
+    }
+};
+Tensor mlp_keep8(const Tensor &x, const Tensor &g, const Tensor &b, const Tensor &w1, const Tensor &b1, const Tensor &w2, const Tensor &b2, double eps) {
+    const Rows r(x);
+    dtype_code(x);
+    if (w1.dim() != 2 || w1.size(1) != r.C || w1.size(0) == 0) throw py::value_error("weight1 must be [hidden, " + std::to_string(r.C) + "]");
+    if (w2.dim() != 2 || w2.size(1) != w1.size(0) || w2.size(0) == 0) throw py::value_error("weight2 must be [features, " + std::to_string(w1.size(0)) + "]");
+    need_numel(g, r.C, "weight");
+    need_numel(b, r.C, "bias");
+    need_numel(b1, w1.size(0), "bias1");
+    need_numel(b2, w2.size(0), "bias2");
+    if (w1.scalar_type() != x.scalar_type() || w2.scalar_type() != x.scalar_type() || b2.scalar_type() != x.scalar_type())
+        throw py::type_error("x and the Linear layers' parameters must have the same dtype");
+    need_cuda(x);
+    for (const Tensor *t : {&g, &b, &w1, &b1, &w2, &b2}) need_device(*t, x, "a parameter");
+    const c10::cuda::CUDAGuard guard(x.device());
+    bool any = wants_grad(x);
+    for (const Tensor *t : {&g, &b, &w1, &b1, &w2, &b2}) any = any || wants_grad(*t);
+    if (at::GradMode::is_enabled() && any) return MlpKeep8Fn::apply(x, g, b, w1, b1, w2, b2, eps);
+    return at::linear(std::get<0>(gelu_forward(at::linear(std::get<0>(ln_keep_forward(x, g, b, eps)), w1), b1, false)), w2, b2);
+}
+
 // ---- softmax cross entropy of a linear classifier ----------------------------------------------------
 struct XentShape {
     int64_t N, D, V;
@@ -705,6 +767,7 @@ PYBIND11_MODULE(_o1d_torch, m) {
     m.def("keep8", &keep8, py::call_guard<py::gil_scoped_release>());
     m.def("restore8", &restore8, py::call_guard<py::gil_scoped_release>());
     m.def("gelu_keep8", &gelu_keep8, py::call_guard<py::gil_scoped_release>());
+    m.def("mlp_keep8", &mlp_keep8, py::call_guard<py::gil_scoped_release>());
     m.def("linear_xent", &linear_xent, py::call_guard<py::gil_scoped_release>());
     m.def("layer_norm_keep8", &layer_norm_keep8, py::call_guard<py::gil_scoped_release>());
 }

@@ -203,6 +203,14 @@ def layer_norm_keep8(x, weight, bias, eps: float = 1e-6):
     return ext.layer_norm_keep8(x, weight, bias, float(eps))
 
 
+def mlp_keep8(x, norm_weight, norm_bias, weight1, bias1, weight2, bias2, eps: float = 1e-6):
+    """Linear2(GELU(Linear1(LayerNorm(x)))) of a block (models/convnext.py:308-313), keeping for the backward pass the
+    8-bit checkpoints of layer_norm_keep8 and gelu_keep8 only: 1.06 bytes for each element of x and of the hidden tensor,
+    in place of x, LayerNorm's output, and the hidden tensor before and after GELU.  The output is that of the separate
+    layers; the gradients are taken at the kept values.  The matrix products stay with the GEMM library."""
+    return ext.mlp_keep8(x, norm_weight, norm_bias, weight1, bias1, weight2, bias2, float(eps))
+
+
 def uses_tiled(plan: Plan, N: int, H: int, W: int, stride: int, nhwc: bool, dtype: torch.dtype) -> bool:
     """Would this request run on one of the TMA-staged families (tiled, direct, segments; True) or on the
     general kernels (False)?"""

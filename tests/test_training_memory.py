@@ -1,0 +1,196 @@
+"""The training step that keeps little: blocks with 8-bit checkpoints, the head's loss without logits, all together."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import oriented1d_b200 as o1d
+from oriented1d_b200 import backbone, convnext1d
+
+ops = o1d.ops
+gpu = pytest.mark.gpu
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+def mlp_args(rows, C, hidden, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x = r(rows, C) * (0.5 + torch.rand(C, generator=g)) + 0.3 * r(C)
+    out = [x, 1 + 0.1 * r(C), 0.1 * r(C), r(hidden, C) * (1.5 / C ** 0.5), 0.2 * r(hidden), r(C, hidden) / hidden ** 0.5, 0.1 * r(C)]
+    return [t.to(DT[dtype]).cuda().requires_grad_(True) for t in out]
+
+
+def kept_of(x):
+    """What the checkpoint of a float32 matrix stands for, float64."""
+    return ops.restore8(*ops.keep8(x.float().reshape(-1, x.shape[-1]))).double().reshape(x.shape)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,C,hidden", [(1, 8, 16), (50, 96, 384), (333, 100, 130), (2000, 128, 512)])
+def test_mlp_keep8(rows, C, hidden, dtype):
+    """Output and gradients against float64: the gradient of each layer at the values its checkpoint stands for.  The GEMM
+    library rounds every product's result to the type (2^-8 relative for bf16) and the hidden tensor's rounding shows in its
+    codes; fp32 products carry 2^-24 sqrt(K) or so.  Norm-wise tolerance: four such roundings in a row."""
+    torch.backends.cuda.matmul.allow_tf32 = False
+    leaves = mlp_args(rows, C, hidden, dtype)
+    dz = torch.randn(rows, C, generator=torch.Generator().manual_seed(9)).to(DT[dtype]).cuda()
+    out = ops.mlp_keep8(*leaves)
+    grads = torch.autograd.grad(out, leaves, dz)
+    with torch.no_grad():
+        assert torch.equal(ops.mlp_keep8(*leaves), out)
+        x, g, b, w1, b1, w2, b2 = (t.detach() for t in leaves)
+        # the stored hidden tensor is the library's rounded one; its checkpoint is taken of that plus the bias
+        hidden32 = F.linear(ops.layer_norm_keep8(x, g, b), w1).float() + b1.float()
+        kx, kh = kept_of(x), kept_of(hidden32)
+        x, g, b, w1, b1, w2, b2, d = (t.double() for t in (x, g, b, w1, b1, w2, b2, dz))
+        mean = x.mean(1, keepdim=True)
+        rstd = 1 / torch.sqrt((x - mean).square().mean(1, keepdim=True) + 1e-6)
+        ref_out = F.gelu(((x - mean) * rstd * g + b) @ w1.t() + b1) @ w2.t() + b2
+        xhat = (kx - mean) * rstd
+        da = d @ w2
+        slope = 0.5 * (1 + torch.erf(kh / 2 ** 0.5)) + kh * torch.exp(-kh * kh / 2) / (2 * torch.pi) ** 0.5
+        dh = da * slope
+        dy = dh @ w1
+        gg = dy * g
+        dx = rstd * (gg - gg.mean(1, keepdim=True) - xhat * (gg * xhat).mean(1, keepdim=True))
+        refs = [dx, (dy * xhat).sum(0), dy.sum(0), dh.t() @ (xhat * g + b), dh.sum(0), d.t() @ F.gelu(kh), d.sum(0)]
+    tol = 4 * 2.0 ** -8 if dtype == "bf16" else 2e-5
+    assert float((out.detach().double() - ref_out).norm()) <= tol * float(ref_out.norm())
+    for name, a, r, leaf in zip(("dx", "dgamma", "dbeta", "dw1", "db1", "dw2", "db2"), grads, refs, leaves):
+        assert a.dtype == leaf.dtype and a.shape == leaf.shape
+        assert float((a.double() - r).norm()) <= tol * float(r.norm()) + 1e-6, name
+
+
+@gpu
+def test_mlp_keep8_is_near_the_whole_gradient():
+    """Against the gradient with everything kept: a code is off by at most half a 255th of its group's range, about six
+    standard deviations of normal data, so by 0.007 of one, r.m.s.; that reaches the gradients scaled by slopes of about one."""
+    leaves = mlp_args(1500, 96, 384, "fp32")
+    dz = torch.randn(1500, 96, device="cuda")
+    grads = torch.autograd.grad(ops.mlp_keep8(*leaves), leaves, dz)
+    x, g, b, w1, b1, w2, b2 = leaves
+    full = torch.autograd.grad(F.linear(F.gelu(F.linear(F.layer_norm(x, (96,), g, b, 1e-6), w1, b1)), w2, b2), leaves, dz)
+    for a, r in zip(grads, full):
+        assert float((a - r).norm()) <= 0.02 * float(r.norm())
+
+
+@gpu
+def test_only_the_gradients_asked_for():
+    leaves = mlp_args(40, 32, 64, "fp32")
+    dz = torch.randn(40, 32, device="cuda")
+    full = torch.autograd.grad(ops.mlp_keep8(*leaves), leaves, dz)
+    for i in range(7):
+        part = [t.detach().requires_grad_(k == i) for k, t in enumerate(leaves)]
+        assert torch.equal(torch.autograd.grad(ops.mlp_keep8(*part), part[i], dz)[0], full[i])
+
+
+def small(keep8, variant="1d"):
+    torch.manual_seed(3)
+    m = convnext1d.ConvNeXt1D(depths=(1, 1, 2, 1), dims=(32, 64, 96, 128), variant=variant, stem_dim1=16, layer_scale_init_value=0.5,
+                              num_classes=37, keep8=keep8)
+    for p in m.parameters():
+        if p.dim() > 1:
+            torch.nn.init.normal_(p, std=0.1)
+    return m.cuda().train()
+
+
+@gpu
+@pytest.mark.parametrize("variant", ["1d", "2d"])
+def test_a_training_step_together(variant):
+    """loss() against F.cross_entropy of forward(), with and without checkpoints, on the same weights and batch."""
+    torch.backends.cudnn.allow_tf32 = torch.backends.cuda.matmul.allow_tf32 = False
+    img = torch.randn(4, 3, 64, 64, generator=torch.Generator().manual_seed(0)).cuda()
+    t = torch.tensor([3, 36, -100, 0], device="cuda")
+    models = [small(False, variant), small(True, variant)]
+    losses, grads = [], []
+    for m in models:
+        loss = m.loss(img, t, label_smoothing=0.1)
+        loss.backward()
+        want = F.cross_entropy(m(img).float(), t, label_smoothing=0.1)
+        assert abs(float(loss - want)) <= 1e-5 * float(want)
+        losses.append(loss.detach())
+        grads.append({k: p.grad for k, p in m.named_parameters() if p.grad is not None})
+    assert abs(float(losses[0] - losses[1])) <= 1e-5 * float(losses[0])          # the forward pass is the same arithmetic
+    assert grads[0].keys() == grads[1].keys()
+    for k, a in grads[0].items():
+        assert float((a - grads[1][k]).norm()) <= 0.05 * float(a.norm()) + 1e-6, k
+    m = models[0]
+    m.zero_grad(set_to_none=True)
+    F.cross_entropy(m(img), t, label_smoothing=0.1).backward()
+    for k, p in m.named_parameters():
+        if p.grad is not None:
+            assert float((p.grad - grads[0][k]).norm()) <= 1e-4 * float(p.grad.norm()) + 1e-7, k
+
+
+@gpu
+def test_a_captured_training_step_repeats():
+    m = small(True)
+    img = torch.randn(2, 3, 64, 64, device="cuda")
+    t = torch.tensor([1, 5], device="cuda")
+    params = [p for p in m.parameters() if p.requires_grad]
+
+    def step():
+        loss = m.loss(img, t)
+        return [loss.detach(), *[g for g in torch.autograd.grad(loss, params, allow_unused=True) if g is not None]]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        first = step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, captured))
+
+
+@gpu
+def test_memory_between_the_passes():
+    """A block's MLP keeps 1.06 bytes an element of x and of the hidden tensor: of 2 x (1 + 1 + 4 + 4) bytes, 5.3."""
+    for keep8, least, most in ((False, 19.0, 21.0), (True, 5.0, 5.6)):
+        block = convnext1d.Block1D(128).cuda().bfloat16().train()
+        block.keep8 = keep8
+        x = torch.randn(8, 56, 56, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        block._mlp(x * 1).sum().backward()                                     # the library's workspaces are there now
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = block._mlp(x * 1)                                                  # an input that only the block holds on to
+        torch.cuda.synchronize()
+        got = (torch.cuda.memory_allocated() - before - y.numel() * 2) / (x.numel())
+        assert least <= got <= most, (keep8, got)
+        del y
+
+
+@gpu
+def test_backbone_with_checkpoints():
+    torch.manual_seed(0)
+    m = backbone.ConvNeXt1DBackbone(depths=(1, 1, 1, 1), dims=(32, 64, 96, 128), stem_dim1=16, keep8=True).cuda().train()
+    x = torch.randn(1, 3, 75, 90, device="cuda")
+    with torch.no_grad():
+        want = m(x)
+    outs = m(x)
+    assert all(float((a - b).norm()) <= 1e-5 * float(b.norm()) for a, b in zip(outs, want))
+    sum(o.square().mean() for o in outs).backward()
+    for k, p in m.stages.named_parameters():
+        if not k.endswith("theta"):                                            # angles never receive a gradient
+            assert p.grad is not None and p.grad.isfinite().all(), k
+
+
+def test_refusals():
+    with pytest.raises(ValueError, match="keep8"):
+        convnext1d.ConvNeXt1D(variant="1dpp", depths=(1, 1, 1, 1), dims=(8, 8, 8, 8), keep8=True)
+    t = torch.zeros
+    ok = [t(4, 8), t(8), t(8), t(16, 8), t(16), t(8, 16), t(8)]
+    for i, bad, what in ((1, t(7), "weight has"), (2, t(7), "bias has"), (3, t(16, 7), "weight1"), (4, t(15), "bias1"), (5, t(8, 15), "weight2"),
+                         (6, t(9), "bias2")):
+        with pytest.raises(ValueError, match=what):
+            ops.mlp_keep8(*[bad if k == i else a for k, a in enumerate(ok)])
+    with pytest.raises(TypeError, match="same dtype"):
+        ops.mlp_keep8(*ok[:3], ok[3].bfloat16(), *ok[4:])
+    with pytest.raises(TypeError, match="float32 and bfloat16"):
+        ops.mlp_keep8(ok[0].half(), *ok[1:])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.mlp_keep8(*ok)

@@ -21,11 +21,27 @@ __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+// (cluster scope: some of the arrivals come from the other CTA of a pair)
 __device__ __forceinline__ bool bar_poll(uint64_t *bar, uint32_t parity) {
     uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
     return done != 0;
+}
+// The address of a CTA's variable in CTA `rank` of its cluster.
+__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_in(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %cluster_ctarank;" : "=r"(r)); return r; }
+// Every thread of both CTAs.
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Every wait has a limit of two seconds, thousands of times what a tile takes.  Running out raises the device flag and
 // `dead`, which ends the other waits of the CTA.
@@ -60,15 +76,30 @@ __device__ __forceinline__ void tma_load3(void *dst, const CUtensorMap *map, uin
                  "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
+// The same for one CTA of a pair: the bytes are counted by a barrier of the pair's first CTA (`bar`: its address there).
+__device__ __forceinline__ void tma_load3_pair(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                     smem_addr(dst)),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- tcgen05 ----------------------------------------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) {      // one whole warp
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// PAIR: two CTAs of a cluster work on one tile of twice the rows; each holds its half of both operands and of the accumulator,
+// and the first one's thread issues the products for both.
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) {      // one whole warp (of each CTA)
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
 }
-__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {        // the same warp
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {        // the same warp
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -79,18 +110,29 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ uint64_t operand(const void *p, uint32_t inner, uint32_t outer) {
     return (uint64_t)((smem_addr(p) & 0x3ffffu) >> 4) | (uint64_t)(inner >> 4) << 16 | (uint64_t)(outer >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
-// bf16 x bf16 -> fp32, M = 128
-template <int N, bool A_MN, bool B_MN> constexpr uint32_t instruction() {
-    return 1u << 4 | 1u << 7 | 1u << 10 | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) | (uint32_t)(N >> 3) << 17 | (128u >> 4) << 24;
+// bf16 x bf16 -> fp32
+template <int M, int N, bool A_MN, bool B_MN> constexpr uint32_t instruction() {
+    return 1u << 4 | 1u << 7 | 1u << 10 | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) | (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24;
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {      // one thread
-    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
-                 "r"(instr), "r"((uint32_t)add)
-                 : "memory");
+template <bool PAIR> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {      // one thread
+    if constexpr (PAIR)
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
+                     "r"(instr), "r"((uint32_t)add)
+                     : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
+                     "r"(instr), "r"((uint32_t)add)
+                     : "memory");
 }
-// The barrier gets one arrival when every product this thread has issued so far is done.
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// The barrier (of a pair: the one at this place in either CTA) gets one arrival when every product this thread has issued so
+// far is done.
+template <bool PAIR> __device__ __forceinline__ void commit(uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 // 32 columns of the warp's 32 accumulator rows: register i of a lane is column i of its row.
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {

@@ -6,6 +6,8 @@
 // ones (O1D_FLAG_PARAMS_BF16); otherwise, or when the library has no such kernel for the request, they are
 // converted to fp32 first.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -371,6 +373,19 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 Tensor linear_train(const Tensor &x, const Tensor &w, const Tensor &b) { return LinearFn::apply(x, w, b); }
 
 // ---- 8-bit activation checkpoints --------------------------------------------------------------------
+// Outputs and workspaces straight from the allocator, without the dispatcher (1.8 us a tensor, up to eight a call).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
+    return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+// Device memory for the length of a call (kernels on the current stream may still use it: it is only handed out again there).
+struct Scratch {
+    c10::DataPtr mem;
+    size_t bytes;
+    explicit Scratch(size_t n) : bytes(n) { if (n) mem = c10::cuda::CUDACachingAllocator::get()->allocate(n); }
+    void *get() const { return mem.get(); }
+};
+Tensor as_type(const Tensor &t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
+Tensor as_shape(const Tensor &t, const Tensor &like) { return t.sizes() == like.sizes() ? t : t.reshape(like.sizes()); }
 // All tensors of a call live on one device: the library launches there, on that device's current stream.
 void need_device(const Tensor &t, const Tensor &like, const char *what) {
     need_cuda(t);
@@ -391,12 +406,17 @@ struct Rows {
         if (C > INT32_MAX) throw py::value_error("rows of more than 2^31 - 1 elements are not supported");
     }
 };
+// A vector for a gradient; zeros where no kernel will write it.
+Tensor vector_of(int64_t n, at::ScalarType type, const Tensor &like, bool zero) {
+    Tensor t = fresh({n}, type, like);
+    return zero ? t.zero_() : t;
+}
 struct Kept { Tensor codes, ranges; };
 Kept empty_kept(const Tensor &x) {
     auto shape = x.sizes().vec();
     shape.back() = (shape.back() + 127) / 128;
     shape.push_back(2);
-    return {at::empty(x.sizes(), x.options().dtype(at::kByte)), at::empty(shape, x.options().dtype(at::kFloat))};
+    return {fresh(x.sizes(), at::kByte, x), fresh(shape, at::kFloat, x)};
 }
 void need_kept(const Tensor &codes, const Tensor &ranges) {
     if (codes.scalar_type() != at::kByte || ranges.scalar_type() != at::kFloat)
@@ -430,7 +450,7 @@ Tensor restore8(const Tensor &codes_, const Tensor &ranges_, bool bf16) {
     need_cuda(codes_); need_device(ranges_, codes_, "ranges");
     const c10::cuda::CUDAGuard guard(codes_.device());
     const Tensor codes = codes_.contiguous(), ranges = ranges_.contiguous();
-    Tensor y = at::empty(codes.sizes(), codes.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+    Tensor y = fresh(codes.sizes(), bf16 ? at::kBFloat16 : at::kFloat, codes);
     if (r.rows)
         check(o1d_restore8((const uint8_t *)ptr(codes), (const float *)ptr(ranges), y.data_ptr(), r.rows, (int)r.C, bf16 ? O1D_BF16 : O1D_F32, stream()),
               "o1d_restore8");
@@ -447,8 +467,8 @@ std::tuple<Tensor, Kept> gelu_forward(const Tensor &x_, const OptTensor &bias, b
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = x_.contiguous();
     Tensor b;
-    if (bias) b = is_bf16(*bias) ? bias->contiguous() : as_f32(*bias);
-    Tensor y = at::empty(x.sizes(), x.options());
+    if (bias) b = is_bf16(*bias) || bias->scalar_type() == at::kFloat ? bias->contiguous() : as_f32(*bias);
+    Tensor y = fresh(x.sizes(), x.scalar_type(), x);
     Kept k;
     if (keep) k = empty_kept(x);
     if (r.rows)
@@ -466,23 +486,17 @@ GeluGrads gelu_backward(const Kept &k, const Tensor &dy_, bool with_db, at::Scal
     const c10::cuda::CUDAGuard guard(dy_.device());
     const Tensor dy = dy_.contiguous();
     const int code = dtype_code(dy);
-    GeluGrads g{at::empty(dy.sizes(), dy.options()), {}, {}};
-    if (with_y) g.y = at::empty(dy.sizes(), dy.options());
+    GeluGrads g{fresh(dy.sizes(), dy.scalar_type(), dy), {}, {}};
+    if (with_y) g.y = fresh(dy.sizes(), dy.scalar_type(), dy);
     const bool db16 = db_type == at::kBFloat16;
-    Tensor ws;
-    size_t bytes = 0;
-    if (with_db) {
-        auto opts = dy.options().dtype(db16 ? at::kBFloat16 : at::kFloat);
-        g.db = r.rows ? at::empty({r.C}, opts) : at::zeros({r.C}, opts);
-        bytes = o1d_gelu_keep8_bwd_workspace_bytes(r.rows, (int)r.C);
-        ws = at::empty({(int64_t)std::max<size_t>(bytes, 4)}, dy.options().dtype(at::kByte));
-    }
+    const Scratch ws(with_db ? o1d_gelu_keep8_bwd_workspace_bytes(r.rows, (int)r.C) : 0);
+    if (with_db) g.db = vector_of(r.C, db16 ? at::kBFloat16 : at::kFloat, dy, r.rows == 0);
     if (r.rows)
         check(o1d_gelu_keep8_bwd((const uint8_t *)ptr(k.codes), (const float *)ptr(k.ranges), ptr(dy), g.dx.data_ptr(),
                                  with_y ? g.y.data_ptr() : nullptr, with_db ? (float *)g.db.data_ptr() : nullptr,
-                                 with_db ? ws.data_ptr() : nullptr, bytes, r.rows, (int)r.C, code | (db16 ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+                                 ws.get(), ws.bytes, r.rows, (int)r.C, code | (db16 ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
               "o1d_gelu_keep8_bwd");
-    if (with_db && g.db.scalar_type() != db_type) g.db = g.db.to(db_type);
+    if (with_db) g.db = as_type(g.db, db_type);
     return g;
 }
 
@@ -501,7 +515,7 @@ struct GeluKeep8Fn : torch::autograd::Function<GeluKeep8Fn> {
         const auto saved = ctx->get_saved_variables();
         const auto p = ctx->saved_data["p"].toIntVector();
         const bool need_db = p[2] && ctx->needs_input_grad(1);
-        GeluGrads g = gelu_backward({saved[0], saved[1]}, grads[0].to((at::ScalarType)p[0]), need_db, (at::ScalarType)p[1], false);
+        GeluGrads g = gelu_backward({saved[0], saved[1]}, as_type(grads[0], (at::ScalarType)p[0]), need_db, (at::ScalarType)p[1], false);
         if (ctx->needs_input_grad(0)) out[0] = g.dx;
         if (need_db) out[1] = g.db;
         return out;
@@ -524,8 +538,8 @@ std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, co
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = x_.contiguous();
     Params p(g, b);
-    Tensor y = at::empty(x.sizes(), x.options());
-    LnKept k{empty_kept(x), at::empty({r.rows, 2}, x.options().dtype(at::kFloat))};
+    Tensor y = fresh(x.sizes(), x.scalar_type(), x);
+    LnKept k{empty_kept(x), fresh({r.rows, 2}, at::kFloat, x)};
     if (r.rows)
         check(o1d_layernorm_keep8(ptr(x), (const float *)ptr(p.w), (const float *)ptr(p.b), y.data_ptr(), (uint8_t *)k.x.codes.data_ptr(),
                                   (float *)k.x.ranges.data_ptr(), (float *)k.stats.data_ptr(), r.rows, (int)r.C, (float)eps, code | p.flag(), stream()),
@@ -540,21 +554,20 @@ LnGrads ln_keep_backward(const LnKept &k, const Tensor &dy_, const Tensor &g, co
     const Tensor dy = dy_.contiguous();
     const int code = dtype_code(dy);
     Params p(g, b);
-    LnGrads out{at::empty(dy.sizes(), dy.options()), {}, {}, {}};
-    auto opts = dy.options().dtype(p.bf16 ? at::kBFloat16 : at::kFloat);
-    out.dg = r.rows ? at::empty({r.C}, opts) : at::zeros({r.C}, opts);
-    out.db = r.rows ? at::empty({r.C}, opts) : at::zeros({r.C}, opts);
-    if (with_y) out.y = at::empty(dy.sizes(), dy.options());
-    const size_t bytes = o1d_layernorm_keep8_bwd_workspace_bytes(r.rows, (int)r.C);
-    Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 4)}, dy.options().dtype(at::kByte));
+    LnGrads out{fresh(dy.sizes(), dy.scalar_type(), dy), {}, {}, {}};
+    const auto type = p.bf16 ? at::kBFloat16 : at::kFloat;
+    out.dg = vector_of(r.C, type, dy, r.rows == 0);
+    out.db = vector_of(r.C, type, dy, r.rows == 0);
+    if (with_y) out.y = fresh(dy.sizes(), dy.scalar_type(), dy);
+    const Scratch ws(o1d_layernorm_keep8_bwd_workspace_bytes(r.rows, (int)r.C));
     if (r.rows)
         check(o1d_layernorm_keep8_bwd((const uint8_t *)ptr(k.x.codes), (const float *)ptr(k.x.ranges), (const float *)ptr(k.stats), ptr(dy),
                                       (const float *)ptr(p.w), (const float *)ptr(p.b), out.dx.data_ptr(), with_y ? out.y.data_ptr() : nullptr,
-                                      (float *)out.dg.data_ptr(), (float *)out.db.data_ptr(), ws.data_ptr(), bytes, r.rows, (int)r.C,
+                                      (float *)out.dg.data_ptr(), (float *)out.db.data_ptr(), ws.get(), ws.bytes, r.rows, (int)r.C,
                                       code | p.flag(), stream()),
               "o1d_layernorm_keep8_bwd");
-    if (out.dg.scalar_type() != g.scalar_type()) out.dg = out.dg.to(g.scalar_type());
-    if (out.db.scalar_type() != b.scalar_type()) out.db = out.db.to(b.scalar_type());
+    out.dg = as_shape(as_type(out.dg, g.scalar_type()), g);
+    out.db = as_shape(as_type(out.db, b.scalar_type()), b);
     return out;
 }
 
@@ -571,10 +584,10 @@ struct LayerNormKeep8Fn : torch::autograd::Function<LayerNormKeep8Fn> {
         if (!grads[0].defined()) return out;
         need_first_order("layer_norm_keep8");
         const auto s = ctx->get_saved_variables();
-        LnGrads g = ln_keep_backward({{s[0], s[1]}, s[2]}, grads[0].to((at::ScalarType)ctx->saved_data["dtype"].toInt()), s[3], s[4], false);
+        LnGrads g = ln_keep_backward({{s[0], s[1]}, s[2]}, as_type(grads[0], (at::ScalarType)ctx->saved_data["dtype"].toInt()), s[3], s[4], false);
         if (ctx->needs_input_grad(0)) out[0] = g.dx;
-        if (ctx->needs_input_grad(1)) out[1] = g.dg.reshape(s[3].sizes());
-        if (ctx->needs_input_grad(2)) out[2] = g.db.reshape(s[4].sizes());
+        if (ctx->needs_input_grad(1)) out[1] = g.dg;
+        if (ctx->needs_input_grad(2)) out[2] = g.db;
         return out;
     }
 };
@@ -607,7 +620,7 @@ struct MlpKeep8Fn : torch::autograd::Function<MlpKeep8Fn> {
         need_first_order("mlp_keep8");
         const auto s = ctx->get_saved_variables();
         const auto p = ctx->saved_data["p"].toIntVector();
-        const Tensor &w1 = s[7], &w2 = s[8], dz = grads[0].to((at::ScalarType)p[0]);
+        const Tensor &w1 = s[7], &w2 = s[8], dz = as_type(grads[0], (at::ScalarType)p[0]);
         const Tensor dz2 = dz.reshape({-1, dz.size(-1)});
         const c10::cuda::CUDAGuard guard(dz.device());
         auto need = [&](int i) { return ctx->needs_input_grad(i); };
@@ -619,8 +632,8 @@ struct MlpKeep8Fn : torch::autograd::Function<MlpKeep8Fn> {
         if (!(need(0) || need(1) || need(2) || need(3))) return out;
         LnGrads n = ln_keep_backward({{s[0], s[1]}, s[2]}, h.dx.matmul(w1), s[3], s[4], need(3));
         if (need(0)) out[0] = n.dx;
-        if (need(1)) out[1] = n.dg.reshape(s[3].sizes());
-        if (need(2)) out[2] = n.db.reshape(s[4].sizes());
+        if (need(1)) out[1] = n.dg;
+        if (need(2)) out[2] = n.db;
         if (need(3)) out[3] = h.dx.reshape({-1, h.dx.size(-1)}).t().matmul(n.y.reshape({-1, n.y.size(-1)}));
         return out;
     }
@@ -669,11 +682,7 @@ struct XentShape {
         if (bias) need_device(*bias, x, "bias");
     }
 };
-Tensor xent_bias(const OptTensor &b) { return !b ? Tensor() : is_bf16(*b) ? b->contiguous() : as_f32(*b); }
-Tensor xent_workspace(const XentShape &s, const Tensor &like, int code, bool backward, size_t *bytes) {
-    *bytes = o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, backward);
-    return at::empty({(int64_t)std::max<size_t>(*bytes, 256)}, like.options().dtype(at::kByte));
-}
+Tensor xent_bias(const OptTensor &b) { return !b ? Tensor() : is_bf16(*b) || b->scalar_type() == at::kFloat ? b->contiguous() : as_f32(*b); }
 struct XentOut { Tensor loss, lse, count; };
 XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, const Tensor &target_, int64_t ignore, double smoothing,
                      int64_t reduction) {
@@ -681,17 +690,15 @@ XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, 
     const XentShape s(x_, w_, bias, target_, smoothing);
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = x_.contiguous(), w = w_.contiguous(), target = target_.contiguous(), b = xent_bias(bias);
-    const auto f32 = x.options().dtype(at::kFloat);
     const bool each = reduction == O1D_XENT_NONE;
-    XentOut o{each ? at::empty(target.sizes(), f32) : at::empty({}, f32), at::empty({s.N}, f32), each ? Tensor() : at::empty({}, f32)};
+    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), fresh({s.N}, at::kFloat, x), each ? Tensor() : fresh({}, at::kFloat, x)};
     if (s.N == 0) {                                       // the sum of nothing, the mean of nothing
         if (!each) { o.loss.fill_(reduction == O1D_XENT_SUM ? 0. : NAN); o.count.zero_(); }
         return o;
     }
-    size_t bytes;
-    Tensor ws = xent_workspace(s, x, code, false, &bytes);
+    const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, 0));
     check(o1d_linear_xent(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (float *)o.loss.data_ptr(), (float *)o.lse.data_ptr(),
-                          each ? nullptr : (float *)o.count.data_ptr(), ws.data_ptr(), bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing,
+                          each ? nullptr : (float *)o.count.data_ptr(), ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing,
                           (int)reduction, code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
           "o1d_linear_xent");
     return o;
@@ -718,23 +725,22 @@ struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
         const XentShape s(saved[0], saved[1], bias, saved[3], smoothing);
         const c10::cuda::CUDAGuard guard(saved[0].device());
         const Tensor x = saved[0].contiguous(), w = saved[1].contiguous(), target = saved[3].contiguous(), b = xent_bias(bias), lse = saved[4], count = saved[5];
-        const Tensor dloss = as_f32(grads[0]);
+        const Tensor dloss = as_type(grads[0], at::kFloat).contiguous();
         const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), b.defined() && ctx->needs_input_grad(2)};
         const bool none = s.N == 0;
-        if (need[0]) out[0] = at::empty(x.sizes(), x.options());
-        if (need[1]) out[1] = none ? at::zeros(w.sizes(), w.options()) : at::empty(w.sizes(), w.options());
-        if (need[2]) out[2] = none ? at::zeros(b.sizes(), b.options()) : at::empty(b.sizes(), b.options());
+        if (need[0]) out[0] = fresh(x.sizes(), x.scalar_type(), x);
+        if (need[1]) { out[1] = fresh(w.sizes(), w.scalar_type(), w); if (none) out[1].zero_(); }
+        if (need[2]) out[2] = vector_of(s.V, b.scalar_type(), x, none);
         if (!none) {
             const int code = dtype_code(x);
-            size_t bytes;
-            Tensor ws = xent_workspace(s, x, code, true, &bytes);
+            const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, 1));
             check(o1d_linear_xent_bwd(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (const float *)ptr(lse), (const float *)ptr(count),
                                       (const float *)ptr(dloss), need[0] ? out[0].data_ptr() : nullptr, need[1] ? out[1].data_ptr() : nullptr,
-                                      need[2] ? out[2].data_ptr() : nullptr, ws.data_ptr(), bytes, s.N, (int)s.D, (int)s.V, p[0], (float)smoothing,
+                                      need[2] ? out[2].data_ptr() : nullptr, ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, p[0], (float)smoothing,
                                       (int)p[1], code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
                   "o1d_linear_xent_bwd");
         }
-        if (need[2]) out[2] = out[2].to(bias->scalar_type()).reshape(bias->sizes());
+        if (need[2]) out[2] = as_shape(as_type(out[2], bias->scalar_type()), *bias);
         return out;
     }
 };

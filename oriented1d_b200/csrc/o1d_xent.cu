@@ -11,7 +11,7 @@ namespace {
 // sums, which is worth more than finding a piece in the L2 cache; 4096 x 1024 x 21841 bf16, gradient alone: 40 MB 557 us,
 // 80 MB 512, 128 MB 489, all 179 MB in one piece 452.
 constexpr long long kPieceBytes = 128ll << 20;
-constexpr int kMinSplitSteps = 8;                // K steps that a part of a split axis has at least
+constexpr int kMinSplitSteps = 16;               // K steps that a part of a split axis has at least (joining parts costs a launch)
 constexpr int kSlicesAtOnce = 512;               // column sums of more slices are added in two steps
 
 inline long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
@@ -50,13 +50,18 @@ int encode(CUtensorMap *map, const Mat &m, int box_rows) {
     return (int)r;
 }
 
-// Columns of a tile: 256 reads a third less for each product, 128 wastes less of a narrow matrix and gives twice the tiles.  Waves of
-// tiles times their steps, a step of 128 columns being 0.6 of one of 256 (measured: 0.25 and 0.42 us).
-int width_of(long long m, long long n, long long k, bool split, int sms) {
-    if (split) return 128;
-    const long long steps = cdiv(k, kXK) + 6, wide = cdiv((long long)cdiv(m, kXM) * cdiv(n, 256), sms) * steps * 5,
-                    narrow = cdiv((long long)cdiv(m, kXM) * cdiv(n, 128), sms) * steps * 3;
-    return narrow < wide ? 128 : 256;
+// How a product is tiled.  Waves of tiles times their steps; a step of 128 x 128 takes 0.6 of one of 128 x 256, a pair's
+// (256 x 256 on two SMs) 0.9 (measured: 0.25, 0.42 and 0.38 us).
+struct Shape { int tile_rows, bn, units; };      // units: CTAs, or pairs of them, that the device runs at once
+Shape shape_of(long long m, long long n, long long k, bool split, int sms) {
+    const Shape narrow{kXM, 128, sms}, wide{kXM, 256, sms}, pair{2 * kXM, 256, sms / 2};
+    if (split) return narrow;
+    const long long steps = cdiv(k, kXK) + 6;
+    auto cost = [&](const Shape &s, int weight) { return cdiv((long long)cdiv(m, s.tile_rows) * cdiv(n, s.bn), s.units) * steps * weight; };
+    const long long cn = cost(narrow, 6), cw = cost(wide, 10), cp = cost(pair, 9);
+    // (a pair's two epilogues wait for each other; with few steps a tile they are what counts: 133200 x 150 x 96 logits 30.6 us,
+    // one CTA a tile 25.9)
+    return k >= 512 && cp <= cw && cp <= cn ? pair : cn < cw ? narrow : wide;
 }
 
 struct Run {                 // of one call
@@ -70,19 +75,22 @@ struct Run {                 // of one call
     template <int KIND, bool SPLIT>
     int product(const Mat &ma, const Mat &mb, const XentParams &p) {
         constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
-        if constexpr (!SPLIT)
-            if (width_of(A_MN ? ma.cols : ma.rows, B_MN ? mb.cols : mb.rows, A_MN ? ma.rows : ma.cols, false, sms) == 256) return run<KIND, false, 256>(ma, mb, p);
-        return run<KIND, SPLIT, 128>(ma, mb, p);
+        if constexpr (!SPLIT) {
+            const Shape s = shape_of(A_MN ? ma.cols : ma.rows, B_MN ? mb.cols : mb.rows, A_MN ? ma.rows : ma.cols, false, sms);
+            if (s.tile_rows != kXM) return run<KIND, false, 256, true>(ma, mb, p);
+            if (s.bn == 256) return run<KIND, false, 256, false>(ma, mb, p);
+        }
+        return run<KIND, SPLIT, 128, false>(ma, mb, p);
     }
-    template <int KIND, bool SPLIT, int BN>
+    template <int KIND, bool SPLIT, int BN, bool PAIR>
     int run(const Mat &ma, const Mat &mb, XentParams p) {
-        using S = XentShape<SPLIT, BN>;
+        using S = XentShape<SPLIT, BN, PAIR>;
         constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
         CUtensorMap a_map, b_map;
-        if ((*enc = encode(&a_map, ma, A_MN ? kXK : kXM)) || (*enc = encode(&b_map, mb, B_MN ? kXK : BN))) return O1D_ERR_CUDA;
+        if ((*enc = encode(&a_map, ma, A_MN ? kXK : kXM)) || (*enc = encode(&b_map, mb, B_MN ? kXK : S::B_COLS))) return O1D_ERR_CUDA;
         p.M = (int)(A_MN ? ma.cols : ma.rows);
         p.N = (int)(B_MN ? mb.cols : mb.rows);
-        const long long m_tiles = cdiv(p.M, kXM), n_tiles = cdiv(p.N, BN);
+        const long long m_tiles = cdiv(p.M, S::TM), n_tiles = cdiv(p.N, BN);
         p.k_steps = cdiv(A_MN ? ma.rows : ma.cols, kXK);
         if (p.splits < 1) p.splits = 1;
         if (m_tiles * n_tiles * p.splits > 0x7fffffff) return O1D_ERR_UNSUPPORTED;
@@ -90,11 +98,22 @@ struct Run {                 // of one call
         p.n_tiles = (int)n_tiles;
         p.tiles = p.m_tiles * p.n_tiles * p.splits;
         p.err_flag = err_flag;
-        auto kern = xent_kernel<KIND, SPLIT, BN>;
+        auto kern = xent_kernel<KIND, SPLIT, BN, PAIR>;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
         if (e != cudaSuccess) return fail(e);
-        kern<<<p.tiles < sms ? p.tiles : sms, kXThreads, S::SMEM, st>>>(a_map, b_map, p);
-        e = cudaGetLastError();
+        const int units = PAIR ? sms / 2 : sms;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((p.tiles < units ? p.tiles : units) * (PAIR ? 2 : 1));
+        cfg.blockDim = dim3(kXThreads);
+        cfg.dynamicSmemBytes = S::SMEM;
+        cfg.stream = st;
+        cudaLaunchAttribute pair_attr;
+        pair_attr.id = cudaLaunchAttributeClusterDimension;
+        pair_attr.val.clusterDim.x = 2;
+        pair_attr.val.clusterDim.y = pair_attr.val.clusterDim.z = 1;
+        cfg.attrs = &pair_attr;
+        cfg.numAttrs = PAIR ? 1 : 0;
+        e = cudaLaunchKernelEx(&cfg, kern, a_map, b_map, p);
         return e == cudaSuccess ? O1D_OK : fail(e);
     }
 };
@@ -127,10 +146,18 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
     return e == cudaSuccess ? O1D_OK : r.fail(e);
 }
 
-// Forward: CTAs that a row tile's vocabulary is spread over, at most.
+bool few_rows(long long N, int D) { return N <= kFewRows && (N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8) * up_to(D, 8) * 4 <= kFewBytes; }
+int few_ctas(long long N, int V, int sms) {
+    const int need = cdiv(V, 8 * (N > 4 ? 2 : 4));
+    return need < 2 * sms ? need : 2 * sms;
+}
+
+// Forward: statistics that a row has, at most.
 int forward_slots(long long N, int D, int V, bool bf16, int sms) {
-    const long long n_tiles = cdiv(V, width_of(N, V, D, !bf16, sms)), tiles = cdiv(N, kXM) * n_tiles;
-    const long long ctas = tiles < sms ? tiles : sms, least = tiles / ctas;
+    if (few_rows(N, D)) return few_ctas(N, V, sms);
+    const Shape s = shape_of(N, V, D, !bf16, sms);
+    const long long n_tiles = cdiv(V, s.bn), tiles = cdiv(N, s.tile_rows) * n_tiles;
+    const long long ctas = tiles < s.units ? tiles : s.units, least = tiles / ctas;
     return 4 * (int)(cdiv(n_tiles, least) + 1);
 }
 
@@ -145,9 +172,9 @@ struct Cut {
     bool col_once() const { return pieces == 1 && col_blocks() == 1; }
 };
 int parts_of(long long m, long long n, long long k, bool split, int sms, bool adds) {
-    const int bn = width_of(m, n, k, split, sms);
-    const long long tiles = (long long)cdiv(m, kXM) * cdiv(n, bn), steps = cdiv(k, kXK);
-    long long s = sms / tiles;
+    const Shape shape = shape_of(m, n, k, split, sms);
+    const long long tiles = (long long)cdiv(m, shape.tile_rows) * cdiv(n, shape.bn), steps = cdiv(k, kXK);
+    long long s = shape.units / tiles;
     if (s > steps / kMinSplitSteps) s = steps / kMinSplitSteps;
     if (s < 1) s = 1;
     return s == 1 && !adds ? 0 : (int)s;
@@ -214,14 +241,50 @@ BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
     return b;
 }
 
+XentRows rows_of(const XentArgs &a, const XentParams &p, double2 *sums) {
+    XentRows q{};
+    q.part = p.part; q.part_sum = p.part_sum; q.target_logit = p.target_logit; q.target = a.target; q.ignore = a.ignore; q.rows = a.N;
+    q.smoothing = a.smoothing; q.V = a.V; q.mean = a.reduction == O1D_XENT_MEAN; q.lse = a.lse; q.sums = sums;
+    if (a.reduction == O1D_XENT_NONE) q.loss_rows = a.loss;
+    else { q.loss = a.loss; q.count = a.count; }
+    return q;
+}
+// The rows' statistics to the loss.  More lanes a row where it has many slots and there are few rows (their vocabulary spread over
+// all SMs); a lane's slots are far apart, so that with many rows one lane a row reads less (133200 rows, 8 slots: 5.5 us, 17 with
+// eight lanes).
+int reduce(Run &r, const XentRows &q) {
+    const int lanes = q.slots <= 4 || q.rows > 16384 ? 1 : q.slots <= 64 ? 8 : 32;
+    const int threads = q.rows * lanes <= 1024 ? 1024 : 256, blocks = cdiv(q.rows * lanes, threads);      // one block where it can be
+    if (lanes == 1) xent_rows_kernel<1><<<blocks, threads, 0, r.st>>>(q);
+    else if (lanes == 8) xent_rows_kernel<8><<<blocks, threads, 0, r.st>>>(q);
+    else xent_rows_kernel<32><<<blocks, threads, 0, r.st>>>(q);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && !q.loss_rows && blocks > 1) {
+        xent_total_kernel<<<1, 256, 0, r.st>>>(q.sums, blocks, q.mean, q.loss, q.count);
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? O1D_OK : r.fail(e);
+}
+
+template <typename T, int NR>
+void few(const XentArgs &a, const XentParams &p, int ctas, bool vec, cudaStream_t st) {
+    const int smem = NR * (int)up_to(a.D, 8) * 4;
+    if (vec) xent_few_kernel<T, NR, true><<<ctas, 256, smem, st>>>((const T *)a.x, (const T *)a.w, p, a.D);
+    else xent_few_kernel<T, NR, false><<<ctas, 256, smem, st>>>((const T *)a.x, (const T *)a.w, p, a.D);
+}
+template <typename T>
+void few(const XentArgs &a, const XentParams &p, int ctas, cudaStream_t st) {
+    const bool vec = a.D % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)a.w & 15) == 0;
+    if (a.N <= 1) few<T, 1>(a, p, ctas, vec, st);
+    else if (a.N <= 2) few<T, 2>(a, p, ctas, vec, st);
+    else if (a.N <= 4) few<T, 4>(a, p, ctas, vec, st);
+    else few<T, 8>(a, p, ctas, vec, st);
+}
+
 template <bool SPLIT>
 int forward(Run &r) {
     const XentArgs &a = r.a;
     unsigned char *ws = (unsigned char *)a.workspace;
-    Mat x, w;
-    int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
-    if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
-    if (rc) return rc;
     const int slots = forward_slots(a.N, a.D, a.V, a.bf16, r.sms);
     XentParams p{};
     p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
@@ -229,20 +292,27 @@ int forward(Run &r) {
     p.target_logit = (float *)ws; ws += up_to(4 * a.N, 256);
     p.smooth = a.smoothing > 0.f;
     p.part_sum = (float *)ws; ws += up_to(4ll * slots * a.N, 256);
-    double2 *sums = (double2 *)ws;
+    double2 *sums = (double2 *)ws; ws += up_to(16ll * cdiv(a.N, 8), 256);
     p.part_rows = a.N;
-    rc = r.product<XENT_LOGITS, SPLIT>(x, w, p);
-    if (rc) return rc;
-    const int n_tiles = cdiv(a.V, width_of(a.N, a.V, a.D, SPLIT, r.sms)), tiles = cdiv(a.N, kXM) * n_tiles, blocks = cdiv(a.N, 256);
-    const bool each = a.reduction == O1D_XENT_NONE;
-    xent_rows_kernel<<<blocks, 256, 0, r.st>>>(p.part, p.part_sum, p.target_logit, a.target, a.ignore, a.smoothing, a.V, a.N, a.N, n_tiles, tiles,
-                                               tiles < r.sms ? tiles : r.sms, a.lse, each ? a.loss : nullptr, each ? nullptr : sums);
-    cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess && !each) {
-        xent_total_kernel<<<1, 256, 0, r.st>>>(sums, blocks, a.reduction == O1D_XENT_MEAN, a.loss, a.count);
-        e = cudaGetLastError();
+    XentRows q = rows_of(a, p, sums);
+    q.slots = slots;
+    if (few_rows(a.N, a.D)) {
+        p.M = (int)a.N;
+        if (SPLIT) few<float>(a, p, slots, r.st); else few<__nv_bfloat16>(a, p, slots, r.st);
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? reduce(r, q) : r.fail(e);
     }
-    return e == cudaSuccess ? O1D_OK : r.fail(e);
+    Mat x, w;
+    int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
+    if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
+    if (!rc) rc = r.product<XENT_LOGITS, SPLIT>(x, w, p);
+    if (rc) return rc;
+    const Shape s = shape_of(a.N, a.V, a.D, SPLIT, r.sms);
+    q.tile_rows = s.tile_rows;
+    q.n_tiles = cdiv(a.V, s.bn);
+    q.tiles = cdiv(a.N, s.tile_rows) * q.n_tiles;
+    q.units = q.tiles < s.units ? q.tiles : s.units;
+    return reduce(r, q);
 }
 
 template <typename T>
@@ -350,8 +420,9 @@ size_t xent_workspace(const XentArgs &a, bool back, int sms) {
         return b.x + b.w + b.g + b.dx + b.dw + b.col + b.more;
     }
     const int slots = forward_slots(a.N, a.D, a.V, a.bf16, sms);
+    if (few_rows(a.N, a.D)) return (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) + up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
     return operand_bytes(a.N, a.D, a.bf16) + operand_bytes(a.V, a.D, a.bf16) + (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) +
-           up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 256), 256));
+           up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
 }
 int xent_forward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {
     Run r{a, sms, err_flag, st, cuda, enc};

@@ -35,11 +35,14 @@ constexpr int kXFinish = 16;                     // warps that finish tiles: fou
 constexpr int kXThreads = 128 + 32 * kXFinish;   // warp 0 loads, 1 multiplies, 2 owns tensor memory, 4-19 finish tiles
 constexpr int kXStaging = 2048;                  // bytes of a warp's store buffer: 32 rows of 64 bytes
 constexpr int kXChunk = 4;                       // fp32: stages of one accumulation
-// Tiles of 256 columns, or of 128: fp32 (its two accumulators would not fit twice), and bf16 products of few columns or too
-// few tiles to go round (see width_of in o1d_xent.cu).
-template <bool SPLIT, int BN_> struct XentShape {
-    static constexpr int BN = BN_, PL = SPLIT ? 3 : 1, STAGES = SPLIT ? 2 : BN == 256 ? 4 : 6;
-    static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = BN * kXK * 2, STAGE = PL * (A_BYTES + B_BYTES);
+// Tiles of 128 x 128 (fp32, whose two accumulators of 256 columns would not fit twice, and products with too few tiles to go
+// round), 128 x 256, or 256 x 256 on a pair of CTAs (each loads half of either operand: a third less than 128 x 256 reads
+// for the same products).  See shape_of in o1d_xent.cu.
+template <bool SPLIT, int BN_, bool PAIR> struct XentShape {
+    static constexpr int TM = PAIR ? 2 * kXM : kXM, BN = BN_, PL = SPLIT ? 3 : 1;
+    static constexpr int B_COLS = PAIR ? BN / 2 : BN;               // columns that one CTA loads
+    static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = B_COLS * kXK * 2, STAGE = PL * (A_BYTES + B_BYTES);
+    static constexpr int STAGES = SPLIT ? 2 : B_COLS == 256 ? 4 : 6;
     static constexpr int SMEM = STAGES * STAGE + kXFinish * kXStaging + 256 + 1024;
 };
 
@@ -150,13 +153,13 @@ __device__ __forceinline__ float column_sums(const float (&a)[32], int lane) {
     return t[0];
 }
 
-template <int KIND, bool SPLIT, int BN>
+template <int KIND, bool SPLIT, int BN, bool PAIR>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XentParams p) {
-    using S = XentShape<SPLIT, BN>;
+    using S = XentShape<SPLIT, BN, PAIR>;
     constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
     constexpr int PIECES = BN / 128;                 // of 32 columns, for each of the four warps that share 32 rows
-    constexpr uint32_t INSTR = tc::instruction<BN, A_MN, B_MN>();
+    constexpr uint32_t INSTR = tc::instruction<S::TM, BN, A_MN, B_MN>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *smem = raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u);
     char *staging = reinterpret_cast<char *>(smem + S::STAGES * S::STAGE);
@@ -165,24 +168,26 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(taken + 2);
     volatile int *dead = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // PAIR: `me` and `all` count pairs; rank 0 of a pair issues the products
+    const int rank = PAIR ? (int)tc::cluster_rank() : 0, me = PAIR ? blockIdx.x >> 1 : blockIdx.x, all = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; i++) { tc::bar_init(full + i, 1); tc::bar_init(empty + i, 1); }
-        for (int i = 0; i < 2; i++) { tc::bar_init(done + i, 1); tc::bar_init(taken + i, kXFinish); }
+        for (int i = 0; i < 2; i++) { tc::bar_init(done + i, 1); tc::bar_init(taken + i, PAIR ? 2 * kXFinish : kXFinish); }
         *dead = 0;
         tc::bar_init_fence();
         tc::tma_prefetch(&map_a);
         tc::tma_prefetch(&map_b);
     }
-    if (warp == 2) tc::tmem_alloc(tmem_slot, 512);
+    if (warp == 2) tc::tmem_alloc<PAIR>(tmem_slot, 512);
     tc::fence_before();
-    __syncthreads();
+    if (PAIR) tc::cluster_sync(); else __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    const int t_begin = KIND == XENT_LOGITS ? xent_run(blockIdx.x, p.tiles, gridDim.x) : blockIdx.x;
-    const int t_end = KIND == XENT_LOGITS ? xent_run(blockIdx.x + 1, p.tiles, gridDim.x) : p.tiles;
-    const int t_step = KIND == XENT_LOGITS ? 1 : gridDim.x;
+    const int t_begin = KIND == XENT_LOGITS ? xent_run(me, p.tiles, all) : me;
+    const int t_end = KIND == XENT_LOGITS ? xent_run(me + 1, p.tiles, all) : p.tiles;
+    const int t_step = KIND == XENT_LOGITS ? 1 : all;
 
     if (warp == 0 && lane == 0) {                                   // ---- loads
         int stage = 0, issued = 0;
@@ -192,37 +197,41 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const XentTile w = xent_tile<KIND>(p, t);
             for (int k = w.k0; k < w.k1; k++) {
                 if (!(ok = tc::bar_wait(empty + stage, phase ^ 1, dead, p.err_flag))) break;
-                tc::bar_expect(full + stage, S::STAGE);
                 unsigned char *a = smem + stage * S::STAGE, *b = a + S::PL * S::A_BYTES;
+                if (rank == 0) tc::bar_expect(full + stage, PAIR ? 2 * S::STAGE : S::STAGE);
+                const uint32_t bar = PAIR ? tc::in_cta(full + stage, 0) : 0;
+                auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
+                    if constexpr (PAIR) tc::tma_load3_pair(dst, map, bar, x, y, z);
+                    else tc::tma_load3(dst, map, full + stage, x, y, z);
+                };
+                const int row = w.m * S::TM + rank * kXM, col = w.n * BN + rank * S::B_COLS;
 #pragma unroll
                 for (int pl = 0; pl < S::PL; pl++) {
                     if (A_MN) {
 #pragma unroll
-                        for (int j = 0; j < kXM / 64; j++)
-                            tc::tma_load3(a + pl * S::A_BYTES + j * 8192, &map_a, full + stage, w.m * kXM + j * 64, k * kXK, pl);
+                        for (int j = 0; j < kXM / 64; j++) load(a + pl * S::A_BYTES + j * 8192, &map_a, row + j * 64, k * kXK, pl);
                     } else {
-                        tc::tma_load3(a + pl * S::A_BYTES, &map_a, full + stage, k * kXK, w.m * kXM, pl);
+                        load(a + pl * S::A_BYTES, &map_a, k * kXK, row, pl);
                     }
                     if (B_MN) {
 #pragma unroll
-                        for (int j = 0; j < BN / 64; j++)
-                            tc::tma_load3(b + pl * S::B_BYTES + j * 8192, &map_b, full + stage, w.n * BN + j * 64, k * kXK, pl);
+                        for (int j = 0; j < S::B_COLS / 64; j++) load(b + pl * S::B_BYTES + j * 8192, &map_b, col + j * 64, k * kXK, pl);
                     } else {
-                        tc::tma_load3(b + pl * S::B_BYTES, &map_b, full + stage, k * kXK, w.n * BN, pl);
+                        load(b + pl * S::B_BYTES, &map_b, k * kXK, col, pl);
                     }
                 }
                 issued++;
                 if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
             }
         }
-        if (!ok) {                                                  // copies in flight end before the CTA does
+        if (!ok && rank == 0) {                                     // copies in flight (a pair's all count here) end before the CTA does
             for (int i = 0; i < S::STAGES && i < issued; i++) {
                 stage = stage == 0 ? S::STAGES - 1 : stage - 1;
                 if (stage == S::STAGES - 1) phase ^= 1;
                 tc::bar_drain(full + stage, phase);
             }
         }
-    } else if (warp == 1 && lane == 0) {                            // ---- products
+    } else if (warp == 1 && lane == 0 && rank == 0) {               // ---- products
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
@@ -247,26 +256,26 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     for (int kk = 0; kk < kXK / 16; kk++) {         // 16 of K: 32 bytes of a K-major row, or 16 rows
                         const uint64_t oa = kk * (A_MN ? 128 : 2), ob = kk * (B_MN ? 128 : 2);
                         const bool add = k > c || kk > 0;
-                        tc::mma(d, da[0] + oa, db[0] + ob, INSTR, add);
+                        tc::mma<PAIR>(d, da[0] + oa, db[0] + ob, INSTR, add);
                         if constexpr (SPLIT) {
-                            tc::mma(d + 128, da[0] + oa, db[2] + ob, INSTR, add);
-                            tc::mma(d + 128, da[1] + oa, db[1] + ob, INSTR, true);
-                            tc::mma(d + 128, da[2] + oa, db[0] + ob, INSTR, true);
-                            tc::mma(d + 128, da[0] + oa, db[1] + ob, INSTR, true);
-                            tc::mma(d + 128, da[1] + oa, db[0] + ob, INSTR, true);
+                            tc::mma<PAIR>(d + 128, da[0] + oa, db[2] + ob, INSTR, add);
+                            tc::mma<PAIR>(d + 128, da[1] + oa, db[1] + ob, INSTR, true);
+                            tc::mma<PAIR>(d + 128, da[2] + oa, db[0] + ob, INSTR, true);
+                            tc::mma<PAIR>(d + 128, da[0] + oa, db[1] + ob, INSTR, true);
+                            tc::mma<PAIR>(d + 128, da[1] + oa, db[0] + ob, INSTR, true);
                         }
                     }
-                    tc::commit(empty + stage);
+                    tc::commit<PAIR>(empty + stage);
                     if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
                 }
                 if (!ok) break;
-                tc::commit(done + acc);
+                tc::commit<PAIR>(done + acc);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1;
             }
         }
         if (!ok) {                                                  // products in flight read shared memory: wait for them
-            tc::commit(done + acc);
+            tc::commit<PAIR>(done + acc);
             tc::bar_drain(done + acc, acc_phase);
         }
     } else if (warp >= 4) {                                         // ---- epilogue: a thread owns a quarter of a row
@@ -284,10 +293,13 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         float alpha = 1.f;
         if (KIND >= XENT_DX && p.out_kind < 2) alpha = xent_alpha(p.alpha_up, p.alpha_count, p.alpha);
 
+        auto release = [&](int i) {                                 // the accumulator may be written again
+            if (rank == 0) tc::bar_arrive(taken + i); else tc::bar_arrive_in(tc::in_cta(taken + i, 0));
+        };
         auto flush = [&]() {
-            const long long row = (long long)m_now * kXM + quarter * 32 + lane;
+            const long long row = (long long)m_now * S::TM + rank * kXM + quarter * 32 + lane;
             if (row >= p.M) return;
-            const int slot = ((int)blockIdx.x - xent_owner(m_now * p.n_tiles, p.tiles, gridDim.x)) * 4 + part;
+            const int slot = (me - xent_owner(m_now * p.n_tiles, p.tiles, all)) * 4 + part;
             p.part[(long long)slot * p.part_rows + row] = make_float2(mx, sum);
             if (p.smooth) p.part_sum[(long long)slot * p.part_rows + row] = total;
         };
@@ -299,7 +311,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             Ahead f{p.ignore, 0.f, 1.f, {}};
             if (KIND > XENT_GRAD || t >= t_end) return f;
             const XentTile w = xent_tile<KIND>(p, t);
-            const int row = w.m * kXM + quarter * 32 + lane;
+            const int row = w.m * S::TM + rank * kXM + quarter * 32 + lane;
             if (row < p.M) {
                 f.tgt = __ldg(p.target + row);
                 if (KIND == XENT_GRAD) {
@@ -317,7 +329,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         Ahead next = fetch(t_begin);
         for (int t = t_begin; ok && t < t_end; t += t_step) {
             const XentTile w = xent_tile<KIND>(p, t);
-            const int row = w.m * kXM + quarter * 32 + lane, n0 = w.n * BN;
+            const int r0 = w.m * S::TM + rank * kXM + quarter * 32, row = r0 + lane, n0 = w.n * BN;
             float bias[PIECES];
             if constexpr (KIND <= XENT_GRAD) {
                 if (w.m != m_now) {
@@ -355,7 +367,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         }
                     tc::fence_before();
                     __syncwarp();
-                    if (lane == 0) tc::bar_arrive(taken + acc);
+                    if (lane == 0) release(acc);
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1;
                 }
@@ -380,7 +392,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (pc == PIECES - 1) {
                         tc::fence_before();
                         __syncwarp();
-                        if (lane == 0) tc::bar_arrive(taken + acc);
+                        if (lane == 0) release(acc);
                         acc ^= 1;
                         if (acc == 0) acc_phase ^= 1;
                     }
@@ -451,7 +463,6 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                             for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i];
                         }
-                        const int r0 = w.m * kXM + quarter * 32;
                         if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + lane] = column_sums(a, lane);
 #pragma unroll
                         for (int pl = 0; pl < S::PL; pl++) {
@@ -473,7 +484,6 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         }
                     }
                 } else {
-                    const int r0 = w.m * kXM + quarter * 32;
                     if (p.out_kind == 0) {
                         uint4 out[4];
                         uint32_t *o = reinterpret_cast<uint32_t *>(out);
@@ -524,9 +534,9 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (KIND == XENT_LOGITS && ok && m_now >= 0) flush();
     }
     tc::fence_before();
-    __syncthreads();
+    if (PAIR) tc::cluster_sync(); else __syncthreads();             // a pair ends together: either reads and signals in the other
     tc::fence_after();
-    if (warp == 2) tc::tmem_free(tmem, 512);
+    if (warp == 2) tc::tmem_free<PAIR>(tmem, 512);
 }
 
 // One matrix as the bf16 planes that tensor copies read: fp32 cut into three, bf16 whose rows do not start on 16 bytes
@@ -569,44 +579,160 @@ xent_planes_kernel(const T *__restrict__ x, __nv_bfloat16 *__restrict__ planes, 
     }
 }
 
-// Loss of every row from the CTAs' statistics, and lse (in units of log2) for the backward pass.  Each block also sums its
-// rows' losses and counts the rows that have one.
+// LOGITS for up to eight rows (an evaluation of single images): a tile of 128 rows would be nearly all padding, and fp32 would
+// be cut into planes first.  What counts is to read w once, over all SMs: a warp takes CU classes at a time, its lanes 16 bytes
+// each, with the rows of x in shared memory, fp32 sums.  Lane n keeps the statistics of row n; a slot for each CTA.
+// Measured, one row, 768 x 1000 fp32: 4 us; tiles and planes 22 us.
+constexpr int kFewRows = 8, kFewBytes = 32768;         // rows; bytes of x in shared memory
+template <typename T, int NR, bool VEC>
 __global__ void __launch_bounds__(256)
-xent_rows_kernel(const float2 *__restrict__ part, const float *__restrict__ part_sum, const float *__restrict__ target_logit,
-                 const long long *__restrict__ target, long long ignore, float smoothing, int V, long long rows, long long part_rows, int n_tiles,
-                 int tiles, int ctas, float *__restrict__ lse, float *__restrict__ loss_rows, double2 *__restrict__ sums) {
-    const long long row = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    double loss = 0., counted = 0.;
-    if (row < rows) {
-        const int m = (int)(row / kXM);
-        const int slots = 4 * (xent_owner((m + 1) * n_tiles - 1, tiles, ctas) - xent_owner(m * n_tiles, tiles, ctas) + 1);
-        float top = __int_as_float(0xff800000), total = 0.f;
-        for (int s = 0; s < slots; s++) top = fmaxf(top, part[s * part_rows + row].x);
-        const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
-        float sum = 0.f;
-        for (int s = 0; s < slots; s++) {
-            const float2 v = part[s * part_rows + row];
-            sum += v.y * exp2f(v.x - ref);
-            if (smoothing > 0.f) total += part_sum[s * part_rows + row];
+xent_few_kernel(const T *__restrict__ x, const T *__restrict__ w, const XentParams p, int D) {
+    constexpr int CU = NR == 8 ? 2 : 4, VE = 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) float few_x[];         // [NR][D4], D4 = D to a multiple of 8
+    __shared__ float stats[3][8][kFewRows];
+    const int D4 = (D + 7) & ~7, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < NR * D4; i += 256) {
+        const int n = i / D4, c = i - n * D4;
+        few_x[i] = n < p.M && c < D ? ld(x + (long long)n * D + c) : 0.f;
+    }
+    __syncthreads();
+    const int row = lane < NR && lane < p.M ? lane : -1;
+    const long long tgt = row >= 0 ? __ldg(p.target + row) : -1;
+    float mx = __int_as_float(0xff800000), sum = 0.f, total = 0.f;
+    for (int v0 = (blockIdx.x * 8 + warp) * CU; v0 < p.V; v0 += gridDim.x * 8 * CU) {
+        float acc[CU][NR];
+#pragma unroll
+        for (int c = 0; c < CU; c++)
+#pragma unroll
+            for (int n = 0; n < NR; n++) acc[c][n] = 0.f;
+        if constexpr (VEC) {
+#pragma unroll 2
+            for (int d = lane * VE; d < D; d += 32 * VE) {
+                float f[CU][VE];
+#pragma unroll
+                for (int c = 0; c < CU; c++) {
+                    const uint4 q = v0 + c < p.V ? __ldg(reinterpret_cast<const uint4 *>(w + (long long)(v0 + c) * D + d)) : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if constexpr (sizeof(T) == 4) f[c][i] = __uint_as_float(u[i]);
+                        else { f[c][2 * i] = __uint_as_float(u[i] << 16); f[c][2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NR; n++)
+#pragma unroll
+                    for (int i = 0; i < VE; i += 4) {
+                        const float4 a = *reinterpret_cast<const float4 *>(few_x + n * D4 + d + i);
+#pragma unroll
+                        for (int c = 0; c < CU; c++)
+                            acc[c][n] = fmaf(f[c][i], a.x, fmaf(f[c][i + 1], a.y, fmaf(f[c][i + 2], a.z, fmaf(f[c][i + 3], a.w, acc[c][n]))));
+                    }
+            }
+        } else {
+            for (int d = lane; d < D; d += 32)
+#pragma unroll
+                for (int c = 0; c < CU; c++) {
+                    const float f = v0 + c < p.V ? ld(w + (long long)(v0 + c) * D + d) : 0.f;
+#pragma unroll
+                    for (int n = 0; n < NR; n++) acc[c][n] = fmaf(f, few_x[n * D4 + d], acc[c][n]);
+                }
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int c = 0; c < CU; c++)
+#pragma unroll
+                for (int n = 0; n < NR; n++) acc[c][n] += __shfl_xor_sync(0xffffffffu, acc[c][n], o);
+#pragma unroll
+        for (int c = 0; c < CU; c++) {
+            if (v0 + c >= p.V) break;
+            float l = acc[c][0];
+#pragma unroll
+            for (int n = 1; n < NR; n++) l = lane == n ? acc[c][n] : l;
+            l *= 1.4426950408889634f;
+            if (p.bias) l += 1.4426950408889634f * ld_param(p.bias, v0 + c, p.bias_bf16);
+            if (tgt == v0 + c) p.target_logit[row] = l;
+            total += l;
+            const float top = fmaxf(mx, l), ref = top == __int_as_float(0xff800000) ? 0.f : top;
+            sum = sum * exp2_fast(mx - ref) + exp2_fast(l - ref);
+            mx = top;
+        }
+    }
+    if (lane < NR) { stats[0][warp][lane] = mx; stats[1][warp][lane] = sum; stats[2][warp][lane] = total; }
+    __syncthreads();
+    if (threadIdx.x < NR && threadIdx.x < p.M) {
+        const int n = threadIdx.x;
+        float top = stats[0][0][n], s = 0.f, t = 0.f;
+#pragma unroll
+        for (int k = 1; k < 8; k++) top = fmaxf(top, stats[0][k][n]);
+        const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < 8; k++) { s += stats[1][k][n] * exp2_fast(stats[0][k][n] - ref); t += stats[2][k][n]; }
+        p.part[(long long)blockIdx.x * p.part_rows + n] = make_float2(top, s);
+        if (p.smooth) p.part_sum[(long long)blockIdx.x * p.part_rows + n] = t;
+    }
+}
+
+// Loss of every row from the statistics of its tiles' runs, and lse (in units of log2) for the backward pass; L lanes a row.  Each
+// block also sums its rows' losses and counts the rows that have one; a block alone finishes the reduction.
+struct XentRows {
+    const float2 *part;
+    const float *part_sum, *target_logit;
+    const long long *target;
+    long long ignore, rows;
+    float smoothing;
+    int V, tile_rows, n_tiles, tiles, units;     // as the runs were cut; tile_rows 0: `slots` for every row
+    int slots, mean;
+    float *lse, *loss_rows, *loss, *count;       // loss_rows, or loss and count
+    double2 *sums;
+};
+template <int L>
+__global__ void __launch_bounds__(1024)
+xent_rows_kernel(const XentRows a) {
+    const long long row = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / L;
+    const int lane = threadIdx.x % L;
+    const bool real = row < a.rows;
+    int slots = real ? a.slots : 0;
+    if (real && a.tile_rows) {
+        const int m = (int)(row / a.tile_rows);
+        slots = 4 * (xent_owner((m + 1) * a.n_tiles - 1, a.tiles, a.units) - xent_owner(m * a.n_tiles, a.tiles, a.units) + 1);
+    }
+    float top = __int_as_float(0xff800000), total = 0.f, sum = 0.f;
+    for (int s = lane; s < slots; s += L) top = fmaxf(top, a.part[s * a.rows + row].x);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
+    for (int s = lane; s < slots; s += L) {
+        const float2 v = a.part[s * a.rows + row];
+        sum += v.y * exp2f(v.x - ref);
+        if (a.smoothing > 0.f) total += a.part_sum[s * a.rows + row];
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    double loss = 0., counted = 0.;
+    if (real && lane == 0) {
         const float l2 = ref + log2f(sum);
-        lse[row] = l2;
-        const long long t = target[row];
+        a.lse[row] = l2;
+        const long long t = a.target[row];
         float out = 0.f;
-        if (t != ignore) {
-            if (t < 0 || t >= V) out = __int_as_float(0x7fffffff);
+        if (t != a.ignore) {
+            if (t < 0 || t >= a.V) out = __int_as_float(0x7fffffff);
             else {
-                out = smoothing < 1.f ? l2 - (1.f - smoothing) * target_logit[row] : l2;
-                if (smoothing > 0.f) out -= smoothing / (float)V * total;
+                out = a.smoothing < 1.f ? l2 - (1.f - a.smoothing) * a.target_logit[row] : l2;
+                if (a.smoothing > 0.f) out -= a.smoothing / (float)a.V * total;
                 out *= 0.6931471805599453f;
             }
             loss = out;
             counted = 1.;
         }
-        if (loss_rows) loss_rows[row] = out;
+        if (a.loss_rows) a.loss_rows[row] = out;
     }
-    if (!sums) return;
-    __shared__ double red[2][8];
+    if (a.loss_rows) return;
+    __shared__ double red[2][32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         loss += __shfl_xor_sync(0xffffffffu, loss, o);
@@ -615,9 +741,11 @@ xent_rows_kernel(const float2 *__restrict__ part, const float *__restrict__ part
     if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = loss; red[1][threadIdx.x >> 5] = counted; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        double a = 0., b = 0.;
-        for (int w = 0; w < 8; w++) { a += red[0][w]; b += red[1][w]; }
-        sums[blockIdx.x] = make_double2(a, b);
+        double s = 0., n = 0.;
+        for (int w = 0; w < blockDim.x / 32; w++) { s += red[0][w]; n += red[1][w]; }
+        if (gridDim.x > 1) { a.sums[blockIdx.x] = make_double2(s, n); return; }
+        *a.count = (float)n;
+        *a.loss = (float)(a.mean ? s / n : s);                               // no row counts: 0 / 0, as the mean of nothing
     }
 }
 __global__ void __launch_bounds__(256)
@@ -633,7 +761,7 @@ xent_total_kernel(const double2 *__restrict__ sums, int blocks, int mean, float 
     }
     if (threadIdx.x == 0) {
         *count = (float)red[1][0];
-        *loss = (float)(mean ? red[0][0] / red[1][0] : red[0][0]);        // no row counts: 0 / 0, as the mean of nothing
+        *loss = (float)(mean ? red[0][0] / red[1][0] : red[0][0]);
     }
 }
 

@@ -97,6 +97,7 @@ struct Run {                 // of one call
         p.m_tiles = (int)m_tiles;
         p.n_tiles = (int)n_tiles;
         p.tiles = p.m_tiles * p.n_tiles * p.splits;
+        p.along_n = p.M > p.N;
         p.err_flag = err_flag;
         auto kern = xent_kernel<KIND, SPLIT, BN, PAIR>;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);

@@ -51,6 +51,7 @@ struct XentParams {
     int m_tiles, n_tiles, k_steps;
     int splits;                  // OUT: parts of the K axis
     int tiles;                   // m_tiles * n_tiles * splits
+    int along_n;                 // neighbouring tiles share rows of A (the larger operand: B then stays in the L2 cache), not of B
     // LOGITS, GRAD
     const void *bias;
     int bias_bf16;
@@ -99,7 +100,7 @@ __device__ __forceinline__ XentTile xent_tile(const XentParams &p, int t) {
     } else {
         const int mn = p.m_tiles * p.n_tiles;
         r.split = t / mn; t -= r.split * mn;
-        r.n = t / p.m_tiles; r.m = t - r.n * p.m_tiles;
+        if (p.along_n) { r.m = t / p.n_tiles; r.n = t - r.m * p.n_tiles; } else { r.n = t / p.m_tiles; r.m = t - r.n * p.m_tiles; }
         r.k0 = (int)((long long)p.k_steps * r.split / p.splits); r.k1 = (int)((long long)p.k_steps * (r.split + 1) / p.splits);
     }
     return r;
@@ -150,6 +151,19 @@ __device__ __forceinline__ float column_sums(const float (&a)[32], int lane) {
 #pragma unroll
         for (int i = 0; i < o; i++) t[i] = (v ? t[i + o] : t[i]) + __shfl_xor_sync(0xffffffffu, v ? t[i] : t[i + o], o);
     }
+    return t[0];
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+// a[at], 0 <= at < 32, by halves.
+__device__ __forceinline__ float pick(const float (&a)[32], int at) {
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) t[i] = at & 16 ? a[i + 16] : a[i];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; i++) t[i] = at & o ? t[i + o] : t[i];
     return t[0];
 }
 
@@ -416,18 +430,17 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     const bool hit = __any_sync(0xffffffffu, at >= 0);
                     if constexpr (KIND == XENT_LOGITS) {
                         if (hit) {
-                            float l = 0.f;
-#pragma unroll
-                            for (int i = 0; i < 32; i++) l = at == i ? a[i] : l;
+                            const float l = pick(a, at);
                             if (at >= 0 && row < p.M) p.target_logit[row] = l;
                         }
                         if (p.smooth) {
 #pragma unroll
                             for (int i = 0; i < 32; i++) total += c0 + i < p.N ? a[i] : 0.f;
                         }
-                        float top = mx;
+                        float top = mx, top2 = a[0];
 #pragma unroll
-                        for (int i = 0; i < 32; i++) top = fmaxf(top, a[i]);
+                        for (int i = 0; i < 32; i += 4) { top = max3(top, a[i], a[i + 1]); top2 = max3(top2, a[i + 2], a[i + 3]); }
+                        top = fmaxf(top, top2);
                         const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
                         F2 s0 = both(0.f), s1 = both(0.f);
 #pragma unroll

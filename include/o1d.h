@@ -249,7 +249,7 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y,
 /* Softmax cross entropy of a linear classifier (the reference's head and criterion: models/convnext.py:495-610 and
  * the loss of engine.py:14-132), without the logits: with l = x w^T + bias,
  *   loss[n] = logsumexp(l[n]) - (1 - e) l[n, t_n] - (e / V) sum_v l[n, v],   e = label_smoothing in [0, 1].
- * x [N, D] and w [V, D] of type `dtype`, bias [V] (or NULL) fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16; target [N].
+ * x [N, D] and w [V, D] of type `dtype`, each starting on 16 bytes, bias [V] (or NULL) fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16; target [N].
  * A row whose target is ignore_index has no loss and no gradient; one whose target is outside [0, V) has a NaN loss
  * (and a NaN gradient).  reduction: O1D_XENT_NONE (loss [N]), _SUM, _MEAN (over the rows not ignored; loss [1]).
  * lse [N] and count [1] (not written for _NONE) are for the backward call.
@@ -295,7 +295,7 @@ int o1d_gelu_keep8_bwd(const uint8_t *codes, const float *ranges, const void *dy
 
 /* LayerNorm over rows of any length up to 8192, y = (x - mean) * rstd * gamma + beta, and the checkpoint of x in the
  * same pass; stats: [rows, 2] floats (mean, rstd), 8-byte aligned.  gamma, beta [C] fp32, or bf16 with
- * dtype | O1D_FLAG_PARAMS_BF16.  (models/convnext.py:28-56; o1d_layernorm_cl keeps x whole and takes rows of whole
+ * dtype | O1D_FLAG_PARAMS_BF16.  codes, ranges and stats NULL: nothing is kept.  (models/convnext.py:28-56; o1d_layernorm_cl keeps x whole and takes rows of whole
  * vectors only.) */
 int o1d_layernorm_keep8(const void *x, const float *gamma, const float *beta, void *y, uint8_t *codes, float *ranges,
                         float *stats, long long rows, int C, float eps, int dtype, void *stream);

@@ -1292,7 +1292,7 @@ bool bad_xent(const XentArgs &a, int dtype) {
            !(a.smoothing >= 0.f && a.smoothing <= 1.f) || a.reduction < O1D_XENT_NONE || a.reduction > O1D_XENT_MEAN;
 }
 int xent_call(const XentArgs &a, bool backward, void *stream) {
-    if (a.N > 0x7fffff00LL || a.V > 0x7fffff00) return O1D_ERR_UNSUPPORTED;
+    if (a.N > 0x7fffff00LL || a.V > 0x7fffff00 || (((uintptr_t)a.x | (uintptr_t)a.w) & 15)) return O1D_ERR_UNSUPPORTED;
     DeviceInfo d;
     int rc = device_info(&d), *flag = nullptr;
     if (!rc) rc = device_flag_ptr(&flag);
@@ -1417,7 +1417,7 @@ int o1d_layernorm_keep8(const void *x, const float *gamma, const float *beta, vo
                         long long rows, int C, float eps, int dtype, void *stream) {
     const int pbf16 = (dtype & O1D_FLAG_PARAMS_BF16) != 0;
     dtype &= ~O1D_FLAG_PARAMS_BF16;
-    if (!x || !gamma || !beta || !y || !codes || !ranges || !stats || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
+    if (!x || !gamma || !beta || !y || !codes != !ranges || !codes != !stats || bad_rows(rows, C, dtype)) return O1D_ERR_INVALID;
     LnKeepArgs a{};
     a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.codes = codes; a.ranges = ranges; a.stats = stats; a.rows = rows; a.C = C;
     a.eps = eps; a.pbf16 = pbf16;

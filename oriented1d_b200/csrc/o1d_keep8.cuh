@@ -471,7 +471,7 @@ ln_keep_kernel(const LnKeepArgs a) {
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             s[u] = rsqrtf(s[u] * inv_c + a.eps);
-            if (act[u] && w.lane == 0 && w.half == 0 && w.wt == 0) stats[u * R::ROWS + w.row] = make_float2(mean[u], s[u]);
+            if (a.codes && act[u] && w.lane == 0 && w.half == 0 && w.wt == 0) stats[u * R::ROWS + w.row] = make_float2(mean[u], s[u]);
         }
 #pragma unroll
         for (int j = 0; j < NG; j++) {
@@ -489,6 +489,7 @@ ln_keep_kernel(const LnKeepArgs a) {
                 for (int i = 0; i < 4; i++) o[i] = fma2(mul2(add2(f[u][i], both(-mean[u])), both(s[u])), gm[j][i], bt[j][i]);
                 store8<VEC, L>(y + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end[u], o);
             }
+            if (!a.codes) continue;
             keep_groups<VEC, L, UN>(f, c[j], end, q, range);
 #pragma unroll
             for (int u = 0; u < UN; u++) {

@@ -32,8 +32,8 @@ cudaError_t keep_launch(int kind, bool bf16, const KeepArgs &a, int sms, cudaStr
 struct LnKeepArgs {
     const void *x;           // forward: the input; backward: dy
     const void *gamma, *beta;
-    uint8_t *codes;
-    float *ranges, *stats;   // stats [rows][2]: mean, 1 / standard deviation
+    uint8_t *codes;          // forward: null, nothing is kept
+    float *ranges, *stats;   // stats [rows][2]: mean, 1 / standard deviation (forward: null with codes)
     void *y;                 // forward: the output; backward: may be null, else the output once more, from the codes
     void *dx, *dgamma, *dbeta;
     float *partial;          // backward: ln_keep_ctas() x 2 x C floats

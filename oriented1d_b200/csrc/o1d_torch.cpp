@@ -385,7 +385,13 @@ struct Scratch {
     void *get() const { return mem.get(); }
 };
 Tensor as_type(const Tensor &t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
-Tensor as_shape(const Tensor &t, const Tensor &like) { return t.sizes() == like.sizes() ? t : t.reshape(like.sizes()); }
+Tensor as_sizes(const Tensor &t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.reshape(sizes); }
+Tensor as_shape(const Tensor &t, const Tensor &like) { return as_sizes(t, like.sizes()); }
+// Contiguous, and starting on 16 bytes, as tensor copies and vector loads want it.
+Tensor as_vectors(const Tensor &t) {
+    const Tensor c = t.contiguous();
+    return ((uintptr_t)c.const_data_ptr() & 15) ? c.clone() : c;
+}
 // All tensors of a call live on one device: the library launches there, on that device's current stream.
 void need_device(const Tensor &t, const Tensor &like, const char *what) {
     need_cuda(t);
@@ -506,6 +512,7 @@ struct GeluKeep8Fn : torch::autograd::Function<GeluKeep8Fn> {
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({k.codes, k.ranges});
         ctx->saved_data["p"] = std::vector<int64_t>{(int64_t)x.scalar_type(), bias ? (int64_t)bias->scalar_type() : (int64_t)at::kFloat, bias.has_value()};
+        if (bias) ctx->saved_data["bias"] = bias->sizes().vec();
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
@@ -517,7 +524,7 @@ struct GeluKeep8Fn : torch::autograd::Function<GeluKeep8Fn> {
         const bool need_db = p[2] && ctx->needs_input_grad(1);
         GeluGrads g = gelu_backward({saved[0], saved[1]}, as_type(grads[0], (at::ScalarType)p[0]), need_db, (at::ScalarType)p[1], false);
         if (ctx->needs_input_grad(0)) out[0] = g.dx;
-        if (need_db) out[1] = g.db;
+        if (need_db) out[1] = as_sizes(g.db, ctx->saved_data["bias"].toIntVector());
         return out;
     }
 };
@@ -529,7 +536,8 @@ Tensor gelu_keep8(const Tensor &x, const OptTensor &bias) {
 }
 
 struct LnKept { Kept x; Tensor stats; };
-std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, const Tensor &b, double eps) {
+// The checkpoint and the statistics only when `keep` is set.
+std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, const Tensor &b, double eps, bool keep) {
     const Rows r(x_);
     const int code = dtype_code(x_);
     need_numel(g, r.C, "weight");
@@ -539,10 +547,12 @@ std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, co
     const Tensor x = x_.contiguous();
     Params p(g, b);
     Tensor y = fresh(x.sizes(), x.scalar_type(), x);
-    LnKept k{empty_kept(x), fresh({r.rows, 2}, at::kFloat, x)};
+    LnKept k;
+    if (keep) k = {empty_kept(x), fresh({r.rows, 2}, at::kFloat, x)};
+    auto out = [&](const Tensor &t) { return keep ? t.data_ptr() : nullptr; };
     if (r.rows)
-        check(o1d_layernorm_keep8(ptr(x), (const float *)ptr(p.w), (const float *)ptr(p.b), y.data_ptr(), (uint8_t *)k.x.codes.data_ptr(),
-                                  (float *)k.x.ranges.data_ptr(), (float *)k.stats.data_ptr(), r.rows, (int)r.C, (float)eps, code | p.flag(), stream()),
+        check(o1d_layernorm_keep8(ptr(x), (const float *)ptr(p.w), (const float *)ptr(p.b), y.data_ptr(), (uint8_t *)out(k.x.codes),
+                                  (float *)out(k.x.ranges), (float *)out(k.stats), r.rows, (int)r.C, (float)eps, code | p.flag(), stream()),
               "o1d_layernorm_keep8");
     return {y, k};
 }
@@ -573,7 +583,7 @@ LnGrads ln_keep_backward(const LnKept &k, const Tensor &dy_, const Tensor &g, co
 
 struct LayerNormKeep8Fn : torch::autograd::Function<LayerNormKeep8Fn> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
-        auto [y, k] = ln_keep_forward(x, g, b, eps);
+        auto [y, k] = ln_keep_forward(x, g, b, eps, true);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({k.x.codes, k.x.ranges, k.stats, g, b});
         ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
@@ -593,7 +603,7 @@ struct LayerNormKeep8Fn : torch::autograd::Function<LayerNormKeep8Fn> {
 };
 Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(g) || wants_grad(b))) return LayerNormKeep8Fn::apply(x, g, b, eps);
-    return std::get<0>(ln_keep_forward(x, g, b, eps));
+    return std::get<0>(ln_keep_forward(x, g, b, eps, false));
 }
 
 // ---- a block's LayerNorm -> Linear -> GELU -> Linear with 8-bit checkpoints -------------------------------
@@ -601,17 +611,18 @@ Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, doubl
 // of the first Linear's output (from which the activation is); the four matrix products stay with the GEMM library.
 Tensor sum_rows(const Tensor &dy, at::ScalarType dt) {
     const int64_t ve = dy.scalar_type() == at::kFloat ? 4 : 8;
-    Tensor s = dy.numel() && dy.size(-1) % ve == 0 ? colsum(dy, dt == at::kBFloat16) : dy.sum(0, false, at::kFloat);
-    return s.scalar_type() == dt ? s : s.to(dt);
+    return as_type(dy.numel() && dy.size(-1) % ve == 0 ? colsum(as_vectors(dy), dt == at::kBFloat16) : dy.sum(0, false, at::kFloat), dt);
 }
 struct MlpKeep8Fn : torch::autograd::Function<MlpKeep8Fn> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &g, const Tensor &b, const Tensor &w1, const Tensor &b1,
                           const Tensor &w2, const Tensor &b2, double eps) {
-        auto [y, kx] = ln_keep_forward(x, g, b, eps);
+        auto [y, kx] = ln_keep_forward(x, g, b, eps, true);
         auto [a, kh] = gelu_forward(at::linear(y, w1), b1, true);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({kx.x.codes, kx.x.ranges, kx.stats, g, b, kh.codes, kh.ranges, w1, w2});
         ctx->saved_data["p"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)b1.scalar_type(), (int64_t)b2.scalar_type()};
+        ctx->saved_data["b1"] = b1.sizes().vec();
+        ctx->saved_data["b2"] = b2.sizes().vec();
         return at::linear(a, w2, b2);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
@@ -624,9 +635,9 @@ struct MlpKeep8Fn : torch::autograd::Function<MlpKeep8Fn> {
         const Tensor dz2 = dz.reshape({-1, dz.size(-1)});
         const c10::cuda::CUDAGuard guard(dz.device());
         auto need = [&](int i) { return ctx->needs_input_grad(i); };
-        if (need(6)) out[6] = sum_rows(dz2, (at::ScalarType)p[2]);
+        if (need(6)) out[6] = as_sizes(sum_rows(dz2, (at::ScalarType)p[2]), ctx->saved_data["b2"].toIntVector());
         GeluGrads h = gelu_backward({s[5], s[6]}, dz.matmul(w2), need(4), (at::ScalarType)p[1], need(5));
-        if (need(4)) out[4] = h.db;
+        if (need(4)) out[4] = as_sizes(h.db, ctx->saved_data["b1"].toIntVector());
         if (need(5)) out[5] = dz2.t().matmul(h.y.reshape({-1, h.y.size(-1)}));
         h.y = Tensor();
         if (!(need(0) || need(1) || need(2) || need(3))) return out;
@@ -652,10 +663,11 @@ Tensor mlp_keep8(const Tensor &x, const Tensor &g, const Tensor &b, const Tensor
     need_cuda(x);
     for (const Tensor *t : {&g, &b, &w1, &b1, &w2, &b2}) need_device(*t, x, "a parameter");
     const c10::cuda::CUDAGuard guard(x.device());
+    const c10::impl::ExcludeDispatchKeyGuard as_given(c10::autocast_dispatch_keyset);      // the products' dtype is x's
     bool any = wants_grad(x);
     for (const Tensor *t : {&g, &b, &w1, &b1, &w2, &b2}) any = any || wants_grad(*t);
     if (at::GradMode::is_enabled() && any) return MlpKeep8Fn::apply(x, g, b, w1, b1, w2, b2, eps);
-    return at::linear(std::get<0>(gelu_forward(at::linear(std::get<0>(ln_keep_forward(x, g, b, eps)), w1), b1, false)), w2, b2);
+    return at::linear(std::get<0>(gelu_forward(at::linear(std::get<0>(ln_keep_forward(x, g, b, eps, false)), w1), b1, false)), w2, b2);
 }
 
 // ---- softmax cross entropy of a linear classifier ----------------------------------------------------
@@ -689,7 +701,7 @@ XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, 
     const int code = dtype_code(x_);
     const XentShape s(x_, w_, bias, target_, smoothing);
     const c10::cuda::CUDAGuard guard(x_.device());
-    const Tensor x = x_.contiguous(), w = w_.contiguous(), target = target_.contiguous(), b = xent_bias(bias);
+    const Tensor x = as_vectors(x_), w = as_vectors(w_), target = target_.contiguous(), b = xent_bias(bias);
     const bool each = reduction == O1D_XENT_NONE;
     XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), fresh({s.N}, at::kFloat, x), each ? Tensor() : fresh({}, at::kFloat, x)};
     if (s.N == 0) {                                       // the sum of nothing, the mean of nothing
@@ -724,7 +736,7 @@ struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
         const double smoothing = ctx->saved_data["smoothing"].toDouble();
         const XentShape s(saved[0], saved[1], bias, saved[3], smoothing);
         const c10::cuda::CUDAGuard guard(saved[0].device());
-        const Tensor x = saved[0].contiguous(), w = saved[1].contiguous(), target = saved[3].contiguous(), b = xent_bias(bias), lse = saved[4], count = saved[5];
+        const Tensor x = as_vectors(saved[0]), w = as_vectors(saved[1]), target = saved[3].contiguous(), b = xent_bias(bias), lse = saved[4], count = saved[5];
         const Tensor dloss = as_type(grads[0], at::kFloat).contiguous();
         const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), b.defined() && ctx->needs_input_grad(2)};
         const bool none = s.N == 0;

@@ -121,18 +121,15 @@ struct Run {                 // of one call
 
 // x or w as planes: in place where it can be, else in the workspace.
 struct Operand { bool copy; long long rows; int D, ld, planes; size_t bytes; };
-Operand operand_of(const void *p, long long rows, int D, bool bf16) {
+Operand operand_of(long long rows, int D, bool bf16) {
     Operand o;
-    o.copy = !bf16 || D % 8 != 0 || ((uintptr_t)p & 15);
+    o.copy = !bf16 || D % 8 != 0;
     o.rows = rows; o.D = D;
     o.planes = bf16 ? 1 : 3;
     o.ld = o.copy ? (int)up_to(D, 8) : D;
     o.bytes = o.copy ? (size_t)up_to((long long)o.planes * rows * o.ld * 2, 256) : 0;
     return o;
 }
-// Workspaces are sized for operands that need the copy: an address is not part of the request.
-size_t operand_bytes(long long rows, int D, bool bf16) { return operand_of((const void *)1, rows, D, bf16).bytes; }
-
 int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, Mat *m) {
     m->rows = o.rows; m->cols = o.D; m->ld = o.ld; m->plane = o.rows * o.ld; m->planes = o.planes;
     if (!o.copy) { m->p = (const __nv_bfloat16 *)src; return O1D_OK; }
@@ -140,7 +137,7 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
     *ws += o.bytes;
     m->p = to;
     const long long blocks = (o.rows + 7) / 8;
-    const int grid = (int)(blocks < (long long)r.sms * 16 ? blocks : (long long)r.sms * 16), vec = o.D % 4 == 0 && ((uintptr_t)src & 15) == 0;
+    const int grid = (int)(blocks < (long long)r.sms * 16 ? blocks : (long long)r.sms * 16), vec = o.D % 4 == 0;
     if (o.planes == 3) xent_planes_kernel<float><<<grid, 256, 0, r.st>>>((const float *)src, to, o.rows, o.D, o.ld, vec);
     else xent_planes_kernel<__nv_bfloat16><<<grid, 256, 0, r.st>>>((const __nv_bfloat16 *)src, to, o.rows, o.D, o.ld, vec);
     const cudaError_t e = cudaGetLastError();
@@ -230,8 +227,8 @@ struct BackwardBytes { size_t x, w, g, dx, dw, col, more; };
 BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
     const int planes = a.bf16 ? 1 : 3;
     BackwardBytes b;
-    b.x = operand_bytes(a.N, a.D, a.bf16);
-    b.w = operand_bytes(a.V, a.D, a.bf16);
+    b.x = operand_of(a.N, a.D, a.bf16).bytes;
+    b.w = operand_of(a.V, a.D, a.bf16).bytes;
     b.g = (size_t)up_to(2ll * planes * c.rows * c.ld, 256);
     // by rows, dx is complete with its piece; by vocabulary, dw is
     b.dx = (size_t)up_to(4ll * c.dx_parts * c.rows * a.D, 256);
@@ -275,7 +272,7 @@ void few(const XentArgs &a, const XentParams &p, int ctas, bool vec, cudaStream_
 }
 template <typename T>
 void few(const XentArgs &a, const XentParams &p, int ctas, cudaStream_t st) {
-    const bool vec = a.D % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)a.w & 15) == 0;
+    const bool vec = a.D % (16 / (int)sizeof(T)) == 0;
     if (a.N <= 1) few<T, 1>(a, p, ctas, vec, st);
     else if (a.N <= 2) few<T, 2>(a, p, ctas, vec, st);
     else if (a.N <= 4) few<T, 4>(a, p, ctas, vec, st);
@@ -304,8 +301,8 @@ int forward(Run &r) {
         return e == cudaSuccess ? reduce(r, q) : r.fail(e);
     }
     Mat x, w;
-    int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
-    if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
+    int rc = make_operand(r, a.x, operand_of(a.N, a.D, a.bf16), &ws, &x);
+    if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, a.bf16), &ws, &w);
     if (!rc) rc = r.product<XENT_LOGITS, SPLIT>(x, w, p);
     if (rc) return rc;
     const Shape s = shape_of(a.N, a.V, a.D, SPLIT, r.sms);
@@ -335,8 +332,8 @@ int backward(Run &r) {
     float *cols = (float *)ws; ws += b.col;
     float *more = (float *)ws; ws += b.more;
     Mat x, w;
-    int rc = make_operand(r, a.x, operand_of(a.x, a.N, a.D, a.bf16), &ws, &x);
-    if (!rc) rc = make_operand(r, a.w, operand_of(a.w, a.V, a.D, a.bf16), &ws, &w);
+    int rc = make_operand(r, a.x, operand_of(a.N, a.D, a.bf16), &ws, &x);
+    if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, a.bf16), &ws, &w);
     if (rc) return rc;
 
     const bool each = a.reduction == O1D_XENT_NONE;
@@ -422,7 +419,7 @@ size_t xent_workspace(const XentArgs &a, bool back, int sms) {
     }
     const int slots = forward_slots(a.N, a.D, a.V, a.bf16, sms);
     if (few_rows(a.N, a.D)) return (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) + up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
-    return operand_bytes(a.N, a.D, a.bf16) + operand_bytes(a.V, a.D, a.bf16) + (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) +
+    return operand_of(a.N, a.D, a.bf16).bytes + operand_of(a.V, a.D, a.bf16).bytes + (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) +
            up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
 }
 int xent_forward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {

@@ -207,7 +207,9 @@ def mlp_keep8(x, norm_weight, norm_bias, weight1, bias1, weight2, bias2, eps: fl
     """Linear2(GELU(Linear1(LayerNorm(x)))) of a block (models/convnext.py:308-313), keeping for the backward pass the
     8-bit checkpoints of layer_norm_keep8 and gelu_keep8 only: 1.06 bytes for each element of x and of the hidden tensor,
     in place of x, LayerNorm's output, and the hidden tensor before and after GELU.  The output is that of the separate
-    layers; the gradients are taken at the kept values.  The matrix products stay with the GEMM library."""
+    layers; the gradients are taken at the kept values.  The matrix products stay with the GEMM library, in x's dtype: the
+    Linear layers' parameters are brought to it where they differ."""
+    weight1, weight2, bias2 = (p if p.dtype == x.dtype else p.to(x.dtype) for p in (weight1, weight2, bias2))
     return ext.mlp_keep8(x, norm_weight, norm_bias, weight1, bias1, weight2, bias2, float(eps))
 
 

@@ -239,6 +239,48 @@ def test_layouts_views_and_empty_tensors():
 
 
 @gpu
+def test_parameters_of_any_shape():
+    """Only the number of elements counts; a gradient has its parameter's shape."""
+    x = make(6, 40, "fp32").cuda()
+    for shape in ((40,), (1, 40), (1, 1, 40), (5, 8)):
+        w, b = (torch.rand(shape, device="cuda").requires_grad_(True) for _ in range(2))
+        gb, = torch.autograd.grad(ops.gelu_keep8(x, b).sum(), b)
+        gw, gc = torch.autograd.grad(ops.layer_norm_keep8(x, w, b).sum(), (w, b))
+        assert gb.shape == gw.shape == gc.shape == shape
+        flat = b.detach().reshape(40).requires_grad_(True)
+        assert torch.equal(torch.autograd.grad(ops.gelu_keep8(x, flat).sum(), flat)[0], gb.reshape(40))
+
+
+@gpu
+def test_more_than_32_bits_of_elements():
+    """2.2e9 elements: the last rows are those of the same rows alone."""
+    rows, C = 67000, 33000
+    x = torch.empty(rows, C, device="cuda", dtype=torch.bfloat16)
+    x.normal_(generator=torch.Generator(device="cuda").manual_seed(0))
+    tail = x[-3:].clone()
+    codes, ranges = ops.keep8(x)
+    c, r = ops.keep8(tail)
+    assert torch.equal(codes[-3:], c) and torch.equal(ranges[-3:], r)
+    back = ops.restore8(codes, ranges, torch.bfloat16)
+    assert torch.equal(back[-3:], ops.restore8(c, r, torch.bfloat16))
+    del codes, ranges, back
+    b = torch.linspace(-1, 1, C, device="cuda")
+    y = ops.gelu_keep8(x.requires_grad_(True), b)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    t = tail.clone().requires_grad_(True)
+    z = ops.gelu_keep8(t, b)
+    assert torch.equal(y[-3:], z) and torch.equal(dx[-3:], torch.autograd.grad(z, t, tail)[0])
+    del y, dx
+    x = x.detach().reshape(-1)[:33000 * 67000 // 4096 * 4096].reshape(-1, 4096).requires_grad_(True)
+    w = torch.linspace(0.5, 1, 4096, device="cuda")
+    y = ops.layer_norm_keep8(x, w, w)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    t = x.detach()[-3:].clone().requires_grad_(True)
+    z = ops.layer_norm_keep8(t, w, w)
+    assert torch.equal(y[-3:], z) and torch.equal(dx[-3:], torch.autograd.grad(z, t, t.detach())[0])
+
+
+@gpu
 def test_sums_repeat_bit_for_bit_and_streams():
     x, dy = make(5000, 385, "bf16").cuda(), make(5000, 385, "bf16", 1).cuda()
     w, b = torch.rand(385, device="cuda"), torch.rand(385, device="cuda")
@@ -319,7 +361,8 @@ def test_entry_points_reject_bad_arguments():
     assert lib.o1d_restore8(p, None, p, 1, 8, 0, None) == 1
     assert lib.o1d_gelu_keep8(p, None, p, p, None, 1, 8, 0, None) == 1          # codes without ranges
     assert lib.o1d_gelu_keep8_bwd(p, p, p, None, None, None, None, 0, 1, 8, 0, None) == 1
-    assert lib.o1d_layernorm_keep8(p, p, p, p, p, p, None, 1, 8, 1e-6, 0, None) == 1
+    assert lib.o1d_layernorm_keep8(p, p, p, p, p, p, None, 1, 8, 1e-6, 0, None) == 1          # codes without statistics
+    assert lib.o1d_layernorm_keep8(p, p, p, p, None, p, p, 1, 8, 1e-6, 0, None) == 1
     assert lib.o1d_layernorm_keep8(p, p, p, p, p, p, p, 1, 8193, 1e-6, 0, None) == 2
     assert lib.o1d_layernorm_keep8_bwd(p, p, p, p, p, None, p, p, p, p, p, 64, 1, 8, 0, None) == 1      # y wanted, beta missing
     assert lib.o1d_layernorm_keep8_bwd(p, p, p, p, p, p, p, None, p, p, None, 0, 1, 8, 0, None) == 4

@@ -255,6 +255,21 @@ def test_only_the_gradients_asked_for_and_empty_batches():
 
 
 @gpu
+def test_more_than_32_bits_of_logits():
+    """70000 x 32768 logits, 2.3e9: the last rows' losses and gradients are those of the same rows alone."""
+    x, w, b, t = make(70000, 8, 32768, "bf16")
+    rows = ops.linear_cross_entropy(x.requires_grad_(True), w.requires_grad_(True), t, b, reduction="none")
+    up = torch.ones_like(rows)
+    dx, dw = torch.autograd.grad(rows, (x, w), up)
+    tail = x.detach()[-200:].clone().requires_grad_(True)
+    want = ops.linear_cross_entropy(tail, w.detach(), t[-200:], b, reduction="none")
+    assert float((rows[-200:] - want).detach().abs().max()) <= 1e-4
+    ref, = torch.autograd.grad(want, tail, up[-200:])
+    assert float((dx[-200:] - ref).float().norm()) <= 2.0 ** -8 * float(ref.float().norm())
+    assert dw.isfinite().all() and dx.isfinite().all()
+
+
+@gpu
 def test_repeats_bit_for_bit_streams_and_graphs():
     x, w, b, t = make(700, 96, 2000, "bf16", ignored=0.1)
     leaves = [v.requires_grad_(True) for v in (x, w, b)]

@@ -1288,7 +1288,7 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y, 
 extern "C++" {
 namespace {
 bool bad_xent(const XentArgs &a, int dtype) {
-    return !a.x || !a.w || !a.target || !a.lse || a.N <= 0 || a.D <= 0 || a.V <= 0 || (dtype != O1D_F32 && dtype != O1D_BF16) ||
+    return !a.x || !a.w || !a.target || a.N <= 0 || a.D <= 0 || a.V <= 0 || (dtype != O1D_F32 && dtype != O1D_BF16) ||
            !(a.smoothing >= 0.f && a.smoothing <= 1.f) || a.reduction < O1D_XENT_NONE || a.reduction > O1D_XENT_MEAN;
 }
 int xent_call(const XentArgs &a, bool backward, void *stream) {
@@ -1308,12 +1308,16 @@ int xent_call(const XentArgs &a, bool backward, void *stream) {
 }  // namespace
 }  // extern "C++"
 
-size_t o1d_linear_xent_workspace_bytes(long long N, int D, int V, int dtype, int backward) {
+size_t o1d_linear_xent_workspace_bytes(long long N, int D, int V, int dtype, int pass) {
     XentArgs a{};
+    float any;
     a.N = N; a.D = D; a.V = V; a.bf16 = dtype == O1D_BF16;
+    a.lse = pass == O1D_XENT_EVALUATION ? nullptr : &any;                 // (a request with or without it; not read)
     DeviceInfo d;
-    if (N <= 0 || D <= 0 || V <= 0 || N > 0x7fffff00LL || V > 0x7fffff00 || (dtype != O1D_F32 && dtype != O1D_BF16) || device_info(&d)) return 0;
-    return xent_workspace(a, backward != 0, d.sms);
+    if (N <= 0 || D <= 0 || V <= 0 || N > 0x7fffff00LL || V > 0x7fffff00 || (dtype != O1D_F32 && dtype != O1D_BF16) ||
+        pass < O1D_XENT_FORWARD || pass > O1D_XENT_EVALUATION || device_info(&d))
+        return 0;
+    return xent_workspace(a, pass == O1D_XENT_BACKWARD, d.sms);
 }
 
 int o1d_linear_xent(const void *x, const void *w, const void *bias, const long long *target, float *loss, float *lse, float *count,
@@ -1338,7 +1342,7 @@ int o1d_linear_xent_bwd(const void *x, const void *w, const void *bias, const lo
     a.x = x; a.w = w; a.bias = bias; a.target = target; a.N = N; a.D = D; a.V = V; a.bf16 = dtype == O1D_BF16; a.ignore = ignore_index;
     a.smoothing = label_smoothing; a.reduction = reduction; a.lse = const_cast<float *>(lse); a.count = const_cast<float *>(count);
     a.dloss = dloss; a.dx = dx; a.dw = dw; a.db = db; a.workspace = workspace; a.workspace_bytes = workspace_bytes;
-    if (bad_xent(a, dtype) || !dloss || (!count && reduction == O1D_XENT_MEAN)) return O1D_ERR_INVALID;
+    if (bad_xent(a, dtype) || !lse || !dloss || (!count && reduction == O1D_XENT_MEAN)) return O1D_ERR_INVALID;
     return xent_call(a, true, stream);
 }
 

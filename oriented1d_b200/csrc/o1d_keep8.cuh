@@ -37,13 +37,26 @@ __device__ __forceinline__ void lane_sums(float (&v)[U]) {
 
 // Exact GELU and its slope without erff, of which the passes below would be nothing else (20 instructions a value each).
 //   P(-|h|) = erfc(z)/2,  z = |h|/sqrt 2,  erfc(z) = t q(t) exp(-z^2),  t = 1/(1 + 0.33 z)
-// the form of Abramowitz and Stegun 7.1.26, with a polynomial q of degree 7 fitted to exp(z^2) erfc(z) on 0 <= z <= 10 by
-// iterated weighted least squares: relative error 1e-7 in both tails.  One reciprocal and one exponential, which the slope
+// the form of Abramowitz and Stegun 7.1.26, with a polynomial q fitted to exp(z^2) erfc(z) on 0 <= z <= 10 by iterated weighted
+// least squares: of degree 7 for bf16 (relative error 1e-7, in the tail too), of degree 9 for fp32 (3e-9; an error of the fit is
+// alike for like values, and the bias gradient adds them up).  One reciprocal and one exponential, which the slope
 // needs anyway.
 // For a pair of values: m = |h| (at most 64), q = -P(-|h|), bell = exp(-h^2/2).  Then GELU(h) = max(h, 0) + m q and
 // GELU'(h) = 1/2 + sign(h) (1/2 + q + m bell / sqrt(2 pi)).
 struct Normal { F2 m, q, bell; };
+template <bool FP32>
 __device__ __forceinline__ Normal normal_of(F2 h) {
+    constexpr int N = FP32 ? 10 : 8;
+    constexpr float fit[10] = {FP32 ? 0.1861456036567688f : 0.1863577961921692f,
+                               FP32 ? 0.1870007961988449f : 0.1829560101032257f,
+                               FP32 ? 0.16811791062355042f : 0.2012234777212143f,
+                               FP32 ? 0.1999620497226715f : 0.04722202196717262f,
+                               FP32 ? -0.029606999829411507f : 0.40849733352661133f,
+                               FP32 ? 0.45996400713920593f : -0.35114675760269165f,
+                               FP32 ? -0.5105049014091492f : 0.4602353572845459f,
+                               FP32 ? 0.5900521874427795f : -0.1353452503681183f,
+                               FP32 ? -0.3076556622982025f : 0.f,
+                               FP32 ? 0.05652497336268425f : 0.f};
     const float2 a = apart(h);
     const F2 m = two(fminf(fabsf(a.x), 64.f), fminf(fabsf(a.y), 64.f));      // (q is 0 there: an infinity times it would be NaN)
     const float2 d = apart(fma2(m, both(0.33f * 0.70710678f), both(1.f))), z = apart(mul2(mul2(h, h), both(-0.72134752f)));
@@ -53,13 +66,9 @@ __device__ __forceinline__ Normal normal_of(F2 h) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(z.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(z.y));
     const F2 t = two(r.x, r.y), bell = two(e.x, e.y);
-    F2 q = fma2(t, both(0.5f * 0.1353452503681183f), both(-0.5f * 0.4602353572845459f));
-    q = fma2(t, q, both(0.5f * 0.35114675760269165f));
-    q = fma2(t, q, both(-0.5f * 0.40849733352661133f));
-    q = fma2(t, q, both(-0.5f * 0.04722202196717262f));
-    q = fma2(t, q, both(-0.5f * 0.2012234777212143f));
-    q = fma2(t, q, both(-0.5f * 0.1829560101032257f));
-    q = fma2(t, q, both(-0.5f * 0.1863577961921692f));
+    F2 q = both(-0.5f * fit[N - 1]);
+#pragma unroll
+    for (int i = N - 2; i >= 0; i--) q = fma2(t, q, both(-0.5f * fit[i]));
     return {m, mul2(q, mul2(t, bell)), bell};
 }
 __device__ __forceinline__ F2 gelu_of(F2 h, const Normal &n) {
@@ -296,7 +305,7 @@ keep_kernel(const KeepArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         f[u][i] = add2(f[u][i], b[i]);
-                        v[i] = gelu_of(f[u][i], normal_of(f[u][i]));
+                        v[i] = gelu_of(f[u][i], normal_of<sizeof(T) == 4>(f[u][i]));
                     }
                     store8<VEC, L>(y + (long long)(u * ROWS) * C + off, c, end[u], v);
                 }
@@ -321,7 +330,7 @@ keep_kernel(const KeepArgs a) {
                     unpack8<T, VEC>(raw[u], f);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const Normal n = normal_of(v[i]);
+                        const Normal n = normal_of<sizeof(T) == 4>(v[i]);
                         d[i] = mul2(f[i], gelu_slope(v[i], n));
                         sum[i] = add2(sum[i], d[i]);             // rows that do not exist add zeros; columns are never read
                         if (a.y) v[i] = gelu_of(v[i], n);

@@ -696,20 +696,21 @@ struct XentShape {
 };
 Tensor xent_bias(const OptTensor &b) { return !b ? Tensor() : is_bf16(*b) || b->scalar_type() == at::kFloat ? b->contiguous() : as_f32(*b); }
 struct XentOut { Tensor loss, lse, count; };
+// lse only when `train` is set.
 XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, const Tensor &target_, int64_t ignore, double smoothing,
-                     int64_t reduction) {
+                     int64_t reduction, bool train) {
     const int code = dtype_code(x_);
     const XentShape s(x_, w_, bias, target_, smoothing);
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = as_vectors(x_), w = as_vectors(w_), target = target_.contiguous(), b = xent_bias(bias);
     const bool each = reduction == O1D_XENT_NONE;
-    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), fresh({s.N}, at::kFloat, x), each ? Tensor() : fresh({}, at::kFloat, x)};
+    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), train ? fresh({2, s.N}, at::kFloat, x) : Tensor(), each ? Tensor() : fresh({}, at::kFloat, x)};
     if (s.N == 0) {                                       // the sum of nothing, the mean of nothing
         if (!each) { o.loss.fill_(reduction == O1D_XENT_SUM ? 0. : NAN); o.count.zero_(); }
         return o;
     }
-    const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, 0));
-    check(o1d_linear_xent(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (float *)o.loss.data_ptr(), (float *)o.lse.data_ptr(),
+    const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, train ? O1D_XENT_FORWARD : O1D_XENT_EVALUATION));
+    check(o1d_linear_xent(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (float *)o.loss.data_ptr(), train ? (float *)o.lse.data_ptr() : nullptr,
                           each ? nullptr : (float *)o.count.data_ptr(), ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing,
                           (int)reduction, code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
           "o1d_linear_xent");
@@ -719,7 +720,7 @@ XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, 
 struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target,
                           int64_t ignore, double smoothing, int64_t reduction) {
-        XentOut o = xent_forward(x, w, bias, target, ignore, smoothing, reduction);
+        XentOut o = xent_forward(x, w, bias, target, ignore, smoothing, reduction, true);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, w, bias ? *bias : Tensor(), target, o.lse, o.count});
         ctx->saved_data["p"] = std::vector<int64_t>{ignore, reduction};
@@ -745,7 +746,7 @@ struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
         if (need[2]) out[2] = vector_of(s.V, b.scalar_type(), x, none);
         if (!none) {
             const int code = dtype_code(x);
-            const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, 1));
+            const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, O1D_XENT_BACKWARD));
             check(o1d_linear_xent_bwd(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (const float *)ptr(lse), (const float *)ptr(count),
                                       (const float *)ptr(dloss), need[0] ? out[0].data_ptr() : nullptr, need[1] ? out[1].data_ptr() : nullptr,
                                       need[2] ? out[2].data_ptr() : nullptr, ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, p[0], (float)smoothing,
@@ -759,7 +760,7 @@ struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
 Tensor linear_xent(const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target, int64_t ignore, double smoothing, int64_t reduction) {
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(bias)))
         return LinearXentFn::apply(x, w, bias, target, ignore, smoothing, reduction);
-    return xent_forward(x, w, bias, target, ignore, smoothing, reduction).loss;
+    return xent_forward(x, w, bias, target, ignore, smoothing, reduction, false).loss;
 }
 
 Tensor conv(const Tensor &x, const Tensor &w, const Tensor &theta, const OptTensor &bias, const Tensor &host, const Tensor &dev,

@@ -53,9 +53,10 @@ int encode(CUtensorMap *map, const Mat &m, int box_rows) {
 // How a product is tiled.  Waves of tiles times their steps; a step of 128 x 128 takes 0.6 of one of 128 x 256, a pair's
 // (256 x 256 on two SMs) 0.9 (measured: 0.25, 0.42 and 0.38 us).
 struct Shape { int tile_rows, bn, units; };      // units: CTAs, or pairs of them, that the device runs at once
-Shape shape_of(long long m, long long n, long long k, bool split, int sms) {
+// `narrow_only`: operands of more than one plane.
+Shape shape_of(long long m, long long n, long long k, bool narrow_only, int sms) {
     const Shape narrow{kXM, 128, sms}, wide{kXM, 256, sms}, pair{2 * kXM, 256, sms / 2};
-    if (split) return narrow;
+    if (narrow_only) return narrow;
     const long long steps = cdiv(k, kXK) + 6;
     auto cost = [&](const Shape &s, int weight) { return cdiv((long long)cdiv(m, s.tile_rows) * cdiv(n, s.bn), s.units) * steps * weight; };
     const long long cn = cost(narrow, 6), cw = cost(wide, 10), cp = cost(pair, 9);
@@ -72,19 +73,19 @@ struct Run {                 // of one call
     int *enc;
     int fail(cudaError_t e) { *cuda = e; return O1D_ERR_CUDA; }
 
-    template <int KIND, bool SPLIT>
+    template <int KIND, int MODE>
     int product(const Mat &ma, const Mat &mb, const XentParams &p) {
         constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
-        if constexpr (!SPLIT) {
+        if constexpr (MODE == XENT_BF16) {
             const Shape s = shape_of(A_MN ? ma.cols : ma.rows, B_MN ? mb.cols : mb.rows, A_MN ? ma.rows : ma.cols, false, sms);
-            if (s.tile_rows != kXM) return run<KIND, false, 256, true>(ma, mb, p);
-            if (s.bn == 256) return run<KIND, false, 256, false>(ma, mb, p);
+            if (s.tile_rows != kXM) return run<KIND, MODE, 256, true>(ma, mb, p);
+            if (s.bn == 256) return run<KIND, MODE, 256, false>(ma, mb, p);
         }
-        return run<KIND, SPLIT, 128, false>(ma, mb, p);
+        return run<KIND, MODE, 128, false>(ma, mb, p);
     }
-    template <int KIND, bool SPLIT, int BN, bool PAIR>
+    template <int KIND, int MODE, int BN, bool PAIR>
     int run(const Mat &ma, const Mat &mb, XentParams p) {
-        using S = XentShape<SPLIT, BN, PAIR>;
+        using S = XentShape<KIND, MODE, BN, PAIR>;
         constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
         CUtensorMap a_map, b_map;
         if ((*enc = encode(&a_map, ma, A_MN ? kXK : kXM)) || (*enc = encode(&b_map, mb, B_MN ? kXK : S::B_COLS))) return O1D_ERR_CUDA;
@@ -99,7 +100,7 @@ struct Run {                 // of one call
         p.tiles = p.m_tiles * p.n_tiles * p.splits;
         p.along_n = p.M > p.N;
         p.err_flag = err_flag;
-        auto kern = xent_kernel<KIND, SPLIT, BN, PAIR>;
+        auto kern = xent_kernel<KIND, MODE, BN, PAIR>;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
         if (e != cudaSuccess) return fail(e);
         const int units = PAIR ? sms / 2 : sms;
@@ -144,6 +145,12 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
     return e == cudaSuccess ? O1D_OK : r.fail(e);
 }
 
+// G in two planes?  Up to 2^30 products, 2 us of a whole GPU, the second plane costs latency at most; and there are then few rows
+// or classes over which the rounding of G to one plane could average out (without: errors of dx up to 1.8 times those of the
+// same sums in fp32, rounded to bf16 once).
+bool fine_of(const XentArgs &a) { return a.bf16 && (double)a.N * a.V * a.D <= (double)(1ll << 30); }
+int planes_of(const XentArgs &a) { return !a.bf16 ? 3 : fine_of(a) ? 2 : 1; }
+
 bool few_rows(long long N, int D) { return N <= kFewRows && (N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8) * up_to(D, 8) * 4 <= kFewBytes; }
 int few_ctas(long long N, int V, int sms) {
     const int need = cdiv(V, 8 * (N > 4 ? 2 : 4));
@@ -151,10 +158,10 @@ int few_ctas(long long N, int V, int sms) {
 }
 
 // Forward: statistics that a row has, at most.
-int forward_slots(long long N, int D, int V, bool bf16, int sms) {
-    if (few_rows(N, D)) return few_ctas(N, V, sms);
-    const Shape s = shape_of(N, V, D, !bf16, sms);
-    const long long n_tiles = cdiv(V, s.bn), tiles = cdiv(N, s.tile_rows) * n_tiles;
+int forward_slots(const XentArgs &a, int sms) {
+    if (few_rows(a.N, a.D) && !a.lse) return few_ctas(a.N, a.V, sms);
+    const Shape s = shape_of(a.N, a.V, a.D, !a.bf16, sms);
+    const long long n_tiles = cdiv(a.V, s.bn), tiles = cdiv(a.N, s.tile_rows) * n_tiles;
     const long long ctas = tiles < s.units ? tiles : s.units, least = tiles / ctas;
     return 4 * (int)(cdiv(n_tiles, least) + 1);
 }
@@ -169,8 +176,8 @@ struct Cut {
     int col_blocks() const { return cdiv(cdiv(rows, 32), kSlicesAtOnce); }
     bool col_once() const { return pieces == 1 && col_blocks() == 1; }
 };
-int parts_of(long long m, long long n, long long k, bool split, int sms, bool adds) {
-    const Shape shape = shape_of(m, n, k, split, sms);
+int parts_of(long long m, long long n, long long k, bool narrow_only, int sms, bool adds) {
+    const Shape shape = shape_of(m, n, k, narrow_only, sms);
     const long long tiles = (long long)cdiv(m, shape.tile_rows) * cdiv(n, shape.bn), steps = cdiv(k, kXK);
     long long s = shape.units / tiles;
     if (s > steps / kMinSplitSteps) s = steps / kMinSplitSteps;
@@ -192,7 +199,7 @@ long long cost_of(const XentArgs &a, bool by_rows, long long piece, int sms, int
     return total;
 }
 Cut cut_of(const XentArgs &a, int sms) {
-    const int bn = a.bf16 ? 256 : 128, planes = a.bf16 ? 1 : 3;
+    const int planes = planes_of(a), bn = planes == 1 ? 256 : 128;
     Cut c;
     c.by_rows = a.N > a.V;
     const long long all_ld = up_to(a.V, 64), axis = c.by_rows ? a.N : a.V;
@@ -219,13 +226,13 @@ Cut cut_of(const XentArgs &a, int sms) {
     c.pieces = cdiv(axis, c.piece);
     c.ld = (int)(c.by_rows ? all_ld : up_to(c.piece, 64));
     c.rows = c.by_rows ? c.piece : a.N;
-    c.dx_parts = parts_of(c.rows, a.D, c.by_rows ? a.V : c.piece, !a.bf16, sms, !c.by_rows && c.pieces > 1);
-    c.dw_parts = parts_of(c.by_rows ? a.V : c.piece, a.D, c.rows, !a.bf16, sms, c.by_rows && c.pieces > 1);
+    c.dx_parts = parts_of(c.rows, a.D, c.by_rows ? a.V : c.piece, planes > 1, sms, !c.by_rows && c.pieces > 1);
+    c.dw_parts = parts_of(c.by_rows ? a.V : c.piece, a.D, c.rows, planes > 1, sms, c.by_rows && c.pieces > 1);
     return c;
 }
 struct BackwardBytes { size_t x, w, g, dx, dw, col, more; };
 BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
-    const int planes = a.bf16 ? 1 : 3;
+    const int planes = planes_of(a);
     BackwardBytes b;
     b.x = operand_of(a.N, a.D, a.bf16).bytes;
     b.w = operand_of(a.V, a.D, a.bf16).bytes;
@@ -279,11 +286,12 @@ void few(const XentArgs &a, const XentParams &p, int ctas, cudaStream_t st) {
     else few<T, 8>(a, p, ctas, vec, st);
 }
 
-template <bool SPLIT>
+template <int MODE>
 int forward(Run &r) {
+    constexpr bool SPLIT = MODE == XENT_F32;
     const XentArgs &a = r.a;
     unsigned char *ws = (unsigned char *)a.workspace;
-    const int slots = forward_slots(a.N, a.D, a.V, a.bf16, r.sms);
+    const int slots = forward_slots(a, r.sms);
     XentParams p{};
     p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
     p.part = (float2 *)ws; ws += up_to(8ll * slots * a.N, 256);
@@ -294,7 +302,7 @@ int forward(Run &r) {
     p.part_rows = a.N;
     XentRows q = rows_of(a, p, sums);
     q.slots = slots;
-    if (few_rows(a.N, a.D)) {
+    if (few_rows(a.N, a.D) && !a.lse) {              // (a backward pass wants the logits that its own tiles will form)
         p.M = (int)a.N;
         if (SPLIT) few<float>(a, p, slots, r.st); else few<__nv_bfloat16>(a, p, slots, r.st);
         const cudaError_t e = cudaGetLastError();
@@ -303,7 +311,7 @@ int forward(Run &r) {
     Mat x, w;
     int rc = make_operand(r, a.x, operand_of(a.N, a.D, a.bf16), &ws, &x);
     if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, a.bf16), &ws, &w);
-    if (!rc) rc = r.product<XENT_LOGITS, SPLIT>(x, w, p);
+    if (!rc) rc = r.product<XENT_LOGITS, MODE>(x, w, p);
     if (rc) return rc;
     const Shape s = shape_of(a.N, a.V, a.D, SPLIT, r.sms);
     q.tile_rows = s.tile_rows;
@@ -319,7 +327,7 @@ cudaError_t finish(const float *sums, void *out, long long n, int slots, const f
     else xent_finish_few_kernel<T><<<cdiv(n, 1024), 256, 0, st>>>(sums, (T *)out, n, slots, up, count, f);
     return cudaGetLastError();
 }
-template <bool SPLIT>
+template <int MODE>
 int backward(Run &r) {
     const XentArgs &a = r.a;
     const Cut c = cut_of(a, r.sms);
@@ -362,22 +370,22 @@ int backward(Run &r) {
         const long long row0 = c.by_rows ? at : 0, rows = c.by_rows ? n : a.N;
         const int col0 = c.by_rows ? 0 : (int)at, colsn = c.by_rows ? a.V : (int)n, ld = (int)up_to(colsn, 64);
         const Mat xs = sub_rows(x, row0, rows), wp = sub_rows(w, col0, colsn);
-        const Mat gm{g, rows, ld, ld, rows * ld, SPLIT ? 3 : 1};
+        const Mat gm{g, rows, ld, ld, rows * ld, planes_of(a)};
         XentParams p{};
         p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.col0 = col0; p.V = a.V; p.target = a.target + row0; p.ignore = a.ignore;
         p.smooth = a.smoothing > 0.f;
-        p.lse = a.lse + row0; p.up = each ? a.dloss + row0 : nullptr;
+        p.lse = a.lse + row0; p.lse_lo = a.lse + a.N + row0; p.up = each ? a.dloss + row0 : nullptr;
         p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
         p.g = g; p.g_plane = gm.plane; p.g_ld = ld;
         p.cols = a.db ? cols : nullptr; p.cols_ld = ld;
         // exp(l - lse) / f = exp2(l2 - (lse2 + log2 f))
-        if ((rc = r.product<XENT_GRAD, SPLIT>(xs, wp, p))) return rc;
+        if ((rc = r.product<XENT_GRAD, MODE>(xs, wp, p))) return rc;
         cudaError_t e = cudaSuccess;
         if (a.dx) {
             XentParams q{};
             void *to = (char *)a.dx + row0 * a.D * es;
             out_of(q, c.dx_parts, c.by_rows || i == 0, to, dxs, rows * a.D, ld);
-            if ((rc = r.product<XENT_DX, SPLIT>(gm, wp, q))) return rc;
+            if ((rc = r.product<XENT_DX, MODE>(gm, wp, q))) return rc;
             if (c.by_rows || i == c.pieces - 1) e = end(c.dx_parts, dxs, to, rows * a.D);
         }
         if (e == cudaSuccess && a.dw) {
@@ -386,7 +394,7 @@ int backward(Run &r) {
             Mat gv = gm;
             gv.cols = colsn;                                          // rows of dw that exist
             out_of(q, c.dw_parts, !c.by_rows || i == 0, to, dws, (long long)colsn * a.D, rows);
-            if ((rc = r.product<XENT_DW, SPLIT>(gv, xs, q))) return rc;
+            if ((rc = r.product<XENT_DW, MODE>(gv, xs, q))) return rc;
             if (!c.by_rows || i == c.pieces - 1) e = end(c.dw_parts, dws, to, (long long)colsn * a.D);
         }
         if (e == cudaSuccess && a.db) {
@@ -417,18 +425,18 @@ size_t xent_workspace(const XentArgs &a, bool back, int sms) {
         const BackwardBytes b = backward_bytes(a, cut_of(a, sms));
         return b.x + b.w + b.g + b.dx + b.dw + b.col + b.more;
     }
-    const int slots = forward_slots(a.N, a.D, a.V, a.bf16, sms);
-    if (few_rows(a.N, a.D)) return (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) + up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
+    const int slots = forward_slots(a, sms);
+    if (few_rows(a.N, a.D) && !a.lse) return (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) + up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
     return operand_of(a.N, a.D, a.bf16).bytes + operand_of(a.V, a.D, a.bf16).bytes + (size_t)(up_to(8ll * slots * a.N, 256) + up_to(4 * a.N, 256) +
            up_to(4ll * slots * a.N, 256) + up_to(16ll * cdiv(a.N, 8), 256));
 }
 int xent_forward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {
     Run r{a, sms, err_flag, st, cuda, enc};
-    return a.bf16 ? forward<false>(r) : forward<true>(r);
+    return a.bf16 ? forward<XENT_BF16>(r) : forward<XENT_F32>(r);
 }
 int xent_backward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {
     Run r{a, sms, err_flag, st, cuda, enc};
-    return a.bf16 ? backward<false>(r) : backward<true>(r);
+    return !a.bf16 ? backward<XENT_F32>(r) : fine_of(a) ? backward<XENT_FINE>(r) : backward<XENT_BF16>(r);
 }
 
 }  // namespace o1d

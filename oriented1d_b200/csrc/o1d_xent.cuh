@@ -28,6 +28,9 @@
 namespace o1d {
 
 enum : int { XENT_LOGITS = 0, XENT_GRAD, XENT_DX, XENT_DW };
+// What the operands are.  XENT_FINE: bf16, but G in two planes (16 bits), so that dx and dw are as exact as their own rounding
+// lets them be; taken where the products are small (see fine_of in o1d_xent.cu).
+enum : int { XENT_BF16 = 0, XENT_F32, XENT_FINE };
 
 constexpr int kXM = 128, kXK = 64;               // tile rows; K elements of a stage (one 128-byte swizzled row)
 constexpr int kXFinish = 16;                     // warps that finish tiles: four a scheduler (with two, half the issue slots stayed
@@ -38,11 +41,12 @@ constexpr int kXChunk = 4;                       // fp32: stages of one accumula
 // Tiles of 128 x 128 (fp32, whose two accumulators of 256 columns would not fit twice, and products with too few tiles to go
 // round), 128 x 256, or 256 x 256 on a pair of CTAs (each loads half of either operand: a third less than 128 x 256 reads
 // for the same products).  See shape_of in o1d_xent.cu.
-template <bool SPLIT, int BN_, bool PAIR> struct XentShape {
-    static constexpr int TM = PAIR ? 2 * kXM : kXM, BN = BN_, PL = SPLIT ? 3 : 1;
+template <int KIND, int MODE, int BN_, bool PAIR> struct XentShape {
+    static constexpr int TM = PAIR ? 2 * kXM : kXM, BN = BN_;
+    static constexpr int PLA = MODE == XENT_F32 ? 3 : MODE == XENT_FINE && KIND >= XENT_DX ? 2 : 1, PLB = MODE == XENT_F32 ? 3 : 1;
     static constexpr int B_COLS = PAIR ? BN / 2 : BN;               // columns that one CTA loads
-    static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = B_COLS * kXK * 2, STAGE = PL * (A_BYTES + B_BYTES);
-    static constexpr int STAGES = SPLIT ? 2 : B_COLS == 256 ? 4 : 6;
+    static constexpr int A_BYTES = kXM * kXK * 2, B_BYTES = B_COLS * kXK * 2, STAGE = PLA * A_BYTES + PLB * B_BYTES;
+    static constexpr int STAGES = MODE == XENT_F32 ? 2 : STAGE > 32768 ? 4 : 6;
     static constexpr int SMEM = STAGES * STAGE + kXFinish * kXStaging + 256 + 1024;
 };
 
@@ -64,7 +68,7 @@ struct XentParams {
     long long part_rows;
     int smooth;
     // GRAD
-    const float *lse, *up;       // up: per-row gradient of the loss, or null
+    const float *lse, *lse_lo, *up;      // lse + lse_lo; up: per-row gradient of the loss, or null
     float factor_log2, one, eps_v;   // log2(1-e), coefficient of the target, e/V; both divided by 1-e
     __nv_bfloat16 *g;
     long long g_plane;           // elements of a plane of G
@@ -167,10 +171,12 @@ __device__ __forceinline__ float pick(const float (&a)[32], int at) {
     return t[0];
 }
 
-template <int KIND, bool SPLIT, int BN, bool PAIR>
+template <int KIND, int MODE, int BN, bool PAIR>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XentParams p) {
-    using S = XentShape<SPLIT, BN, PAIR>;
+    using S = XentShape<KIND, MODE, BN, PAIR>;
+    constexpr bool SPLIT = MODE == XENT_F32;
+    constexpr int GPL = SPLIT ? 3 : MODE == XENT_FINE ? 2 : 1;      // planes of G
     constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
     constexpr int PIECES = BN / 128;                 // of 32 columns, for each of the four warps that share 32 rows
     constexpr uint32_t INSTR = tc::instruction<S::TM, BN, A_MN, B_MN>();
@@ -211,7 +217,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const XentTile w = xent_tile<KIND>(p, t);
             for (int k = w.k0; k < w.k1; k++) {
                 if (!(ok = tc::bar_wait(empty + stage, phase ^ 1, dead, p.err_flag))) break;
-                unsigned char *a = smem + stage * S::STAGE, *b = a + S::PL * S::A_BYTES;
+                unsigned char *a = smem + stage * S::STAGE, *b = a + S::PLA * S::A_BYTES;
                 if (rank == 0) tc::bar_expect(full + stage, PAIR ? 2 * S::STAGE : S::STAGE);
                 const uint32_t bar = PAIR ? tc::in_cta(full + stage, 0) : 0;
                 auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
@@ -220,13 +226,16 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 };
                 const int row = w.m * S::TM + rank * kXM, col = w.n * BN + rank * S::B_COLS;
 #pragma unroll
-                for (int pl = 0; pl < S::PL; pl++) {
+                for (int pl = 0; pl < S::PLA; pl++) {
                     if (A_MN) {
 #pragma unroll
                         for (int j = 0; j < kXM / 64; j++) load(a + pl * S::A_BYTES + j * 8192, &map_a, row + j * 64, k * kXK, pl);
                     } else {
                         load(a + pl * S::A_BYTES, &map_a, k * kXK, row, pl);
                     }
+                }
+#pragma unroll
+                for (int pl = 0; pl < S::PLB; pl++) {
                     if (B_MN) {
 #pragma unroll
                         for (int j = 0; j < S::B_COLS / 64; j++) load(b + pl * S::B_BYTES + j * 8192, &map_b, col + j * 64, k * kXK, pl);
@@ -259,18 +268,18 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 for (int k = c; k < c_end; k++) {
                     if (!(ok = tc::bar_wait(full + stage, phase, dead, p.err_flag))) break;
                     tc::fence_after();
-                    unsigned char *a = smem + stage * S::STAGE, *b = a + S::PL * S::A_BYTES;
-                    uint64_t da[S::PL], db[S::PL];
+                    unsigned char *a = smem + stage * S::STAGE, *b = a + S::PLA * S::A_BYTES;
+                    uint64_t da[S::PLA], db[S::PLB];
 #pragma unroll
-                    for (int pl = 0; pl < S::PL; pl++) {
-                        da[pl] = tc::operand(a + pl * S::A_BYTES, A_MN ? 8192 : 16, 1024);
-                        db[pl] = tc::operand(b + pl * S::B_BYTES, B_MN ? 8192 : 16, 1024);
-                    }
+                    for (int pl = 0; pl < S::PLA; pl++) da[pl] = tc::operand(a + pl * S::A_BYTES, A_MN ? 8192 : 16, 1024);
+#pragma unroll
+                    for (int pl = 0; pl < S::PLB; pl++) db[pl] = tc::operand(b + pl * S::B_BYTES, B_MN ? 8192 : 16, 1024);
 #pragma unroll
                     for (int kk = 0; kk < kXK / 16; kk++) {         // 16 of K: 32 bytes of a K-major row, or 16 rows
                         const uint64_t oa = kk * (A_MN ? 128 : 2), ob = kk * (B_MN ? 128 : 2);
                         const bool add = k > c || kk > 0;
-                        tc::mma<PAIR>(d, da[0] + oa, db[0] + ob, INSTR, add);
+                        if constexpr (S::PLA == 2) tc::mma<PAIR>(d, da[1] + oa, db[0] + ob, INSTR, add);
+                        tc::mma<PAIR>(d, da[0] + oa, db[0] + ob, INSTR, add || S::PLA == 2);
                         if constexpr (SPLIT) {
                             tc::mma<PAIR>(d + 128, da[0] + oa, db[2] + ob, INSTR, add);
                             tc::mma<PAIR>(d + 128, da[1] + oa, db[1] + ob, INSTR, true);
@@ -302,7 +311,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // LOGITS: running maximum and sum of the row's columns that this warp sees, in units of log2
         float mx = 0.f, sum = 0.f, total = 0.f;
         long long tgt = -1;
-        float lse = 0.f, scale = 0.f;
+        float lse = 0.f, lse_lo = 0.f, scale = 0.f;
         bool ignored = false;
         float alpha = 1.f;
         if (KIND >= XENT_DX && p.out_kind < 2) alpha = xent_alpha(p.alpha_up, p.alpha_count, p.alpha);
@@ -320,16 +329,17 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 
         // What a tile needs from memory, fetched while the one before it is worked on.  Bias in units of log2; -inf where the
         // vocabulary ends, so that those columns weigh nothing.
-        struct Ahead { long long tgt; float lse, scale, bias[PIECES]; };
+        struct Ahead { long long tgt; float lse, lse_lo, scale, bias[PIECES]; };
         auto fetch = [&](int t) {
-            Ahead f{p.ignore, 0.f, 1.f, {}};
+            Ahead f{p.ignore, 0.f, 0.f, 1.f, {}};
             if (KIND > XENT_GRAD || t >= t_end) return f;
             const XentTile w = xent_tile<KIND>(p, t);
             const int row = w.m * S::TM + rank * kXM + quarter * 32 + lane;
             if (row < p.M) {
                 f.tgt = __ldg(p.target + row);
                 if (KIND == XENT_GRAD) {
-                    f.lse = __ldg(p.lse + row) + p.factor_log2;
+                    f.lse = __ldg(p.lse + row);
+                    f.lse_lo = __ldg(p.lse_lo + row) + p.factor_log2;
                     if (p.up) f.scale = __ldg(p.up + row);
                 }
             }
@@ -354,6 +364,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 tgt = next.tgt;
                 ignored = tgt == p.ignore;
                 lse = !ignored && (tgt < 0 || tgt >= p.V) ? __int_as_float(0x7fffffff) : next.lse;      // no such class: NaN, not silence
+                lse_lo = next.lse_lo;
                 scale = next.scale;
 #pragma unroll
                 for (int i = 0; i < PIECES; i++) bias[i] = next.bias[i];
@@ -418,34 +429,56 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     float *bs = reinterpret_cast<float *>(stage);
                     bs[lane] = bias[pc];
                     __syncwarp();
+                    // fp32: the piece's exponents relative to `ref` (the row's greatest so far, or lse in two parts).  The product is
+                    // taken from ref in one operation, so that what is rounded is small where it counts.
+                    auto exponents = [&](float ref, float lo) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 b = *reinterpret_cast<const float4 *>(bs + i);
-                        const float2 u = apart(fma2(two(a[i], a[i + 1]), log2e, two(b.x, b.y))), v = apart(fma2(two(a[i + 2], a[i + 3]), log2e, two(b.z, b.w)));
-                        a[i] = u.x; a[i + 1] = u.y; a[i + 2] = v.x; a[i + 3] = v.y;
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 b = *reinterpret_cast<const float4 *>(bs + i);
+                            const F2 u = add2(fma2(two(a[i], a[i + 1]), log2e, both(-ref)), add2(two(b.x, b.y), both(-lo)));
+                            const F2 v = add2(fma2(two(a[i + 2], a[i + 3]), log2e, both(-ref)), add2(two(b.z, b.w), both(-lo)));
+                            a[i] = apart(u).x; a[i + 1] = apart(u).y; a[i + 2] = apart(v).x; a[i + 3] = apart(v).y;
+                        }
+                        __syncwarp();
+                    };
+                    float top = mx;                                  // LOGITS
+                    if constexpr (SPLIT && KIND == XENT_GRAD) {
+                        exponents(lse, lse_lo);
+                    } else {
+                        float top2 = __int_as_float(0xff800000);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 b = *reinterpret_cast<const float4 *>(bs + i);
+                            const float2 u = apart(fma2(two(a[i], a[i + 1]), log2e, two(b.x, b.y))), v = apart(fma2(two(a[i + 2], a[i + 3]), log2e, two(b.z, b.w)));
+                            if constexpr (KIND == XENT_LOGITS) {
+                                top = max3(top, u.x, u.y);
+                                top2 = max3(top2, v.x, v.y);
+                                if (p.smooth) {
+                                    const int left = p.N - (c0 + i);
+                                    total += ((left > 0 ? u.x : 0.f) + (left > 1 ? u.y : 0.f)) + ((left > 2 ? v.x : 0.f) + (left > 3 ? v.y : 0.f));
+                                }
+                            }
+                            if constexpr (!SPLIT) { a[i] = u.x; a[i + 1] = u.y; a[i + 2] = v.x; a[i + 3] = v.y; }
+                        }
+                        top = fmaxf(top, top2);
+                        if (!SPLIT) __syncwarp();
                     }
-                    __syncwarp();
                     const long long off = tgt - p.col0 - c0;         // where the target lies in this piece
                     const int at = off >= 0 && off < 32 ? (int)off : -1;
                     const bool hit = __any_sync(0xffffffffu, at >= 0);
                     if constexpr (KIND == XENT_LOGITS) {
                         if (hit) {
-                            const float l = pick(a, at);
+                            float l = pick(a, at);
+                            if (SPLIT) l = fmaf(l, 1.4426950408889634f, bs[at & 31]);
                             if (at >= 0 && row < p.M) p.target_logit[row] = l;
                         }
-                        if (p.smooth) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) total += c0 + i < p.N ? a[i] : 0.f;
-                        }
-                        float top = mx, top2 = a[0];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) { top = max3(top, a[i], a[i + 1]); top2 = max3(top2, a[i + 2], a[i + 3]); }
-                        top = fmaxf(top, top2);
                         const float ref = top == __int_as_float(0xff800000) ? 0.f : top;
                         F2 s0 = both(0.f), s1 = both(0.f);
+                        if constexpr (SPLIT) exponents(ref, 0.f);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const float2 u = apart(add2(two(a[i], a[i + 1]), both(-ref))), v = apart(add2(two(a[i + 2], a[i + 3]), both(-ref)));
+                            float2 u = make_float2(a[i], a[i + 1]), v = make_float2(a[i + 2], a[i + 3]);
+                            if constexpr (!SPLIT) { u = apart(add2(two(u.x, u.y), both(-ref))); v = apart(add2(two(v.x, v.y), both(-ref))); }
                             s0 = add2(s0, two(exp2_fast(u.x), exp2_fast(u.y)));
                             s1 = add2(s1, two(exp2_fast(v.x), exp2_fast(v.y)));
                         }
@@ -453,20 +486,26 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         sum = sum * exp2_fast(mx - ref) + (s2.x + s2.y);
                         mx = top;
                     } else {
+                        if constexpr (!SPLIT) {
+                            const F2 l = both(-(lse + lse_lo));
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 u = apart(add2(two(a[i], a[i + 1]), both(-lse)));
-                            a[i] = exp2_fast(u.x);
-                            a[i + 1] = exp2_fast(u.y);
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 u = apart(add2(two(a[i], a[i + 1]), l));
+                                a[i] = u.x;
+                                a[i + 1] = u.y;
+                            }
+                        }
+                        float hot = 0.f;                             // the target's value: p - 1 without its cancellation
+                        if (hit && p.one != 0.f) hot = expm1f(0.6931471805599453f * pick(a, at));
+#pragma unroll
+                        for (int i = 0; i < 32; i++) a[i] = exp2_fast(a[i]);
+                        if (hit && p.one != 0.f) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) a[i] = at == i ? hot : a[i];
                         }
                         if (p.smooth) {
 #pragma unroll
                             for (int i = 0; i < 32; i++) a[i] -= c0 + i < p.N ? p.eps_v : 0.f;
-                        }
-                        if (hit) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (at == i) a[i] -= p.one;
                         }
                         if (p.up) {
 #pragma unroll
@@ -478,7 +517,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         }
                         if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + lane] = column_sums(a, lane);
 #pragma unroll
-                        for (int pl = 0; pl < S::PL; pl++) {
+                        for (int pl = 0; pl < GPL; pl++) {
                             uint4 out[4];
                             uint32_t *o = reinterpret_cast<uint32_t *>(out);
 #pragma unroll
@@ -488,6 +527,10 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                     o[i] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
                                 } else {
                                     o[i] = pack_bf16(a[2 * i], a[2 * i + 1]);
+                                    if (GPL > 1) {
+                                        a[2 * i] -= __uint_as_float(o[i] << 16);
+                                        a[2 * i + 1] -= __uint_as_float(o[i] & 0xffff0000u);
+                                    }
                                 }
                             }
                             __nv_bfloat16 *to = p.g + pl * p.g_plane + c0;
@@ -728,15 +771,23 @@ xent_rows_kernel(const XentRows a) {
     }
     double loss = 0., counted = 0.;
     if (real && lane == 0) {
-        const float l2 = ref + log2f(sum);
-        a.lse[row] = l2;
+        // lse = ref + log2(sum), as two floats; the loss from its parts (where the target is the greatest, ref is its logit)
+        const float ls = log2f(sum), hi = ref + ls;
+        if (a.lse) {
+            const float r1 = hi - ls;
+            a.lse[row] = hi;
+            a.lse[a.rows + row] = fabsf(hi) <= 3.402823466e38f ? (ref - r1) + (ls - (hi - r1)) : 0.f;
+        }
         const long long t = a.target[row];
         float out = 0.f;
         if (t != a.ignore) {
             if (t < 0 || t >= a.V) out = __int_as_float(0x7fffffff);
             else {
-                out = a.smoothing < 1.f ? l2 - (1.f - a.smoothing) * a.target_logit[row] : l2;
-                if (a.smoothing > 0.f) out -= a.smoothing / (float)a.V * total;
+                if (a.smoothing == 0.f) out = (ref - a.target_logit[row]) + ls;
+                else {
+                    out = a.smoothing < 1.f ? (1.f - a.smoothing) * ((ref - a.target_logit[row]) + ls) : 0.f;
+                    out += a.smoothing * ((ref - total / (float)a.V) + ls);
+                }
                 out *= 0.6931471805599453f;
             }
             loss = out;
@@ -782,19 +833,19 @@ xent_total_kernel(const double2 *__restrict__ sums, int blocks, int mean, float 
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_finish_kernel(const float *__restrict__ sums, T *__restrict__ out, long long n, int slots, const float *up, const float *count, float f) {
-    __shared__ float part[8][33];
+    __shared__ double part[8][33];
     const long long i = (long long)blockIdx.x * 32 + threadIdx.x;
-    float s = 0.f;
+    double s = 0.;
     if (i < n)
 #pragma unroll 4
         for (int k = threadIdx.y; k < slots; k += 8) s += sums[k * n + i];
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && i < n) {
-        float t = 0.f;
+        double t = 0.;
 #pragma unroll
         for (int y = 0; y < 8; y++) t += part[y][threadIdx.x];
-        st(out + i, xent_alpha(up, count, f) * t);
+        st(out + i, xent_alpha(up, count, f) * (float)t);
     }
 }
 // The same where there are few slots and many elements: four elements a thread.
@@ -824,20 +875,20 @@ xent_finish_few_kernel(const float *__restrict__ sums, T *__restrict__ out, long
 __global__ void __launch_bounds__(1024)
 xent_bias_kernel(const float *__restrict__ partial, long long part_ld, int slices, int per, void *__restrict__ db, int bf16, float *__restrict__ more,
                  long long more_ld, int V, const float *up, const float *count, float f) {
-    __shared__ float part[32][33];
+    __shared__ double part[32][33];
     const int c = blockIdx.x * 32 + threadIdx.x, end = min(slices, (int)(blockIdx.y + 1) * per);
-    float s = 0.f;
+    double s = 0.;
     if (c < V)
 #pragma unroll 4
         for (int k = blockIdx.y * per + threadIdx.y; k < end; k += 32) s += partial[k * part_ld + c];
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < V) {
-        float t = 0.f;
+        double t = 0.;
 #pragma unroll
         for (int y = 0; y < 32; y++) t += part[y][threadIdx.x];
-        if (more) more[blockIdx.y * more_ld + c] = t;
-        else st_param(db, c, bf16, xent_alpha(up, count, f) * t);
+        if (more) more[blockIdx.y * more_ld + c] = (float)t;
+        else st_param(db, c, bf16, xent_alpha(up, count, f) * (float)t);
     }
 }
 

@@ -95,7 +95,9 @@ def check(N, D, V, dtype, bias="same", smoothing=0.0, reduction="mean", ignored=
         if n > 1e-3 * float(up.mean()):
             assert float((o.double() - r).norm()) <= ((2.0 ** -8 if torch.bfloat16 in (x.dtype, leaf.dtype) else 3e-6) + most) * n
     with torch.no_grad():
-        assert torch.equal(ops.linear_cross_entropy(x, w, t, b, **kw), got)
+        alone = ops.linear_cross_entropy(x, w, t, b, **kw)               # up to eight rows: a kernel of its own, in another order
+        assert torch.equal(alone, got) if N > 8 else True
+        within(alone, loss, e_loss, "loss without gradients")
     assert o1d.ops.device_status() == 0
     return out
 
@@ -221,7 +223,7 @@ def test_extreme_logits(dtype):
 def test_layouts(dtype):
     """More axes, strided and misaligned inputs, a channels-last map with a label a pixel, one row without a batch axis."""
     x, w, b, t = make(96, 40, 50, dtype)
-    want = ops.linear_cross_entropy(x, w, t, b, reduction="none")
+    want = ops.linear_cross_entropy(x, w, t, b, reduction="none").detach()
     assert torch.equal(ops.linear_cross_entropy(x.view(4, 24, 40), w, t.view(4, 24), b, reduction="none"), want.view(4, 24))
     assert torch.equal(ops.linear_cross_entropy(x.t().contiguous().t(), w.t().contiguous().t(), t, b, reduction="none"), want)
     pad = torch.empty(96 * 40 + 1, device="cuda", dtype=x.dtype)
@@ -309,7 +311,7 @@ def test_the_logits_are_not_kept():
     base = torch.cuda.memory_allocated()
     torch.cuda.reset_peak_memory_stats()
     loss = ops.linear_cross_entropy(*leaves[:2], t, leaves[2])
-    assert torch.cuda.memory_allocated() - base <= 16384 * 4 + 8192       # one float a row
+    assert torch.cuda.memory_allocated() - base <= 16384 * 8 + 8192       # two floats a row
     torch.autograd.grad(loss, leaves)
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - base <= 256 << 20
@@ -348,7 +350,7 @@ def test_entry_points_reject_bad_arguments():
     p = buf.data_ptr()
     ok = dict(x=p, w=p, b=None, t=p, loss=p, lse=p, count=p, ws=p, n=0, N=4, D=8, V=10, ig=-100, s=0.0, red=2, dt=0, st=None)
     call = lambda **k: lib.o1d_linear_xent(*{**ok, **k}.values())  # noqa: E731
-    for k in ("x", "w", "t", "loss", "lse", "count"):
+    for k in ("x", "w", "t", "loss", "count"):
         assert call(**{k: None}) == 1, k
     for k in (dict(N=0), dict(D=0), dict(V=-1), dict(s=-1.0), dict(s=float("nan")), dict(red=3), dict(dt=2)):
         assert call(**k) == 1, k

@@ -17,7 +17,7 @@
 // would show.
 //
 // Rounding: G is rounded to bf16 for bf16 inputs (half a unit of 2^-8, random from element to element; dx and dw are
-// rounded so themselves).  So that the rounding of the coefficient 1-e, which every row shares, cannot add up, G is kept divided
+// rounded so themselves), or to two planes of it where that costs nothing (XENT_FINE).  So that the rounding of the coefficient 1-e, which every row shares, cannot add up, G is kept divided
 // by 1-e and the factor applied to the fp32 sums.  All sums, statistics and the loss are fp32 or wider.
 #pragma once
 
@@ -304,8 +304,11 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     } else if (warp >= 4) {                                         // ---- epilogue: a thread owns a quarter of a row
         const int quarter = warp & 3, part = (warp - 4) >> 2;
         char *stage = staging + (warp - 4) * kXStaging;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + part * 32;      // every fourth piece of 32 columns
-        int acc = 0, m_now = -1;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+        // The four warps of 32 rows take every fourth piece of 32 columns, each starting one further with every tile: where the
+        // columns end inside a tile, no warp has more to do than another (133200 x 150 classes have 5 pieces a tile).
+        auto piece_of = [&](int pc, int tile) { return 4 * pc + ((part + tile) & 3); };
+        int acc = 0, m_now = -1, tile = 0;                          // tile: of this CTA
         uint32_t acc_phase = 0;
         bool ok = true;
         // LOGITS: running maximum and sum of the row's columns that this warp sees, in units of log2
@@ -327,10 +330,10 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             if (p.smooth) p.part_sum[(long long)slot * p.part_rows + row] = total;
         };
 
-        // What a tile needs from memory, fetched while the one before it is worked on.  Bias in units of log2; -inf where the
-        // vocabulary ends, so that those columns weigh nothing.
-        struct Ahead { long long tgt; float lse, lse_lo, scale, bias[PIECES]; };
-        auto fetch = [&](int t) {
+        // What a tile needs from memory, fetched while the one before it is worked on: bits as they are stored, since any arithmetic
+        // on them here would wait for them.
+        struct Ahead { long long tgt; float lse, lse_lo, scale; uint32_t bias[PIECES]; };
+        auto fetch = [&](int t, int tile) {
             Ahead f{p.ignore, 0.f, 0.f, 1.f, {}};
             if (KIND > XENT_GRAD || t >= t_end) return f;
             const XentTile w = xent_tile<KIND>(p, t);
@@ -339,19 +342,23 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 f.tgt = __ldg(p.target + row);
                 if (KIND == XENT_GRAD) {
                     f.lse = __ldg(p.lse + row);
-                    f.lse_lo = __ldg(p.lse_lo + row) + p.factor_log2;
+                    f.lse_lo = __ldg(p.lse_lo + row);
                     if (p.up) f.scale = __ldg(p.up + row);
                 }
             }
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
-                const int c = w.n * BN + (4 * i + part) * 32 + lane;
-                f.bias[i] = c >= p.N ? __int_as_float(0xff800000) : p.bias ? 1.4426950408889634f * ld_param(p.bias, p.col0 + c, p.bias_bf16) : 0.f;
+                const int c = w.n * BN + piece_of(i, tile) * 32 + lane;
+                f.bias[i] = 0u;
+                if (p.bias && c < p.N) {
+                    if (p.bias_bf16) f.bias[i] = __ldg(static_cast<const unsigned short *>(p.bias) + p.col0 + c);
+                    else f.bias[i] = __ldg(static_cast<const uint32_t *>(p.bias) + p.col0 + c);
+                }
             }
             return f;
         };
-        Ahead next = fetch(t_begin);
-        for (int t = t_begin; ok && t < t_end; t += t_step) {
+        Ahead next = fetch(t_begin, 0);
+        for (int t = t_begin; ok && t < t_end; t += t_step, tile++) {
             const XentTile w = xent_tile<KIND>(p, t);
             const int r0 = w.m * S::TM + rank * kXM + quarter * 32, row = r0 + lane, n0 = w.n * BN;
             float bias[PIECES];
@@ -364,11 +371,14 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 tgt = next.tgt;
                 ignored = tgt == p.ignore;
                 lse = !ignored && (tgt < 0 || tgt >= p.V) ? __int_as_float(0x7fffffff) : next.lse;      // no such class: NaN, not silence
-                lse_lo = next.lse_lo;
+                lse_lo = next.lse_lo + p.factor_log2;
                 scale = next.scale;
+                // in units of log2; -inf where the vocabulary ends, so that those columns weigh nothing
 #pragma unroll
-                for (int i = 0; i < PIECES; i++) bias[i] = next.bias[i];
-                next = fetch(t + t_step);
+                for (int i = 0; i < PIECES; i++)
+                    bias[i] = n0 + piece_of(i, tile) * 32 + lane < p.N ? 1.4426950408889634f * __uint_as_float(p.bias_bf16 ? next.bias[i] << 16 : next.bias[i])
+                                                                      : __int_as_float(0xff800000);
+                next = fetch(t + t_step, tile + 1);
             }
             float v[SPLIT ? PIECES : 1][32];
             if constexpr (SPLIT) {
@@ -385,7 +395,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                         for (int part_sum = 1; part_sum >= 0; part_sum--) {          // the five small products, then x0 w0
                             uint32_t r[32];
-                            tc::tmem_load32(lane_base + acc * 256 + part_sum * 128 + pc * 128, r);
+                            tc::tmem_load32(lane_base + acc * 256 + part_sum * 128 + piece_of(pc, tile) * 32, r);
                             tc::tmem_wait32(r);
 #pragma unroll
                             for (int i = 0; i < 32; i++) v[pc][i] += __uint_as_float(r[i]);
@@ -404,12 +414,12 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
             for (int pc = 0; pc < PIECES; pc++) {
                 float (&a)[32] = v[SPLIT ? pc : 0];
-                const int c0 = n0 + (4 * pc + part) * 32;           // first column of the piece
+                const int c0 = n0 + piece_of(pc, tile) * 32;        // first column of the piece
                 const bool some = c0 < (KIND == XENT_GRAD ? p.g_ld : p.N);      // the same for the whole warp
                 if constexpr (!SPLIT) {
                     if (some) {
                         uint32_t r[32];
-                        tc::tmem_load32(lane_base + acc * 256 + pc * 128, r);
+                        tc::tmem_load32(lane_base + acc * 256 + piece_of(pc, tile) * 32, r);
                         tc::tmem_wait32(r);
 #pragma unroll
                         for (int i = 0; i < 32; i++) a[i] = __uint_as_float(r[i]);

@@ -94,23 +94,61 @@ __device__ __forceinline__ float xent_alpha(const float *up, const float *count,
 
 __device__ __forceinline__ float exp2_fast(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 
-// Tile t of a CTA's work.
-struct XentTile { int m, n, k0, k1, split; };
+// The tiles of a CTA (or pair), one after the other.  Found by division once and by steps from there: a tile of a narrow product
+// takes 2 us, of which the divisions of sixteen warps were a quarter.
+struct XentTile {
+    int m, n, split, k0, k1;
+    int left;                                        // tiles still to come, this one included
+    int dm, dn, dsplit;                              // a step, in tiles
+};
 template <int KIND>
-__device__ __forceinline__ XentTile xent_tile(const XentParams &p, int t) {
+__device__ __forceinline__ void xent_span(const XentParams &p, XentTile &t) {
+    t.k0 = 0; t.k1 = p.k_steps;
+    if (KIND >= XENT_DX && p.splits > 1) {
+        t.k0 = (int)((long long)p.k_steps * t.split / p.splits);
+        t.k1 = (int)((long long)p.k_steps * (t.split + 1) / p.splits);
+    }
+}
+template <int KIND>
+__device__ __forceinline__ XentTile xent_first(const XentParams &p, int me, int all) {
     XentTile r;
     if (KIND == XENT_LOGITS) {                       // along the vocabulary: a CTA keeps its rows' statistics in registers
-        r.m = t / p.n_tiles; r.n = t - r.m * p.n_tiles; r.k0 = 0; r.k1 = p.k_steps; r.split = 0;
+        const int t = (int)((long long)me * p.tiles / all);
+        r.left = (int)((long long)(me + 1) * p.tiles / all) - t;
+        r.m = t / p.n_tiles; r.n = t - r.m * p.n_tiles;
+        r.split = r.dm = r.dn = r.dsplit = 0;
     } else {
-        const int mn = p.m_tiles * p.n_tiles;
-        r.split = t / mn; t -= r.split * mn;
-        if (p.along_n) { r.m = t / p.n_tiles; r.n = t - r.m * p.n_tiles; } else { r.n = t / p.m_tiles; r.m = t - r.n * p.m_tiles; }
-        r.k0 = (int)((long long)p.k_steps * r.split / p.splits); r.k1 = (int)((long long)p.k_steps * (r.split + 1) / p.splits);
+        const int inner = p.along_n ? p.n_tiles : p.m_tiles, mn = p.m_tiles * p.n_tiles;
+        r.left = me < p.tiles ? (p.tiles - 1 - me) / all + 1 : 0;
+        auto cut = [&](int t, int &m, int &n, int &split) {
+            split = t / mn; t -= split * mn;
+            const int o = t / inner, i = t - o * inner;
+            m = p.along_n ? o : i; n = p.along_n ? i : o;
+        };
+        cut(me, r.m, r.n, r.split);
+        cut(all, r.dm, r.dn, r.dsplit);
     }
+    xent_span<KIND>(p, r);
     return r;
 }
-// First tile of CTA i: LOGITS gives each a contiguous run, so that the runs differ by one tile at most.
-__host__ __device__ inline int xent_run(int i, int tiles, int ctas) { return (int)((long long)i * tiles / ctas); }
+template <int KIND>
+__device__ __forceinline__ void xent_next(const XentParams &p, XentTile &t) {
+    t.left--;
+    if (KIND == XENT_LOGITS) {
+        if (++t.n == p.n_tiles) { t.n = 0; t.m++; }
+        return;
+    }
+    t.m += t.dm; t.n += t.dn; t.split += t.dsplit;
+    if (p.along_n) {                                 // n is the inner axis
+        if (t.n >= p.n_tiles) { t.n -= p.n_tiles; t.m++; }
+        if (t.m >= p.m_tiles) { t.m -= p.m_tiles; t.split++; }
+    } else {
+        if (t.m >= p.m_tiles) { t.m -= p.m_tiles; t.n++; }
+        if (t.n >= p.n_tiles) { t.n -= p.n_tiles; t.split++; }
+    }
+    xent_span<KIND>(p, t);
+}
+// LOGITS: the runs of CTAs differ by one tile at most (CTA i begins at i * tiles / ctas).
 // CTA whose run holds tile t.
 __host__ __device__ inline int xent_owner(int t, int tiles, int ctas) { return (int)((((long long)t + 1) * ctas - 1) / tiles); }
 
@@ -205,16 +243,11 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     tc::fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    const int t_begin = KIND == XENT_LOGITS ? xent_run(me, p.tiles, all) : me;
-    const int t_end = KIND == XENT_LOGITS ? xent_run(me + 1, p.tiles, all) : p.tiles;
-    const int t_step = KIND == XENT_LOGITS ? 1 : all;
-
     if (warp == 0 && lane == 0) {                                   // ---- loads
         int stage = 0, issued = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int t = t_begin; ok && t < t_end; t += t_step) {
-            const XentTile w = xent_tile<KIND>(p, t);
+        for (XentTile w = xent_first<KIND>(p, me, all); ok && w.left > 0; xent_next<KIND>(p, w)) {
             for (int k = w.k0; k < w.k1; k++) {
                 if (!(ok = tc::bar_wait(empty + stage, phase ^ 1, dead, p.err_flag))) break;
                 unsigned char *a = smem + stage * S::STAGE, *b = a + S::PLA * S::A_BYTES;
@@ -258,8 +291,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        for (int t = t_begin; ok && t < t_end; t += t_step) {
-            const XentTile w = xent_tile<KIND>(p, t);
+        for (XentTile w = xent_first<KIND>(p, me, all); ok && w.left > 0; xent_next<KIND>(p, w)) {
             for (int c = w.k0; ok && c < w.k1; c += SPLIT ? kXChunk : w.k1 - w.k0) {
                 const int c_end = SPLIT ? min(c + kXChunk, w.k1) : w.k1;
                 if (!(ok = tc::bar_wait(taken + acc, acc_phase ^ 1, dead, p.err_flag))) break;
@@ -322,10 +354,11 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         auto release = [&](int i) {                                 // the accumulator may be written again
             if (rank == 0) tc::bar_arrive(taken + i); else tc::bar_arrive_in(tc::in_cta(taken + i, 0));
         };
+        int run = 0;                                                // LOGITS: of the runs that share the row tile, which this one is
         auto flush = [&]() {
             const long long row = (long long)m_now * S::TM + rank * kXM + quarter * 32 + lane;
             if (row >= p.M) return;
-            const int slot = (me - xent_owner(m_now * p.n_tiles, p.tiles, all)) * 4 + part;
+            const int slot = run * 4 + part;
             p.part[(long long)slot * p.part_rows + row] = make_float2(mx, sum);
             if (p.smooth) p.part_sum[(long long)slot * p.part_rows + row] = total;
         };
@@ -333,10 +366,9 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // What a tile needs from memory, fetched while the one before it is worked on: bits as they are stored, since any arithmetic
         // on them here would wait for them.
         struct Ahead { long long tgt; float lse, lse_lo, scale; uint32_t bias[PIECES]; };
-        auto fetch = [&](int t, int tile) {
+        auto fetch = [&](const XentTile &w, int tile) {
             Ahead f{p.ignore, 0.f, 0.f, 1.f, {}};
-            if (KIND > XENT_GRAD || t >= t_end) return f;
-            const XentTile w = xent_tile<KIND>(p, t);
+            if (KIND > XENT_GRAD || w.left <= 0) return f;
             const int row = w.m * S::TM + rank * kXM + quarter * 32 + lane;
             if (row < p.M) {
                 f.tgt = __ldg(p.target + row);
@@ -357,14 +389,17 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
             return f;
         };
-        Ahead next = fetch(t_begin, 0);
-        for (int t = t_begin; ok && t < t_end; t += t_step, tile++) {
-            const XentTile w = xent_tile<KIND>(p, t);
+        XentTile coming = xent_first<KIND>(p, me, all);
+        if (KIND == XENT_LOGITS) run = me - xent_owner(coming.m * p.n_tiles, p.tiles, all);
+        Ahead next = fetch(coming, 0);
+        for (; ok && coming.left > 0; tile++) {
+            const XentTile w = coming;
+            xent_next<KIND>(p, coming);
             const int r0 = w.m * S::TM + rank * kXM + quarter * 32, row = r0 + lane, n0 = w.n * BN;
             float bias[PIECES];
             if constexpr (KIND <= XENT_GRAD) {
                 if (w.m != m_now) {
-                    if (KIND == XENT_LOGITS && m_now >= 0) flush();
+                    if (KIND == XENT_LOGITS && m_now >= 0) { flush(); run = 0; }      // the next row tile begins here
                     m_now = w.m;
                     mx = __int_as_float(0xff800000); sum = 0.f; total = 0.f;
                 }
@@ -378,7 +413,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 for (int i = 0; i < PIECES; i++)
                     bias[i] = n0 + piece_of(i, tile) * 32 + lane < p.N ? 1.4426950408889634f * __uint_as_float(p.bias_bf16 ? next.bias[i] << 16 : next.bias[i])
                                                                       : __int_as_float(0xff800000);
-                next = fetch(t + t_step, tile + 1);
+                next = fetch(coming, tile + 1);
             }
             float v[SPLIT ? PIECES : 1][32];
             if constexpr (SPLIT) {

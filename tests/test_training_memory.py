@@ -136,6 +136,22 @@ def test_under_autocast():
 
 
 @gpu
+def test_no_rows_and_inference_mode():
+    leaves = mlp_args(3, 32, 64, "fp32")
+    empty = leaves[0].detach()[:0].requires_grad_(True)
+    out = ops.mlp_keep8(empty, *leaves[1:])
+    grads = torch.autograd.grad(out, [empty, *leaves[1:]], torch.zeros_like(out))
+    assert out.shape == (0, 32) and grads[0].shape == (0, 32)
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(grads[1:], leaves[1:]))
+    with torch.inference_mode():
+        x, g, b, w1, b1 = (t.detach() for t in leaves[:5])
+        t = torch.tensor([0, 5, 63], device="cuda")
+        outs = [ops.mlp_keep8(*(v.detach() for v in leaves)), ops.gelu_keep8(x), ops.layer_norm_keep8(x, g, b), ops.linear_cross_entropy(x, w1, t, b1),
+                *ops.keep8(x)]
+    assert all(not o.requires_grad for o in outs) and torch.equal(outs[0], ops.mlp_keep8(*leaves).detach())
+
+
+@gpu
 def test_gradients_that_start_off_a_vector():
     leaves = mlp_args(30, 32, 64, "bf16")
     dz = torch.randn(30 * 32 + 1, device="cuda").bfloat16()

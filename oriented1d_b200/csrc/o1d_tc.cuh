@@ -111,8 +111,8 @@ __device__ __forceinline__ uint64_t operand(const void *p, uint32_t inner, uint3
     return (uint64_t)((smem_addr(p) & 0x3ffffu) >> 4) | (uint64_t)(inner >> 4) << 16 | (uint64_t)(outer >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 // bf16 x bf16 -> fp32
-template <int M, int N, bool A_MN, bool B_MN> constexpr uint32_t instruction() {
-    return 1u << 4 | 1u << 7 | 1u << 10 | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) | (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24;
+__host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_mn, bool b_mn) {
+    return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 template <bool PAIR> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {      // one thread
     if constexpr (PAIR)

@@ -1,5 +1,6 @@
 // Linear cross entropy: cutting the work into pieces, tensor maps, launches.
 #include "o1d_xent.cuh"
+#include "o1d_xent_dense.cuh"
 #include "o1d_tma_host.cuh"
 #include "o1d_xent.h"
 
@@ -150,6 +151,10 @@ int make_operand(Run &r, const void *src, const Operand &o, unsigned char **ws, 
 // same sums in fp32, rounded to bf16 once).
 bool fine_of(const XentArgs &a) { return a.bf16 && (double)a.N * a.V * a.D <= (double)(1ll << 30); }
 int planes_of(const XentArgs &a) { return !a.bf16 ? 3 : fine_of(a) ? 2 : 1; }
+
+// Few classes and narrow features: one kernel for all of the backward pass (o1d_xent_dense.cuh), with one plane of G.
+bool dense_of(const XentArgs &a) { return a.bf16 && !fine_of(a) && a.V <= kDenseV && a.D <= kDenseD; }
+int dense_ctas(const XentArgs &a, int sms) { return cdiv(a.N, kXM) < sms ? cdiv(a.N, kXM) : sms; }
 
 bool few_rows(long long N, int D) { return N <= kFewRows && (N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8) * up_to(D, 8) * 4 <= kFewBytes; }
 int few_ctas(long long N, int V, int sms) {
@@ -327,6 +332,42 @@ cudaError_t finish(const float *sums, void *out, long long n, int slots, const f
     else xent_finish_few_kernel<T><<<cdiv(n, 1024), 256, 0, st>>>(sums, (T *)out, n, slots, up, count, f);
     return cudaGetLastError();
 }
+int backward_dense(Run &r) {
+    const XentArgs &a = r.a;
+    const int ctas = dense_ctas(a, r.sms);
+    unsigned char *ws = (unsigned char *)a.workspace;
+    float *dws = (float *)ws; ws += up_to(4ll * ctas * a.V * a.D, 256);
+    float *cols = (float *)ws; ws += up_to(4ll * ctas * 4 * kDenseV, 256);
+    Mat x, w;
+    int rc = make_operand(r, a.x, operand_of(a.N, a.D, true), &ws, &x);
+    if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, true), &ws, &w);
+    if (rc) return rc;
+    CUtensorMap x_map, w_map;
+    if ((*r.enc = encode(&x_map, x, kXM)) || (*r.enc = encode(&w_map, w, (int)up_to(a.V, 32)))) return O1D_ERR_CUDA;
+    const bool each = a.reduction == O1D_XENT_NONE;
+    const float f = a.smoothing < 1.f ? 1.f - a.smoothing : 1.f;
+    const float *up = each ? nullptr : a.dloss, *count = a.reduction == O1D_XENT_MEAN ? a.count : nullptr;
+    XentParams p{};
+    p.M = (int)a.N; p.N = a.V; p.tiles = cdiv(a.N, kXM);
+    p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
+    p.smooth = a.smoothing > 0.f;
+    p.lse = a.lse; p.lse_lo = a.lse + a.N; p.up = each ? a.dloss : nullptr;
+    p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
+    p.cols = a.db ? cols : nullptr; p.cols_ld = kDenseV;
+    p.vec = ((uintptr_t)a.dx & 15) == 0 && a.D % 8 == 0;
+    p.alpha_up = up; p.alpha_count = count; p.alpha = f;
+    p.err_flag = r.err_flag;
+    cudaError_t e = cudaFuncSetAttribute(xent_dense_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
+    if (e != cudaSuccess) return r.fail(e);
+    xent_dense_kernel<<<ctas, kXThreads, kDenseSmem, r.st>>>(x_map, w_map, p, a.D, (__nv_bfloat16 *)a.dx, a.dw ? dws : nullptr);
+    e = cudaGetLastError();
+    if (e == cudaSuccess && a.dw) e = finish<__nv_bfloat16>(dws, a.dw, (long long)a.V * a.D, ctas, up, count, f, r.st);
+    if (e == cudaSuccess && a.db) {
+        xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(cols, kDenseV, 4 * ctas, 4 * ctas, a.db, a.bias_bf16, nullptr, 0, a.V, up, count, f);
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? O1D_OK : r.fail(e);
+}
 template <int MODE>
 int backward(Run &r) {
     const XentArgs &a = r.a;
@@ -421,6 +462,10 @@ int backward(Run &r) {
 }  // namespace
 
 size_t xent_workspace(const XentArgs &a, bool back, int sms) {
+    if (back && dense_of(a)) {
+        const int ctas = dense_ctas(a, sms);
+        return operand_of(a.N, a.D, true).bytes + operand_of(a.V, a.D, true).bytes + (size_t)(up_to(4ll * ctas * a.V * a.D, 256) + up_to(4ll * ctas * 4 * kDenseV, 256));
+    }
     if (back) {
         const BackwardBytes b = backward_bytes(a, cut_of(a, sms));
         return b.x + b.w + b.g + b.dx + b.dw + b.col + b.more;
@@ -436,6 +481,7 @@ int xent_forward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cud
 }
 int xent_backward(const XentArgs &a, int sms, int *err_flag, cudaStream_t st, cudaError_t *cuda, int *enc) {
     Run r{a, sms, err_flag, st, cuda, enc};
+    if (dense_of(a)) return backward_dense(r);
     return !a.bf16 ? backward<XENT_F32>(r) : fine_of(a) ? backward<XENT_FINE>(r) : backward<XENT_BF16>(r);
 }
 

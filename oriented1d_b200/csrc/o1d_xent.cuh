@@ -209,6 +209,42 @@ __device__ __forceinline__ float pick(const float (&a)[32], int at) {
     return t[0];
 }
 
+// The gradient of 32 columns of a row from their exponents log2 p: u (p - (1-e) [target] - e/V), all over 1-e.  off: where the target
+// lies in the piece, if it does; the whole warp calls.
+__device__ __forceinline__ void xent_gradient(float (&a)[32], long long off, int c0, bool ignored, float scale, const XentParams &p) {
+    const int at = off >= 0 && off < 32 ? (int)off : -1;
+    const bool hit = p.one != 0.f && __any_sync(0xffffffffu, at >= 0);
+    float hot = 0.f;                                 // the target's value: p - 1 without its cancellation
+    if (hit) hot = expm1f(0.6931471805599453f * pick(a, at));
+#pragma unroll
+    for (int i = 0; i < 32; i++) a[i] = exp2_fast(a[i]);
+    if (hit) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) a[i] = at == i ? hot : a[i];
+    }
+    if (p.smooth) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) a[i] -= c0 + i < p.N ? p.eps_v : 0.f;
+    }
+    if (p.up) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) a[i] *= scale;
+    }
+    if (__any_sync(0xffffffffu, ignored)) {          // (whatever the row held: nothing comes of it)
+#pragma unroll
+        for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i];
+    }
+}
+// Eight values of a row of `n`, from column c on.
+__device__ __forceinline__ void xent_store8(__nv_bfloat16 *row, int c, int n, int vec, uint4 val) {
+    if (c >= n) return;
+    if (vec && c + 8 <= n) { *reinterpret_cast<uint4 *>(row + c) = val; return; }
+    const uint32_t x[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (c + i < n) row[c + i] = __ushort_as_bfloat16((unsigned short)(x[i >> 1] >> (16 * (i & 1))));
+}
+
 template <int KIND, int MODE, int BN, bool PAIR>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const XentParams p) {
@@ -217,7 +253,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     constexpr int GPL = SPLIT ? 3 : MODE == XENT_FINE ? 2 : 1;      // planes of G
     constexpr bool A_MN = KIND == XENT_DW, B_MN = KIND == XENT_DX || KIND == XENT_DW;
     constexpr int PIECES = BN / 128;                 // of 32 columns, for each of the four warps that share 32 rows
-    constexpr uint32_t INSTR = tc::instruction<S::TM, BN, A_MN, B_MN>();
+    constexpr uint32_t INSTR = tc::instruction(S::TM, BN, A_MN, B_MN);
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *smem = raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u);
     char *staging = reinterpret_cast<char *>(smem + S::STAGES * S::STAGE);
@@ -509,10 +545,9 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         if (!SPLIT) __syncwarp();
                     }
                     const long long off = tgt - p.col0 - c0;         // where the target lies in this piece
-                    const int at = off >= 0 && off < 32 ? (int)off : -1;
-                    const bool hit = __any_sync(0xffffffffu, at >= 0);
                     if constexpr (KIND == XENT_LOGITS) {
-                        if (hit) {
+                        const int at = off >= 0 && off < 32 ? (int)off : -1;
+                        if (__any_sync(0xffffffffu, at >= 0)) {
                             float l = pick(a, at);
                             if (SPLIT) l = fmaf(l, 1.4426950408889634f, bs[at & 31]);
                             if (at >= 0 && row < p.M) p.target_logit[row] = l;
@@ -540,26 +575,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                 a[i + 1] = u.y;
                             }
                         }
-                        float hot = 0.f;                             // the target's value: p - 1 without its cancellation
-                        if (hit && p.one != 0.f) hot = expm1f(0.6931471805599453f * pick(a, at));
-#pragma unroll
-                        for (int i = 0; i < 32; i++) a[i] = exp2_fast(a[i]);
-                        if (hit && p.one != 0.f) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) a[i] = at == i ? hot : a[i];
-                        }
-                        if (p.smooth) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) a[i] -= c0 + i < p.N ? p.eps_v : 0.f;
-                        }
-                        if (p.up) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) a[i] *= scale;
-                        }
-                        if (__any_sync(0xffffffffu, ignored)) {      // (whatever the row held: nothing comes of it)
-#pragma unroll
-                            for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i];
-                        }
+                        xent_gradient(a, off, c0, ignored, scale, p);
                         if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + lane] = column_sums(a, lane);
 #pragma unroll
                         for (int pl = 0; pl < GPL; pl++) {
@@ -592,14 +608,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         for (int i = 0; i < 16; i++) o[i] = pack_bf16(alpha * a[2 * i], alpha * a[2 * i + 1]);
                         __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(p.out);
                         xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
-                            const int c = c0 + piece * 8;
-                            if (r0 + r >= p.M || c >= p.N) return;
-                            __nv_bfloat16 *q = to + (long long)(r0 + r) * p.N + c;
-                            if (p.vec && c + 8 <= p.N) { *reinterpret_cast<uint4 *>(q) = val; return; }
-                            const uint32_t x[4] = {val.x, val.y, val.z, val.w};
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                if (c + i < p.N) q[i] = __ushort_as_bfloat16((unsigned short)(x[i >> 1] >> (16 * (i & 1))));
+                            if (r0 + r < p.M) xent_store8(to + (long long)(r0 + r) * p.N, c0 + piece * 8, p.N, p.vec, val);
                         });
                     } else {
                         float *to = static_cast<float *>(p.out) + (p.out_kind >= 2 ? w.split * p.split_elems : 0);

@@ -141,6 +141,50 @@ def test_pieces_and_parts(N, D, V, dtype, reduction):
     check(N, D, V, dtype, reduction=reduction, smoothing=0.1, ignored=0.1)
 
 
+# more than 2^30 products, up to 192 classes and 128 features: one kernel for the gradients.  Around its blocks of 64 and pieces of 32
+DENSE = [(75001, 96, 150), (43700, 128, 192), (60001, 100, 180), (270000, 63, 64), (530011, 64, 33), (2100007, 24, 22), (700001, 8, 192),
+         (260000, 65, 65), (560003, 120, 16), (4200001, 128, 2), (2300001, 3, 160), (90112, 127, 97)]
+
+
+@gpu
+@pytest.mark.parametrize("N,D,V", DENSE)
+def test_few_classes_and_narrow_features(N, D, V):
+    check(N, D, V, "bf16", ignored=0.1)
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("bias", [None, "same", "other"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 1.0])
+def test_options_of_few_classes(smoothing, bias, reduction):
+    check(100001, 96, 120, "bf16", bias, smoothing, reduction, ignored=0.3, ignore_index=7)
+
+
+@gpu
+def test_parts_of_the_gradient_of_few_classes():
+    """Any of the three gradients alone is the same, bits and all; labels that are no class and rows without a loss."""
+    x, w, b, t = make(80003, 96, 150, "bf16", ignored=0.2)
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    up = torch.rand(80003, device="cuda")
+    f = lambda t, r, *v: ops.linear_cross_entropy(v[0], v[1], t, v[2], reduction=r)  # noqa: E731
+    all_of = torch.autograd.grad(f(t, "none", *leaves), leaves, up)
+    again = torch.autograd.grad(f(t, "none", *leaves), leaves, up)
+    for i in range(3):
+        alone, = torch.autograd.grad(f(t, "none", *(v if k == i else v.detach() for k, v in enumerate(leaves))), leaves[i], up)
+        assert torch.equal(alone, all_of[i]) and torch.equal(again[i], all_of[i])
+    assert not all_of[0][t == -100].any() and all_of[0][t != -100].any(1).all()
+    none = torch.autograd.grad(f(torch.full_like(t, -100), "mean", *leaves), leaves)
+    assert not any(g.any() for g in none)
+    wrong = t.clone()
+    wrong[[5, 79999]] = torch.tensor([150, -1], device="cuda")
+    rows = f(wrong, "none", *leaves)
+    dx, = torch.autograd.grad(rows, x, up)
+    bad = torch.zeros(80003, dtype=torch.bool, device="cuda")
+    bad[[5, 79999]] = True
+    assert rows[bad].isnan().all() and dx[bad].isnan().all()
+    assert torch.equal(dx[~bad], all_of[0][~bad])
+
+
 @gpu
 def test_gradients_against_differences():
     """The fp32 gradient against central differences of the float64 loss along random directions."""

@@ -252,7 +252,7 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y,
  * x [N, D] and w [V, D] of type `dtype`, each starting on 16 bytes, bias [V] (or NULL) fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16; target [N].
  * A row whose target is ignore_index has no loss and no gradient; one whose target is outside [0, V) has a NaN loss
  * (and a NaN gradient).  reduction: O1D_XENT_NONE (loss [N]), _SUM, _MEAN (over the rows not ignored; loss [1]).
- * lse [2, N] (the log-sum-exp of a row, base 2, in two floats) and count [1] (not written for _NONE) are for the backward
+ * lse [3, N] (the log-sum-exp of a row, base 2, in two floats, and log2 of the target's probability) and count [1] (not written for _NONE) are for the backward
  * call; lse NULL: none will follow, which lets a few rows take a shorter way.
  * Sums, softmax statistics and the loss are fp32 or wider; fp32 products are exact to fp32 rounding (three bf16 planes
  * an operand on the tensor cores).  workspace: uninitialised, o1d_linear_xent_workspace_bytes() bytes, 256-byte aligned

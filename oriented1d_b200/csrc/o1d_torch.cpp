@@ -704,7 +704,7 @@ XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, 
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = as_vectors(x_), w = as_vectors(w_), target = target_.contiguous(), b = xent_bias(bias);
     const bool each = reduction == O1D_XENT_NONE;
-    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), train ? fresh({2, s.N}, at::kFloat, x) : Tensor(), each ? Tensor() : fresh({}, at::kFloat, x)};
+    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), train ? fresh({3, s.N}, at::kFloat, x) : Tensor(), each ? Tensor() : fresh({}, at::kFloat, x)};
     if (s.N == 0) {                                       // the sum of nothing, the mean of nothing
         if (!each) { o.loss.fill_(reduction == O1D_XENT_SUM ? 0. : NAN); o.count.zero_(); }
         return o;

@@ -1,4 +1,6 @@
 // Linear cross entropy: cutting the work into pieces, tensor maps, launches.
+#include <atomic>
+
 #include "o1d_xent.cuh"
 #include "o1d_xent_dense.cuh"
 #include "o1d_tma_host.cuh"
@@ -66,6 +68,16 @@ Shape shape_of(long long m, long long n, long long k, bool narrow_only, int sms)
     return k >= 512 && cp <= cw && cp <= cn ? pair : cn < cw ? narrow : wide;
 }
 
+// Sets a kernel's limit of shared memory once a device (a microsecond a call otherwise).
+cudaError_t size_once(std::atomic<uint64_t> &sized, const void *kern, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (sized.load(std::memory_order_acquire) >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) sized.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+}
+
 struct Run {                 // of one call
     const XentArgs &a;
     int sms, *err_flag;
@@ -102,7 +114,8 @@ struct Run {                 // of one call
         p.along_n = p.M > p.N;
         p.err_flag = err_flag;
         auto kern = xent_kernel<KIND, MODE, BN, PAIR>;
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        static std::atomic<uint64_t> sized{0};       // devices that know how much shared memory the kernel takes
+        cudaError_t e = size_once(sized, (const void *)kern, S::SMEM);
         if (e != cudaSuccess) return fail(e);
         const int units = PAIR ? sms / 2 : sms;
         cudaLaunchConfig_t cfg = {};
@@ -328,7 +341,7 @@ int forward(Run &r) {
 
 template <typename T>
 cudaError_t finish(const float *sums, void *out, long long n, int slots, const float *up, const float *count, float f, cudaStream_t st) {
-    if (slots > 4) xent_finish_kernel<T><<<cdiv(n, 32), dim3(32, 8), 0, st>>>(sums, (T *)out, n, slots, up, count, f);
+    if (slots > 4) xent_finish_kernel<T, 8><<<cdiv(n, 32), dim3(32, 8), 0, st>>>(sums, (T *)out, n, slots, nullptr, nullptr, 0, 0, 0, 0, up, count, f);
     else xent_finish_few_kernel<T><<<cdiv(n, 1024), 256, 0, st>>>(sums, (T *)out, n, slots, up, count, f);
     return cudaGetLastError();
 }
@@ -337,7 +350,7 @@ int backward_dense(Run &r) {
     const int ctas = dense_ctas(a, r.sms);
     unsigned char *ws = (unsigned char *)a.workspace;
     float *dws = (float *)ws; ws += up_to(4ll * ctas * a.V * a.D, 256);
-    float *cols = (float *)ws; ws += up_to(4ll * ctas * 4 * kDenseV, 256);
+    float *cols = (float *)ws; ws += up_to(4ll * ctas * kDenseV, 256);
     Mat x, w;
     int rc = make_operand(r, a.x, operand_of(a.N, a.D, true), &ws, &x);
     if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, true), &ws, &w);
@@ -351,19 +364,22 @@ int backward_dense(Run &r) {
     p.M = (int)a.N; p.N = a.V; p.tiles = cdiv(a.N, kXM);
     p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
     p.smooth = a.smoothing > 0.f;
-    p.lse = a.lse; p.lse_lo = a.lse + a.N; p.up = each ? a.dloss : nullptr;
+    p.lse = a.lse; p.lse_lo = a.lse + a.N; p.log2p = a.lse + 2 * a.N; p.up = each ? a.dloss : nullptr;
     p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
     p.cols = a.db ? cols : nullptr; p.cols_ld = kDenseV;
     p.vec = ((uintptr_t)a.dx & 15) == 0 && a.D % 8 == 0;
     p.alpha_up = up; p.alpha_count = count; p.alpha = f;
     p.err_flag = r.err_flag;
-    cudaError_t e = cudaFuncSetAttribute(xent_dense_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
+    static std::atomic<uint64_t> sized{0};
+    cudaError_t e = size_once(sized, (const void *)xent_dense_kernel, kDenseSmem);
     if (e != cudaSuccess) return r.fail(e);
     xent_dense_kernel<<<ctas, kXThreads, kDenseSmem, r.st>>>(x_map, w_map, p, a.D, (__nv_bfloat16 *)a.dx, a.dw ? dws : nullptr);
     e = cudaGetLastError();
-    if (e == cudaSuccess && a.dw) e = finish<__nv_bfloat16>(dws, a.dw, (long long)a.V * a.D, ctas, up, count, f, r.st);
-    if (e == cudaSuccess && a.db) {
-        xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(cols, kDenseV, 4 * ctas, 4 * ctas, a.db, a.bias_bf16, nullptr, 0, a.V, up, count, f);
+    const long long dw_n = a.dw ? (long long)a.V * a.D : 0;
+    const int db_n = a.db ? a.V : 0;
+    if (e == cudaSuccess && dw_n + db_n > 0) {
+        xent_finish_kernel<__nv_bfloat16, 16><<<cdiv(dw_n, 32) + cdiv(db_n, 32), dim3(32, 16), 0, r.st>>>(
+            dws, (__nv_bfloat16 *)a.dw, dw_n, ctas, cols, a.db, db_n, kDenseV, ctas, a.bias_bf16, up, count, f);
         e = cudaGetLastError();
     }
     return e == cudaSuccess ? O1D_OK : r.fail(e);
@@ -415,7 +431,7 @@ int backward(Run &r) {
         XentParams p{};
         p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.col0 = col0; p.V = a.V; p.target = a.target + row0; p.ignore = a.ignore;
         p.smooth = a.smoothing > 0.f;
-        p.lse = a.lse + row0; p.lse_lo = a.lse + a.N + row0; p.up = each ? a.dloss + row0 : nullptr;
+        p.lse = a.lse + row0; p.lse_lo = a.lse + a.N + row0; p.log2p = a.lse + 2 * a.N + row0; p.up = each ? a.dloss + row0 : nullptr;
         p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
         p.g = g; p.g_plane = gm.plane; p.g_ld = ld;
         p.cols = a.db ? cols : nullptr; p.cols_ld = ld;
@@ -464,7 +480,7 @@ int backward(Run &r) {
 size_t xent_workspace(const XentArgs &a, bool back, int sms) {
     if (back && dense_of(a)) {
         const int ctas = dense_ctas(a, sms);
-        return operand_of(a.N, a.D, true).bytes + operand_of(a.V, a.D, true).bytes + (size_t)(up_to(4ll * ctas * a.V * a.D, 256) + up_to(4ll * ctas * 4 * kDenseV, 256));
+        return operand_of(a.N, a.D, true).bytes + operand_of(a.V, a.D, true).bytes + (size_t)(up_to(4ll * ctas * a.V * a.D, 256) + up_to(4ll * ctas * kDenseV, 256));
     }
     if (back) {
         const BackwardBytes b = backward_bytes(a, cut_of(a, sms));

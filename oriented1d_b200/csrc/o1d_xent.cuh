@@ -68,7 +68,7 @@ struct XentParams {
     long long part_rows;
     int smooth;
     // GRAD
-    const float *lse, *lse_lo, *up;      // lse + lse_lo; up: per-row gradient of the loss, or null
+    const float *lse, *lse_lo, *log2p, *up;      // lse + lse_lo; of the target's probability; per-row gradient of the loss, or null
     float factor_log2, one, eps_v;   // log2(1-e), coefficient of the target, e/V; both divided by 1-e
     __nv_bfloat16 *g;
     long long g_plane;           // elements of a plane of G
@@ -154,18 +154,22 @@ __host__ __device__ inline int xent_owner(int t, int tiles, int ctas) { return (
 
 // Moves 32 rows x 64 bytes from the lanes that own the rows to memory: `vals` are the lane's four 16-byte pieces.
 // Rows go out as whole 64-byte segments.  F(row, piece, value) stores one piece.
-template <typename F>
-__device__ __forceinline__ void xent_transpose(char *stage, int lane, const uint4 (&vals)[4], F &&store) {
+__device__ __forceinline__ char *xent_staged(char *stage, int lane, int j) { return stage + lane * 64 + ((j ^ (lane >> 1)) & 3) * 16; }
+template <typename F, typename P>
+__device__ __forceinline__ void xent_transpose(char *stage, int lane, const uint4 (&vals)[4], F &&store, P &&patch) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) *reinterpret_cast<uint4 *>(stage + lane * 64 + ((j ^ (lane >> 1)) & 3) * 16) = vals[j];
+    for (int j = 0; j < 4; j++) *reinterpret_cast<uint4 *>(xent_staged(stage, lane, j)) = vals[j];
+    patch();                                             // what the lane puts over its row
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int row = i * 8 + (lane >> 2), piece = lane & 3;
-        store(row, piece, *reinterpret_cast<const uint4 *>(stage + row * 64 + ((piece ^ (row >> 1)) & 3) * 16));
+        store(row, piece, *reinterpret_cast<const uint4 *>(xent_staged(stage, row, piece)));
     }
     __syncwarp();
 }
+template <typename F>
+__device__ __forceinline__ void xent_transpose(char *stage, int lane, const uint4 (&vals)[4], F &&store) { xent_transpose(stage, lane, vals, store, [] {}); }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -180,20 +184,33 @@ __device__ __forceinline__ float take_bf16(float &v) {
     return r;
 }
 
-// Sums over the warp's lanes of 32 values each: lane i gets the sum of value i.  Each step exchanges half of what is left
-// (31 shuffles; 32 sums one after the other would be 160).  All lanes add in the same fixed order.
-__device__ __forceinline__ float column_sums(const float (&a)[32], int lane) {
-    float t[16];
-    const bool u = lane & 16;
+// Sums over the warp's lanes of 32 values each, of which a lane may have one (`at`, or -1) that is `hot` instead; in a fixed order.
+// The lane gets the sum of value column_of(lane).  Through the store buffer, half of the values at a time, the target's put over
+// what is there: a lane adds four rows of four columns, and three exchanges join the eight lanes of a column.  76 instructions;
+// by exchanges alone 124, and 64 to put the target among the registers (xent_dense_kernel, 133200 x 96 x 150: 33.5 us and 37.5).
+__device__ __forceinline__ int column_of(int lane) { return (lane & 4) * 4 + (lane & 3) * 4 + (lane >> 3 & 2) + (lane >> 3 & 1); }
+__device__ __forceinline__ float column_sums(const float (&a)[32], int lane, char *stage, int at, float hot) {
+    float s[2];
 #pragma unroll
-    for (int i = 0; i < 16; i++) t[i] = (u ? a[i + 16] : a[i]) + __shfl_xor_sync(0xffffffffu, u ? a[i] : a[i + 16], 16);
+    for (int h = 0; h < 2; h++) {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        const bool v = lane & o;
+        for (int j = 0; j < 4; j++)
+            *reinterpret_cast<float4 *>(xent_staged(stage, lane, j)) = make_float4(a[h * 16 + j * 4], a[h * 16 + j * 4 + 1], a[h * 16 + j * 4 + 2], a[h * 16 + j * 4 + 3]);
+        if (at >> 4 == h) reinterpret_cast<float *>(xent_staged(stage, lane, at >> 2 & 3))[at & 3] = hot;
+        __syncwarp();
+        float4 v[4];
 #pragma unroll
-        for (int i = 0; i < o; i++) t[i] = (v ? t[i + o] : t[i]) + __shfl_xor_sync(0xffffffffu, v ? t[i] : t[i + o], o);
+        for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const float4 *>(xent_staged(stage, i * 8 + (lane >> 2), lane & 3));
+        __syncwarp();
+        const float2 x = apart(add2(add2(two(v[0].x, v[0].y), two(v[1].x, v[1].y)), add2(two(v[2].x, v[2].y), two(v[3].x, v[3].y))));
+        const float2 y = apart(add2(add2(two(v[0].z, v[0].w), two(v[1].z, v[1].w)), add2(two(v[2].z, v[2].w), two(v[3].z, v[3].w))));
+        const bool p = lane & 16, q = lane & 8;
+        const float t0 = (p ? y.x : x.x) + __shfl_xor_sync(0xffffffffu, p ? x.x : y.x, 16);
+        const float t1 = (p ? y.y : x.y) + __shfl_xor_sync(0xffffffffu, p ? x.y : y.y, 16);
+        s[h] = (q ? t1 : t0) + __shfl_xor_sync(0xffffffffu, q ? t0 : t1, 8);
     }
-    return t[0];
+    const bool u = lane & 4;
+    return (u ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, u ? s[0] : s[1], 4);
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
@@ -209,32 +226,58 @@ __device__ __forceinline__ float pick(const float (&a)[32], int at) {
     return t[0];
 }
 
-// The gradient of 32 columns of a row from their exponents log2 p: u (p - (1-e) [target] - e/V), all over 1-e.  off: where the target
-// lies in the piece, if it does; the whole warp calls.
-__device__ __forceinline__ void xent_gradient(float (&a)[32], long long off, int c0, bool ignored, float scale, const XentParams &p) {
-    const int at = off >= 0 && off < 32 ? (int)off : -1;
-    const bool hit = p.one != 0.f && __any_sync(0xffffffffu, at >= 0);
-    float hot = 0.f;                                 // the target's value: p - 1 without its cancellation
-    if (hit) hot = expm1f(0.6931471805599453f * pick(a, at));
+// What a row's gradient G needs besides its logits.  G = u (p - (1-e) [target] - e/V), all over 1-e.  The target's value is formed
+// once a row, as expm1 of its own exponent (p - 1 without cancellation), and put over what the other columns' formula gives
+// where the row is in shared memory on its way out: in registers it would cost an instruction or two for every column.
+struct XentRow {
+    long long tgt;               // -1: none of these columns
+    float lse, lse_lo;           // what the exponents are taken from; +inf for a row without a loss, whose G then is zero
+    float eps, scale, hot;
+    bool bad;                    // a row without a loss whose logits are not finite: nothing comes of it either
+};
+struct XentAhead { long long tgt; float lse, lse_lo, log2p, scale; };      // as they are stored
+__device__ __forceinline__ XentAhead xent_fetch(long long row, const XentParams &p) {
+    XentAhead f{p.ignore, __int_as_float(0x7f800000), 0.f, 0.f, 1.f};
+    if (row < p.M) {
+        f.tgt = __ldg(p.target + row);
+        f.lse = __ldg(p.lse + row);
+        f.lse_lo = __ldg(p.lse_lo + row);
+        f.log2p = __ldg(p.log2p + row);
+        if (p.up) f.scale = __ldg(p.up + row);
+    }
+    return f;
+}
+__device__ __forceinline__ XentRow xent_row(const XentAhead &f, const XentParams &p) {
+    const bool ignored = f.tgt == p.ignore, none = f.tgt < 0 || f.tgt >= p.V;
+    XentRow r;
+    r.tgt = ignored || none || p.one == 0.f ? -1 : f.tgt - p.col0;
+    r.lse = ignored ? __int_as_float(0x7f800000) : none ? __int_as_float(0x7fffffff) : f.lse;      // no such class: NaN, not silence
+    r.lse_lo = f.lse_lo + p.factor_log2;
+    r.bad = ignored && !(fabsf(f.lse) <= 3.402823466e38f);
+    r.eps = ignored || !p.smooth ? 0.f : p.eps_v;
+    r.scale = ignored ? 0.f : f.scale;
+    r.hot = (expm1f(0.6931471805599453f * (f.log2p - p.factor_log2)) - r.eps) * r.scale;
+    return r;
+}
+// G of 32 columns, from c0 on, but for the target: from exponents log2 p.
+__device__ __forceinline__ void xent_gradient(float (&a)[32], int c0, const XentRow &r, const XentParams &p) {
 #pragma unroll
     for (int i = 0; i < 32; i++) a[i] = exp2_fast(a[i]);
-    if (hit) {
-#pragma unroll
-        for (int i = 0; i < 32; i++) a[i] = at == i ? hot : a[i];
-    }
     if (p.smooth) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) a[i] -= c0 + i < p.N ? p.eps_v : 0.f;
+        for (int i = 0; i < 32; i++) a[i] -= c0 + i < p.N ? r.eps : 0.f;
     }
     if (p.up) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) a[i] *= scale;
+        for (int i = 0; i < 32; i++) a[i] *= r.scale;
     }
-    if (__any_sync(0xffffffffu, ignored)) {          // (whatever the row held: nothing comes of it)
+    if (__any_sync(0xffffffffu, r.bad)) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) a[i] = ignored ? 0.f : a[i];
+        for (int i = 0; i < 32; i++) a[i] = r.bad ? 0.f : a[i];
     }
 }
+// Of 32 columns from c0 on, which one is the target; or -1.
+__device__ __forceinline__ int xent_at(const XentRow &r, int c0) { const long long off = r.tgt - c0; return off >= 0 && off < 32 ? (int)off : -1; }
 // Eight values of a row of `n`, from column c on.
 __device__ __forceinline__ void xent_store8(__nv_bfloat16 *row, int c, int n, int vec, uint4 val) {
     if (c >= n) return;
@@ -382,8 +425,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // LOGITS: running maximum and sum of the row's columns that this warp sees, in units of log2
         float mx = 0.f, sum = 0.f, total = 0.f;
         long long tgt = -1;
-        float lse = 0.f, lse_lo = 0.f, scale = 0.f;
-        bool ignored = false;
+        XentRow mine{};                                              // GRAD
         float alpha = 1.f;
         if (KIND >= XENT_DX && p.out_kind < 2) alpha = xent_alpha(p.alpha_up, p.alpha_count, p.alpha);
 
@@ -401,19 +443,13 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 
         // What a tile needs from memory, fetched while the one before it is worked on: bits as they are stored, since any arithmetic
         // on them here would wait for them.
-        struct Ahead { long long tgt; float lse, lse_lo, scale; uint32_t bias[PIECES]; };
+        struct Ahead { XentAhead row; uint32_t bias[PIECES]; };
         auto fetch = [&](const XentTile &w, int tile) {
-            Ahead f{p.ignore, 0.f, 0.f, 1.f, {}};
+            Ahead f{};
             if (KIND > XENT_GRAD || w.left <= 0) return f;
-            const int row = w.m * S::TM + rank * kXM + quarter * 32 + lane;
-            if (row < p.M) {
-                f.tgt = __ldg(p.target + row);
-                if (KIND == XENT_GRAD) {
-                    f.lse = __ldg(p.lse + row);
-                    f.lse_lo = __ldg(p.lse_lo + row);
-                    if (p.up) f.scale = __ldg(p.up + row);
-                }
-            }
+            const long long row = (long long)w.m * S::TM + rank * kXM + quarter * 32 + lane;
+            if (KIND == XENT_GRAD) f.row = xent_fetch(row, p);
+            else f.row.tgt = row < p.M ? __ldg(p.target + row) : p.ignore;
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
                 const int c = w.n * BN + piece_of(i, tile) * 32 + lane;
@@ -439,11 +475,8 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     m_now = w.m;
                     mx = __int_as_float(0xff800000); sum = 0.f; total = 0.f;
                 }
-                tgt = next.tgt;
-                ignored = tgt == p.ignore;
-                lse = !ignored && (tgt < 0 || tgt >= p.V) ? __int_as_float(0x7fffffff) : next.lse;      // no such class: NaN, not silence
-                lse_lo = next.lse_lo + p.factor_log2;
-                scale = next.scale;
+                tgt = next.row.tgt;
+                if (KIND == XENT_GRAD) mine = xent_row(next.row, p);
                 // in units of log2; -inf where the vocabulary ends, so that those columns weigh nothing
 #pragma unroll
                 for (int i = 0; i < PIECES; i++)
@@ -524,7 +557,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     };
                     float top = mx;                                  // LOGITS
                     if constexpr (SPLIT && KIND == XENT_GRAD) {
-                        exponents(lse, lse_lo);
+                        exponents(mine.lse, mine.lse_lo);
                     } else {
                         float top2 = __int_as_float(0xff800000);
 #pragma unroll
@@ -544,8 +577,8 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         top = fmaxf(top, top2);
                         if (!SPLIT) __syncwarp();
                     }
-                    const long long off = tgt - p.col0 - c0;         // where the target lies in this piece
                     if constexpr (KIND == XENT_LOGITS) {
+                        const long long off = tgt - p.col0 - c0;     // where the target lies in this piece
                         const int at = off >= 0 && off < 32 ? (int)off : -1;
                         if (__any_sync(0xffffffffu, at >= 0)) {
                             float l = pick(a, at);
@@ -567,7 +600,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         mx = top;
                     } else {
                         if constexpr (!SPLIT) {
-                            const F2 l = both(-(lse + lse_lo));
+                            const F2 l = both(-(mine.lse + mine.lse_lo));
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const float2 u = apart(add2(two(a[i], a[i + 1]), l));
@@ -575,8 +608,10 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                 a[i + 1] = u.y;
                             }
                         }
-                        xent_gradient(a, off, c0, ignored, scale, p);
-                        if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + lane] = column_sums(a, lane);
+                        xent_gradient(a, c0, mine, p);
+                        const int at = xent_at(mine, c0);
+                        if (p.cols && r0 < p.M) p.cols[(long long)(r0 >> 5) * p.cols_ld + c0 + column_of(lane)] = column_sums(a, lane, stage, at, mine.hot);
+                        float hot = mine.hot;
 #pragma unroll
                         for (int pl = 0; pl < GPL; pl++) {
                             uint4 out[4];
@@ -594,10 +629,12 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                     }
                                 }
                             }
+                            const __nv_bfloat16 hot_now = __float2bfloat16_rn(SPLIT ? take_bf16(hot) : hot);
+                            if (!SPLIT) hot -= __bfloat162float(hot_now);
                             __nv_bfloat16 *to = p.g + pl * p.g_plane + c0;
                             xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
                                 if (r0 + r < p.M) *reinterpret_cast<uint4 *>(to + (long long)(r0 + r) * p.g_ld + piece * 8) = val;
-                            });
+                            }, [&] { if (at >= 0) reinterpret_cast<__nv_bfloat16 *>(xent_staged(stage, lane, at >> 3))[at & 7] = hot_now; });
                         }
                     }
                 } else {
@@ -825,7 +862,7 @@ xent_rows_kernel(const XentRows a) {
     }
     double loss = 0., counted = 0.;
     if (real && lane == 0) {
-        // lse = ref + log2(sum), as two floats; the loss from its parts (where the target is the greatest, ref is its logit)
+        // lse = ref + log2(sum), as two floats; the loss, and log2 of the target's probability, from its parts (where the target is the greatest, ref is its logit)
         const float ls = log2f(sum), hi = ref + ls;
         if (a.lse) {
             const float r1 = hi - ls;
@@ -833,13 +870,14 @@ xent_rows_kernel(const XentRows a) {
             a.lse[a.rows + row] = fabsf(hi) <= 3.402823466e38f ? (ref - r1) + (ls - (hi - r1)) : 0.f;
         }
         const long long t = a.target[row];
-        float out = 0.f;
+        float out = 0.f, log2p = 0.f;
         if (t != a.ignore) {
             if (t < 0 || t >= a.V) out = __int_as_float(0x7fffffff);
             else {
-                if (a.smoothing == 0.f) out = (ref - a.target_logit[row]) + ls;
-                else {
-                    out = a.smoothing < 1.f ? (1.f - a.smoothing) * ((ref - a.target_logit[row]) + ls) : 0.f;
+                out = (ref - a.target_logit[row]) + ls;
+                log2p = -out;
+                if (a.smoothing != 0.f) {
+                    out = a.smoothing < 1.f ? (1.f - a.smoothing) * out : 0.f;
                     out += a.smoothing * ((ref - total / (float)a.V) + ls);
                 }
                 out *= 0.6931471805599453f;
@@ -847,6 +885,7 @@ xent_rows_kernel(const XentRows a) {
             loss = out;
             counted = 1.;
         }
+        if (a.lse) a.lse[2 * a.rows + row] = log2p;
         if (a.loss_rows) a.loss_rows[row] = out;
     }
     if (a.loss_rows) return;
@@ -883,23 +922,30 @@ xent_total_kernel(const double2 *__restrict__ sums, int blocks, int mean, float 
     }
 }
 
-// out = alpha * sum over slots of sums[slot], in a fixed order.  Block (32, 8): 32 elements, the slots congruent to y modulo 8.
-template <typename T>
-__global__ void __launch_bounds__(256)
-xent_finish_kernel(const float *__restrict__ sums, T *__restrict__ out, long long n, int slots, const float *up, const float *count, float f) {
-    __shared__ double part[8][33];
-    const long long i = (long long)blockIdx.x * 32 + threadIdx.x;
+// out = alpha * sum over slots of sums[slot], in a fixed order.  Block (32, Y): 32 elements, the slots congruent to y modulo Y.  The
+// blocks behind the first n elements add another matrix of sums (of n2 elements, rows of ld2) to out2.
+template <typename T, int Y>
+__global__ void __launch_bounds__(32 * Y)
+xent_finish_kernel(const float *__restrict__ sums, T *__restrict__ out, long long n, int slots, const float *__restrict__ sums2, void *__restrict__ out2, int n2,
+                   int ld2, int slots2, int bf16_2, const float *up, const float *count, float f) {
+    __shared__ double part[Y][33];
+    const long long first = (n + 31) / 32;
+    const bool more = blockIdx.x >= first;
+    const long long i = ((long long)blockIdx.x - (more ? first : 0)) * 32 + threadIdx.x, all = more ? n2 : n, step = more ? ld2 : n;
+    const float *from = (more ? sums2 : sums) + i;
+    const int rows = more ? slots2 : slots;
     double s = 0.;
-    if (i < n)
-#pragma unroll 4
-        for (int k = threadIdx.y; k < slots; k += 8) s += sums[k * n + i];
+    if (i < all)
+#pragma unroll 8
+        for (int k = threadIdx.y; k < rows; k += Y) s += from[k * step];
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && i < n) {
+    if (threadIdx.y == 0 && i < all) {
         double t = 0.;
 #pragma unroll
-        for (int y = 0; y < 8; y++) t += part[y][threadIdx.x];
-        st(out + i, xent_alpha(up, count, f) * (float)t);
+        for (int y = 0; y < Y; y++) t += part[y][threadIdx.x];
+        const float r = xent_alpha(up, count, f) * (float)t;
+        if (more) st_param(out2, i, bf16_2, r); else st(out + i, r);
     }
 }
 // The same where there are few slots and many elements: four elements a thread.

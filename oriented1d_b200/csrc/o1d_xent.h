@@ -18,7 +18,7 @@ struct XentArgs {
     float smoothing;
     int reduction;                            // O1D_XENT_*
     // forward
-    float *loss, *lse, *count;                // lse [2, N], null: no backward pass will follow
+    float *loss, *lse, *count;                // lse [3, N], null: no backward pass will follow
     // backward (lse and count are read)
     const float *dloss;
     void *dx, *dw, *db;                       // any may be null

@@ -168,32 +168,19 @@ xent_dense_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 });
             }
         };
-        // The rows' targets and statistics, fetched while the tile before is worked on
-        struct Ahead { long long tgt; float lse, lse_lo, scale; };
-        auto fetch = [&](int i) {
-            Ahead f{p.ignore, 0.f, 0.f, 1.f};
-            if (i >= mine) return f;
-            const int row = row_of(i) + lane;
-            if (row < p.M) {
-                f.tgt = __ldg(p.target + row);
-                f.lse = __ldg(p.lse + row);
-                f.lse_lo = __ldg(p.lse_lo + row);
-                if (p.up) f.scale = __ldg(p.up + row);
-            }
-            return f;
-        };
+        // (fetched while the tile before is worked on)
+        auto fetch = [&](int i) { return xent_fetch(i < mine ? (long long)row_of(i) + lane : p.M, p); };
         if ((g_pieces & 1) && part == 0) {                          // the rest of the last block of G, which nothing writes
             const int row = quarter * 32 + lane;
 #pragma unroll
             for (int j = 4; j < 8; j++) *reinterpret_cast<uint4 *>(sg + (g_pieces >> 1) * 16384 + row * 128 + ((j ^ (row & 7)) * 16)) = make_uint4(0u, 0u, 0u, 0u);
         }
         bool ok = true;
-        Ahead next = fetch(0);
+        XentAhead next = fetch(0);
         for (int i = 0; i < mine; i++) {
-            const Ahead f = next;
+            const XentRow me = xent_row(next, p);
+            const F2 lse = both(-(me.lse + me.lse_lo));
             next = fetch(i + 1);
-            const bool ignored = f.tgt == p.ignore;                  // (rows behind the last one, too)
-            const float lse = -((!ignored && (f.tgt < 0 || f.tgt >= p.V) ? __int_as_float(0x7fffffff) : f.lse) + (f.lse_lo + p.factor_log2));
             if (!(ok = await(logits, i))) break;
             if (part >= g_pieces) release(read);
             for (int j = 0, pc = part; pc < g_pieces; j++, pc += 4) {
@@ -204,13 +191,14 @@ xent_dense_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) {
                     const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + k);
-                    const float2 u = apart(add2(fma2(two(a[k], a[k + 1]), both(1.4426950408889634f), two(b.x, b.y)), both(lse)));
-                    const float2 v = apart(add2(fma2(two(a[k + 2], a[k + 3]), both(1.4426950408889634f), two(b.z, b.w)), both(lse)));
+                    const float2 u = apart(add2(fma2(two(a[k], a[k + 1]), both(1.4426950408889634f), two(b.x, b.y)), lse));
+                    const float2 v = apart(add2(fma2(two(a[k + 2], a[k + 3]), both(1.4426950408889634f), two(b.z, b.w)), lse));
                     a[k] = u.x; a[k + 1] = u.y; a[k + 2] = v.x; a[k + 3] = v.y;
                 }
-                xent_gradient(a, f.tgt - c0, c0, ignored, f.scale, p);
+                xent_gradient(a, c0, me, p);
+                const int at = xent_at(me, c0);
                 if (p.cols) {
-                    const float s = column_sums(a, lane);
+                    const float s = column_sums(a, lane, stage, at, me.hot);
                     if (j == 0) cols[0] += s; else cols[1] += s;
                 }
                 uint4 out[4];
@@ -219,9 +207,11 @@ xent_dense_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 for (int k = 0; k < 16; k++) o[k] = pack_bf16(a[2 * k], a[2 * k + 1]);
                 if (j == 0 && i > 0 && !(ok = await(done, i - 1))) break;      // G of the tile before is read
                 const int row = quarter * 32 + lane;
+                unsigned char *to = sg + (pc >> 1) * 16384 + row * 128;
+                auto chunk = [&](int k) { return to + (((pc & 1) * 4 + k) ^ (row & 7)) * 16; };
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    *reinterpret_cast<uint4 *>(sg + (pc >> 1) * 16384 + row * 128 + ((((pc & 1) * 4 + k) ^ (row & 7)) * 16)) = out[k];
+                for (int k = 0; k < 4; k++) *reinterpret_cast<uint4 *>(chunk(k)) = out[k];
+                if (at >= 0) reinterpret_cast<__nv_bfloat16 *>(chunk(at >> 3))[at & 7] = __float2bfloat16_rn(me.hot);
             }
             if (ok && part >= g_pieces && i > 0) ok = await(done, i - 1);
             if (!ok) break;
@@ -243,10 +233,17 @@ xent_dense_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                         if (d < D && pc * 32 + k < p.V) to[(long long)(pc * 32 + k) * D] = a[k];
                 }
             }
-            if (p.cols) {
-                float *to = p.cols + (long long)(blockIdx.x * 4 + quarter) * p.cols_ld + lane;
-                if (part < g_pieces) to[part * 32] = (float)cols[0];
-                if (part + 4 < g_pieces) to[part * 32 + 128] = (float)cols[1];
+        }
+        if (p.cols) {                                               // the four quarters' sums of a column in one
+            double *mine_of = reinterpret_cast<double *>(stage);
+            mine_of[lane] = cols[0];
+            mine_of[lane + 32] = cols[1];
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kXFinish) : "memory");      // (those that gave up come here, too)
+            for (int h = quarter; h < 2; h += 4) {
+                double t = 0.;
+#pragma unroll
+                for (int q = 0; q < 4; q++) t += reinterpret_cast<const double *>(staging + (part * 4 + q) * kXStaging)[h * 32 + lane];
+                if (ok && part + 4 * h < g_pieces) p.cols[(long long)blockIdx.x * p.cols_ld + (part + 4 * h) * 32 + column_of(lane)] = (float)t;
             }
         }
     }

@@ -164,7 +164,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index: int = -100,
     """F.cross_entropy(F.linear(x, weight, bias), target, ...) without the logits: features x [..., D], weight [V, D],
     bias [V] or None, int64 class indices target [...]; the loss is fp32, a scalar or (reduction="none") of target's
     shape.  Differentiable in x, weight and bias.  The logits exist a tile at a time on the chip, and their gradient a piece
-    of the classes at a time; what is kept between the passes is two floats a row.
+    of the classes at a time; what is kept between the passes is three floats a row.
 
     A row with target == ignore_index has no loss and no gradient; a target that is no class makes the row's loss (and the
     gradients) NaN, where torch stops the process.  weight is brought to x's dtype where it differs."""

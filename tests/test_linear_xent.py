@@ -355,7 +355,7 @@ def test_the_logits_are_not_kept():
     base = torch.cuda.memory_allocated()
     torch.cuda.reset_peak_memory_stats()
     loss = ops.linear_cross_entropy(*leaves[:2], t, leaves[2])
-    assert torch.cuda.memory_allocated() - base <= 16384 * 8 + 8192       # two floats a row
+    assert torch.cuda.memory_allocated() - base <= 16384 * 12 + 8192       # three floats a row
     torch.autograd.grad(loss, leaves)
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - base <= 256 << 20

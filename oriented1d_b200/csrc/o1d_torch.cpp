@@ -9,6 +9,9 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 #include "../../include/o1d.h"
@@ -398,10 +401,42 @@ void need_device(const Tensor &t, const Tensor &like, const char *what) {
     if (t.device() != like.device())
         throw py::value_error(std::string(what) + " is on " + t.device().str() + ", the first tensor on " + like.device().str());
 }
-// The nodes below differentiate once; a graph of their backward pass would silently leave them out.
-void need_first_order(const char *what) {
-    if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + " has no second derivative (create_graph=True)");
+// Nodes of the graph for the operators below: their own, since torch::autograd::Function keeps what a node needs in a dictionary of
+// boxed values and wraps outputs for every kind of operator (6-10 us a step, of which the kernels of a small call take 6).
+using torch::autograd::variable_list;
+struct TrainNode : torch::autograd::Node {
+    using torch::autograd::Node::Node;
+    std::vector<torch::autograd::SavedVariable> saved;
+    void keep(std::initializer_list<Tensor> tensors) {
+        saved.reserve(tensors.size());
+        for (const Tensor &t : tensors) saved.emplace_back(t, false);
+    }
+    Tensor kept(size_t i) const { return saved[i].unpack(); }
+    bool need(size_t i) const { return task_should_compute_output(i); }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (auto &s : saved) s.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(num_outputs());
+        if (!grads[0].defined()) return out;
+        // these differentiate once; a graph of their backward pass would silently leave them out
+        if (at::GradMode::is_enabled()) throw std::runtime_error(name() + " has no second derivative (create_graph=True)");
+        backward(grads[0], out);
+        return out;
+    }
+    virtual void backward(const Tensor &grad, variable_list &out) = 0;
+};
+template <class N, class... In> std::shared_ptr<N> make_node(const In &...in) {
+    return std::shared_ptr<N>(new N(torch::autograd::collect_next_edges(in...)), torch::autograd::deleteNode);
 }
+bool wants_grad(const Tensor &t) {
+    if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error("no forward-mode derivative");
+    return t.defined() && t.requires_grad();
+}
+bool wants_grad(const OptTensor &t) { return t && wants_grad(*t); }
+template <class... In> bool trains(const In &...in) { return (static_cast<int>(wants_grad(in)) + ...) > 0 && at::GradMode::is_enabled(); }
 // [rows, C] of a tensor whose last axis is a row; no rows is a valid tensor, no columns is not.
 struct Rows {
     int64_t rows, C;
@@ -417,13 +452,23 @@ Tensor vector_of(int64_t n, at::ScalarType type, const Tensor &like, bool zero) 
     Tensor t = fresh({n}, type, like);
     return zero ? t.zero_() : t;
 }
-struct Kept { Tensor codes, ranges; };
-Kept empty_kept(const Tensor &x) {
-    auto shape = x.sizes().vec();
-    shape.back() = (shape.back() + 127) / 128;
-    shape.push_back(2);
-    return {fresh(x.sizes(), at::kByte, x), fresh(shape, at::kFloat, x)};
-}
+// The checkpoint of a tensor of [rows, C]; behind the ranges two floats a row where LayerNorm needs them.  (All in one allocation
+// would be rounded up to the next 2 MB where it is large.)
+struct Kept {
+    Tensor codes_, side;
+    int64_t rows = 0, C = 0;
+    void make(const Rows &r, const Tensor &like, bool with_stats) {
+        rows = r.rows; C = r.C;
+        codes_ = fresh({rows * C}, at::kByte, like);
+        side = fresh({rows * ((C + 127) / 128 + with_stats) * 2}, at::kFloat, like);
+    }
+    uint8_t *codes() const { return codes_.defined() ? (uint8_t *)codes_.data_ptr() : nullptr; }
+    float *ranges() const { return side.defined() ? (float *)side.data_ptr() : nullptr; }
+    float *stats() const { return side.defined() ? ranges() + rows * ((C + 127) / 128) * 2 : nullptr; }
+    // in a node the memory is in saved variables, the rest is kept as it is
+    Kept without() const { Kept k; k.rows = rows; k.C = C; return k; }
+    Kept with(const Tensor &c, const Tensor &s) const { Kept k = *this; k.codes_ = c; k.side = s; return k; }
+};
 void need_kept(const Tensor &codes, const Tensor &ranges) {
     if (codes.scalar_type() != at::kByte || ranges.scalar_type() != at::kFloat)
         throw py::type_error("a checkpoint is uint8 codes and float32 ranges");
@@ -444,10 +489,13 @@ std::tuple<Tensor, Tensor> keep8(const Tensor &x_) {
     need_cuda(x_);
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = x_.contiguous();
-    Kept k = empty_kept(x);
+    auto shape = x.sizes().vec();
+    shape.back() = (shape.back() + 127) / 128;
+    shape.push_back(2);
+    const Tensor codes = fresh(x.sizes(), at::kByte, x), ranges = fresh(shape, at::kFloat, x);
     if (r.rows)
-        check(o1d_keep8(ptr(x), (uint8_t *)k.codes.data_ptr(), (float *)k.ranges.data_ptr(), r.rows, (int)r.C, code, stream()), "o1d_keep8");
-    return {k.codes, k.ranges};
+        check(o1d_keep8(ptr(x), (uint8_t *)codes.data_ptr(), (float *)ranges.data_ptr(), r.rows, (int)r.C, code, stream()), "o1d_keep8");
+    return {codes, ranges};
 }
 
 Tensor restore8(const Tensor &codes_, const Tensor &ranges_, bool bf16) {
@@ -476,10 +524,9 @@ std::tuple<Tensor, Kept> gelu_forward(const Tensor &x_, const OptTensor &bias, b
     if (bias) b = is_bf16(*bias) || bias->scalar_type() == at::kFloat ? bias->contiguous() : as_f32(*bias);
     Tensor y = fresh(x.sizes(), x.scalar_type(), x);
     Kept k;
-    if (keep) k = empty_kept(x);
+    if (keep) k.make(r, x, false);
     if (r.rows)
-        check(o1d_gelu_keep8(ptr(x), (const float *)ptr(b), y.data_ptr(), keep ? (uint8_t *)k.codes.data_ptr() : nullptr,
-                             keep ? (float *)k.ranges.data_ptr() : nullptr, r.rows, (int)r.C,
+        check(o1d_gelu_keep8(ptr(x), (const float *)ptr(b), y.data_ptr(), k.codes(), k.ranges(), r.rows, (int)r.C,
                              code | (bias && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
               "o1d_gelu_keep8");
     return {y, k};
@@ -488,56 +535,50 @@ std::tuple<Tensor, Kept> gelu_forward(const Tensor &x_, const OptTensor &bias, b
 struct GeluGrads { Tensor dx, db, y; };
 // dx; the bias gradient in `db_type` when `with_db` is set; the activation once more when `with_y` is.
 GeluGrads gelu_backward(const Kept &k, const Tensor &dy_, bool with_db, at::ScalarType db_type, bool with_y) {
-    const Rows r(k.codes);
     const c10::cuda::CUDAGuard guard(dy_.device());
     const Tensor dy = dy_.contiguous();
     const int code = dtype_code(dy);
     GeluGrads g{fresh(dy.sizes(), dy.scalar_type(), dy), {}, {}};
     if (with_y) g.y = fresh(dy.sizes(), dy.scalar_type(), dy);
     const bool db16 = db_type == at::kBFloat16;
-    const Scratch ws(with_db ? o1d_gelu_keep8_bwd_workspace_bytes(r.rows, (int)r.C) : 0);
-    if (with_db) g.db = vector_of(r.C, db16 ? at::kBFloat16 : at::kFloat, dy, r.rows == 0);
-    if (r.rows)
-        check(o1d_gelu_keep8_bwd((const uint8_t *)ptr(k.codes), (const float *)ptr(k.ranges), ptr(dy), g.dx.data_ptr(),
-                                 with_y ? g.y.data_ptr() : nullptr, with_db ? (float *)g.db.data_ptr() : nullptr,
-                                 ws.get(), ws.bytes, r.rows, (int)r.C, code | (db16 ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+    const Scratch ws(with_db ? o1d_gelu_keep8_bwd_workspace_bytes(k.rows, (int)k.C) : 0);
+    if (with_db) g.db = vector_of(k.C, db16 ? at::kBFloat16 : at::kFloat, dy, k.rows == 0);
+    if (k.rows)
+        check(o1d_gelu_keep8_bwd(k.codes(), k.ranges(), ptr(dy), g.dx.data_ptr(), with_y ? g.y.data_ptr() : nullptr,
+                                 with_db ? (float *)g.db.data_ptr() : nullptr, ws.get(), ws.bytes, k.rows, (int)k.C, code | (db16 ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
               "o1d_gelu_keep8_bwd");
     if (with_db) g.db = as_type(g.db, db_type);
     return g;
 }
 
-struct GeluKeep8Fn : torch::autograd::Function<GeluKeep8Fn> {
-    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const OptTensor &bias) {
-        auto [y, k] = gelu_forward(x, bias, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({k.codes, k.ranges});
-        ctx->saved_data["p"] = std::vector<int64_t>{(int64_t)x.scalar_type(), bias ? (int64_t)bias->scalar_type() : (int64_t)at::kFloat, bias.has_value()};
-        if (bias) ctx->saved_data["bias"] = bias->sizes().vec();
-        return y;
-    }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        torch::autograd::variable_list out(2);
-        if (!grads[0].defined()) return out;
-        need_first_order("gelu_keep8");
-        const auto saved = ctx->get_saved_variables();
-        const auto p = ctx->saved_data["p"].toIntVector();
-        const bool need_db = p[2] && ctx->needs_input_grad(1);
-        GeluGrads g = gelu_backward({saved[0], saved[1]}, as_type(grads[0], (at::ScalarType)p[0]), need_db, (at::ScalarType)p[1], false);
-        if (ctx->needs_input_grad(0)) out[0] = g.dx;
-        if (need_db) out[1] = as_sizes(g.db, ctx->saved_data["bias"].toIntVector());
-        return out;
+struct GeluKeep8 : TrainNode {
+    using TrainNode::TrainNode;
+    Kept k;
+    at::ScalarType type, bias_type = at::kFloat;
+    std::vector<int64_t> bias_sizes;
+    std::string name() const override { return "gelu_keep8"; }
+    void backward(const Tensor &grad, variable_list &out) override {
+        const bool need_db = need(1);
+        GeluGrads g = gelu_backward(k.with(kept(0), kept(1)), as_type(grad, type), need_db, bias_type, false);
+        if (need(0)) out[0] = g.dx;
+        if (need_db) out[1] = as_sizes(g.db, bias_sizes);
     }
 };
-bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
-bool wants_grad(const OptTensor &t) { return t && t->requires_grad(); }
 Tensor gelu_keep8(const Tensor &x, const OptTensor &bias) {
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(bias))) return GeluKeep8Fn::apply(x, bias);
-    return std::get<0>(gelu_forward(x, bias, false));
+    if (!trains(x, bias)) return std::get<0>(gelu_forward(x, bias, false));
+    const auto node = make_node<GeluKeep8>(x, bias);
+    const at::AutoGradMode off(false);
+    auto [y, k] = gelu_forward(x, bias, true);
+    node->keep({k.codes_, k.side});
+    node->k = k.without();
+    node->type = x.scalar_type();
+    if (bias) { node->bias_type = bias->scalar_type(); node->bias_sizes = bias->sizes().vec(); }
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
-struct LnKept { Kept x; Tensor stats; };
 // The checkpoint and the statistics only when `keep` is set.
-std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, const Tensor &b, double eps, bool keep) {
+std::tuple<Tensor, Kept> ln_keep_forward(const Tensor &x_, const Tensor &g, const Tensor &b, double eps, bool keep) {
     const Rows r(x_);
     const int code = dtype_code(x_);
     need_numel(g, r.C, "weight");
@@ -547,33 +588,31 @@ std::tuple<Tensor, LnKept> ln_keep_forward(const Tensor &x_, const Tensor &g, co
     const Tensor x = x_.contiguous();
     Params p(g, b);
     Tensor y = fresh(x.sizes(), x.scalar_type(), x);
-    LnKept k;
-    if (keep) k = {empty_kept(x), fresh({r.rows, 2}, at::kFloat, x)};
-    auto out = [&](const Tensor &t) { return keep ? t.data_ptr() : nullptr; };
+    Kept k;
+    if (keep) k.make(r, x, true);
     if (r.rows)
-        check(o1d_layernorm_keep8(ptr(x), (const float *)ptr(p.w), (const float *)ptr(p.b), y.data_ptr(), (uint8_t *)out(k.x.codes),
-                                  (float *)out(k.x.ranges), (float *)out(k.stats), r.rows, (int)r.C, (float)eps, code | p.flag(), stream()),
+        check(o1d_layernorm_keep8(ptr(x), (const float *)ptr(p.w), (const float *)ptr(p.b), y.data_ptr(), k.codes(), k.ranges(), k.stats(), r.rows,
+                                  (int)r.C, (float)eps, code | p.flag(), stream()),
               "o1d_layernorm_keep8");
     return {y, k};
 }
 
 struct LnGrads { Tensor dx, dg, db, y; };
-LnGrads ln_keep_backward(const LnKept &k, const Tensor &dy_, const Tensor &g, const Tensor &b, bool with_y) {
-    const Rows r(k.x.codes);
+LnGrads ln_keep_backward(const Kept &k, const Tensor &dy_, const Tensor &g, const Tensor &b, bool with_y) {
     const c10::cuda::CUDAGuard guard(dy_.device());
     const Tensor dy = dy_.contiguous();
     const int code = dtype_code(dy);
     Params p(g, b);
     LnGrads out{fresh(dy.sizes(), dy.scalar_type(), dy), {}, {}, {}};
     const auto type = p.bf16 ? at::kBFloat16 : at::kFloat;
-    out.dg = vector_of(r.C, type, dy, r.rows == 0);
-    out.db = vector_of(r.C, type, dy, r.rows == 0);
+    out.dg = vector_of(k.C, type, dy, k.rows == 0);
+    out.db = vector_of(k.C, type, dy, k.rows == 0);
     if (with_y) out.y = fresh(dy.sizes(), dy.scalar_type(), dy);
-    const Scratch ws(o1d_layernorm_keep8_bwd_workspace_bytes(r.rows, (int)r.C));
-    if (r.rows)
-        check(o1d_layernorm_keep8_bwd((const uint8_t *)ptr(k.x.codes), (const float *)ptr(k.x.ranges), (const float *)ptr(k.stats), ptr(dy),
-                                      (const float *)ptr(p.w), (const float *)ptr(p.b), out.dx.data_ptr(), with_y ? out.y.data_ptr() : nullptr,
-                                      (float *)out.dg.data_ptr(), (float *)out.db.data_ptr(), ws.get(), ws.bytes, r.rows, (int)r.C,
+    const Scratch ws(o1d_layernorm_keep8_bwd_workspace_bytes(k.rows, (int)k.C));
+    if (k.rows)
+        check(o1d_layernorm_keep8_bwd(k.codes(), k.ranges(), k.stats(), ptr(dy), (const float *)ptr(p.w), (const float *)ptr(p.b), out.dx.data_ptr(),
+                                      with_y ? out.y.data_ptr() : nullptr, (float *)out.dg.data_ptr(), (float *)out.db.data_ptr(), ws.get(), ws.bytes,
+                                      k.rows, (int)k.C,
                                       code | p.flag(), stream()),
               "o1d_layernorm_keep8_bwd");
     out.dg = as_shape(as_type(out.dg, g.scalar_type()), g);
@@ -581,29 +620,28 @@ LnGrads ln_keep_backward(const LnKept &k, const Tensor &dy_, const Tensor &g, co
     return out;
 }
 
-struct LayerNormKeep8Fn : torch::autograd::Function<LayerNormKeep8Fn> {
-    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
-        auto [y, k] = ln_keep_forward(x, g, b, eps, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({k.x.codes, k.x.ranges, k.stats, g, b});
-        ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
-        return y;
-    }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        torch::autograd::variable_list out(4);
-        if (!grads[0].defined()) return out;
-        need_first_order("layer_norm_keep8");
-        const auto s = ctx->get_saved_variables();
-        LnGrads g = ln_keep_backward({{s[0], s[1]}, s[2]}, as_type(grads[0], (at::ScalarType)ctx->saved_data["dtype"].toInt()), s[3], s[4], false);
-        if (ctx->needs_input_grad(0)) out[0] = g.dx;
-        if (ctx->needs_input_grad(1)) out[1] = g.dg;
-        if (ctx->needs_input_grad(2)) out[2] = g.db;
-        return out;
+struct LayerNormKeep8 : TrainNode {
+    using TrainNode::TrainNode;
+    Kept k;
+    at::ScalarType type;
+    std::string name() const override { return "layer_norm_keep8"; }
+    void backward(const Tensor &grad, variable_list &out) override {
+        LnGrads g = ln_keep_backward(k.with(kept(0), kept(1)), as_type(grad, type), kept(2), kept(3), false);
+        if (need(0)) out[0] = g.dx;
+        if (need(1)) out[1] = g.dg;
+        if (need(2)) out[2] = g.db;
     }
 };
 Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(g) || wants_grad(b))) return LayerNormKeep8Fn::apply(x, g, b, eps);
-    return std::get<0>(ln_keep_forward(x, g, b, eps, false));
+    if (!trains(x, g, b)) return std::get<0>(ln_keep_forward(x, g, b, eps, false));
+    const auto node = make_node<LayerNormKeep8>(x, g, b);
+    const at::AutoGradMode off(false);
+    auto [y, k] = ln_keep_forward(x, g, b, eps, true);
+    node->keep({k.codes_, k.side, g, b});
+    node->k = k.without();
+    node->type = x.scalar_type();
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 // ---- a block's LayerNorm -> Linear -> GELU -> Linear with 8-bit checkpoints -------------------------------
@@ -613,40 +651,27 @@ Tensor sum_rows(const Tensor &dy, at::ScalarType dt) {
     const int64_t ve = dy.scalar_type() == at::kFloat ? 4 : 8;
     return as_type(dy.numel() && dy.size(-1) % ve == 0 ? colsum(as_vectors(dy), dt == at::kBFloat16) : dy.sum(0, false, at::kFloat), dt);
 }
-struct MlpKeep8Fn : torch::autograd::Function<MlpKeep8Fn> {
-    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &g, const Tensor &b, const Tensor &w1, const Tensor &b1,
-                          const Tensor &w2, const Tensor &b2, double eps) {
-        auto [y, kx] = ln_keep_forward(x, g, b, eps, true);
-        auto [a, kh] = gelu_forward(at::linear(y, w1), b1, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({kx.x.codes, kx.x.ranges, kx.stats, g, b, kh.codes, kh.ranges, w1, w2});
-        ctx->saved_data["p"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)b1.scalar_type(), (int64_t)b2.scalar_type()};
-        ctx->saved_data["b1"] = b1.sizes().vec();
-        ctx->saved_data["b2"] = b2.sizes().vec();
-        return at::linear(a, w2, b2);
-    }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        torch::autograd::variable_list out(8);
-        if (!grads[0].defined()) return out;
-        need_first_order("mlp_keep8");
-        const auto s = ctx->get_saved_variables();
-        const auto p = ctx->saved_data["p"].toIntVector();
-        const Tensor &w1 = s[7], &w2 = s[8], dz = as_type(grads[0], (at::ScalarType)p[0]);
+struct MlpKeep8 : TrainNode {
+    using TrainNode::TrainNode;
+    Kept kx, kh;
+    at::ScalarType type, b1_type, b2_type;
+    std::vector<int64_t> b1_sizes, b2_sizes;
+    std::string name() const override { return "mlp_keep8"; }
+    void backward(const Tensor &grad, variable_list &out) override {
+        const Tensor g = kept(4), b = kept(5), w1 = kept(6), w2 = kept(7), dz = as_type(grad, type);
         const Tensor dz2 = dz.reshape({-1, dz.size(-1)});
         const c10::cuda::CUDAGuard guard(dz.device());
-        auto need = [&](int i) { return ctx->needs_input_grad(i); };
-        if (need(6)) out[6] = as_sizes(sum_rows(dz2, (at::ScalarType)p[2]), ctx->saved_data["b2"].toIntVector());
-        GeluGrads h = gelu_backward({s[5], s[6]}, dz.matmul(w2), need(4), (at::ScalarType)p[1], need(5));
-        if (need(4)) out[4] = as_sizes(h.db, ctx->saved_data["b1"].toIntVector());
+        if (need(6)) out[6] = as_sizes(sum_rows(dz2, b2_type), b2_sizes);
+        GeluGrads h = gelu_backward(kh.with(kept(2), kept(3)), dz.matmul(w2), need(4), b1_type, need(5));
+        if (need(4)) out[4] = as_sizes(h.db, b1_sizes);
         if (need(5)) out[5] = dz2.t().matmul(h.y.reshape({-1, h.y.size(-1)}));
         h.y = Tensor();
-        if (!(need(0) || need(1) || need(2) || need(3))) return out;
-        LnGrads n = ln_keep_backward({{s[0], s[1]}, s[2]}, h.dx.matmul(w1), s[3], s[4], need(3));
+        if (!(need(0) || need(1) || need(2) || need(3))) return;
+        LnGrads n = ln_keep_backward(kx.with(kept(0), kept(1)), h.dx.matmul(w1), g, b, need(3));
         if (need(0)) out[0] = n.dx;
         if (need(1)) out[1] = n.dg;
         if (need(2)) out[2] = n.db;
         if (need(3)) out[3] = h.dx.reshape({-1, h.dx.size(-1)}).t().matmul(n.y.reshape({-1, n.y.size(-1)}));
-        return out;
     }
 };
 Tensor mlp_keep8(const Tensor &x, const Tensor &g, const Tensor &b, const Tensor &w1, const Tensor &b1, const Tensor &w2, const Tensor &b2, double eps) {
@@ -664,10 +689,19 @@ Tensor mlp_keep8(const Tensor &x, const Tensor &g, const Tensor &b, const Tensor
     for (const Tensor *t : {&g, &b, &w1, &b1, &w2, &b2}) need_device(*t, x, "a parameter");
     const c10::cuda::CUDAGuard guard(x.device());
     const c10::impl::ExcludeDispatchKeyGuard as_given(c10::autocast_dispatch_keyset);      // the products' dtype is x's
-    bool any = wants_grad(x);
-    for (const Tensor *t : {&g, &b, &w1, &b1, &w2, &b2}) any = any || wants_grad(*t);
-    if (at::GradMode::is_enabled() && any) return MlpKeep8Fn::apply(x, g, b, w1, b1, w2, b2, eps);
-    return at::linear(std::get<0>(gelu_forward(at::linear(std::get<0>(ln_keep_forward(x, g, b, eps, false)), w1), b1, false)), w2, b2);
+    if (!trains(x, g, b, w1, b1, w2, b2))
+        return at::linear(std::get<0>(gelu_forward(at::linear(std::get<0>(ln_keep_forward(x, g, b, eps, false)), w1), b1, false)), w2, b2);
+    const auto node = make_node<MlpKeep8>(x, g, b, w1, b1, w2, b2);
+    const at::AutoGradMode off(false);
+    auto [y, kx] = ln_keep_forward(x, g, b, eps, true);
+    auto [a, kh] = gelu_forward(at::linear(y, w1), b1, true);
+    node->keep({kx.codes_, kx.side, kh.codes_, kh.side, g, b, w1, w2});
+    node->kx = kx.without(); node->kh = kh.without();
+    node->type = x.scalar_type(); node->b1_type = b1.scalar_type(); node->b2_type = b2.scalar_type();
+    node->b1_sizes = b1.sizes().vec(); node->b2_sizes = b2.sizes().vec();
+    Tensor z = at::linear(a, w2, b2);
+    torch::autograd::set_history(z, node);
+    return z;
 }
 
 // ---- softmax cross entropy of a linear classifier ----------------------------------------------------
@@ -695,8 +729,7 @@ struct XentShape {
     }
 };
 Tensor xent_bias(const OptTensor &b) { return !b ? Tensor() : is_bf16(*b) || b->scalar_type() == at::kFloat ? b->contiguous() : as_f32(*b); }
-struct XentOut { Tensor loss, lse, count; };
-// lse only when `train` is set.
+struct XentOut { Tensor loss, kept; };       // kept: three floats a row for the backward pass, and the number of rows that have a loss
 XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, const Tensor &target_, int64_t ignore, double smoothing,
                      int64_t reduction, bool train) {
     const int code = dtype_code(x_);
@@ -704,63 +737,59 @@ XentOut xent_forward(const Tensor &x_, const Tensor &w_, const OptTensor &bias, 
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = as_vectors(x_), w = as_vectors(w_), target = target_.contiguous(), b = xent_bias(bias);
     const bool each = reduction == O1D_XENT_NONE;
-    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), train ? fresh({3, s.N}, at::kFloat, x) : Tensor(), each ? Tensor() : fresh({}, at::kFloat, x)};
+    const int64_t rows = train ? 3 * s.N : 0;
+    XentOut o{fresh(each ? target.sizes() : at::IntArrayRef{}, at::kFloat, x), fresh({rows + 1}, at::kFloat, x)};
+    float *kept = (float *)o.kept.data_ptr();
     if (s.N == 0) {                                       // the sum of nothing, the mean of nothing
-        if (!each) { o.loss.fill_(reduction == O1D_XENT_SUM ? 0. : NAN); o.count.zero_(); }
+        if (!each) o.loss.fill_(reduction == O1D_XENT_SUM ? 0. : NAN);
         return o;
     }
     const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, train ? O1D_XENT_FORWARD : O1D_XENT_EVALUATION));
-    check(o1d_linear_xent(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (float *)o.loss.data_ptr(), train ? (float *)o.lse.data_ptr() : nullptr,
-                          each ? nullptr : (float *)o.count.data_ptr(), ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing,
+    check(o1d_linear_xent(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (float *)o.loss.data_ptr(), train ? kept : nullptr,
+                          each ? nullptr : kept + rows, ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing,
                           (int)reduction, code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
           "o1d_linear_xent");
     return o;
 }
 
-struct LinearXentFn : torch::autograd::Function<LinearXentFn> {
-    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target,
-                          int64_t ignore, double smoothing, int64_t reduction) {
-        XentOut o = xent_forward(x, w, bias, target, ignore, smoothing, reduction, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({x, w, bias ? *bias : Tensor(), target, o.lse, o.count});
-        ctx->saved_data["p"] = std::vector<int64_t>{ignore, reduction};
-        ctx->saved_data["smoothing"] = smoothing;
-        return o.loss;
-    }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        torch::autograd::variable_list out(7);
-        if (!grads[0].defined()) return out;
-        need_first_order("linear_cross_entropy");
-        const auto saved = ctx->get_saved_variables();
-        const OptTensor bias = saved[2].defined() ? OptTensor(saved[2]) : std::nullopt;
-        const auto p = ctx->saved_data["p"].toIntVector();
-        const double smoothing = ctx->saved_data["smoothing"].toDouble();
-        const XentShape s(saved[0], saved[1], bias, saved[3], smoothing);
-        const c10::cuda::CUDAGuard guard(saved[0].device());
-        const Tensor x = as_vectors(saved[0]), w = as_vectors(saved[1]), target = saved[3].contiguous(), b = xent_bias(bias), lse = saved[4], count = saved[5];
-        const Tensor dloss = as_type(grads[0], at::kFloat).contiguous();
-        const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), b.defined() && ctx->needs_input_grad(2)};
-        const bool none = s.N == 0;
-        if (need[0]) out[0] = fresh(x.sizes(), x.scalar_type(), x);
-        if (need[1]) { out[1] = fresh(w.sizes(), w.scalar_type(), w); if (none) out[1].zero_(); }
-        if (need[2]) out[2] = vector_of(s.V, b.scalar_type(), x, none);
+struct LinearXent : TrainNode {
+    using TrainNode::TrainNode;
+    int64_t ignore, reduction;
+    double smoothing;
+    std::string name() const override { return "linear_cross_entropy"; }
+    void backward(const Tensor &grad, variable_list &out) override {
+        const Tensor x_ = kept(0), w_ = kept(1), bias_ = kept(2), target_ = kept(3), stats = kept(4);
+        const OptTensor bias = bias_.defined() ? OptTensor(bias_) : std::nullopt;
+        const XentShape s(x_, w_, bias, target_, smoothing);
+        const c10::cuda::CUDAGuard guard(x_.device());
+        const Tensor x = as_vectors(x_), w = as_vectors(w_), target = target_.contiguous(), b = xent_bias(bias);
+        const Tensor dloss = as_type(grad, at::kFloat).contiguous();
+        const bool dx = need(0), dw = need(1), db = need(2), none = s.N == 0;
+        if (dx) out[0] = fresh(x.sizes(), x.scalar_type(), x);
+        if (dw) { out[1] = fresh(w.sizes(), w.scalar_type(), w); if (none) out[1].zero_(); }
+        if (db) out[2] = vector_of(s.V, b.scalar_type(), x, none);
         if (!none) {
             const int code = dtype_code(x);
+            const float *lse = (const float *)ptr(stats);
             const Scratch ws(o1d_linear_xent_workspace_bytes(s.N, (int)s.D, (int)s.V, code, O1D_XENT_BACKWARD));
-            check(o1d_linear_xent_bwd(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), (const float *)ptr(lse), (const float *)ptr(count),
-                                      (const float *)ptr(dloss), need[0] ? out[0].data_ptr() : nullptr, need[1] ? out[1].data_ptr() : nullptr,
-                                      need[2] ? out[2].data_ptr() : nullptr, ws.get(), ws.bytes, s.N, (int)s.D, (int)s.V, p[0], (float)smoothing,
-                                      (int)p[1], code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), stream()),
+            check(o1d_linear_xent_bwd(ptr(x), ptr(w), ptr(b), (const long long *)ptr(target), lse, lse + 3 * s.N, (const float *)ptr(dloss),
+                                      dx ? out[0].data_ptr() : nullptr, dw ? out[1].data_ptr() : nullptr, db ? out[2].data_ptr() : nullptr, ws.get(),
+                                      ws.bytes, s.N, (int)s.D, (int)s.V, ignore, (float)smoothing, (int)reduction,
+                                      code | (b.defined() && is_bf16(b) ? O1D_FLAG_PARAMS_BF16 : 0), ::stream()),
                   "o1d_linear_xent_bwd");
         }
-        if (need[2]) out[2] = as_shape(as_type(out[2], bias->scalar_type()), *bias);
-        return out;
+        if (db) out[2] = as_shape(as_type(out[2], bias->scalar_type()), *bias);
     }
 };
 Tensor linear_xent(const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target, int64_t ignore, double smoothing, int64_t reduction) {
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(bias)))
-        return LinearXentFn::apply(x, w, bias, target, ignore, smoothing, reduction);
-    return xent_forward(x, w, bias, target, ignore, smoothing, reduction, false).loss;
+    if (!trains(x, w, bias)) return xent_forward(x, w, bias, target, ignore, smoothing, reduction, false).loss;
+    const auto node = make_node<LinearXent>(x, w, bias);
+    const at::AutoGradMode off(false);
+    XentOut o = xent_forward(x, w, bias, target, ignore, smoothing, reduction, true);
+    node->keep({x, w, bias ? *bias : Tensor(), target, o.kept});
+    node->ignore = ignore; node->reduction = reduction; node->smoothing = smoothing;
+    torch::autograd::set_history(o.loss, node);
+    return o.loss;
 }
 
 Tensor conv(const Tensor &x, const Tensor &w, const Tensor &theta, const OptTensor &bias, const Tensor &host, const Tensor &dev,

@@ -192,7 +192,7 @@ struct Cut {
     long long rows;          // rows of a piece
     int dx_parts, dw_parts;  // fp32 sums; 0: the product writes its result
     int col_blocks() const { return cdiv(cdiv(rows, 32), kSlicesAtOnce); }
-    bool col_once() const { return pieces == 1 && col_blocks() == 1; }
+    bool col_once() const { return (pieces == 1 || !by_rows) && col_blocks() == 1; }      // a class's sum is complete with its piece
 };
 int parts_of(long long m, long long n, long long k, bool narrow_only, int sms, bool adds) {
     const Shape shape = shape_of(m, n, k, narrow_only, sms);
@@ -406,18 +406,23 @@ int backward(Run &r) {
     const float *up = each ? nullptr : a.dloss, *count = a.reduction == O1D_XENT_MEAN ? a.count : nullptr;
     const long long part_ld = up_to(a.V, 64);
     // One product's way out: its result at once, or sums that `finish` turns into it.
-    auto out_of = [&](XentParams &p, int parts, bool first, void *result, float *sums, long long elems, long long k) {
+    // (the last piece of a product whose pieces have one part adds the others to what it writes)
+    auto out_of = [&](XentParams &p, int parts, bool first, bool last, void *result, float *sums, long long elems, long long k) {
         p.splits = parts < 1 ? 1 : parts;
         const long long steps = cdiv(k, kXK);
         if (p.splits > steps) p.splits = (int)steps;                  // a short last piece
-        p.out = parts ? (void *)sums : result;
+        const bool joins = parts == 1 && last && !first;
+        p.out = parts && !joins ? (void *)sums : result;
+        p.before = sums;
         p.split_elems = elems;
-        p.out_kind = parts ? (first ? 2 : 3) : a.bf16 ? 0 : 1;
-        p.vec = ((uintptr_t)p.out & 15) == 0 && (long long)a.D * (p.out_kind == 0 ? 2 : 4) % 16 == 0;
+        p.out_kind = joins ? (a.bf16 ? 4 : 5) : parts ? (first ? 2 : 3) : a.bf16 ? 0 : 1;
+        // (rows of fp32 sums and of the result start on their vectors alike: four elements of the one, four or eight of the other)
+        p.vec = p.out_kind == 0 ? ((uintptr_t)p.out & 15) == 0 && a.D % 8 == 0
+                                : ((uintptr_t)p.out & 15) == 0 && a.D % 4 == 0;
         p.alpha_up = up; p.alpha_count = count; p.alpha = f;
     };
-    auto end = [&](int parts, float *sums, void *result, long long elems) {
-        if (!parts) return cudaSuccess;
+    auto end = [&](int parts, bool joined, float *sums, void *result, long long elems) {
+        if (!parts || (parts == 1 && joined)) return cudaSuccess;
         return a.bf16 ? finish<__nv_bfloat16>(sums, result, elems, parts, up, count, f, r.st)
                       : finish<float>(sums, result, elems, parts, up, count, f, r.st);
     };
@@ -441,23 +446,24 @@ int backward(Run &r) {
         if (a.dx) {
             XentParams q{};
             void *to = (char *)a.dx + row0 * a.D * es;
-            out_of(q, c.dx_parts, c.by_rows || i == 0, to, dxs, rows * a.D, ld);
+            out_of(q, c.dx_parts, c.by_rows || i == 0, i == c.pieces - 1, to, dxs, rows * a.D, ld);
             if ((rc = r.product<XENT_DX, MODE>(gm, wp, q))) return rc;
-            if (c.by_rows || i == c.pieces - 1) e = end(c.dx_parts, dxs, to, rows * a.D);
+            if (c.by_rows || i == c.pieces - 1) e = end(c.dx_parts, !c.by_rows && i > 0, dxs, to, rows * a.D);
         }
         if (e == cudaSuccess && a.dw) {
             XentParams q{};
             void *to = (char *)a.dw + (long long)col0 * a.D * es;
             Mat gv = gm;
             gv.cols = colsn;                                          // rows of dw that exist
-            out_of(q, c.dw_parts, !c.by_rows || i == 0, to, dws, (long long)colsn * a.D, rows);
+            out_of(q, c.dw_parts, !c.by_rows || i == 0, i == c.pieces - 1, to, dws, (long long)colsn * a.D, rows);
             if ((rc = r.product<XENT_DW, MODE>(gv, xs, q))) return rc;
-            if (!c.by_rows || i == c.pieces - 1) e = end(c.dw_parts, dws, to, (long long)colsn * a.D);
+            if (!c.by_rows || i == c.pieces - 1) e = end(c.dw_parts, c.by_rows && i > 0, dws, to, (long long)colsn * a.D);
         }
         if (e == cudaSuccess && a.db) {
             const int slices = cdiv(rows, 32);
             if (c.col_once())
-                xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(cols, ld, slices, slices, a.db, a.bias_bf16, nullptr, 0, a.V, up, count, f);
+                xent_bias_kernel<<<cdiv(colsn, 32), dim3(32, 32), 0, r.st>>>(cols, ld, slices, slices, (char *)a.db + (long long)col0 * (a.bias_bf16 ? 2 : 4),
+                                                                             a.bias_bf16, nullptr, 0, colsn, up, count, f);
             else
                 xent_bias_kernel<<<dim3(cdiv(colsn, 32), cdiv(slices, kSlicesAtOnce)), dim3(32, 32), 0, r.st>>>(
                     cols, ld, slices, kSlicesAtOnce, nullptr, 0, more + (long long)(c.by_rows ? i : 0) * c.col_blocks() * part_ld + col0, part_ld, colsn, nullptr,

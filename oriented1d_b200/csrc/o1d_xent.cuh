@@ -78,7 +78,9 @@ struct XentParams {
     // OUT
     void *out;                   // dx or dw (rows of N elements), or the fp32 sums of split 0
     long long split_elems;       // elements of one split's sums
-    int out_kind;                // 0: bf16 result, 1: fp32 result, 2: fp32 sums, written, 3: fp32 sums, added to
+    int out_kind;                // 0: bf16 result, 1: fp32 result, 2: fp32 sums, written, 3: fp32 sums, added to; 4, 5: bf16 / fp32 result from
+                                 // `before`, the sums of earlier pieces, and this product
+    const float *before;
     int vec;                     // rows of the output start on 16 bytes
     const float *alpha_up, *alpha_count;
     float alpha;
@@ -427,7 +429,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         long long tgt = -1;
         XentRow mine{};                                              // GRAD
         float alpha = 1.f;
-        if (KIND >= XENT_DX && p.out_kind < 2) alpha = xent_alpha(p.alpha_up, p.alpha_count, p.alpha);
+        if (KIND >= XENT_DX && (p.out_kind < 2 || p.out_kind > 3)) alpha = xent_alpha(p.alpha_up, p.alpha_count, p.alpha);
 
         auto release = [&](int i) {                                 // the accumulator may be written again
             if (rank == 0) tc::bar_arrive(taken + i); else tc::bar_arrive_in(tc::in_cta(taken + i, 0));
@@ -648,30 +650,40 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                             if (r0 + r < p.M) xent_store8(to + (long long)(r0 + r) * p.N, c0 + piece * 8, p.N, p.vec, val);
                         });
                     } else {
-                        float *to = static_cast<float *>(p.out) + (p.out_kind >= 2 ? w.split * p.split_elems : 0);
+                        float *to = static_cast<float *>(p.out) + (p.out_kind == 2 || p.out_kind == 3 ? w.split * p.split_elems : 0);
+                        const float *before = p.out_kind >= 4 ? p.before : to;
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             uint4 out[4];
                             float *o = reinterpret_cast<float *>(out);
 #pragma unroll
-                            for (int i = 0; i < 16; i++) o[i] = alpha * a[h * 16 + i];
+                            for (int i = 0; i < 16; i++) o[i] = p.out_kind == 1 ? alpha * a[h * 16 + i] : a[h * 16 + i];
                             xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
                                 const int c = c0 + h * 16 + piece * 4;
                                 if (r0 + r >= p.M || c >= p.N) return;
-                                float *q = to + (long long)(r0 + r) * p.N + c;
-                                const float x[4] = {__uint_as_float(val.x), __uint_as_float(val.y), __uint_as_float(val.z), __uint_as_float(val.w)};
+                                const long long at = (long long)(r0 + r) * p.N + c;
+                                float x[4] = {__uint_as_float(val.x), __uint_as_float(val.y), __uint_as_float(val.z), __uint_as_float(val.w)};
                                 if (p.vec && c + 4 <= p.N) {
-                                    float4 s = make_float4(x[0], x[1], x[2], x[3]);
-                                    if (p.out_kind == 3) {
-                                        const float4 old = *reinterpret_cast<const float4 *>(q);
-                                        s.x += old.x; s.y += old.y; s.z += old.z; s.w += old.w;
+                                    if (p.out_kind >= 3) {
+                                        const float4 old = *reinterpret_cast<const float4 *>(before + at);
+                                        x[0] += old.x; x[1] += old.y; x[2] += old.z; x[3] += old.w;
                                     }
-                                    *reinterpret_cast<float4 *>(q) = s;
+                                    if (p.out_kind == 4) {
+                                        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + at) =
+                                            make_uint2(pack_bf16(alpha * x[0], alpha * x[1]), pack_bf16(alpha * x[2], alpha * x[3]));
+                                        return;
+                                    }
+                                    const float f = p.out_kind == 5 ? alpha : 1.f;
+                                    *reinterpret_cast<float4 *>(to + at) = make_float4(f * x[0], f * x[1], f * x[2], f * x[3]);
                                     return;
                                 }
 #pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    if (c + i < p.N) q[i] = p.out_kind == 3 ? q[i] + x[i] : x[i];
+                                for (int i = 0; i < 4; i++) {
+                                    if (c + i >= p.N) continue;
+                                    if (p.out_kind >= 3) x[i] += before[at + i];
+                                    if (p.out_kind == 4) static_cast<__nv_bfloat16 *>(p.out)[at + i] = __float2bfloat16_rn(alpha * x[i]);
+                                    else to[at + i] = p.out_kind == 5 ? alpha * x[i] : x[i];
+                                }
                             });
                         }
                     }

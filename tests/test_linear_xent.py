@@ -136,6 +136,10 @@ def test_options(smoothing, bias, reduction, dtype):
     (9000, 100, 3, "fp32", "sum"),
     (5, 64, 30011, "bf16", "sum"),            # dx has one tile and a long K axis
     (3, 40, 9001, "fp32", "mean"),
+    (4100, 1000, 17001, "bf16", "mean"),      # pieces whose products have one part: the last one adds the others to what it writes
+    (4101, 997, 17001, "bf16", "none"),
+    (2500, 1100, 9001, "fp32", "sum"),        # the same in fp32
+    (14001, 1002, 5000, "bf16", "sum"),       # and of the rows
 ])
 def test_pieces_and_parts(N, D, V, dtype, reduction):
     check(N, D, V, dtype, reduction=reduction, smoothing=0.1, ignored=0.1)

@@ -15,26 +15,39 @@ inline bool vectors(int C, const void *x, const void *y, const void *dx, const v
     return C % 8 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(dx, 16) && aligned(codes, 8);
 }
 
-// Rows of a lane in flight: two where there are rows enough for four CTAs on every SM, else one, so that short tensors
-// reach all SMs.  100352 x 768 bf16, GELU forward / backward: one 95 / 93 us, two 80 / 84, three 90 / 99.
+// Vectors of a lane in flight: two where there are rows enough for four CTAs on every SM, else one, so that short tensors
+// reach all SMs.  Of two rows, or (bf16, whole vectors) of one row that eight lanes hold: an exchange less and half as many ranges a
+// value, but more registers.  100352 x 768 bf16, GELU forward / backward: one 92 / 87 us, two rows 82 / 85, three 90 / 99, eight
+// lanes 84 / 81; 12544 x 2048 bf16, there / back: two rows 20.6 / 12.7, eight lanes 17.7 / 10.3, four lanes of four vectors
+// 17.9 / 10.9; fp32: two rows 26.0 / 28.2, eight lanes 25.5 / 28.7.
 constexpr int kKeepFlight = 2;
 inline bool keep_many(long long rows, int C, int sms) { return rows * groups_of(C) >= (long long)kKeepWarps * (32 / lanes_of(C)) * kKeepFlight * sms * 4; }
 
-template <int KIND, typename T, bool VEC, int L>
+// Slices of the rows that the grid has along y, for CTAs that take `per` rows a round.
+int slices_of(long long rows, int C, int per, int sms) {
+    const int G = groups_of(C);
+    const long long most = (rows + per - 1) / per;
+    long long s = ((long long)sms * 16 + G - 1) / G;
+    s = s < most ? s : most;
+    return (int)(s < 1 ? 1 : s > 65535 ? 65535 : s);
+}
+
+template <int KIND, typename T, bool VEC, int L, int NV, int UN>
 cudaError_t keep_go(const KeepArgs &a, int sms, cudaStream_t st) {
-    const dim3 grid(groups_of(a.C), keep_slices(a.rows, a.C, sms));
-    if (keep_many(a.rows, a.C, sms)) keep_kernel<KIND, T, VEC, L, kKeepFlight><<<grid, kKeepThreads, 0, st>>>(a);
-    else keep_kernel<KIND, T, VEC, L, 1><<<grid, kKeepThreads, 0, st>>>(a);
+    const dim3 grid(groups_of(a.C), slices_of(a.rows, a.C, kKeepWarps * (32 / L) * UN, sms));
+    keep_kernel<KIND, T, VEC, L, NV, UN><<<grid, kKeepThreads, 0, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess && KIND == KEEP_GELU_BWD && a.dbias ? sum_slices(a.partial, a.dbias, a.C, nullptr, 0, a.pbf16, (int)grid.y, st) : e;
 }
 template <int KIND, typename T, bool VEC>
 cudaError_t keep_lanes(const KeepArgs &a, int sms, cudaStream_t st) {
-    switch (lanes_of(a.C)) {
-        case 4: return keep_go<KIND, T, VEC, 4>(a, sms, st);
-        case 8: return keep_go<KIND, T, VEC, 8>(a, sms, st);
-        default: return keep_go<KIND, T, VEC, 16>(a, sms, st);
-    }
+    const bool many = keep_many(a.rows, a.C, sms);
+    constexpr int N = kKeepFlight;
+    if (a.C <= 32) return many ? keep_go<KIND, T, VEC, 4, 1, N>(a, sms, st) : keep_go<KIND, T, VEC, 4, 1, 1>(a, sms, st);
+    if (a.C <= 64) return many ? keep_go<KIND, T, VEC, 8, 1, N>(a, sms, st) : keep_go<KIND, T, VEC, 8, 1, 1>(a, sms, st);
+    if (!many) return keep_go<KIND, T, VEC, 16, 1, 1>(a, sms, st);
+    if constexpr (VEC && sizeof(T) == 2 && KIND != KEEP_GELU_FWD) return keep_go<KIND, T, VEC, 8, 2, 1>(a, sms, st);
+    else return keep_go<KIND, T, VEC, 16, 1, N>(a, sms, st);
 }
 template <int KIND, typename T>
 cudaError_t keep_vec(const KeepArgs &a, int sms, cudaStream_t st) {
@@ -56,37 +69,41 @@ inline int ln_team(int C) { return C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 
 inline int ln_cta_rows(int C) { return C <= 128 ? kKeepWarps * (32 / lanes_of(C)) : kKeepWarps / ln_team(C); }
 
 // Short rows: several of a lane in flight where there are rows enough for four CTAs on every SM.  401408 x 96 bf16, forward /
-// backward: two 58 / 57 us, three 52 / 61, four 54 / 81 (registers).
+// backward: two 58 / 57 us, three 52 / 61, four 54 / 81 (registers).  Forward, bf16, whole vectors, 65 to 96 columns: four lanes hold a
+// row instead, three vectors each (two exchanges a sum instead of four, and at 96 no lane without values): 40.  Not elsewhere:
+// 200000 x 128 (four vectors a lane) 41 instead of 28, fp32 200000 x 96 42 instead of 33, backward 61 instead of 57 (registers).
 constexpr int kLnFlightFwd = 3, kLnFlightBwd = 2;
 template <bool BWD> inline int ln_flight(long long rows, int C, int sms) {
     constexpr int n = BWD ? kLnFlightBwd : kLnFlightFwd;
     return C <= 256 && rows >= (long long)n * ln_cta_rows(C) * sms * 4 ? n : 1;
 }
-template <bool BWD> int ln_ctas(long long rows, int C, int sms) {
-    const int per = ln_cta_rows(C) * ln_flight<BWD>(rows, C, sms);
+int ln_ctas(long long rows, int per, int sms) {
     const long long need = (rows + per - 1) / per, cap = (long long)sms * 4;
     return (int)(need < cap ? need : cap);
 }
 
-template <bool BWD, typename T, bool VEC, int LR, int TEAM, int NG, int UN>
+template <bool BWD, typename T, bool VEC, int LR, int TEAM, int NG, int NV, int UN>
 cudaError_t ln_go(const LnKeepArgs &a, int sms, cudaStream_t st) {
-    const int grid = ln_ctas<BWD>(a.rows, a.C, sms);
+    const int grid = ln_ctas(a.rows, LnRow<LR, TEAM, NG, NV>::ROWS * UN, sms);
     if constexpr (BWD) {
         constexpr int TEAMS = kKeepWarps / TEAM;
         const int smem = TEAMS > 1 ? TEAMS * 2 * a.C * (int)sizeof(float) : 0;        // at most 32 KB
-        ln_keep_bwd_kernel<T, VEC, LR, TEAM, NG, UN><<<grid, kKeepThreads, smem, st>>>(a);
+        ln_keep_bwd_kernel<T, VEC, LR, TEAM, NG, NV, UN><<<grid, kKeepThreads, smem, st>>>(a);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         return sum_slices(a.partial, a.dgamma, a.C, a.dbeta, a.C, a.pbf16, grid, st);
     } else {
-        ln_keep_kernel<T, VEC, LR, TEAM, NG, UN><<<grid, kKeepThreads, 0, st>>>(a);
+        ln_keep_kernel<T, VEC, LR, TEAM, NG, NV, UN><<<grid, kKeepThreads, 0, st>>>(a);
         return cudaGetLastError();
     }
 }
 template <bool BWD, typename T, bool VEC, int LR>
 cudaError_t ln_short(const LnKeepArgs &a, int sms, cudaStream_t st) {
     constexpr int n = BWD ? kLnFlightBwd : kLnFlightFwd;
-    return ln_flight<BWD>(a.rows, a.C, sms) == n ? ln_go<BWD, T, VEC, LR, 1, 1, n>(a, sms, st) : ln_go<BWD, T, VEC, LR, 1, 1, 1>(a, sms, st);
+    if (ln_flight<BWD>(a.rows, a.C, sms) == 1) return ln_go<BWD, T, VEC, LR, 1, 1, 1, 1>(a, sms, st);
+    if constexpr (!BWD && VEC && LR == 16 && sizeof(T) == 2)
+        if (a.C <= 96) return ln_go<false, T, true, 4, 1, 1, 3, 1>(a, sms, st);
+    return ln_go<BWD, T, VEC, LR, 1, 1, 1, n>(a, sms, st);
 }
 template <bool BWD, typename T, bool VEC>
 cudaError_t ln_width(const LnKeepArgs &a, int sms, cudaStream_t st) {
@@ -95,11 +112,11 @@ cudaError_t ln_width(const LnKeepArgs &a, int sms, cudaStream_t st) {
     if (C <= 64) return ln_short<BWD, T, VEC, 8>(a, sms, st);
     if (C <= 128) return ln_short<BWD, T, VEC, 16>(a, sms, st);
     if (C <= 256) return ln_short<BWD, T, VEC, 32>(a, sms, st);
-    if (C <= 512) return ln_go<BWD, T, VEC, 32, 1, 2, 1>(a, sms, st);
-    if (C <= 1024) return ln_go<BWD, T, VEC, 32, 2, 2, 1>(a, sms, st);
-    if (C <= 2048) return ln_go<BWD, T, VEC, 32, 4, 2, 1>(a, sms, st);
-    if (C <= 4096) return ln_go<BWD, T, VEC, 32, 8, 2, 1>(a, sms, st);
-    return ln_go<BWD, T, VEC, 32, 8, 4, 1>(a, sms, st);
+    if (C <= 512) return ln_go<BWD, T, VEC, 32, 1, 2, 1, 1>(a, sms, st);
+    if (C <= 1024) return ln_go<BWD, T, VEC, 32, 2, 2, 1, 1>(a, sms, st);
+    if (C <= 2048) return ln_go<BWD, T, VEC, 32, 4, 2, 1, 1>(a, sms, st);
+    if (C <= 4096) return ln_go<BWD, T, VEC, 32, 8, 2, 1, 1>(a, sms, st);
+    return ln_go<BWD, T, VEC, 32, 8, 4, 1, 1>(a, sms, st);
 }
 template <bool BWD, typename T>
 cudaError_t ln_vec(const LnKeepArgs &a, int sms, cudaStream_t st) {
@@ -108,19 +125,15 @@ cudaError_t ln_vec(const LnKeepArgs &a, int sms, cudaStream_t st) {
 
 }  // namespace
 
-int keep_slices(long long rows, int C, int sms) {
-    const int per = kKeepWarps * (32 / lanes_of(C)) * (keep_many(rows, C, sms) ? kKeepFlight : 1), G = groups_of(C);
-    const long long most = (rows + per - 1) / per;                       // rows of one round of a CTA
-    long long s = ((long long)sms * 16 + G - 1) / G;
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s > 65535 ? 65535 : s);
-}
+// (of the kernels that take fewest rows a round)
+int keep_slices(long long rows, int C, int sms) { return slices_of(rows, C, kKeepWarps * (32 / lanes_of(C)), sms); }
 
 cudaError_t keep_launch(int kind, bool bf16, const KeepArgs &a, int sms, cudaStream_t st) {
     return bf16 ? keep_kind<__nv_bfloat16>(kind, a, sms, st) : keep_kind<float>(kind, a, sms, st);
 }
 
-int ln_keep_ctas(long long rows, int C, int sms) { return ln_ctas<true>(rows, C, sms); }
+// (of the kernels that take fewest rows a round)
+int ln_keep_ctas(long long rows, int C, int sms) { return ln_ctas(rows, ln_cta_rows(C), sms); }
 
 cudaError_t ln_keep_launch(bool backward, bool bf16, const LnKeepArgs &a, int sms, cudaStream_t st) {
     if (backward) return bf16 ? ln_vec<true, __nv_bfloat16>(a, sms, st) : ln_vec<true, float>(a, sms, st);

@@ -19,7 +19,7 @@ namespace o1d {
 
 constexpr int kKeepThreads = 256;
 constexpr int kKeepWarps = kKeepThreads / 32;
-constexpr int kKeepLane = 8;             // values of a lane: 16 lanes hold a group, 16 bytes of bf16 each
+constexpr int kKeepLane = 8;             // values of a vector: 16 bytes of bf16
 
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -86,6 +86,7 @@ __device__ __forceinline__ F2 gelu_slope(F2 h, const Normal &n) {
 // of its part, that exist.
 template <bool VEC, int L> __device__ __forceinline__ int col_of(int c, int i) { return VEC ? c + i : c + i * L; }
 template <bool VEC> __device__ __forceinline__ int first_col(int lane) { return VEC ? lane * kKeepLane : lane; }
+// A lane has NV vectors of a group, L * 8 columns apart.  Lanes with more of a row need fewer exchanges to find its range and its sums.
 
 __device__ __forceinline__ float from_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float from_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
@@ -168,26 +169,32 @@ __device__ __forceinline__ void restore_codes(uint2 q, float2 range, F2 (&f)[4])
 // Codes of the lane's eight values and their group's range, for U groups at once (each step of the butterflies waits for the
 // one before it, and shuffles stay in the order they are written in: one group after the other, those waits were what the
 // kernels did).  end: 0 for a row that does not exist.
-template <bool VEC, int L, int U>
-__device__ __forceinline__ void keep_groups(const F2 (&f)[U][4], int c, const int (&end)[U], uint2 (&codes)[U], float2 (&range)[U]) {
+template <bool VEC, int L, int NV, int U>
+__device__ __forceinline__ void keep_groups(const F2 (&f)[U][NV][4], const int (&c)[NV], const int (&end)[U], uint2 (&codes)[U][NV], float2 (&range)[U]) {
     const float none = __int_as_float(0x7f800000);
     const bool upper = threadIdx.x & (L / 2);
     float m[U], send[U], lo[U], inv[U], step[U];
     uint32_t mask[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const float2 a = apart(f[u][0]), b = apart(f[u][1]), d = apart(f[u][2]), e = apart(f[u][3]);
         float least, most;
-        if (VEC) {
-            least = min_nan(min_nan(a.x, a.y, b.x), min_nan(b.y, d.x, d.y), min_nan(e.x, e.y));
-            most = max_nan(max_nan(a.x, a.y, b.x), max_nan(b.y, d.x, d.y), max_nan(e.x, e.y));
-            if (c >= end[u]) { least = none; most = -none; }
-        } else {
-            const float v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
-            least = none; most = -none;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (c + i * L < end[u]) { least = min_nan(least, v[i]); most = max_nan(most, v[i]); }
+        for (int j = 0; j < NV; j++) {
+            const float2 a = apart(f[u][j][0]), b = apart(f[u][j][1]), d = apart(f[u][j][2]), e = apart(f[u][j][3]);
+            float l, h;
+            if (VEC) {
+                l = min_nan(min_nan(a.x, a.y, b.x), min_nan(b.y, d.x, d.y), min_nan(e.x, e.y));
+                h = max_nan(max_nan(a.x, a.y, b.x), max_nan(b.y, d.x, d.y), max_nan(e.x, e.y));
+                if (c[j] >= end[u]) { l = none; h = -none; }
+            } else {
+                const float v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
+                l = none; h = -none;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (c[j] + i * L < end[u]) { l = min_nan(l, v[i]); h = max_nan(h, v[i]); }
+            }
+            least = j ? min_nan(least, l) : l;
+            most = j ? max_nan(most, h) : h;
         }
         // One butterfly finds both ends: the lanes of the upper half take over the (negated) greatest values, those of the
         // lower half the least ones, and the last exchange hands each the other's result.
@@ -212,22 +219,24 @@ __device__ __forceinline__ void keep_groups(const F2 (&f)[U][4], int c, const in
         inv[u] = some && !lost ? inv[u] : 0.f;
         step[u] = lost ? __int_as_float(0x7fffffff) : some ? step[u] : 0.f;
         mask[u] = lost ? 0u : 0xffffffffu;                            // a NaN or an infinity: the group is lost
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        uint32_t q[8];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            // 2^23 + t has round(t) in its lowest bits.  (Not a packed sum: the assembler makes one operation of a packed
-            // product and the packed sum behind it, with one rounding, which on ties is another code.)
-            const float2 t = apart(mul2(add2(f[u][i], both(-lo[u])), both(inv[u])));
-            q[2 * i] = __float_as_uint(__fadd_rn(t.x, 8388608.f));
-            q[2 * i + 1] = __float_as_uint(__fadd_rn(t.y, 8388608.f));
-        }
-        codes[u] = make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410) & mask[u],
-                              __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410) & mask[u]);
         range[u] = make_float2(lo[u], step[u]);
     }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            uint32_t q[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // 2^23 + t has round(t) in its lowest bits.  (Not a packed sum: the assembler makes one operation of a packed
+                // product and the packed sum behind it, with one rounding, which on ties is another code.)
+                const float2 t = apart(mul2(add2(f[u][j][i], both(-lo[u])), both(inv[u])));
+                q[2 * i] = __float_as_uint(__fadd_rn(t.x, 8388608.f));
+                q[2 * i + 1] = __float_as_uint(__fadd_rn(t.y, 8388608.f));
+            }
+            codes[u][j] = make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410) & mask[u],
+                                     __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410) & mask[u]);
+        }
 }
 template <bool VEC, int L>
 __device__ __forceinline__ void store_codes(uint8_t *row, int c, int end, uint2 q) {
@@ -241,27 +250,33 @@ __device__ __forceinline__ void store_codes(uint8_t *row, int c, int end, uint2 
 }
 
 // The elementwise kinds.  CTA (bx, by): the columns of group bx, blocks of UN * ROWS rows in steps of all the grid's; L lanes
-// hold a row's part of the group, 32/L rows a warp, UN rows of a lane are in flight at once.  Column sums of the GELU
+// hold a row's part of the group, NV vectors each, 32/L rows a warp, UN rows of a lane are in flight at once.  Column sums of the GELU
 // backward (its bias gradient) stay in registers over all rows of a thread and leave as one partial per (by, column),
 // added in a fixed order by sum_slices_kernel.  Addresses are a base that the whole CTA shares plus an offset that never
 // changes: as 64-bit products of row and column for every access they were half of all instructions.
-template <int KIND, typename T, bool VEC, int L, int UN>
+template <int KIND, typename T, bool VEC, int L, int NV, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 keep_kernel(const KeepArgs a) {
     constexpr int RW = 32 / L, ROWS = kKeepWarps * RW;           // rows of a warp, of the CTA
     const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, warp = threadIdx.x >> 5;
     const int g = blockIdx.x, G = gridDim.x, C = a.C;
-    const int c = g * kKeepGroup + first_col<VEC>(lane);
+    const int c0 = g * kKeepGroup + first_col<VEC>(lane);
     const int lim = min(C, (g + 1) * kKeepGroup);                // end of the group
     const int my_row = warp * RW + sub;
-    const unsigned off = (unsigned)my_row * (unsigned)C + (unsigned)c, range_off = (unsigned)my_row * (unsigned)G + (unsigned)g;
-    F2 b[4], sum[4];
-    if (KIND == KEEP_GELU_FWD) load_params<VEC, L>(a.bias, a.pbf16, c, lim, b);
+    const unsigned off = (unsigned)my_row * (unsigned)C + (unsigned)c0, range_off = (unsigned)my_row * (unsigned)G + (unsigned)g;
+    constexpr int NEXT = L * kKeepLane;                          // columns from one of a lane's vectors to the next
+    int c[NV];
+    F2 b[NV][4], sum[NV][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) sum[i] = both(0.f);
+    for (int j = 0; j < NV; j++) {
+        c[j] = c0 + j * NEXT;
+        if (KIND == KEEP_GELU_FWD) load_params<VEC, L>(a.bias, a.pbf16, c[j], lim, b[j]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[j][i] = both(0.f);
+    }
     struct Rows {
-        Raw8<T, VEC> raw[UN];
-        uint2 q[UN];
+        Raw8<T, VEC> raw[UN][NV];
+        uint2 q[UN][NV];
         float2 range[UN];
     };
     // end of the row part of round r0, row u: a row past the last one has no columns
@@ -273,11 +288,13 @@ keep_kernel(const KeepArgs a) {
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             const int end = row_end(r0, u);
-            if (KIND != KEEP_RESTORE) load8<VEC, L>(x + (long long)(u * ROWS) * C + off, c, end, w.raw[u]);
-            if (KIND == KEEP_RESTORE || KIND == KEEP_GELU_BWD) {
-                w.q[u] = load_codes<VEC, L>(codes + (long long)(u * ROWS) * C + off, c, end);
-                w.range[u] = end ? __ldg(ranges + (long long)(u * ROWS) * G + range_off) : make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                if (KIND != KEEP_RESTORE) load8<VEC, L>(x + (long long)(u * ROWS) * C + off + j * NEXT, c[j], end, w.raw[u][j]);
+                if (KIND == KEEP_RESTORE || KIND == KEEP_GELU_BWD) w.q[u][j] = load_codes<VEC, L>(codes + (long long)(u * ROWS) * C + off + j * NEXT, c[j], end);
             }
+            if (KIND == KEEP_RESTORE || KIND == KEEP_GELU_BWD)
+                w.range[u] = end ? __ldg(ranges + (long long)(u * ROWS) * G + range_off) : make_float2(0.f, 0.f);
         }
     };
     // Whole CTAs go round together (the groups' ranges are found with warp-wide instructions).  The next round's values are
@@ -291,66 +308,73 @@ keep_kernel(const KeepArgs a) {
         float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G;
         const Rows now = next;
         load(r0 + round, next);
-        const Raw8<T, VEC> (&raw)[UN] = now.raw;
+        const Raw8<T, VEC> (&raw)[UN][NV] = now.raw;
         int end[UN];
 #pragma unroll
         for (int u = 0; u < UN; u++) end[u] = row_end(r0, u);
         if constexpr (KIND == KEEP_FWD || KIND == KEEP_GELU_FWD) {
-            F2 f[UN][4];
+            F2 f[UN][NV][4];
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                unpack8<T, VEC>(raw[u], f[u]);
-                if constexpr (KIND == KEEP_GELU_FWD) {
-                    F2 v[4];
+            for (int u = 0; u < UN; u++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        f[u][i] = add2(f[u][i], b[i]);
-                        v[i] = gelu_of(f[u][i], normal_of<sizeof(T) == 4>(f[u][i]));
+                for (int j = 0; j < NV; j++) {
+                    unpack8<T, VEC>(raw[u][j], f[u][j]);
+                    if constexpr (KIND == KEEP_GELU_FWD) {
+                        F2 v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            f[u][j][i] = add2(f[u][j][i], b[j][i]);
+                            v[i] = gelu_of(f[u][j][i], normal_of<sizeof(T) == 4>(f[u][j][i]));
+                        }
+                        store8<VEC, L>(y + (long long)(u * ROWS) * C + off + j * NEXT, c[j], end[u], v);
                     }
-                    store8<VEC, L>(y + (long long)(u * ROWS) * C + off, c, end[u], v);
                 }
-            }
             if (KIND == KEEP_FWD || a.codes) {
-                uint2 q[UN];
+                uint2 q[UN][NV];
                 float2 range[UN];
-                keep_groups<VEC, L, UN>(f, c, end, q, range);
+                keep_groups<VEC, L, NV, UN>(f, c, end, q, range);
 #pragma unroll
                 for (int u = 0; u < UN; u++) {
-                    store_codes<VEC, L>(codes + (long long)(u * ROWS) * C + off, c, end[u], q[u]);
+#pragma unroll
+                    for (int j = 0; j < NV; j++) store_codes<VEC, L>(codes + (long long)(u * ROWS) * C + off + j * NEXT, c[j], end[u], q[u][j]);
                     if (end[u] && lane == 0) ranges[(long long)(u * ROWS) * G + range_off] = range[u];
                 }
             }
         } else {
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                F2 v[4];
-                restore_codes(now.q[u], now.range[u], v);
-                if constexpr (KIND == KEEP_GELU_BWD) {
-                    F2 d[4], f[4];
-                    unpack8<T, VEC>(raw[u], f);
+            for (int u = 0; u < UN; u++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const Normal n = normal_of<sizeof(T) == 4>(v[i]);
-                        d[i] = mul2(f[i], gelu_slope(v[i], n));
-                        sum[i] = add2(sum[i], d[i]);             // rows that do not exist add zeros; columns are never read
-                        if (a.y) v[i] = gelu_of(v[i], n);
+                for (int j = 0; j < NV; j++) {
+                    F2 v[4];
+                    restore_codes(now.q[u][j], now.range[u], v);
+                    if constexpr (KIND == KEEP_GELU_BWD) {
+                        F2 d[4], f[4];
+                        unpack8<T, VEC>(raw[u][j], f);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const Normal n = normal_of<sizeof(T) == 4>(v[i]);
+                            d[i] = mul2(f[i], gelu_slope(v[i], n));
+                            sum[j][i] = add2(sum[j][i], d[i]);   // rows that do not exist add zeros; columns are never read
+                            if (a.y) v[i] = gelu_of(v[i], n);
+                        }
+                        store8<VEC, L>(dx + (long long)(u * ROWS) * C + off + j * NEXT, c[j], end[u], d);
                     }
-                    store8<VEC, L>(dx + (long long)(u * ROWS) * C + off, c, end[u], d);
+                    if (KIND == KEEP_RESTORE || a.y) store8<VEC, L>(y + (long long)(u * ROWS) * C + off + j * NEXT, c[j], end[u], v);
                 }
-                if (KIND == KEEP_RESTORE || a.y) store8<VEC, L>(y + (long long)(u * ROWS) * C + off, c, end[u], v);
-            }
         }
     }
     if constexpr (KIND == KEEP_GELU_BWD) {
         if (!a.dbias) return;
         __shared__ float red[kKeepWarps][kKeepGroup];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float t = i & 1 ? apart(sum[i >> 1]).y : apart(sum[i >> 1]).x;
+        for (int j = 0; j < NV; j++)
 #pragma unroll
-            for (int o = L; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (sub == 0) red[warp][col_of<VEC, L>(first_col<VEC>(lane), i)] = t;
-        }
+            for (int i = 0; i < 8; i++) {
+                float t = i & 1 ? apart(sum[j][i >> 1]).y : apart(sum[j][i >> 1]).x;
+#pragma unroll
+                for (int o = L; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                if (sub == 0) red[warp][col_of<VEC, L>(first_col<VEC>(lane) + j * NEXT, i)] = t;
+            }
         __syncthreads();
         if (threadIdx.x < lim - g * kKeepGroup) {
             float s = 0.f;
@@ -382,8 +406,10 @@ __device__ __forceinline__ void team_sum(float (&v)[NV], float (*slot)[NV], int 
 
 // How a row is held: LR lanes (4 to 16 for one group, 32/LR rows a warp; 32 for two groups side by side), a team of TEAM
 // warps, NG passes of a warp's lanes along the row.  L: lanes of a group.
-template <int LR, int TEAM, int NG> struct LnRow {
+// A lane has NV vectors of each of its groups.
+template <int LR, int TEAM, int NG, int NV> struct LnRow {
     static constexpr int L = LR < 16 ? LR : 16, PER_PASS = LR == 32 ? 2 : 1, RW = 32 / LR, TEAMS = kKeepWarps / TEAM;
+    static constexpr int NP = NG * NV;               // vectors of a lane
     static constexpr int ROWS = TEAMS * RW;          // rows of a CTA
     int lane, team, wt, half, row;                   // lane within its group; group of the pass; row of the CTA
     __device__ __forceinline__ LnRow() {
@@ -391,39 +417,41 @@ template <int LR, int TEAM, int NG> struct LnRow {
         lane = l % L; half = LR == 32 ? l / 16 : 0; team = warp / TEAM; wt = warp % TEAM; row = team * RW + l / LR;
     }
     __device__ __forceinline__ int group(int j) const { return (wt * NG + j) * PER_PASS + half; }
+    template <bool VEC> __device__ __forceinline__ int column(int v) const {      // the first of vector v
+        return group(v / NV) * kKeepGroup + first_col<VEC>(lane) + v % NV * (L * kKeepLane);
+    }
 };
 
 // LayerNorm over rows of up to 8192 columns, y = (x - mean) * rstd * gamma + beta, the row held in registers.  Statistics are
 // two-pass, fp32.  Kept for the backward pass: the codes of x, mean and rstd.  UN rows of a lane are in flight at once
 // (short rows: what bounds the kernel is memory, and a lane's piece of a row is 16 bytes).
-template <typename T, bool VEC, int LR, int TEAM, int NG, int UN>
+template <typename T, bool VEC, int LR, int TEAM, int NG, int NV, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 ln_keep_kernel(const LnKeepArgs a) {
-    using R = LnRow<LR, TEAM, NG>;
-    constexpr int L = R::L;
+    using R = LnRow<LR, TEAM, NG, NV>;
+    constexpr int L = R::L, NP = R::NP;
     __shared__ float s1[kKeepWarps][UN], s2[kKeepWarps][UN];
     const R w;
     const int C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
     const float inv_c = 1.f / (float)C;
     const unsigned off = (unsigned)(w.row * C), range_off = (unsigned)(w.row * G);
-    F2 gm[NG][4], bt[NG][4];
-    int c[NG], lim[NG];
+    F2 gm[NP][4], bt[NP][4];
+    int c[NP], lim[NP];
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
-        const int g = w.group(j);
-        c[j] = g * kKeepGroup + first_col<VEC>(w.lane);
-        lim[j] = min(C, (g + 1) * kKeepGroup);
+    for (int j = 0; j < NP; j++) {
+        c[j] = w.template column<VEC>(j);
+        lim[j] = min(C, (w.group(j / NV) + 1) * kKeepGroup);
         load_params<VEC, L>(a.gamma, a.pbf16, c[j], lim[j], gm[j]);
         load_params<VEC, L>(a.beta, a.pbf16, c[j], lim[j], bt[j]);
     }
-    struct Rows { Raw8<T, VEC> raw[UN][NG]; };
+    struct Rows { Raw8<T, VEC> raw[UN][NP]; };
     auto exists = [&](long long r0, int u) { return w.row < a.rows - r0 - u * R::ROWS; };
     auto load = [&](long long r0, Rows &to) {
         const T *x = static_cast<const T *>(a.x) + r0 * C;
 #pragma unroll
         for (int u = 0; u < UN; u++)
 #pragma unroll
-            for (int j = 0; j < NG; j++)
+            for (int j = 0; j < NP; j++)
                 load8<VEC, L>(x + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], exists(r0, u) ? lim[j] : 0, to.raw[u][j]);
     };
     // the next round's rows are on their way while this one's are worked on
@@ -436,7 +464,7 @@ ln_keep_kernel(const LnKeepArgs a) {
         float2 *ranges = reinterpret_cast<float2 *>(a.ranges) + r0 * G, *stats = reinterpret_cast<float2 *>(a.stats) + r0;
         const Rows now = next;
         load(r0 + round, next);
-        const Raw8<T, VEC> (&raw)[UN][NG] = now.raw;
+        const Raw8<T, VEC> (&raw)[UN][NP] = now.raw;
         float s[UN], mean[UN];
         bool act[UN];
 #pragma unroll
@@ -445,7 +473,7 @@ ln_keep_kernel(const LnKeepArgs a) {
         for (int u = 0; u < UN; u++) {
             s[u] = 0.f;
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
+            for (int j = 0; j < NP; j++) {
                 F2 f[4];
                 unpack8<T, VEC>(raw[u][j], f);
                 const float2 t = apart(add2(add2(f[0], f[1]), add2(f[2], f[3])));
@@ -459,7 +487,7 @@ ln_keep_kernel(const LnKeepArgs a) {
             mean[u] = s[u] * inv_c;
             s[u] = 0.f;
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
+            for (int j = 0; j < NP; j++) {
                 F2 f[4], sq = both(0.f);
                 unpack8<T, VEC>(raw[u][j], f);
 #pragma unroll
@@ -483,27 +511,34 @@ ln_keep_kernel(const LnKeepArgs a) {
             if (a.codes && act[u] && w.lane == 0 && w.half == 0 && w.wt == 0) stats[u * R::ROWS + w.row] = make_float2(mean[u], s[u]);
         }
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            if ((w.wt * NG + j) * R::PER_PASS >= G) break;                      // the same for the whole warp
-            F2 f[UN][4];
-            int end[UN];
-            uint2 q[UN];
+        for (int k = 0; k < NG; k++) {
+            if ((w.wt * NG + k) * R::PER_PASS >= G) break;                      // the same for the whole warp
+            F2 f[UN][NV][4];
+            int end[UN], col[NV];
+            uint2 q[UN][NV];
             float2 range[UN];
 #pragma unroll
             for (int u = 0; u < UN; u++) {
-                end[u] = act[u] ? lim[j] : 0;
-                F2 o[4];
-                unpack8<T, VEC>(raw[u][j], f[u]);
+                end[u] = act[u] ? lim[k * NV] : 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = fma2(mul2(add2(f[u][i], both(-mean[u])), both(s[u])), gm[j][i], bt[j][i]);
-                store8<VEC, L>(y + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end[u], o);
+                for (int v = 0; v < NV; v++) {
+                    const int j = k * NV + v;
+                    col[v] = c[j];
+                    F2 o[4];
+                    unpack8<T, VEC>(raw[u][j], f[u][v]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[i] = fma2(mul2(add2(f[u][v][i], both(-mean[u])), both(s[u])), gm[j][i], bt[j][i]);
+                    store8<VEC, L>(y + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end[u], o);
+                }
             }
             if (!a.codes) continue;
-            keep_groups<VEC, L, UN>(f, c[j], end, q, range);
+            keep_groups<VEC, L, NV, UN>(f, col, end, q, range);
 #pragma unroll
             for (int u = 0; u < UN; u++) {
-                store_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end[u], q[u]);
-                if (act[u] && w.lane == 0 && w.group(j) < G) ranges[(long long)(u * R::ROWS) * G + (range_off + w.group(j))] = range[u];
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+                    store_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + col[v]), col[v], end[u], q[u][v]);
+                if (act[u] && w.lane == 0 && w.group(k) < G) ranges[(long long)(u * R::ROWS) * G + (range_off + w.group(k))] = range[u];
             }
         }
     }
@@ -513,24 +548,23 @@ ln_keep_kernel(const LnKeepArgs a) {
 //   dx = rstd * (g - mean_C(g) - xhat * mean_C(g * xhat)),  dgamma = sum_rows dy * xhat,  dbeta = sum_rows dy.
 // Column sums as in layernorm_cl_bwd_kernel: registers, then the CTA's teams in order, then the CTAs in order
 // (sum_slices_kernel).  Dynamic shared memory: teams x 2 x C floats where a CTA has more than one team.
-template <typename T, bool VEC, int LR, int TEAM, int NG, int UN>
+template <typename T, bool VEC, int LR, int TEAM, int NG, int NV, int UN>
 __global__ void __launch_bounds__(kKeepThreads)
 ln_keep_bwd_kernel(const LnKeepArgs a) {
-    using R = LnRow<LR, TEAM, NG>;
-    constexpr int L = R::L;
+    using R = LnRow<LR, TEAM, NG, NV>;
+    constexpr int L = R::L, NP = R::NP;
     extern __shared__ float ln_cols[];
     __shared__ float s1[2][kKeepWarps][2 * UN];
     const R w;
     const int C = a.C, G = (C + kKeepGroup - 1) / kKeepGroup;
     const float inv_c = 1.f / (float)C;
     const unsigned off = (unsigned)(w.row * C), range_off = (unsigned)(w.row * G);
-    F2 gm[NG][4], sg[NG][4], sb[NG][4];
-    int c[NG], lim[NG];
+    F2 gm[NP][4], sg[NP][4], sb[NP][4];
+    int c[NP], lim[NP];
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
-        const int g = w.group(j);
-        c[j] = g * kKeepGroup + first_col<VEC>(w.lane);
-        lim[j] = min(C, (g + 1) * kKeepGroup);
+    for (int j = 0; j < NP; j++) {
+        c[j] = w.template column<VEC>(j);
+        lim[j] = min(C, (w.group(j / NV) + 1) * kKeepGroup);
         load_params<VEC, L>(a.gamma, a.pbf16, c[j], lim[j], gm[j]);
 #pragma unroll
         for (int i = 0; i < 4; i++) sg[j][i] = sb[j][i] = both(0.f);
@@ -548,9 +582,9 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
         }
     };
     struct Rows {
-        Raw8<T, VEC> raw[UN][NG];
+        Raw8<T, VEC> raw[UN][NP];
         float2 st[UN], range[UN][NG];
-        uint2 q[UN][NG];
+        uint2 q[UN][NP];
     };
     auto exists = [&](long long r0, int u) { return w.row < a.rows - r0 - u * R::ROWS; };
     auto load = [&](long long r0, Rows &to) {
@@ -562,12 +596,13 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
             const bool on = exists(r0, u);
             to.st[u] = on ? __ldg(stats + u * R::ROWS + w.row) : make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
+            for (int j = 0; j < NP; j++) {
                 const int end = on ? lim[j] : 0;
                 load8<VEC, L>(dy + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end, to.raw[u][j]);
                 to.q[u][j] = load_codes<VEC, L>(codes + (long long)(u * R::ROWS) * C + (off + c[j]), c[j], end);
-                // (columns that do not exist: dy, gamma and this are zero, whatever their group holds)
-                to.range[u][j] = c[j] < end ? __ldg(ranges + (long long)(u * R::ROWS) * G + (range_off + w.group(j))) : make_float2(0.f, 0.f);
+                // (columns that do not exist: dy, gamma and this are zero, whatever their group holds; with more vectors than one the
+                // row is that group)
+                if (j % NV == 0) to.range[u][j / NV] = c[j] < end ? __ldg(ranges + (long long)(u * R::ROWS) * G + (range_off + w.group(j / NV))) : make_float2(0.f, 0.f);
             }
         }
     };
@@ -582,9 +617,9 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
         if (!AHEAD) load(r0, next);
         const Rows now = next;
         if (AHEAD) load(r0 + round, next);
-        const Raw8<T, VEC> (&raw)[UN][NG] = now.raw;
+        const Raw8<T, VEC> (&raw)[UN][NP] = now.raw;
         const float2 (&st)[UN] = now.st, (&range)[UN][NG] = now.range;
-        const uint2 (&q)[UN][NG] = now.q;
+        const uint2 (&q)[UN][NP] = now.q;
         float s[2 * UN];
         bool act[UN];
 #pragma unroll
@@ -593,9 +628,9 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
         for (int u = 0; u < UN; u++) {
             F2 t1 = both(0.f), t2 = both(0.f);
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
+            for (int j = 0; j < NP; j++) {
                 F2 d[4], h[4];
-                normalised(q[u][j], range[u][j], st[u], j, h);
+                normalised(q[u][j], range[u][j / NV], st[u], j, h);
                 unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -616,10 +651,10 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
         for (int u = 0; u < UN; u++) {
             const float c1 = s[2 * u] * inv_c, c2 = s[2 * u + 1] * inv_c;
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
+            for (int j = 0; j < NP; j++) {
                 const int end = act[u] ? lim[j] : 0;
                 F2 d[4], h[4], o[4];
-                normalised(q[u][j], range[u][j], st[u], j, h);
+                normalised(q[u][j], range[u][j / NV], st[u], j, h);
                 unpack8<T, VEC>(raw[u][j], d);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
@@ -637,7 +672,7 @@ ln_keep_bwd_kernel(const LnKeepArgs a) {
     }
     float *out = a.partial + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
+    for (int j = 0; j < NP; j++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int k = col_of<VEC, L>(c[j], i);

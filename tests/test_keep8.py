@@ -189,6 +189,48 @@ def test_layer_norm_keep8(C, dtype, params):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C", [8, 24, 40, 64, 72, 80, 88, 96, 97, 104, 128, 136, 200])
+def test_many_rows(C, dtype):
+    """Enough rows for the kernels that hold several vectors of a lane at once: a row's checkpoint and GELU are those it has
+    among few rows, bit for bit; LayerNorm, whose sums are in another order, is within the roundings of the formula."""
+    rows, some = 120001, 500
+    x, dy = (make(2 * some, C, dtype, k).cuda().repeat(-(-rows // (2 * some)), 1)[:rows] for k in (8, 9))
+    x = (x.float() * torch.linspace(0.5, 2, rows, device="cuda")[:, None]).to(DT[dtype])
+    b = make(1, C, "fp32", 3)[0].cuda().to(DT[dtype])
+    codes, ranges = ops.keep8(x)
+    back = ops.restore8(codes, ranges, DT[dtype])
+    leaves = [t.requires_grad_(True) for t in (x, b)]
+    y = ops.gelu_keep8(*leaves)
+    dx, db = torch.autograd.grad(y, leaves, dy)
+    for at in (0, 60000, rows - some):
+        part = x.detach()[at:at + some].clone().requires_grad_(True)
+        pc, pr = ops.keep8(part)
+        assert torch.equal(pc, codes[at:at + some]) and torch.equal(pr, ranges[at:at + some])
+        assert torch.equal(ops.restore8(pc, pr, DT[dtype]), back[at:at + some])
+        py = ops.gelu_keep8(part, b.detach())
+        assert torch.equal(py, y[at:at + some])
+        assert torch.equal(torch.autograd.grad(py, part, dy[at:at + some])[0], dx[at:at + some])
+    ref = dx.double() if dtype == "fp32" else None                           # (bf16: the sum is of what dx was rounded from)
+    if ref is not None:
+        assert ((db.double() - ref.sum(0)).abs() <= 2e-6 * ref.abs().sum(0)).all()
+
+    w = (1 + 0.2 * make(1, C, "fp32", 6)[0]).cuda()
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b.float())]
+    y = ops.layer_norm_keep8(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    kept = ops.restore8(codes, ranges).double()                              # fp32: a rounding away from what the kernel holds
+    ry, rdx, rdw, rdb, xhat, rstd, g = _ln_ref(x.detach(), dy, w, b.detach(), 1e-6, kept)
+    hat = (x.detach().double().abs().amax(1, keepdim=True) * rstd) + xhat.abs().amax(1, keepdim=True)
+    half = 2.0 ** -8 if dtype == "bf16" else 0.0
+    assert ((y.double() - ry).abs() <= 2e-6 * (hat * w.abs().max() + b.detach().double().abs().max()) + half * ry.abs()).all()
+    most = rstd * g.abs().amax(1, keepdim=True) * (1 + hat * xhat.abs().amax(1, keepdim=True))
+    assert ((grads[0].double() - rdx).abs() <= 2e-6 * most + half * rdx.abs()).all()
+    assert ((grads[1].double() - rdw).abs() <= 2e-6 * (dy.double().abs() * hat).sum(0)).all()
+    assert ((grads[2].double() - rdb).abs() <= 2e-6 * dy.double().abs().sum(0)).all()
+
+
+@gpu
 def test_gradients_against_differences():
     """The gradient belongs to the function at the kept values: with an input that the checkpoint holds exactly (256
     evenly spaced values a group) it is the derivative of the forward pass itself."""

@@ -428,6 +428,7 @@ struct TrainNode : torch::autograd::Node {
     }
     virtual void backward(const Tensor &grad, variable_list &out) = 0;
 };
+// (What a node's forward pass calls is dispatched below autograd: recorded nowhere, and no view of anything to autograd.)
 template <class N, class... In> std::shared_ptr<N> make_node(const In &...in) {
     return std::shared_ptr<N>(new N(torch::autograd::collect_next_edges(in...)), torch::autograd::deleteNode);
 }
@@ -567,7 +568,7 @@ struct GeluKeep8 : TrainNode {
 Tensor gelu_keep8(const Tensor &x, const OptTensor &bias) {
     if (!trains(x, bias)) return std::get<0>(gelu_forward(x, bias, false));
     const auto node = make_node<GeluKeep8>(x, bias);
-    const at::AutoGradMode off(false);
+    const at::AutoDispatchBelowADInplaceOrView off;
     auto [y, k] = gelu_forward(x, bias, true);
     node->keep({k.codes_, k.side});
     node->k = k.without();
@@ -635,7 +636,7 @@ struct LayerNormKeep8 : TrainNode {
 Tensor layer_norm_keep8(const Tensor &x, const Tensor &g, const Tensor &b, double eps) {
     if (!trains(x, g, b)) return std::get<0>(ln_keep_forward(x, g, b, eps, false));
     const auto node = make_node<LayerNormKeep8>(x, g, b);
-    const at::AutoGradMode off(false);
+    const at::AutoDispatchBelowADInplaceOrView off;
     auto [y, k] = ln_keep_forward(x, g, b, eps, true);
     node->keep({k.codes_, k.side, g, b});
     node->k = k.without();
@@ -692,7 +693,7 @@ Tensor mlp_keep8(const Tensor &x, const Tensor &g, const Tensor &b, const Tensor
     if (!trains(x, g, b, w1, b1, w2, b2))
         return at::linear(std::get<0>(gelu_forward(at::linear(std::get<0>(ln_keep_forward(x, g, b, eps, false)), w1), b1, false)), w2, b2);
     const auto node = make_node<MlpKeep8>(x, g, b, w1, b1, w2, b2);
-    const at::AutoGradMode off(false);
+    const at::AutoDispatchBelowADInplaceOrView off;
     auto [y, kx] = ln_keep_forward(x, g, b, eps, true);
     auto [a, kh] = gelu_forward(at::linear(y, w1), b1, true);
     node->keep({kx.codes_, kx.side, kh.codes_, kh.side, g, b, w1, w2});
@@ -784,7 +785,7 @@ struct LinearXent : TrainNode {
 Tensor linear_xent(const Tensor &x, const Tensor &w, const OptTensor &bias, const Tensor &target, int64_t ignore, double smoothing, int64_t reduction) {
     if (!trains(x, w, bias)) return xent_forward(x, w, bias, target, ignore, smoothing, reduction, false).loss;
     const auto node = make_node<LinearXent>(x, w, bias);
-    const at::AutoGradMode off(false);
+    const at::AutoDispatchBelowADInplaceOrView off;
     XentOut o = xent_forward(x, w, bias, target, ignore, smoothing, reduction, true);
     node->keep({x, w, bias ? *bias : Tensor(), target, o.kept});
     node->ignore = ignore; node->reduction = reduction; node->smoothing = smoothing;

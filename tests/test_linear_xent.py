@@ -190,6 +190,40 @@ def test_parts_of_the_gradient_of_few_classes():
 
 
 @gpu
+def test_extreme_rows_of_few_classes():
+    """Masked classes, targets among them, rows that are not finite with and without a loss: each row alone is affected."""
+    N, D, V = 80003, 96, 150
+    x, w, b, t = make(N, D, V, "bf16", bias=None, ignored=0.1)
+    b = torch.zeros(V, device="cuda")
+    b[140:145], b[145:] = -float("inf"), torch.finfo(torch.float32).min
+    t[t >= 140] = 3
+    t[7], t[8], t[9], t[10] = 141, 2, -100, -100
+    x[8] = float("nan")
+    x[9] = float("inf")
+    x[10, 5] = float("nan")
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    rows = ops.linear_cross_entropy(x, w, t, b, reduction="none")
+    dx, _, db = torch.autograd.grad(rows, leaves, torch.ones_like(rows))
+    odd = torch.zeros(N, dtype=torch.bool, device="cuda")
+    odd[7:11] = True
+    assert rows[7] == float("inf") and rows[8].isnan() and rows[9] == 0 and rows[10] == 0
+    assert dx[8].isnan().all() and not dx[9:11].any() and dx[7].isfinite().all() and rows[~odd].isfinite().all()
+    l = x.detach()[~odd].double() @ w.detach()[:140].double().t()
+    tt = t[~odd]
+    kept = tt != -100
+    p = torch.softmax(l, 1)
+    p[torch.arange(len(tt), device="cuda"), tt.clamp_min(0)] -= 1
+    p[~kept] = 0
+    ref = p @ w.detach()[:140].double()
+    assert float((dx[~odd].double() - ref).norm()) <= 2.0 ** -8 * float(ref.norm())
+    with torch.no_grad():
+        x[8], x[9], x[10] = 0, 0, 0
+    rows = ops.linear_cross_entropy(x, w, t, b, reduction="none")
+    again, db = torch.autograd.grad(rows, (leaves[0], leaves[2]), torch.ones_like(rows))
+    assert torch.equal(again[~odd], dx[~odd]) and not db[145:].any() and not db[142:145].any() and db[141] == -1
+
+
+@gpu
 def test_gradients_against_differences():
     """The fp32 gradient against central differences of the float64 loss along random directions."""
     x, w, b, t = make(70, 48, 90, "fp32", ignored=0.2)

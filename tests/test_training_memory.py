@@ -136,6 +136,48 @@ def test_under_autocast():
 
 
 @gpu
+def test_nodes_of_the_graph():
+    """What autograd does with any node: outputs changed in place, graphs kept and used up, inputs changed behind its back, saved
+    tensors through hooks, hooks on inputs, no forward-mode derivative."""
+    leaves = mlp_args(6, 32, 64, "fp32")
+    x, g, b, w1, b1 = leaves[:5]
+    t = torch.tensor([0, 5, 63, 1, 2, 3], device="cuda")
+    calls = {"mlp": (lambda: ops.mlp_keep8(x.unsqueeze(0), *leaves[1:])[0], leaves),
+             "gelu": (lambda: ops.gelu_keep8(x), [x]),
+             "ln": (lambda: ops.layer_norm_keep8(x, g, b), [x, g, b]),
+             "ce": (lambda: ops.linear_cross_entropy(x, w1, t, b1, reduction="none"), [x, w1, b1])}
+    for name, (f, ins) in calls.items():
+        y = f()
+        up = torch.rand_like(y)
+        want = torch.autograd.grad(y, ins, up, retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(y, ins, up)))
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, ins, up)
+        y = f()
+        y.add_(1).mul_(2)                                                      # before the backward pass
+        assert all(torch.equal(2 * p, q) or torch.allclose(2 * p, q, rtol=1e-5, atol=1e-6) for p, q in zip(want, torch.autograd.grad(y, ins, up)))
+        packed = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: packed.append(v.shape) or v.cpu(), lambda v: v.cuda()):
+            y = f()
+        assert packed and all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(y, ins, up)))
+        seen = []
+        handle = ins[0].register_hook(lambda v: seen.append(v.shape))
+        f().backward(up)
+        handle.remove()
+        assert seen == [ins[0].shape] and torch.equal(ins[0].grad, want[0])
+        for v in ins:
+            v.grad = None
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+            ops.gelu_keep8(dual)
+    y = ops.linear_cross_entropy(x, w1, t, b1)
+    with torch.no_grad():
+        w1.mul_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+
+
+@gpu
 def test_no_rows_and_inference_mode():
     leaves = mlp_args(3, 32, 64, "fp32")
     empty = leaves[0].detach()[:0].requires_grad_(True)

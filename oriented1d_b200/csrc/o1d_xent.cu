@@ -12,8 +12,9 @@ namespace {
 
 // Bytes of G that are held at once.  Larger pieces have fewer waves that end half empty and fewer rounds of adding to fp32
 // sums, which is worth more than finding a piece in the L2 cache; 4096 x 1024 x 21841 bf16, gradient alone: 40 MB 557 us,
-// 80 MB 512, 128 MB 489, all 179 MB in one piece 452.
-constexpr long long kPieceBytes = 128ll << 20;
+// 80 MB 512, 128 MB 489, all 179 MB in one piece 452 (the step 694 -> 673; 2500 x 384 x 10007 fp32, 150 MB, 507 -> 497).  A
+// thousandth of the device's memory.
+constexpr long long kPieceBytes = 192ll << 20;
 constexpr int kMinSplitSteps = 16;               // K steps that a part of a split axis has at least (joining parts costs a launch)
 constexpr int kSlicesAtOnce = 512;               // column sums of more slices are added in two steps
 

@@ -140,6 +140,8 @@ def test_options(smoothing, bias, reduction, dtype):
     (4101, 997, 17001, "bf16", "none"),
     (2500, 1100, 9001, "fp32", "sum"),        # the same in fp32
     (14001, 1002, 5000, "bf16", "sum"),       # and of the rows
+    (2100, 64, 50001, "bf16", "mean"), (1500, 72, 24001, "fp32", "none"), (110001, 32, 1000, "bf16", "none"), (50003, 24, 700, "fp32", "mean"),
+    (4100, 1000, 28001, "bf16", "mean"), (4101, 997, 28001, "bf16", "none"), (2500, 1100, 14001, "fp32", "sum"), (21001, 1002, 5000, "bf16", "sum"),
 ])
 def test_pieces_and_parts(N, D, V, dtype, reduction):
     check(N, D, V, dtype, reduction=reduction, smoothing=0.1, ignored=0.1)

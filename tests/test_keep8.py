@@ -4,6 +4,7 @@ References are float64.  The codes of a checkpoint follow from fp32 operations b
 steps in numpy float32 and the codes have to be equal, one by one.  Tolerances: an fp32 result may be off by the fp32
 operations of its formula (about ten roundings of 2^-24 at the size of its terms: 2e-6 of the largest), a bf16 one by half
 a unit of its last place (2^-8 relative) on top."""
+import gc
 import math
 
 import numpy as np
@@ -15,6 +16,13 @@ import oriented1d_b200 as o1d
 ops = o1d.ops
 gpu = pytest.mark.gpu
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def leave_no_garbage():
+    """Tensors in reference cycles (an exception's frames) are freed here, not in the middle of a test that counts bytes."""
+    yield
+    gc.collect()
 
 
 def ref_codes(x):

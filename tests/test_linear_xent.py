@@ -6,6 +6,8 @@ Tolerances, element by element, from the arithmetic (u = 2^-24):
   softmax and loss add the errors of exp2 and log2 (2^-22 each, absolute in the exponent) and two roundings of the logits;
   the gradient of the logits is off by that, relatively, and for bf16 by its rounding to bf16 (2^-8);
   dx, dw and db add the same bound for their own sums, and their rounding to bf16 (2^-8) where they are bf16."""
+import gc
+
 import pytest
 import torch
 
@@ -15,6 +17,13 @@ ops = o1d.ops
 gpu = pytest.mark.gpu
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
 U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module", autouse=True)
+def leave_no_garbage():
+    """Tensors in reference cycles (an exception's frames) are freed here, not in the middle of a test that counts bytes."""
+    yield
+    gc.collect()
 
 
 def make(N, D, V, dtype, bias="same", seed=0, ignored=0.0, ignore_index=-100, logit=2.0):

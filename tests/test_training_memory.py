@@ -1,4 +1,6 @@
 """The training step that keeps little: blocks with 8-bit checkpoints, the head's loss without logits, all together."""
+import gc
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -9,6 +11,13 @@ from oriented1d_b200 import backbone, convnext1d
 ops = o1d.ops
 gpu = pytest.mark.gpu
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def leave_no_garbage():
+    """Tensors in reference cycles (an exception's frames) are freed here, not in the middle of a test that counts bytes."""
+    yield
+    gc.collect()
 
 
 def mlp_args(rows, C, hidden, dtype, seed=0):

@@ -173,6 +173,22 @@ __device__ __forceinline__ void xent_transpose(char *stage, int lane, const uint
 template <typename F>
 __device__ __forceinline__ void xent_transpose(char *stage, int lane, const uint4 (&vals)[4], F &&store) { xent_transpose(stage, lane, vals, store, [] {}); }
 
+// The same where rows start anywhere: lanes go along a row, an element each, so that its stores meet in as few sectors as they can
+// (eight elements of four lanes a row each: dx of 84547 x 785 bf16 362 us, so 89).  F(row, column, value).
+template <typename T, typename F>
+__device__ __forceinline__ void xent_transpose_any(char *stage, int lane, const uint4 (&vals)[4], F &&store) {
+    constexpr int W = 64 / (int)sizeof(T), V = 16 / (int)sizeof(T);      // columns; of a piece
+#pragma unroll
+    for (int j = 0; j < 4; j++) *reinterpret_cast<uint4 *>(xent_staged(stage, lane, j)) = vals[j];
+    __syncwarp();
+#pragma unroll 8
+    for (int i = 0; i < W; i++) {
+        const int row = i * (32 / W) + lane / W, col = lane % W;
+        store(row, col, reinterpret_cast<const T *>(xent_staged(stage, row, col / V))[col % V]);
+    }
+    __syncwarp();
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -280,14 +296,21 @@ __device__ __forceinline__ void xent_gradient(float (&a)[32], int c0, const Xent
 }
 // Of 32 columns from c0 on, which one is the target; or -1.
 __device__ __forceinline__ int xent_at(const XentRow &r, int c0) { const long long off = r.tgt - c0; return off >= 0 && off < 32 ? (int)off : -1; }
-// Eight values of a row of `n`, from column c on.
-__device__ __forceinline__ void xent_store8(__nv_bfloat16 *row, int c, int n, int vec, uint4 val) {
-    if (c >= n) return;
-    if (vec && c + 8 <= n) { *reinterpret_cast<uint4 *>(row + c) = val; return; }
-    const uint32_t x[4] = {val.x, val.y, val.z, val.w};
+// 32 columns of a bf16 result of rows of `n` from a lane's row of values, for the warp's 32 rows from r0 on.  vec: rows start on vectors.
+__device__ __forceinline__ void xent_store(__nv_bfloat16 *to, char *stage, int lane, const float (&a)[32], float alpha, int r0, int rows, int c0, int n, int vec) {
+    uint4 out[4];
+    uint32_t *o = reinterpret_cast<uint32_t *>(out);
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (c + i < n) row[c + i] = __ushort_as_bfloat16((unsigned short)(x[i >> 1] >> (16 * (i & 1))));
+    for (int i = 0; i < 16; i++) o[i] = pack_bf16(alpha * a[2 * i], alpha * a[2 * i + 1]);
+    if (vec)
+        xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
+            const int c = c0 + piece * 8;
+            if (r0 + r < rows && c < n) *reinterpret_cast<uint4 *>(to + (long long)(r0 + r) * n + c) = val;
+        });
+    else
+        xent_transpose_any<__nv_bfloat16>(stage, lane, out, [&](int r, int c, __nv_bfloat16 val) {
+            if (r0 + r < rows && c0 + c < n) to[(long long)(r0 + r) * n + c0 + c] = val;
+        });
 }
 
 template <int KIND, int MODE, int BN, bool PAIR>
@@ -641,14 +664,7 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     }
                 } else {
                     if (p.out_kind == 0) {
-                        uint4 out[4];
-                        uint32_t *o = reinterpret_cast<uint32_t *>(out);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = pack_bf16(alpha * a[2 * i], alpha * a[2 * i + 1]);
-                        __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(p.out);
-                        xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
-                            if (r0 + r < p.M) xent_store8(to + (long long)(r0 + r) * p.N, c0 + piece * 8, p.N, p.vec, val);
-                        });
+                        xent_store(static_cast<__nv_bfloat16 *>(p.out), stage, lane, a, alpha, r0, p.M, c0, p.N, p.vec);
                     } else {
                         float *to = static_cast<float *>(p.out) + (p.out_kind == 2 || p.out_kind == 3 ? w.split * p.split_elems : 0);
                         const float *before = p.out_kind >= 4 ? p.before : to;
@@ -658,32 +674,31 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                             float *o = reinterpret_cast<float *>(out);
 #pragma unroll
                             for (int i = 0; i < 16; i++) o[i] = p.out_kind == 1 ? alpha * a[h * 16 + i] : a[h * 16 + i];
+                            const float f = p.out_kind >= 4 ? alpha : 1.f;      // (of what is the result of a sum; kind 1 has it already)
+                            if (!p.vec) {
+                                xent_transpose_any<float>(stage, lane, out, [&](int r, int col, float x) {
+                                    const int c = c0 + h * 16 + col;
+                                    if (r0 + r >= p.M || c >= p.N) return;
+                                    const long long at = (long long)(r0 + r) * p.N + c;
+                                    if (p.out_kind >= 3) x += before[at];
+                                    if (p.out_kind == 4) static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(f * x);
+                                    else to[at] = f * x;
+                                });
+                                continue;
+                            }
                             xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
                                 const int c = c0 + h * 16 + piece * 4;
                                 if (r0 + r >= p.M || c >= p.N) return;
                                 const long long at = (long long)(r0 + r) * p.N + c;
                                 float x[4] = {__uint_as_float(val.x), __uint_as_float(val.y), __uint_as_float(val.z), __uint_as_float(val.w)};
-                                if (p.vec && c + 4 <= p.N) {
-                                    if (p.out_kind >= 3) {
-                                        const float4 old = *reinterpret_cast<const float4 *>(before + at);
-                                        x[0] += old.x; x[1] += old.y; x[2] += old.z; x[3] += old.w;
-                                    }
-                                    if (p.out_kind == 4) {
-                                        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + at) =
-                                            make_uint2(pack_bf16(alpha * x[0], alpha * x[1]), pack_bf16(alpha * x[2], alpha * x[3]));
-                                        return;
-                                    }
-                                    const float f = p.out_kind == 5 ? alpha : 1.f;
-                                    *reinterpret_cast<float4 *>(to + at) = make_float4(f * x[0], f * x[1], f * x[2], f * x[3]);
-                                    return;
+                                if (p.out_kind >= 3) {
+                                    const float4 old = *reinterpret_cast<const float4 *>(before + at);
+                                    x[0] += old.x; x[1] += old.y; x[2] += old.z; x[3] += old.w;
                                 }
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    if (c + i >= p.N) continue;
-                                    if (p.out_kind >= 3) x[i] += before[at + i];
-                                    if (p.out_kind == 4) static_cast<__nv_bfloat16 *>(p.out)[at + i] = __float2bfloat16_rn(alpha * x[i]);
-                                    else to[at + i] = p.out_kind == 5 ? alpha * x[i] : x[i];
-                                }
+                                if (p.out_kind == 4)
+                                    *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + at) =
+                                        make_uint2(pack_bf16(f * x[0], f * x[1]), pack_bf16(f * x[2], f * x[3]));
+                                else *reinterpret_cast<float4 *>(to + at) = make_float4(f * x[0], f * x[1], f * x[2], f * x[3]);
                             });
                         }
                     }
@@ -699,8 +714,8 @@ xent_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // One matrix as the bf16 planes that tensor copies read: fp32 cut into three, bf16 whose rows do not start on 16 bytes
-// copied.  planes: [3 or 1][rows][ld], ld a multiple of 8 (what lies past D is never read).  A warp a row; `vec`: four
-// values a lane, where the rows of x start on a vector.
+// copied.  planes: [3 or 1][rows][ld], ld a multiple of 8 (what lies past D is never read).  A warp a row; a lane writes a vector of a
+// plane, from one load where the rows of x start on vectors (`vec`), else from an element each.
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_planes_kernel(const T *__restrict__ x, __nv_bfloat16 *__restrict__ planes, long long rows, int D, int ld, int vec) {
@@ -710,29 +725,31 @@ xent_planes_kernel(const T *__restrict__ x, __nv_bfloat16 *__restrict__ planes, 
         const T *from = x + r * D;
         __nv_bfloat16 *to = planes + r * ld;
         if constexpr (sizeof(T) == 4) {
-            if (vec) {
 #pragma unroll 2
-                for (int c = lane * 4; c < D; c += 128) {
+            for (int c = lane * 4; c < D; c += 128) {
+                float v[4];
+                if (vec) {
                     const float4 q = __ldg(reinterpret_cast<const float4 *>(from + c));
-                    float v[4] = {q.x, q.y, q.z, q.w};
+                    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+                } else {
 #pragma unroll
-                    for (int pl = 0; pl < 3; pl++) {
-                        uint32_t b[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) b[i] = __float_as_uint(take_bf16(v[i]));              // exact: eight bits each
-                        *reinterpret_cast<uint2 *>(to + pl * plane + c) = make_uint2(b[0] >> 16 | (b[1] & 0xffff0000u), b[2] >> 16 | (b[3] & 0xffff0000u));
-                    }
+                    for (int i = 0; i < 4; i++) v[i] = c + i < D ? __ldg(from + c + i) : 0.f;
                 }
-                continue;
-            }
-        }
-        for (int c = lane; c < D; c += 32) {
-            if constexpr (sizeof(T) == 2) {
-                to[c] = from[c];
-            } else {
-                float v = from[c];
 #pragma unroll
-                for (int pl = 0; pl < 3; pl++) to[pl * plane + c] = __float2bfloat16_rn(take_bf16(v));
+                for (int pl = 0; pl < 3; pl++) {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) b[i] = __float_as_uint(take_bf16(v[i]));                  // exact: eight bits each
+                    *reinterpret_cast<uint2 *>(to + pl * plane + c) = make_uint2(b[0] >> 16 | (b[1] & 0xffff0000u), b[2] >> 16 | (b[3] & 0xffff0000u));
+                }
+            }
+        } else {
+            for (int c = lane * 8; c < D; c += 256) {
+                uint32_t v[8];
+                const unsigned short *p = reinterpret_cast<const unsigned short *>(from) + c;
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = c + i < D ? __ldg(p + i) : 0;
+                *reinterpret_cast<uint4 *>(to + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
             }
         }
     }

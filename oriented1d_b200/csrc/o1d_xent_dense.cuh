@@ -159,13 +159,7 @@ xent_dense_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 float a[32];
                 load(kDenseTX + pc * 32, a);
                 if (pc + 4 >= x_pieces) release(taken);
-                uint4 out[4];
-                uint32_t *o = reinterpret_cast<uint32_t *>(out);
-#pragma unroll
-                for (int k = 0; k < 16; k++) o[k] = pack_bf16(alpha * a[2 * k], alpha * a[2 * k + 1]);
-                xent_transpose(stage, lane, out, [&](int r, int piece, uint4 val) {
-                    if (r0 + r < p.M) xent_store8(dx + (long long)(r0 + r) * D, pc * 32 + piece * 8, D, p.vec, val);
-                });
+                xent_store(dx, stage, lane, a, alpha, r0, p.M, pc * 32, D, p.vec);
             }
         };
         // (fetched while the tile before is worked on)

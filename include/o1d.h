@@ -252,8 +252,8 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y,
  * x [N, D] and w [V, D] of type `dtype`, each starting on 16 bytes, bias [V] (or NULL) fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16; target [N].
  * A row whose target is ignore_index has no loss and no gradient; one whose target is outside [0, V) has a NaN loss
  * (and a NaN gradient).  reduction: O1D_XENT_NONE (loss [N]), _SUM, _MEAN (over the rows not ignored; loss [1]).
- * lse [3, N] (the log-sum-exp of a row, base 2, in two floats, and log2 of the target's probability) and count [1] (not written for _NONE) are for the backward
- * call; lse NULL: none will follow, which lets a few rows take a shorter way.
+ * lse [3, N] (the log-sum-exp of a row, base 2, in two floats, and log2 of the target's probability) and count [1] (not
+ * written for _NONE) are for the backward call; lse NULL: none will follow, which lets a few rows take a shorter way.
  * Sums, softmax statistics and the loss are fp32 or wider; fp32 products are exact to fp32 rounding (three bf16 planes
  * an operand on the tensor cores).  workspace: uninitialised, o1d_linear_xent_workspace_bytes() bytes, 256-byte aligned
  * (pass: O1D_XENT_FORWARD, _BACKWARD, or _EVALUATION for a forward call without lse). */
@@ -264,8 +264,8 @@ int o1d_linear_xent(const void *x, const void *w, const void *bias, const long l
                     void *workspace, size_t workspace_bytes, long long N, int D, int V, long long ignore_index,
                     float label_smoothing, int reduction, int dtype, void *stream);
 /* Its backward pass; dloss is the gradient of `loss` (fp32, [N] or [1]).  dx, dw (type `dtype`) and db (the bias's type)
- * may each be NULL.  The softmax is formed again in pieces of the vocabulary (or of the rows, where those are more) that
- * fit the cache; sums over pieces are fp32 and in a fixed order (bit-reproducible, no atomics).  For bf16 the gradient of
+ * may each be NULL.  The softmax is formed again, in pieces of the vocabulary (or of the rows, where those are more) of up
+ * to 192 MB of its gradient; sums over pieces are fp32 and in a fixed order (bit-reproducible, no atomics).  For bf16 the gradient of
  * the logits is rounded to bf16 (to 16 bits up to 2^30 products) before the two products that read it. */
 int o1d_linear_xent_bwd(const void *x, const void *w, const void *bias, const long long *target, const float *lse,
                         const float *count, const float *dloss, void *dx, void *dw, void *db, void *workspace,

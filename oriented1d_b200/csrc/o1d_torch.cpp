@@ -423,6 +423,8 @@ struct TrainNode : torch::autograd::Node {
         if (!grads[0].defined()) return out;
         // these differentiate once; a graph of their backward pass would silently leave them out
         if (at::GradMode::is_enabled()) throw std::runtime_error(name() + " has no second derivative (create_graph=True)");
+        // (the engine brings along the autocast state of the thread that called it: a product would round its operands to that type)
+        const c10::impl::ExcludeDispatchKeyGuard as_given(c10::autocast_dispatch_keyset);
         backward(grads[0], out);
         return out;
     }

@@ -145,6 +145,26 @@ def test_under_autocast():
 
 
 @gpu
+@pytest.mark.parametrize("region", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_a_backward_pass_inside_autocast(dtype, region):
+    """A region around the backward pass (or around both) changes nothing: the products' type is that of x."""
+    leaves = mlp_args(64, 32, 128, dtype)
+    x, g, b, w1, b1 = leaves[:5]
+    dz = torch.randn(64, 32, device="cuda").to(DT[dtype])
+    t = torch.arange(64, device="cuda")
+    calls = [(lambda: ops.mlp_keep8(*leaves), leaves, dz), (lambda: ops.gelu_keep8(x, b), [x, b], dz), (lambda: ops.layer_norm_keep8(x, g, b), [x, g, b], dz),
+             (lambda: ops.linear_cross_entropy(x, w1, t, b1), [x, w1, b1], torch.ones((), device="cuda"))]
+    for f, ins, up in calls:
+        want = torch.autograd.grad(f(), ins, up)
+        y = f()
+        with torch.autocast("cuda", region):
+            got = torch.autograd.grad(y, ins, up)
+            both = torch.autograd.grad(f(), ins, up)
+        assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, got, both))
+
+
+@gpu
 def test_nodes_of_the_graph():
     """What autograd does with any node: outputs changed in place, graphs kept and used up, inputs changed behind its back, saved
     tensors through hooks, hooks on inputs, no forward-mode derivative."""

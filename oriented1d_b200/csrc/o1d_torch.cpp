@@ -5,6 +5,7 @@
 // Parameters (weights, biases, LayerNorm scales) are passed as they are stored when the kernels take bf16
 // ones (O1D_FLAG_PARAMS_BF16); otherwise, or when the library has no such kernel for the request, they are
 // converted to fp32 first.
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -373,7 +374,15 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         return out;
     }
 };
-Tensor linear_train(const Tensor &x, const Tensor &w, const Tensor &b) { return LinearFn::apply(x, w, b); }
+Tensor linear_train(const Tensor &x, const Tensor &w, const Tensor &b) {
+    // An autocast region that converts an operand: the saved tensors would not be those of the product.  torch's own operator then,
+    // whose graph has the conversions in it.
+    if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+        const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+        if (x.scalar_type() != type || w.scalar_type() != type || b.scalar_type() != type) return at::linear(x, w, b);
+    }
+    return LinearFn::apply(x, w, b);
+}
 
 // ---- 8-bit activation checkpoints --------------------------------------------------------------------
 // Outputs and workspaces straight from the allocator, without the dispatcher (1.8 us a tensor, up to eight a call).

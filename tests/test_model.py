@@ -178,3 +178,50 @@ def test_model_training_step_gradients(variant):
         assert err < 5e-4, (k, err)
     err = float((got_img - img.grad.double()).abs().max() / img.grad.abs().max())
     assert err < 5e-4, err
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("region", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("xtype,wtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("inside", [False, True])
+def test_linear_under_autocast(xtype, wtype, region, inside):
+    """linear_cl in an autocast region is nn.Linear there, wherever its backward pass runs.  (Of the same type all round: its own node,
+    whose bias gradient is rounded once from an fp32 sum in another order, 2^-8 of it either way.)"""
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(64, 128).cuda().to(wtype)
+    x = torch.randn(300, 64, device="cuda", dtype=xtype, requires_grad=True)
+    dy = torch.randn(300, 128, device="cuda")
+    outs = []
+    for f in (lambda: o1d.ops.linear_cl(lin, x), lambda: lin(x)):
+        with torch.autocast("cuda", region):
+            y = f()
+            if inside:
+                g = torch.autograd.grad(y, (x, lin.weight, lin.bias), dy.to(y.dtype))
+        if not inside:
+            g = torch.autograd.grad(y, (x, lin.weight, lin.bias), dy.to(y.dtype))
+        outs.append((y.detach(), *g))
+    for a, b in zip(*outs):
+        assert a.dtype == b.dtype and a.shape == b.shape
+        assert float((a - b).float().norm()) <= 2.0 ** -7 * float(b.float().norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", ["1d", "1dpp", "2d"])
+def test_a_training_step_under_autocast(variant):
+    """fp32 parameters, products in bf16, the backward pass outside the region as torch advises: the loss and the gradients of the fp32
+    step, to a few roundings to bf16 a layer (2^-8 each, some twenty layers deep: 0.1 norm-wise)."""
+    torch.manual_seed(3)
+    m = convnext1d.ConvNeXt1D(depths=(1, 1, 2, 1), dims=(32, 64, 96, 128), variant=variant, stem_dim1=16, layer_scale_init_value=0.5, num_classes=37)
+    for p in m.parameters():
+        if p.dim() > 1:
+            torch.nn.init.normal_(p, std=0.1)
+    m = m.cuda().train()
+    img = torch.randn(8, 3, 64, 64, generator=torch.Generator().manual_seed(0)).cuda()
+    t = torch.arange(8, device="cuda")
+    params = {k: p for k, p in m.named_parameters() if not k.endswith("theta")}
+    want = torch.autograd.grad(F.cross_entropy(m(img), t), list(params.values()))
+    with torch.autocast("cuda", torch.bfloat16):
+        loss = F.cross_entropy(m(img).float(), t)
+    got = torch.autograd.grad(loss, list(params.values()))
+    a, b = (torch.cat([g.reshape(-1) for g in gs]) for gs in (got, want))
+    assert float((a - b).norm()) <= 0.1 * float(b.norm())

@@ -130,8 +130,10 @@ class Block1D(nn.Module):
         return F.gelu(h) if gelu else h
 
     def _mlp(self, x):
-        if self.keep8 and x.is_cuda and torch.is_grad_enabled():
-            return ops.mlp_keep8(x, self.norm.weight, self.norm.bias, self.pwconv1.weight, self.pwconv1.bias, self.pwconv2.weight,
+        # under autocast the products run in the region's type, as those of the separate layers do
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        if self.keep8 and x.is_cuda and torch.is_grad_enabled() and dtype in (torch.float32, torch.bfloat16):
+            return ops.mlp_keep8(x.to(dtype), self.norm.weight, self.norm.bias, self.pwconv1.weight, self.pwconv1.bias, self.pwconv2.weight,
                                  self.pwconv2.bias, self.norm.eps)
         return ops.linear_cl(self.pwconv2, self._mlp_in(x))
 

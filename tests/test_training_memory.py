@@ -146,6 +146,29 @@ def test_under_autocast():
 
 @gpu
 @pytest.mark.parametrize("region", [torch.bfloat16, torch.float16])
+def test_blocks_under_autocast_run_their_products_in_its_type(region):
+    """The MLP of a block with checkpoints against the separate layers in the same region, fp32 parameters and input.  Four roundings
+    to the type in a row on either side (the input's, the normalised one's, the hidden tensor's, the result's), 2^-8 of each at most; a
+    region of a type without checkpoints (float16) is served by the separate layers."""
+    torch.manual_seed(0)
+    block = convnext1d.Block1D(64).cuda().train()
+    x = torch.randn(2, 20, 20, 64, device="cuda", requires_grad=True)
+    outs = []
+    for block.keep8 in (False, True):
+        with torch.autocast("cuda", region):
+            y = block._mlp(x)
+        params = [*block.norm.parameters(), *block.pwconv1.parameters(), *block.pwconv2.parameters()]
+        outs.append((y.detach(), *torch.autograd.grad(y, [x, *params], torch.ones_like(y) / 8)))
+    assert all(a.dtype == b.dtype and a.shape == b.shape for a, b in zip(*outs)) and outs[1][0].dtype == region
+    if region == torch.float16:
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert float((outs[0][0] - outs[1][0]).float().norm()) <= 8 * 2.0 ** -8 * float(outs[0][0].float().norm())
+    for a, b in zip(outs[0][1:], outs[1][1:]):                                 # 8-bit codes of normal data on top: 0.007 r.m.s.
+        assert float((a - b).float().norm()) <= 0.05 * float(a.float().norm())
+
+
+@gpu
+@pytest.mark.parametrize("region", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_a_backward_pass_inside_autocast(dtype, region):
     """A region around the backward pass (or around both) changes nothing: the products' type is that of x."""

@@ -305,7 +305,11 @@ class ConvNeXt1D(nn.Module):
             outs.append(x.permute(0, 3, 1, 2))
         return outs if all_stages else outs[-1]
 
-    def forward(self, x):
+    def forward(self, x, target=None, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
+        """Logits of the images x; with target, loss() of them.  A wrapper that does its work around forward has to be called for
+        the loss, too: ddp(x, target), since ddp.module.loss(x, target) would leave the gradients of each rank to itself."""
+        if target is not None:
+            return self.loss(x, target, label_smoothing, ignore_index, reduction)
         x = self.forward_features(x)
         return self.head(self.norm(x.mean([-2, -1])))
 

@@ -59,3 +59,58 @@ def test_batch_sharding_and_gradient_allreduce(tmp_path):
         assert np.array_equal(r["y"], y[lo:hi]) and np.array_equal(r["dx"], dx[lo:hi])   # no exchange needed
         err = np.abs(r["flat"] - ref_flat).max() / np.abs(ref_flat).max()
         assert err <= 1e-4, err                                                           # sum over ranks
+
+
+class _Classifier:
+    """A ConvNeXt1D whose features come from one library conv and whose head's loss is torch's, so that it runs on a CPU rank."""
+
+    def __new__(cls):
+        from oriented1d_b200 import convnext1d
+
+        class Model(convnext1d.ConvNeXt1D):
+            def forward_features(self, x, all_stages=False):
+                return self.features(x)
+
+        torch.manual_seed(0)
+        m = Model(depths=(1, 1, 1, 1), dims=(8, 8, 8, 8), num_classes=5, stem_dim1=8)
+        del m.downsample_layers, m.stages
+        m.features = torch.nn.Conv2d(3, 8, 4, stride=4)
+        convnext1d.ops.linear_cross_entropy = lambda x, w, t, b, **kw: torch.nn.functional.cross_entropy(x @ w.t() + b, t, **kw)
+        return m
+
+
+def _batch():
+    g = torch.Generator().manual_seed(1)
+    return torch.randn(6, 3, 16, 16, generator=g), torch.tensor([0, 1, 2, 3, 4, 0])
+
+
+def _loss_worker(rank, world, port, out_dir):
+    sys.path.insert(0, ROOT)
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        img, t = _batch()
+        lo, hi = rank * 6 // world, (rank + 1) * 6 // world
+        m = _Classifier()
+        ddp = torch.nn.parallel.DistributedDataParallel(m)
+        loss = ddp(img[lo:hi], t[lo:hi], label_smoothing=0.1)
+        loss.backward()
+        torch.save({k: p.grad for k, p in m.named_parameters()}, os.path.join(out_dir, f"grads{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_the_loss_through_a_data_parallel_wrapper(tmp_path, monkeypatch):
+    """The gradients on every rank are those of the whole batch: the wrapper sees the loss as a forward pass."""
+    from oriented1d_b200 import ops
+    monkeypatch.setattr(ops, "linear_cross_entropy", ops.linear_cross_entropy)            # put back what _Classifier replaces
+    world, port = 2, 30111 + os.getpid() % 500
+    mp.start_processes(_loss_worker, args=(world, port, str(tmp_path)), nprocs=world, join=True, start_method="spawn")
+    m = _Classifier()
+    img, t = _batch()
+    m(img, t, label_smoothing=0.1).backward()
+    assert torch.equal(m(img, t, 0.1), m.loss(img, t, 0.1)) and m(img).shape == (6, 5)
+    for rank in range(world):
+        got = torch.load(os.path.join(str(tmp_path), f"grads{rank}.pt"))
+        for k, p in m.named_parameters():                                                  # (equal shards: the mean of means is the mean)
+            assert float((got[k] - p.grad).norm()) <= 1e-5 * float(p.grad.norm()) + 1e-8, k

@@ -132,7 +132,8 @@ class Block1D(nn.Module):
     def _mlp(self, x):
         # under autocast the products run in the region's type, as those of the separate layers do
         dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-        if self.keep8 and x.is_cuda and torch.is_grad_enabled() and dtype in (torch.float32, torch.bfloat16):
+        plain = ops.bare(self.norm, LayerNorm) and ops.bare(self.pwconv1, nn.Linear) and ops.bare(self.pwconv2, nn.Linear)
+        if self.keep8 and plain and x.is_cuda and torch.is_grad_enabled() and dtype in (torch.float32, torch.bfloat16):
             return ops.mlp_keep8(x.to(dtype), self.norm.weight, self.norm.bias, self.pwconv1.weight, self.pwconv1.bias, self.pwconv2.weight,
                                  self.pwconv2.bias, self.norm.eps)
         return ops.linear_cl(self.pwconv2, self._mlp_in(x))
@@ -314,8 +315,11 @@ class ConvNeXt1D(nn.Module):
         return self.head(self.norm(x.mean([-2, -1])))
 
     def loss(self, x, target, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
-        """F.cross_entropy(self(x).float(), target, ...) without the logits (ops.linear_cross_entropy); fp32."""
+        """F.cross_entropy(self(x).float(), target, ...) without the logits (ops.linear_cross_entropy); fp32.  With the logits where the
+        head is another module than a Linear, or has hooks."""
         x = self.norm(self.forward_features(x).mean([-2, -1]))
+        if not ops.bare(self.head, nn.Linear):
+            return F.cross_entropy(self.head(x).float(), target, ignore_index=ignore_index, label_smoothing=label_smoothing, reduction=reduction)
         return ops.linear_cross_entropy(x, self.head.weight, target, self.head.bias, ignore_index=ignore_index,
                                         label_smoothing=label_smoothing, reduction=reduction)
 

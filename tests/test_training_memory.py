@@ -4,6 +4,7 @@ import gc
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.nn.utils.prune
 
 import oriented1d_b200 as o1d
 from oriented1d_b200 import backbone, convnext1d
@@ -185,6 +186,46 @@ def test_a_backward_pass_inside_autocast(dtype, region):
             got = torch.autograd.grad(y, ins, up)
             both = torch.autograd.grad(f(), ins, up)
         assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, got, both))
+
+
+def test_the_loss_calls_a_head_that_is_more_than_a_linear():
+    """Hooks on the head run, a pruned head is pruned anew, and a head that is another module is that module (on the CPU: those take torch's
+    own operators)."""
+    m = convnext1d.ConvNeXt1D(depths=(1, 1, 1, 1), dims=(8, 8, 8, 8), num_classes=5, stem_dim1=8)
+    m.forward_features = lambda x: x
+    x, t = torch.randn(6, 8, 3, 3), torch.tensor([0, 1, -100, 4, 4, 2])
+    want = lambda: F.cross_entropy(m(x), t, label_smoothing=0.1)  # noqa: E731
+    seen = []
+    handle = m.head.register_forward_hook(lambda mod, i, o: seen.append(o.shape) or 2 * o)
+    assert torch.equal(m.loss(x, t, label_smoothing=0.1), want()) and seen == [(6, 5), (6, 5)]
+    handle.remove()
+    torch.nn.utils.prune.l1_unstructured(m.head, "weight", 0.5)
+    for _ in range(2):                                                         # its weight is a new tensor at every call
+        m.loss(x, t).backward()
+    assert torch.equal(m.loss(x, t, label_smoothing=0.1), want())
+    assert (m.head.weight_orig.grad[m.head.weight_mask == 0] == 0).all()
+    m.head = torch.nn.Sequential(torch.nn.Linear(8, 8), torch.nn.ReLU(), torch.nn.Linear(8, 5))
+    assert torch.equal(m.loss(x, t, label_smoothing=0.1), want())
+    m.head = torch.nn.Linear(8, 5)
+    with pytest.raises(RuntimeError, match="CUDA"):                            # the plain head: ops.linear_cross_entropy
+        m.loss(x, t)
+
+
+@gpu
+@pytest.mark.parametrize("keep8", [False, True])
+def test_hooks_on_the_layers_of_a_block(keep8):
+    block = convnext1d.Block1D(64).cuda().train()
+    block.keep8 = keep8
+    x = torch.randn(50, 64, device="cuda", requires_grad=True)
+    for name in ("norm", "pwconv1", "pwconv2"):
+        layer = getattr(block, name)
+        seen = []
+        handles = [layer.register_forward_pre_hook(lambda mod, i: seen.append("before")), layer.register_forward_hook(lambda mod, i, o: seen.append("after") or o * 0),
+                   layer.register_full_backward_hook(lambda mod, i, o: seen.append("back"))]
+        block._mlp(x).sum().backward()
+        assert seen == ["before", "after", "back"], name
+        for h in handles:
+            h.remove()
 
 
 @gpu

@@ -168,7 +168,17 @@ int planes_of(const XentArgs &a) { return !a.bf16 ? 3 : fine_of(a) ? 2 : 1; }
 
 // Few classes and narrow features: one kernel for all of the backward pass (o1d_xent_dense.cuh), with one plane of G.
 bool dense_of(const XentArgs &a) { return a.bf16 && !fine_of(a) && a.V <= kDenseV && a.D <= kDenseD; }
-int dense_ctas(const XentArgs &a, int sms) { return cdiv(a.N, kXM) < sms ? cdiv(a.N, kXM) : sms; }
+// Rows of one launch of it.  dw of a CTA's tiles is one sum in tensor memory, eight additions a tile, and a tensor core truncates as it
+// adds: measured, sums of one sign lose 1.6e-8 of themselves with every addition.  256 tiles are 2048 additions, 3e-5 (19.4 M rows in one
+// launch had 8192, 60 M 25000: 4e-4, a fifth of what a bf16 result is rounded by).  Each launch leaves sums of its own.
+constexpr int kDenseTiles = 256;
+long long dense_rows(int sms) { return (long long)kDenseTiles * sms * kXM; }
+int dense_ctas(long long rows, int sms) { return cdiv(rows, kXM) < sms ? cdiv(rows, kXM) : sms; }
+// Sums that all launches of a call leave: CTAs of each.
+int dense_sums(const XentArgs &a, int sms) {
+    const long long most = dense_rows(sms), rest = a.N % most;
+    return (int)(a.N / most) * sms + (rest ? dense_ctas(rest, sms) : 0);
+}
 
 bool few_rows(long long N, int D) { return N <= kFewRows && (N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8) * up_to(D, 8) * 4 <= kFewBytes; }
 int few_ctas(long long N, int V, int sms) {
@@ -348,39 +358,50 @@ cudaError_t finish(const float *sums, void *out, long long n, int slots, const f
 }
 int backward_dense(Run &r) {
     const XentArgs &a = r.a;
-    const int ctas = dense_ctas(a, r.sms);
+    const int sums = dense_sums(a, r.sms);
     unsigned char *ws = (unsigned char *)a.workspace;
-    float *dws = (float *)ws; ws += up_to(4ll * ctas * a.V * a.D, 256);
-    float *cols = (float *)ws; ws += up_to(4ll * ctas * kDenseV, 256);
+    float *dws = (float *)ws; ws += up_to(4ll * sums * a.V * a.D, 256);
+    float *cols = (float *)ws; ws += up_to(4ll * sums * kDenseV, 256);
     Mat x, w;
     int rc = make_operand(r, a.x, operand_of(a.N, a.D, true), &ws, &x);
     if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, true), &ws, &w);
     if (rc) return rc;
     CUtensorMap x_map, w_map;
-    if ((*r.enc = encode(&x_map, x, kXM)) || (*r.enc = encode(&w_map, w, (int)up_to(a.V, 32)))) return O1D_ERR_CUDA;
+    if ((*r.enc = encode(&w_map, w, (int)up_to(a.V, 32)))) return O1D_ERR_CUDA;
     const bool each = a.reduction == O1D_XENT_NONE;
     const float f = a.smoothing < 1.f ? 1.f - a.smoothing : 1.f;
     const float *up = each ? nullptr : a.dloss, *count = a.reduction == O1D_XENT_MEAN ? a.count : nullptr;
     XentParams p{};
-    p.M = (int)a.N; p.N = a.V; p.tiles = cdiv(a.N, kXM);
-    p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.target = a.target; p.ignore = a.ignore;
+    p.N = a.V;
+    p.bias = a.bias; p.bias_bf16 = a.bias_bf16; p.V = a.V; p.ignore = a.ignore;
     p.smooth = a.smoothing > 0.f;
-    p.lse = a.lse; p.lse_lo = a.lse + a.N; p.log2p = a.lse + 2 * a.N; p.up = each ? a.dloss : nullptr;
     p.factor_log2 = log2f(f); p.one = a.smoothing < 1.f ? 1.f : 0.f; p.eps_v = a.smoothing / (float)a.V / f;
-    p.cols = a.db ? cols : nullptr; p.cols_ld = kDenseV;
-    p.vec = ((uintptr_t)a.dx & 15) == 0 && a.D % 8 == 0;
+    p.cols_ld = kDenseV;
+    p.vec = ((uintptr_t)a.dx & 15) == 0 && a.D % 8 == 0;             // (a launch's rows start on a multiple of 128)
     p.alpha_up = up; p.alpha_count = count; p.alpha = f;
     p.err_flag = r.err_flag;
     static std::atomic<uint64_t> sized{0};
     cudaError_t e = size_once(sized, (const void *)xent_dense_kernel, kDenseSmem);
     if (e != cudaSuccess) return r.fail(e);
-    xent_dense_kernel<<<ctas, kXThreads, kDenseSmem, r.st>>>(x_map, w_map, p, a.D, (__nv_bfloat16 *)a.dx, a.dw ? dws : nullptr);
-    e = cudaGetLastError();
+    int at = 0;                                                       // sums that the launches so far leave
+    for (long long row0 = 0; e == cudaSuccess && row0 < a.N; row0 += dense_rows(r.sms)) {
+        const long long rows = a.N - row0 < dense_rows(r.sms) ? a.N - row0 : dense_rows(r.sms);
+        const int ctas = dense_ctas(rows, r.sms);
+        if ((*r.enc = encode(&x_map, sub_rows(x, row0, rows), kXM))) return O1D_ERR_CUDA;
+        p.M = (int)rows; p.tiles = cdiv(rows, kXM);
+        p.target = a.target + row0;
+        p.lse = a.lse + row0; p.lse_lo = a.lse + a.N + row0; p.log2p = a.lse + 2 * a.N + row0; p.up = each ? a.dloss + row0 : nullptr;
+        p.cols = a.db ? cols + (long long)at * kDenseV : nullptr;
+        xent_dense_kernel<<<ctas, kXThreads, kDenseSmem, r.st>>>(x_map, w_map, p, a.D, a.dx ? (__nv_bfloat16 *)a.dx + row0 * a.D : nullptr,
+                                                                 a.dw ? dws + (long long)at * a.V * a.D : nullptr);
+        e = cudaGetLastError();
+        at += ctas;
+    }
     const long long dw_n = a.dw ? (long long)a.V * a.D : 0;
     const int db_n = a.db ? a.V : 0;
     if (e == cudaSuccess && dw_n + db_n > 0) {
         xent_finish_kernel<__nv_bfloat16, 16><<<cdiv(dw_n, 32) + cdiv(db_n, 32), dim3(32, 16), 0, r.st>>>(
-            dws, (__nv_bfloat16 *)a.dw, dw_n, ctas, cols, a.db, db_n, kDenseV, ctas, a.bias_bf16, up, count, f);
+            dws, (__nv_bfloat16 *)a.dw, dw_n, sums, cols, a.db, db_n, kDenseV, sums, a.bias_bf16, up, count, f);
         e = cudaGetLastError();
     }
     return e == cudaSuccess ? O1D_OK : r.fail(e);
@@ -486,8 +507,8 @@ int backward(Run &r) {
 
 size_t xent_workspace(const XentArgs &a, bool back, int sms) {
     if (back && dense_of(a)) {
-        const int ctas = dense_ctas(a, sms);
-        return operand_of(a.N, a.D, true).bytes + operand_of(a.V, a.D, true).bytes + (size_t)(up_to(4ll * ctas * a.V * a.D, 256) + up_to(4ll * ctas * kDenseV, 256));
+        const int sums = dense_sums(a, sms);
+        return operand_of(a.N, a.D, true).bytes + operand_of(a.V, a.D, true).bytes + (size_t)(up_to(4ll * sums * a.V * a.D, 256) + up_to(4ll * sums * kDenseV, 256));
     }
     if (back) {
         const BackwardBytes b = backward_bytes(a, cut_of(a, sms));

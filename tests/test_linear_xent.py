@@ -201,6 +201,60 @@ def test_parts_of_the_gradient_of_few_classes():
 
 
 @gpu
+def test_sums_over_very_many_rows_do_not_drift():
+    """Few classes, 29 million rows: the upstream gradient of the first half is 1, of the second, the same rows, -1, so that the weight's
+    gradient is zero.  All weights are zero: G = 1/64 (and 1/64 - 1 of class 0) is exact in bf16, and what dw is off by is what the tensor
+    core's additions lose: half a unit (2^-24) of the sum so far, on average, for each of at most 2048 that one sum takes (its mean is half
+    of what its terms add up to)."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    half, D, V = 6 * 128 * sms * 128, 24, 64                                   # six launches' worth of rounds; every SM gets both halves
+    x = torch.rand(half, D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda", dtype=torch.bfloat16) + 0.25
+    x = torch.cat([x, x])
+    w = torch.zeros(V, D, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    b = torch.zeros(V, device="cuda", requires_grad=True)
+    t = torch.zeros(2 * half, dtype=torch.int64, device="cuda")
+    up = torch.ones(2 * half, device="cuda")
+    up[half:] = -1
+    dw, db = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, b, reduction="none"), (w, b), up)
+    terms = 2 * x[:half].double().sum(0) / V * torch.where(torch.arange(V, device="cuda") == 0, V - 1, 1)[:, None]
+    assert float((dw.double().abs() / terms).max()) <= 2048 * 2.0 ** -24 / 2
+    assert not db.any()                                                        # whole numbers of 1/64
+
+
+@gpu
+@pytest.mark.parametrize("extra", [0, 1, 128, 40001])
+def test_few_classes_in_several_launches(extra):
+    """Rows around the number that one launch takes (256 tiles of 128 an SM): each row's gradient is the one it has among few rows, and
+    the sums are those of float64."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    N, D, V = 256 * 128 * sms + extra, 9, 31
+    g = torch.Generator(device="cuda").manual_seed(extra)
+    x = torch.randn(N, D, device="cuda", generator=g).bfloat16().requires_grad_(True)
+    w = torch.randn(V, D, device="cuda", generator=g).bfloat16().requires_grad_(True)
+    b = torch.randn(V, device="cuda", generator=g).requires_grad_(True)
+    t = torch.randint(-1, V, (N,), device="cuda", generator=g)
+    up = torch.rand(N, device="cuda", generator=g)
+    f = lambda x, t, up: torch.autograd.grad(ops.linear_cross_entropy(x, w, t, b, ignore_index=-1, reduction="none"), (x, w, b), up)  # noqa: E731
+    dx, dw, db = f(x, t, up)
+    rdw, rdb, s_db = 0, 0, 0
+    with torch.no_grad():
+        for lo in range(0, N, 1 << 20):
+            xs, ts, us = x[lo:lo + (1 << 20)].double(), t[lo:lo + (1 << 20)], up[lo:lo + (1 << 20)].double()
+            G = torch.softmax(xs @ w.double().t() + b.double(), 1)
+            G[torch.arange(len(ts), device="cuda"), ts.clamp_min(0)] -= 1
+            G *= torch.where(ts == -1, 0, us)[:, None]
+            ref = G @ w.double()
+            # each element of G to half a unit of bf16, a few units of fp32 in its exponent, and the result's own rounding
+            assert ((dx[lo:lo + (1 << 20)].double() - ref).abs() <= 2.0 ** -8 * (G.abs() @ w.double().abs()) + 2.0 ** -8 * ref.abs() + 1e-6).all()
+            rdw, rdb, s_db = rdw + G.t() @ xs, rdb + G.sum(0), s_db + G.abs().sum(0)
+    # (labels are random: a class's sums are of its rows' own size, and the roundings of millions of rows' G cancel in them)
+    assert float((dw.double() - rdw).norm()) <= 2.0 ** -8 * float(rdw.norm())
+    assert ((db.double() - rdb).abs() <= 1e-5 * s_db).all()
+    tail = slice(N - 100_000, N)
+    assert torch.equal(f(x[tail].detach().repeat(40, 1).requires_grad_(True), t[tail].repeat(40), up[tail].repeat(40))[0][:100_000], dx[tail])
+
+
+@gpu
 def test_extreme_rows_of_few_classes():
     """Masked classes, targets among them, rows that are not finite with and without a loss: each row alone is affected."""
     N, D, V = 80003, 96, 150

@@ -38,28 +38,30 @@ __device__ __forceinline__ void lane_sums(float (&v)[U]) {
 // Exact GELU and its slope without erff, of which the passes below would be nothing else (20 instructions a value each).
 //   P(-|h|) = erfc(z)/2,  z = |h|/sqrt 2,  erfc(z) = t q(t) exp(-z^2),  t = 1/(1 + 0.33 z)
 // the form of Abramowitz and Stegun 7.1.26, with a polynomial q fitted to exp(z^2) erfc(z) on 0 <= z <= 10 by iterated weighted
-// least squares: of degree 7 for bf16 (relative error 1e-7, in the tail too), of degree 9 for fp32 (3e-9; an error of the fit is
-// alike for like values, and the bias gradient adds them up).  One reciprocal and one exponential, which the slope
-// needs anyway.
+// least squares: of degree 7 for bf16 (relative error 1e-7, in the tail too), of degree 9 for fp32 (5e-9, its mean 1e-9; an error of
+// the fit is alike for like values, and the bias gradient adds them up).  These are the errors of the numbers below: 0.33 / sqrt 2 was
+// rounded to fp32 before the fit, and the coefficients one after the other, the others fitted anew each time (all at once: 3.5e-8,
+// nearly all of one sign).  One reciprocal and one exponential, which the slope needs anyway.
 // For a pair of values: m = |h| (at most 64), q = -P(-|h|), bell = exp(-h^2/2).  Then GELU(h) = max(h, 0) + m q and
 // GELU'(h) = 1/2 + sign(h) (1/2 + q + m bell / sqrt(2 pi)).
 struct Normal { F2 m, q, bell; };
 template <bool FP32>
 __device__ __forceinline__ Normal normal_of(F2 h) {
     constexpr int N = FP32 ? 10 : 8;
+    constexpr float slope = 0.23334524035453796f;        // 0.33 / sqrt 2
     constexpr float fit[10] = {FP32 ? 0.1861456036567688f : 0.1863577961921692f,
-                               FP32 ? 0.1870007961988449f : 0.1829560101032257f,
-                               FP32 ? 0.16811791062355042f : 0.2012234777212143f,
-                               FP32 ? 0.1999620497226715f : 0.04722202196717262f,
-                               FP32 ? -0.029606999829411507f : 0.40849733352661133f,
-                               FP32 ? 0.45996400713920593f : -0.35114675760269165f,
-                               FP32 ? -0.5105049014091492f : 0.4602353572845459f,
-                               FP32 ? 0.5900521874427795f : -0.1353452503681183f,
-                               FP32 ? -0.3076556622982025f : 0.f,
-                               FP32 ? 0.05652497336268425f : 0.f};
+                               FP32 ? 0.18700088560581207f : 0.18295611441135406f,
+                               FP32 ? 0.16811716556549072f : 0.2012227475643158f,
+                               FP32 ? 0.1999654918909073f : 0.047224510461091995f,
+                               FP32 ? -0.02961677871644497f : 0.4084925055503845f,
+                               FP32 ? 0.45998188853263855f : -0.3511412739753723f,
+                               FP32 ? -0.5105260610580444f : 0.4602320194244385f,
+                               FP32 ? 0.5900679230690002f : -0.13534443080425262f,
+                               FP32 ? -0.30766230821609497f : 0.f,
+                               FP32 ? 0.05652618780732155f : 0.f};
     const float2 a = apart(h);
     const F2 m = two(fminf(fabsf(a.x), 64.f), fminf(fabsf(a.y), 64.f));      // (q is 0 there: an infinity times it would be NaN)
-    const float2 d = apart(fma2(m, both(0.33f * 0.70710678f), both(1.f))), z = apart(mul2(mul2(h, h), both(-0.72134752f)));
+    const float2 d = apart(fma2(m, both(slope), both(1.f))), z = apart(mul2(mul2(h, h), both(-0.72134752f)));
     float2 r, e;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));

@@ -6,6 +6,8 @@ operations of its formula (about ten roundings of 2^-24 at the size of its terms
 a unit of its last place (2^-8 relative) on top."""
 import gc
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -130,6 +132,21 @@ def _gelu_grad(h):
 def _kept(h32):
     rc, rr = ref_codes(h32.numpy())
     return torch.from_numpy(ref_values(rc, rr))
+
+
+def test_the_fit_of_gelu_is_as_good_as_it_says():
+    """The stored fp32 coefficients of t q(t), t = 1/(1 + slope m), against exp(z^2) erfc(z), z = m/sqrt 2, in float64: the relative errors
+    that the comment beside them states, at the centre, in the tail and on average."""
+    src = open(os.path.join(os.path.dirname(o1d.__file__), "csrc", "o1d_keep8.cuh")).read()
+    slope = float(re.search(r"constexpr float slope = ([\d.]+)f;", src).group(1))
+    table = re.findall(r"FP32 \? (-?[\d.]+)f : (-?[\d.]+)f", src[src.index("fit[10]"):src.index("fit[10]") + 1500])[:10]
+    assert len(table) == 10 and np.float32(slope) == slope
+    m = torch.linspace(0, 10 * math.sqrt(2), 40001, dtype=torch.float64)
+    t = 1 / (1 + slope * m)
+    for column, worst, mean in ((0, 5e-9, 1e-9), (1, 1e-7, 1e-8)):
+        coef = [float(np.float32(row[column])) for row in table]
+        e = t * sum(c * t ** k for k, c in enumerate(coef)) / torch.special.erfcx(m / math.sqrt(2)) - 1
+        assert float(e.abs().max()) <= worst and abs(float(e.mean())) <= mean, (column, float(e.abs().max()), float(e.mean()))
 
 
 @gpu

@@ -515,7 +515,9 @@ Tensor restore8(const Tensor &codes_, const Tensor &ranges_, bool bf16) {
     const Rows r(codes_);
     need_cuda(codes_); need_device(ranges_, codes_, "ranges");
     const c10::cuda::CUDAGuard guard(codes_.device());
-    const Tensor codes = codes_.contiguous(), ranges = ranges_.contiguous();
+    const Tensor codes = codes_.contiguous();
+    Tensor ranges = ranges_.contiguous();
+    if ((uintptr_t)ptr(ranges) & 7) ranges = ranges.clone();      // (read in pairs; a view of a larger buffer may start between two)
     Tensor y = fresh(codes.sizes(), bf16 ? at::kBFloat16 : at::kFloat, codes);
     if (r.rows)
         check(o1d_restore8((const uint8_t *)ptr(codes), (const float *)ptr(ranges), y.data_ptr(), r.rows, (int)r.C, bf16 ? O1D_BF16 : O1D_F32, stream()),

@@ -306,6 +306,18 @@ def test_layouts_views_and_empty_tensors():
 
 
 @gpu
+def test_a_checkpoint_stored_anywhere():
+    """Codes and ranges that are views of a larger buffer, off every alignment, or strided."""
+    x = make(64, 200, "fp32").cuda()
+    codes, ranges = ops.keep8(x)
+    want = ops.restore8(codes, ranges)
+    c, r = torch.empty(64 * 200 + 3, dtype=torch.uint8, device="cuda"), torch.empty(64 * 4 + 1, device="cuda")
+    c[3:], r[1:] = codes.reshape(-1), ranges.reshape(-1)
+    assert torch.equal(ops.restore8(c[3:].view(64, 200), r[1:].view(64, 2, 2)), want)
+    assert torch.equal(ops.restore8(codes.t().contiguous().t(), ranges.permute(2, 0, 1).contiguous().permute(1, 2, 0)), want)
+
+
+@gpu
 def test_parameters_of_any_shape():
     """Only the number of elements counts; a gradient has its parameter's shape."""
     x = make(6, 40, "fp32").cuda()

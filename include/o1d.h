@@ -265,7 +265,8 @@ int o1d_linear_xent(const void *x, const void *w, const void *bias, const long l
                     float label_smoothing, int reduction, int dtype, void *stream);
 /* Its backward pass; dloss is the gradient of `loss` (fp32, [N] or [1]).  dx, dw (type `dtype`) and db (the bias's type)
  * may each be NULL.  The softmax is formed again, in pieces of the vocabulary (or of the rows, where those are more) of up
- * to 192 MB of its gradient; sums over pieces are fp32 and in a fixed order (bit-reproducible, no atomics).  For bf16 the gradient of
+ * to 192 MB of its gradient, or 256 rows or columns of it where those are more (beyond 131072 of both in fp32, 393216 in
+ * bf16); sums over pieces are fp32 or wider and in a fixed order (bit-reproducible, no atomics).  For bf16 the gradient of
  * the logits is rounded to bf16 (to 16 bits up to 2^30 products) before the two products that read it. */
 int o1d_linear_xent_bwd(const void *x, const void *w, const void *bias, const long long *target, const float *lse,
                         const float *count, const float *dloss, void *dx, void *dw, void *db, void *workspace,

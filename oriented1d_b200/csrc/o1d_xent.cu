@@ -12,8 +12,10 @@ namespace {
 
 // Bytes of G that are held at once.  Larger pieces have fewer waves that end half empty and fewer rounds of adding to fp32
 // sums, which is worth more than finding a piece in the L2 cache; 4096 x 1024 x 21841 bf16, gradient alone: 40 MB 557 us,
-// 80 MB 512, 128 MB 489, all 179 MB in one piece 452 (the step 694 -> 673; 2500 x 384 x 10007 fp32, 150 MB, 507 -> 497).  A
-// thousandth of the device's memory.
+// 80 MB 512, 128 MB 489, all 179 MB in one piece 452 (the step 694 -> 673; 2500 x 384 x 10007 fp32, 150 MB, 507 -> 497).  Where
+// more pieces than one it is, bf16, with pieces of 128 / 192 / 448 MB: 8192 x 1024 x 21841 957 / 901 / 842 us, 6000 x 512 x 30000
+// 755 / 686 / 646, 16384 x 384 x 10000 640 / 583 / 547, 65536 x 256 x 4000 704 / 737 / 681; fp32 4096 x 384 x 10007 588 / 609 / 589.
+// A thousandth of the device's memory.  (At least 256 rows or columns: the products' tiles.)
 constexpr long long kPieceBytes = 192ll << 20;
 constexpr int kMinSplitSteps = 16;               // K steps that a part of a split axis has at least (joining parts costs a launch)
 constexpr int kSlicesAtOnce = 512;               // column sums of more slices are added in two steps
@@ -269,9 +271,9 @@ BackwardBytes backward_bytes(const XentArgs &a, const Cut &c) {
     // by rows, dx is complete with its piece; by vocabulary, dw is
     b.dx = (size_t)up_to(4ll * c.dx_parts * c.rows * a.D, 256);
     b.dw = (size_t)up_to(4ll * c.dw_parts * (c.by_rows ? a.V : c.piece) * a.D, 256);
-    // column sums of a piece, in slices of 32 rows; and of all pieces, in slices of kSlicesAtOnce of those
+    // column sums of a piece, in slices of 32 rows; and (by rows: of all pieces) of kSlicesAtOnce of those
     b.col = (size_t)up_to(4ll * cdiv(c.rows, 32) * c.ld, 256);
-    b.more = (size_t)up_to(4ll * c.col_blocks() * (c.by_rows ? c.pieces : 1) * up_to(a.V, 64), 256);
+    b.more = c.col_once() ? 0 : (size_t)up_to(8ll * c.col_blocks() * c.ld, 256);
     return b;
 }
 
@@ -417,7 +419,7 @@ int backward(Run &r) {
     float *dxs = (float *)ws; ws += b.dx;
     float *dws = (float *)ws; ws += b.dw;
     float *cols = (float *)ws; ws += b.col;
-    float *more = (float *)ws; ws += b.more;
+    double *more = (double *)ws; ws += b.more;
     Mat x, w;
     int rc = make_operand(r, a.x, operand_of(a.N, a.D, a.bf16), &ws, &x);
     if (!rc) rc = make_operand(r, a.w, operand_of(a.V, a.D, a.bf16), &ws, &w);
@@ -426,7 +428,6 @@ int backward(Run &r) {
     const bool each = a.reduction == O1D_XENT_NONE;
     const float f = a.smoothing < 1.f ? 1.f - a.smoothing : 1.f;
     const float *up = each ? nullptr : a.dloss, *count = a.reduction == O1D_XENT_MEAN ? a.count : nullptr;
-    const long long part_ld = up_to(a.V, 64);
     // One product's way out: its result at once, or sums that `finish` turns into it.
     // (the last piece of a product whose pieces have one part adds the others to what it writes)
     auto out_of = [&](XentParams &p, int parts, bool first, bool last, void *result, float *sums, long long elems, long long k) {
@@ -448,7 +449,6 @@ int backward(Run &r) {
         return a.bf16 ? finish<__nv_bfloat16>(sums, result, elems, parts, up, count, f, r.st)
                       : finish<float>(sums, result, elems, parts, up, count, f, r.st);
     };
-    int more_slices = 0;
     for (int i = 0; i < c.pieces; i++) {
         const long long at = i * c.piece, axis = c.by_rows ? a.N : a.V, n = axis - at < c.piece ? axis - at : c.piece;
         const long long row0 = c.by_rows ? at : 0, rows = c.by_rows ? n : a.N;
@@ -483,21 +483,18 @@ int backward(Run &r) {
         }
         if (e == cudaSuccess && a.db) {
             const int slices = cdiv(rows, 32);
-            if (c.col_once())
-                xent_bias_kernel<<<cdiv(colsn, 32), dim3(32, 32), 0, r.st>>>(cols, ld, slices, slices, (char *)a.db + (long long)col0 * (a.bias_bf16 ? 2 : 4),
-                                                                             a.bias_bf16, nullptr, 0, colsn, up, count, f);
-            else
+            void *to = (char *)a.db + (long long)col0 * (a.bias_bf16 ? 2 : 4);
+            if (c.col_once()) {
+                xent_bias_kernel<<<cdiv(colsn, 32), dim3(32, 32), 0, r.st>>>(cols, ld, slices, slices, to, a.bias_bf16, nullptr, 0, false, colsn, up, count, f);
+            } else {
                 xent_bias_kernel<<<dim3(cdiv(colsn, 32), cdiv(slices, kSlicesAtOnce)), dim3(32, 32), 0, r.st>>>(
-                    cols, ld, slices, kSlicesAtOnce, nullptr, 0, more + (long long)(c.by_rows ? i : 0) * c.col_blocks() * part_ld + col0, part_ld, colsn, nullptr,
-                    nullptr, 1.f);
-            more_slices = c.by_rows ? i * c.col_blocks() + cdiv(slices, kSlicesAtOnce) : c.col_blocks();
+                    cols, ld, slices, kSlicesAtOnce, nullptr, 0, more, c.ld, c.by_rows && i > 0, colsn, nullptr, nullptr, 1.f);
+                if (!c.by_rows || i == c.pieces - 1)
+                    xent_bias_kernel<<<cdiv(colsn, 32), dim3(32, 32), 0, r.st>>>(more, c.ld, c.col_blocks(), c.col_blocks(), to, a.bias_bf16, nullptr, 0, false, colsn,
+                                                                                 up, count, f);
+            }
             e = cudaGetLastError();
         }
-        if (e != cudaSuccess) return r.fail(e);
-    }
-    if (a.db && !c.col_once()) {
-        xent_bias_kernel<<<cdiv(a.V, 32), dim3(32, 32), 0, r.st>>>(more, part_ld, more_slices, more_slices, a.db, a.bias_bf16, nullptr, 0, a.V, up, count, f);
-        const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return r.fail(e);
     }
     return O1D_OK;

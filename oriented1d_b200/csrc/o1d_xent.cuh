@@ -1000,10 +1000,11 @@ xent_finish_few_kernel(const float *__restrict__ sums, T *__restrict__ out, long
 }
 
 // Column sums over slices of 32 rows, in a fixed order.  Block (32, 32); CTA (bx, by): columns 32 bx .., slices by * per ..
-// With one CTA along y the result is db (times alpha), else partial sums again.
+// With one CTA along y the result is db (times alpha), else sums of `per` slices, written or (`add`: of a later piece of the rows) added to.
+template <typename P>
 __global__ void __launch_bounds__(1024)
-xent_bias_kernel(const float *__restrict__ partial, long long part_ld, int slices, int per, void *__restrict__ db, int bf16, float *__restrict__ more,
-                 long long more_ld, int V, const float *up, const float *count, float f) {
+xent_bias_kernel(const P *__restrict__ partial, long long part_ld, int slices, int per, void *__restrict__ db, int bf16, double *__restrict__ more,
+                 long long more_ld, bool add, int V, const float *up, const float *count, float f) {
     __shared__ double part[32][33];
     const int c = blockIdx.x * 32 + threadIdx.x, end = min(slices, (int)(blockIdx.y + 1) * per);
     double s = 0.;
@@ -1016,8 +1017,12 @@ xent_bias_kernel(const float *__restrict__ partial, long long part_ld, int slice
         double t = 0.;
 #pragma unroll
         for (int y = 0; y < 32; y++) t += part[y][threadIdx.x];
-        if (more) more[blockIdx.y * more_ld + c] = (float)t;
-        else st_param(db, c, bf16, xent_alpha(up, count, f) * (float)t);
+        if (more) {
+            double &to = more[blockIdx.y * more_ld + c];
+            to = add ? to + t : t;
+        } else {
+            st_param(db, c, bf16, xent_alpha(up, count, f) * (float)t);
+        }
     }
 }
 

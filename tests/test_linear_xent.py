@@ -289,6 +289,27 @@ def test_extreme_rows_of_few_classes():
 
 
 @gpu
+@pytest.mark.parametrize("N,D,V,dtype", [(20001, 16, 24001, "bf16"), (60001, 16, 4001, "bf16"), (50001, 24, 1000, "bf16"), (17001, 8, 18001, "fp32"),
+                                         (40001, 8, 3001, "fp32")])
+def test_bias_gradient_of_many_rows(N, D, V, dtype):
+    """More than 16384 rows a piece, whose column sums are added in two steps: pieces of the classes, of the rows (a short last one), and one."""
+    check(N, D, V, dtype, "other" if dtype == "bf16" else "same", ignored=0.1, reduction="sum")
+
+
+@gpu
+@pytest.mark.parametrize("N,V", [(131072, 131072), (500_000, 500_000), (2_000_000, 300_000), (300_000, 2_000_000), (4096, 21841), (9, 10_000_000)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_workspace_of_the_backward_pass(N, V, dtype):
+    """What include/o1d.h says of it: the logits' gradient in pieces of 192 MB, or of 256 rows or columns where those are more, and
+    beside it planes of the operands (none for bf16 rows of whole vectors), fp32 sums of the pieces' products and column sums of 32 rows."""
+    D, planes = 8, 1 if dtype else 3
+    piece = max(192 << 20, 256 * 2 * planes * (min(N, V) + 64))
+    operands = 0 if dtype else planes * 2 * D * (N + V)
+    sums = 4 * D * (N + V) + 4 * D * 148 * 4096                              # of one part each, or parts that are short
+    assert o1d._lib.lib.o1d_linear_xent_workspace_bytes(N, D, V, dtype, 1) <= piece * (1 + 1 / 16) + operands + sums + (64 << 20)
+
+
+@gpu
 def test_gradients_against_differences():
     """The fp32 gradient against central differences of the float64 loss along random directions."""
     x, w, b, t = make(70, 48, 90, "fp32", ignored=0.2)

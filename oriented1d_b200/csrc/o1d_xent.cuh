@@ -8,17 +8,23 @@
 //   GRAD     the same tiles once more; the epilogue turns a piece of them into G (bf16) in the workspace.
 //   OUT      G w and G^T x over that piece, to the output or to fp32 sums that later pieces (and the other parts of a
 //            split K axis) add to in a fixed order.
-// Logits are formed twice (8NDV operations where 6NDV would do) because to keep them in fp32 costs more in traffic than
-// the product does, and to keep them in bf16 costs the softmax its accuracy.
+// Logits are formed twice (8NDV operations where 6NDV would do): kept between the passes they are the memory that this operator
+// is there to save (4096 x 1024 x 21841 in fp32: 358 MB, and 109 us to write and read, about what the product takes), and in bf16
+// they cost the softmax its accuracy.
 //
 // fp32 inputs are cut into three bf16 planes each (x = x0 + x1 + x2 exactly, 8 bits a plane); of the nine products of
 // planes the six above 2^-24 are taken.  x0 w0 has an accumulator of its own, the five small ones share another, and
 // both are added to fp32 registers every 256 of K: a tensor core adds with truncation, which over thousands of steps
 // would show.
 //
-// Rounding: G is rounded to bf16 for bf16 inputs (half a unit of 2^-8, random from element to element; dx and dw are
-// rounded so themselves), or to two planes of it where that costs nothing (XENT_FINE).  So that the rounding of the coefficient 1-e, which every row shares, cannot add up, G is kept divided
-// by 1-e and the factor applied to the fp32 sums.  All sums, statistics and the loss are fp32 or wider.
+// Rounding: G is rounded to bf16 for bf16 inputs (2^-8 of an element at most, as dx and dw are themselves), or to two planes of it
+// where that costs nothing (XENT_FINE).  Where rows differ so do these roundings, and they cancel in the sums; where rows have an
+// element of G in common they do not.  The coefficient 1-e of the target is kept out: G is divided by it, so that the target's -1
+// is exact, and the factor applied to the fp32 sums.  What stays is e/V of the classes that a row gives no weight, and all of G
+// where logits are alike: dx and dw are then off by up to 2^-8 before their own rounding (8192 x 512 x 1000, rows sure of their
+// class: e = 0.1 2.2e-3 norm-wise, e = 0.3 2.0e-3; rounding the results alone is 1.7e-3).  All sums, statistics and the loss are
+// fp32 or wider.  A bf16 logit is one accumulator's sum over D, which truncates as it adds: D/16 additions, each off by up to
+// 2^-23 of the sum so far (the loss of 256 x D x 200: within 9.5e-6 at D = 1024, 2.3e-5 at 2048; in fp32 1.3e-6).
 #pragma once
 
 #include "o1d_common.cuh"

@@ -172,7 +172,12 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index: int = -100,
     """F.cross_entropy(F.linear(x, weight, bias), target, ...) without the logits: features x [..., D], weight [V, D],
     bias [V] or None, int64 class indices target [...]; the loss is fp32, a scalar or (reduction="none") of target's
     shape.  Differentiable in x, weight and bias.  The logits exist a tile at a time on the chip, and their gradient a piece
-    of the classes at a time; what is kept between the passes is three floats a row.
+    of the classes or rows at a time (up to 192 MB, or 256 rows or classes where those are more); what is kept between the
+    passes is three floats a row.
+
+    Sums, the softmax and the loss are fp32 or wider.  For bf16 features the gradient of the logits is rounded to bf16 before
+    the products that give x's and weight's gradients (to 16 bits up to 2^30 rows x classes x features), so these are off by up
+    to 2^-8 before they are rounded themselves.
 
     A row with target == ignore_index has no loss and no gradient; a target that is no class makes the row's loss (and the
     gradients) NaN, where torch stops the process.  weight is brought to x's dtype where it differs."""
@@ -199,8 +204,9 @@ def restore8(codes, ranges, dtype: torch.dtype = torch.float32):
 
 def gelu_keep8(x, bias=None):
     """Exact GELU of x + bias (bias [C], broadcast over the rows; or None), keeping for the backward pass 1.06 bytes an
-    element in place of the tensor: the checkpoint keep8() makes of x + bias.  The output is that of F.gelu; dx and the
-    bias gradient are taken at the values the checkpoint stands for.  Without gradients nothing is kept."""
+    element in place of the tensor: the checkpoint keep8() makes of x + bias.  The output is that of F.gelu (at -inf its
+    limit, 0, where F.gelu has NaN); dx and the bias gradient are taken at the values the checkpoint stands for.  Without
+    gradients nothing is kept."""
     return ext.gelu_keep8(x, bias)
 
 

@@ -289,6 +289,31 @@ def test_extreme_rows_of_few_classes():
 
 
 @gpu
+@pytest.mark.parametrize("rows", ["sure", "alike"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 0.3, 0.9])
+@pytest.mark.parametrize("N,D,V", [(80003, 96, 150), (8190, 512, 1000)])
+def test_gradients_that_all_rows_round_alike(N, D, V, smoothing, rows):
+    """More than 2^30 products, where the logits' gradient G is rounded to bf16 (2^-8 of an element at most), and rows whose G are the
+    same numbers, so that roundings do not average out: every row sure of its class (smoothing leaves e/V for each other class), or equal
+    logits everywhere.  They add up to 2^-8 of the gradient at most, and its own rounding is another 2^-8."""
+    x, w, b, t = make(N, D, V, "bf16", bias=None)
+    with torch.no_grad():
+        if rows == "sure":
+            w.copy_(torch.randn(V, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0)))
+            x.copy_(1.5 * w[t].float() + torch.rand(x.shape, device="cuda"))
+        else:
+            w.zero_()
+    up = torch.ones((), device="cuda")
+    loss, e_loss, grads = reference(x, w, None, t, up, -100, smoothing, "mean")
+    leaves = [v.requires_grad_(True) for v in (x, w)]
+    got = ops.linear_cross_entropy(x, w, t, label_smoothing=smoothing)
+    within(got.detach(), loss, e_loss, "loss")
+    for o, (ref, bound), what in zip(torch.autograd.grad(got, leaves), grads, ("dx", "dw")):
+        within(o, ref, bound, what)
+        assert float((o.double() - ref).norm()) <= 2 * 2.0 ** -8 * float(ref.norm()), what
+
+
+@gpu
 @pytest.mark.parametrize("N,D,V,dtype", [(20001, 16, 24001, "bf16"), (60001, 16, 4001, "bf16"), (50001, 24, 1000, "bf16"), (17001, 8, 18001, "fp32"),
                                          (40001, 8, 3001, "fp32")])
 def test_bias_gradient_of_many_rows(N, D, V, dtype):

@@ -249,7 +249,8 @@ int o1d_pointwise_in(const void *x, const float *w, const float *bias, void *y,
 /* Softmax cross entropy of a linear classifier (the reference's head and criterion: models/convnext.py:495-610 and
  * the loss of engine.py:14-132), without the logits: with l = x w^T + bias,
  *   loss[n] = logsumexp(l[n]) - (1 - e) l[n, t_n] - (e / V) sum_v l[n, v],   e = label_smoothing in [0, 1].
- * x [N, D] and w [V, D] of type `dtype`, each starting on 16 bytes, bias [V] (or NULL) fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16; target [N].
+ * x [N, D] and w [V, D] of type `dtype`, each starting on 16 bytes, N, D and V at most 2^31 - 65536; bias
+ * [V] (or NULL) fp32, or bf16 with dtype | O1D_FLAG_PARAMS_BF16; target [N].
  * A row whose target is ignore_index has no loss and no gradient; one whose target is outside [0, V) has a NaN loss
  * (and a NaN gradient).  reduction: O1D_XENT_NONE (loss [N]), _SUM, _MEAN (over the rows not ignored; loss [1]).
  * lse [3, N] (the log-sum-exp of a row, base 2, in two floats, and log2 of the target's probability) and count [1] (not

@@ -1292,7 +1292,7 @@ bool bad_xent(const XentArgs &a, int dtype) {
            !(a.smoothing >= 0.f && a.smoothing <= 1.f) || a.reduction < O1D_XENT_NONE || a.reduction > O1D_XENT_MEAN;
 }
 int xent_call(const XentArgs &a, bool backward, void *stream) {
-    if (a.N > 0x7fffff00LL || a.V > 0x7fffff00 || (((uintptr_t)a.x | (uintptr_t)a.w) & 15)) return O1D_ERR_UNSUPPORTED;
+    if (a.N > kXentMost || a.V > kXentMost || a.D > kXentMost || (((uintptr_t)a.x | (uintptr_t)a.w) & 15)) return O1D_ERR_UNSUPPORTED;
     DeviceInfo d;
     int rc = device_info(&d), *flag = nullptr;
     if (!rc) rc = device_flag_ptr(&flag);
@@ -1314,7 +1314,7 @@ size_t o1d_linear_xent_workspace_bytes(long long N, int D, int V, int dtype, int
     a.N = N; a.D = D; a.V = V; a.bf16 = dtype == O1D_BF16;
     a.lse = pass == O1D_XENT_EVALUATION ? nullptr : &any;                 // (a request with or without it; not read)
     DeviceInfo d;
-    if (N <= 0 || D <= 0 || V <= 0 || N > 0x7fffff00LL || V > 0x7fffff00 || (dtype != O1D_F32 && dtype != O1D_BF16) ||
+    if (N <= 0 || D <= 0 || V <= 0 || N > kXentMost || V > kXentMost || D > kXentMost || (dtype != O1D_F32 && dtype != O1D_BF16) ||
         pass < O1D_XENT_FORWARD || pass > O1D_XENT_EVALUATION || device_info(&d))
         return 0;
     return xent_workspace(a, pass == O1D_XENT_BACKWARD, d.sms);

@@ -737,7 +737,7 @@ struct XentShape {
             throw py::value_error(s.str());
         }
         if (!(smoothing >= 0. && smoothing <= 1.)) throw py::value_error("label_smoothing must be between 0 and 1");
-        if (D > INT32_MAX || V > 0x7fffff00 || N > 0x7fffff00) throw py::value_error("more than 2^31 rows, classes or features are not supported");
+        if (D > 0x7fff0000 || V > 0x7fff0000 || N > 0x7fff0000) throw py::value_error("more than 2^31 - 65536 rows, classes or features are not supported");
         need_cuda(x); need_device(w, x, "weight"); need_device(target, x, "target");
         if (bias) need_device(*bias, x, "bias");
     }

@@ -7,6 +7,9 @@
 
 namespace o1d {
 
+// Rows, classes and features, each: kernels hold their indices in 32 bits and step past an end by up to a grid's worth of classes (10^4).
+constexpr int kXentMost = 0x7fff0000;
+
 struct XentArgs {
     const void *x, *w, *bias;                 // [N, D], [V, D], [V] or null
     const long long *target;                  // [N]

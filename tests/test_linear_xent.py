@@ -538,6 +538,23 @@ def test_refusals():
         f(x, w, t)
 
 
+def test_sizes_that_indices_do_not_hold():
+    """One-row steps past the last class stay within 32 bits up to 2^31 - 65536; sizes above are refused before any device is asked."""
+    lib, p = o1d._lib.lib, torch.zeros(256).data_ptr()
+    for k in range(3):
+        n = [4, 8, 10]
+        n[k] = 2 ** 31 - 65535
+        assert lib.o1d_linear_xent(p, p, None, p, p, None, p, p, 0, *n, -100, 0.0, 2, 0, None) == 2
+        assert lib.o1d_linear_xent_bwd(p, p, None, p, p, p, p, p, p, None, p, 0, *n, -100, 0.0, 2, 0, None) == 2
+        assert lib.o1d_linear_xent_workspace_bytes(*n, 0, 0) == 0
+    one = torch.zeros(1, 1)
+    wide = torch.zeros(1).expand(1, 2 ** 31 - 1)
+    for x, w, t in ((one, one.expand(2 ** 31 - 65535, 1), torch.zeros(1, dtype=torch.int64)), (wide, wide, torch.zeros(1, dtype=torch.int64)),
+                    (one.expand(2 ** 31 - 65535, 1), one, torch.zeros((), dtype=torch.int64).expand(2 ** 31 - 65535))):
+        with pytest.raises(ValueError, match="65536"):
+            ops.linear_cross_entropy(x, w, t)
+
+
 def test_entry_points_reject_bad_arguments():
     lib, buf = o1d._lib.lib, torch.zeros(256)
     p = buf.data_ptr()

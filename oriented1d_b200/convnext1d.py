@@ -130,12 +130,13 @@ class Block1D(nn.Module):
         return F.gelu(h) if gelu else h
 
     def _mlp(self, x):
-        # under autocast the products run in the region's type, as those of the separate layers do
-        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-        plain = ops.bare(self.norm, LayerNorm) and ops.bare(self.pwconv1, nn.Linear) and ops.bare(self.pwconv2, nn.Linear)
-        if self.keep8 and plain and x.is_cuda and torch.is_grad_enabled() and dtype in (torch.float32, torch.bfloat16):
-            return ops.mlp_keep8(x.to(dtype), self.norm.weight, self.norm.bias, self.pwconv1.weight, self.pwconv1.bias, self.pwconv2.weight,
-                                 self.pwconv2.bias, self.norm.eps)
+        if self.keep8 and x.is_cuda and torch.is_grad_enabled():
+            # under autocast the products run in the region's type, as those of the separate layers do
+            dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+            plain = ops.bare(self.norm, LayerNorm) and all(ops.bare(p, nn.Linear) and p.bias is not None for p in (self.pwconv1, self.pwconv2))
+            if plain and dtype in (torch.float32, torch.bfloat16):
+                return ops.mlp_keep8(x.to(dtype), self.norm.weight, self.norm.bias, self.pwconv1.weight, self.pwconv1.bias, self.pwconv2.weight,
+                                     self.pwconv2.bias, self.norm.eps)
         return ops.linear_cl(self.pwconv2, self._mlp_in(x))
 
     def forward(self, x):

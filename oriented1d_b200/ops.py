@@ -152,11 +152,9 @@ def bare(module, kind) -> bool:
 
 def linear_cl(module, x):
     """module(x) for an nn.Linear; on CUDA with gradients enabled the bias gradient runs here."""
-    if not bare(module, torch.nn.Linear):
-        return module(x)
-    C = module.out_features
-    if (x.is_cuda and torch.is_grad_enabled() and module.bias is not None and x.dtype == module.weight.dtype
-            and x.dtype in (torch.float32, torch.bfloat16) and C % (4 if x.dtype == torch.float32 else 8) == 0):
+    if (x.is_cuda and torch.is_grad_enabled() and bare(module, torch.nn.Linear) and module.bias is not None
+            and x.dtype == module.weight.dtype and x.dtype in (torch.float32, torch.bfloat16)
+            and module.out_features % (4 if x.dtype == torch.float32 else 8) == 0):
         return LinearCL.apply(x, module.weight, module.bias)
     return module(x)
 

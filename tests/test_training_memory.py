@@ -226,6 +226,9 @@ def test_hooks_on_the_layers_of_a_block(keep8):
         assert seen == ["before", "after", "back"], name
         for h in handles:
             h.remove()
+    block.pwconv1 = torch.nn.Linear(64, 256, bias=False).cuda()                # a layer in its place that has no bias
+    block._mlp(x).sum().backward()
+    assert block.pwconv1.weight.grad is not None
 
 
 @gpu
